@@ -444,6 +444,96 @@ int sdm_rt_table_backward(const sdm_rt_dims* dims, const sdm_rt_params* params,
                           float* d_keys1, float* d_keys2, float* d_log_scale,
                           void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- the vocabulary's ends: embedding, distillation loss, rules on logits ------------------------------------- */
+
+/* The scaled embedding lookup (OneSdmLM's emb, track4_onesdm_models.py:534-535, with a factor): out[i] =
+ * round(scale * table[ids[i]]), n tokens.  ids int64, each in [0, vocab) (one outside is clamped into it: the host reads
+ * none).  table [vocab][d], out [n][d] in dtype, row strides in elements, any alignment of an element.  At most 2^30
+ * tokens, a vocabulary of 2^25 and rows of 2^20 values. */
+int sdm_rt_embed(const int64_t* ids, int64_t n, const void* table, int64_t table_row_stride, sdm_rt_dtype dtype,
+                 int64_t vocab, int32_t d, float scale, void* out, int64_t out_row_stride, void* stream);
+
+/* Bytes of workspace sdm_rt_embed_backward needs (0 on sizes outside its limits). */
+size_t sdm_rt_embed_backward_workspace_bytes(int64_t n, int64_t vocab, int32_t d);
+
+/* The gradient of sdm_rt_embed's table: d_table[v] = round(scale * the sum over the tokens i of v of dy[i]), every row
+ * written (zeros for a token that does not occur, and for padding_idx; -1: none).  The tokens are put in the order of
+ * their rows and summed in a fixed order in float32, without atomics on floats: the result is deterministic.  ids as
+ * in sdm_rt_embed; dy [n][d], d_table [vocab][d] in dtype. */
+int sdm_rt_embed_backward(const int64_t* ids, int64_t n, const void* dy, int64_t dy_row_stride, sdm_rt_dtype dtype,
+                          int64_t vocab, int32_t d, float scale, int64_t padding_idx, void* d_table,
+                          int64_t d_table_row_stride, void* workspace, size_t workspace_bytes, void* stream);
+
+enum { SDM_RT_NONE = 0, SDM_RT_MEAN = 1, SDM_RT_SUM = 2 };
+
+/* The distillation loss of rows of student logits z against a teacher's top logits, joined by the cross entropy of
+ * labels.  A row's teacher is its entries i with an id in [0, vocab) and a logit t_i whose t_i / temperature is not -inf
+ * (an id may repeat: its shares add up); q = softmax(t / temperature) over them, p = softmax(z / temperature) over the
+ * vocabulary.  A row's label counts if it is in [0, vocab) and not ignore_index.
+ *   row loss = alpha temperature^2 sum_i q_i (log q_i - log p_{id_i}) + (1 - alpha) (-log softmax(z)_label)
+ * with only the terms that the row has: a part of weight 0 (alpha 0, or 1) counts as absent, and a row with neither has
+ * loss 0 and gradient 0 whatever its logits hold.  reduction: SDM_RT_NONE gives the rows' losses, SDM_RT_SUM their sum,
+ * SDM_RT_MEAN that over the number of rows with a target (0 if there is none). */
+typedef struct {
+  int64_t rows;          /* at most 2^22 */
+  int32_t vocab;         /* at most 2^30 */
+  int32_t top_k;         /* teacher entries per row, 0 to 1,024 */
+  float temperature;     /* positive */
+  float alpha;           /* in [0, 1] */
+  int64_t ignore_index;
+  int32_t reduction;
+} sdm_rt_distill;
+
+/* Bytes of workspace sdm_rt_distill_loss needs. */
+size_t sdm_rt_distill_workspace_bytes(const sdm_rt_distill* dims);
+
+/* loss: [rows] (SDM_RT_NONE) or [1] float32.
+ *   logits [rows][vocab] in dtype, top_ids [rows][top_k] int64, top_logits [rows][top_k] float32, row strides in elements;
+ *   labels [rows] int64 or NULL;  stats [rows][4] float32, 16-byte aligned, for sdm_rt_distill_grad, or NULL */
+int sdm_rt_distill_loss(const sdm_rt_distill* dims, const void* logits, int64_t logits_row_stride, sdm_rt_dtype dtype,
+                        const int64_t* top_ids, int64_t top_ids_row_stride, const float* top_logits,
+                        int64_t top_logits_row_stride, const int64_t* labels, float* loss, float* stats, void* workspace,
+                        size_t workspace_bytes, void* stream);
+
+/* d_logits [rows][vocab] in dtype: the gradient of sdm_rt_distill_loss of the same inputs (stats from that call) for
+ * grad_out, the gradient of loss: float32 on the device, [rows] (SDM_RT_NONE) or [1]. */
+int sdm_rt_distill_grad(const sdm_rt_distill* dims, const void* logits, int64_t logits_row_stride, sdm_rt_dtype dtype,
+                        const int64_t* top_ids, int64_t top_ids_row_stride, const float* top_logits,
+                        int64_t top_logits_row_stride, const int64_t* labels, const float* stats, const float* grad_out,
+                        void* d_logits, int64_t d_logits_row_stride, void* stream);
+
+/* The rules of a decode step on its logits, in this order, in float32:
+ *   a token of the stream's history        x = x > 0 ? x / repetition : x * repetition
+ *   one that occurred c > 0 times in it at or after position prompt   x -= c * frequency + presence
+ *   x += bias;  not allowed by the mask     x = -inf (whatever it was)
+ * tokens [rows][width] int64 (ids outside the vocabulary count nowhere), of which the first lengths[row] are a stream's
+ * history; where lengths[row] exceeds width the row is a ring that holds its last width tokens, position p at p mod width
+ * (sdm_rt_append_tokens).  A NULL pointer leaves its rule out; NULL repetition, frequency or presence takes the
+ * *_all value for every row.  A row stride of 0 gives every row the same bias or mask. */
+typedef struct {
+  const int64_t* tokens;
+  int64_t tokens_row_stride;
+  int64_t width;
+  const int64_t* lengths;    /* [rows] */
+  const int64_t* prompt;     /* [rows] or NULL (0) */
+  const float* repetition;   /* [rows] or NULL */
+  const float* frequency;
+  const float* presence;
+  float repetition_all, frequency_all, presence_all;
+  const float* bias;         /* rows of vocab float32 */
+  int64_t bias_row_stride;
+  const uint32_t* mask;      /* rows of ceil(vocab / 32) words, bit v mod 32 of word v / 32 set: token v is allowed */
+  int64_t mask_row_stride;
+} sdm_rt_rules;
+
+/* logits, out [rows][vocab] in dtype, each value rounded once; out may be logits itself.  At most 65,535 rows. */
+int sdm_rt_process_logits(const sdm_rt_rules* rules, const void* logits, int64_t logits_row_stride, sdm_rt_dtype dtype,
+                          int64_t rows, int32_t vocab, void* out, int64_t out_row_stride, void* stream);
+
+/* One token more of each stream: tokens[row][lengths[row] mod width] = new_ids[row], lengths[row] += 1. */
+int sdm_rt_append_tokens(int64_t* tokens, int64_t tokens_row_stride, int64_t width, int64_t* lengths,
+                         const int64_t* new_ids, int64_t rows, void* stream);
+
 /* Description of the last failure on the calling thread ("" if none). */
 const char* sdm_rt_last_error(void);
 

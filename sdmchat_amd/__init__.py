@@ -6,8 +6,9 @@
 ``core``            torch-facing wrappers of the C ABI (addressing, the SDM core)
 ``synthetic``       seeded synthetic parameters and inputs of the layer workloads
 ``DecodeGraph``, ``ForwardGraph``  OneSdmLM.step and OneSdmLM.forward at fixed shapes, captured in HIP graphs
+``TokenRules``      penalties for repeated tokens, a bias and a grammar mask on a decode loop's logits
 ``build``           compiles ``csrc/*.hip`` into ``lib/libsdm_rt.so``
 """
 from .runtime_sdm import RMSNorm, RunTimeSdm  # noqa: F401
 from .trained_sdm import TrainedSdm  # noqa: F401
-from .model import DecodeGraph, ForwardGraph, ModelDecodeState, OneSdmLM, decode_state_bytes  # noqa: F401
+from .model import DecodeGraph, ForwardGraph, ModelDecodeState, OneSdmLM, TokenRules, decode_state_bytes  # noqa: F401

@@ -11,6 +11,8 @@ LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "lib", "libs
 SDM_RT_F32 = 0
 SDM_RT_BF16 = 1
 
+SDM_RT_NONE, SDM_RT_MEAN, SDM_RT_SUM = 0, 1, 2
+
 # every function the header declares, with its ctypes signature
 c_void_p = ctypes.c_void_p
 c_i64 = ctypes.c_int64
@@ -57,6 +59,38 @@ class SdmRtSaved(ctypes.Structure):
         ("scores_r", c_void_p),
         ("read", c_void_p),
         ("den", c_void_p),
+    ]
+
+
+class SdmRtDistill(ctypes.Structure):
+    _fields_ = [
+        ("rows", c_i64),
+        ("vocab", ctypes.c_int32),
+        ("top_k", ctypes.c_int32),
+        ("temperature", ctypes.c_float),
+        ("alpha", ctypes.c_float),
+        ("ignore_index", c_i64),
+        ("reduction", ctypes.c_int32),
+    ]
+
+
+class SdmRtRules(ctypes.Structure):
+    _fields_ = [
+        ("tokens", c_void_p),
+        ("tokens_row_stride", c_i64),
+        ("width", c_i64),
+        ("lengths", c_void_p),
+        ("prompt", c_void_p),
+        ("repetition", c_void_p),
+        ("frequency", c_void_p),
+        ("presence", c_void_p),
+        ("repetition_all", ctypes.c_float),
+        ("frequency_all", ctypes.c_float),
+        ("presence_all", ctypes.c_float),
+        ("bias", c_void_p),
+        ("bias_row_stride", c_i64),
+        ("mask", c_void_p),
+        ("mask_row_stride", c_i64),
     ]
 
 
@@ -170,6 +204,21 @@ SIGNATURES = {
                                              c_void_p, c_i64, c_void_p,
                                              c_void_p, c_void_p, c_void_p,
                                              c_void_p, ctypes.c_size_t, c_void_p]),
+    "sdm_rt_embed": (ctypes.c_int, [c_void_p, c_i64, c_void_p, c_i64, ctypes.c_int, c_i64, ctypes.c_int32, ctypes.c_float,
+                                    c_void_p, c_i64, c_void_p]),
+    "sdm_rt_embed_backward_workspace_bytes": (ctypes.c_size_t, [c_i64, c_i64, ctypes.c_int32]),
+    "sdm_rt_embed_backward": (ctypes.c_int, [c_void_p, c_i64, c_void_p, c_i64, ctypes.c_int, c_i64, ctypes.c_int32,
+                                             ctypes.c_float, c_i64, c_void_p, c_i64, c_void_p, ctypes.c_size_t,
+                                             c_void_p]),
+    "sdm_rt_distill_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(SdmRtDistill)]),
+    "sdm_rt_distill_loss": (ctypes.c_int, [ctypes.POINTER(SdmRtDistill), c_void_p, c_i64, ctypes.c_int, c_void_p, c_i64,
+                                           c_void_p, c_i64, c_void_p, c_void_p, c_void_p, c_void_p, ctypes.c_size_t,
+                                           c_void_p]),
+    "sdm_rt_distill_grad": (ctypes.c_int, [ctypes.POINTER(SdmRtDistill), c_void_p, c_i64, ctypes.c_int, c_void_p, c_i64,
+                                           c_void_p, c_i64, c_void_p, c_void_p, c_void_p, c_void_p, c_i64, c_void_p]),
+    "sdm_rt_process_logits": (ctypes.c_int, [ctypes.POINTER(SdmRtRules), c_void_p, c_i64, ctypes.c_int, c_i64,
+                                             ctypes.c_int32, c_void_p, c_i64, c_void_p]),
+    "sdm_rt_append_tokens": (ctypes.c_int, [c_void_p, c_i64, c_i64, c_void_p, c_void_p, c_i64, c_void_p]),
     "sdm_rt_status": (ctypes.c_int, [ctypes.POINTER(SdmRtDims), c_void_p, c_void_p]),
     "sdm_rt_set_wait_limit": (None, [c_i64]),
     "sdm_rt_set_crowded_threshold": (None, [ctypes.c_int32]),

@@ -4,7 +4,9 @@ Tensors must live on a ROCm device.  Activations are [B, T, width] with unit str
 uniform row stride (a slice of a wider fused projection output is fine).  All work is queued on the current torch
 stream; nothing synchronises.
 """
+import contextlib
 import ctypes
+import math
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -1241,3 +1243,350 @@ class TableSdmFunction(torch.autograd.Function):
         return (g["q"].to(dq) if need[0] else None, g["keys1"].to(dk) if need[1] else None,
                 g["keys2"].to(dk) if need[2] else None, g["log_scale"].to(dl) if need[3] else None,
                 g["values"].to(dv) if need[4] else None, None)
+
+
+# -- the vocabulary's ends: embedding, distillation loss, rules on logits ------------------------------------------
+
+def _on(device):
+    """The device as the current one, for a launch on a tensor of another device than the current one."""
+    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def _same_device(name, device, **tensors):
+    for n, t in tensors.items():
+        if t is not None and t.device != device:
+            raise ValueError(f"{name}: {n} is on {t.device}, expected {device}")
+
+
+def _ids(name, what, t):
+    """Token ids as int64 (int32 is widened)."""
+    if t.dtype not in (torch.int64, torch.int32):
+        raise ValueError(f"{name}: {what} must be int64 or int32, got {t.dtype}")
+    return t.to(torch.int64)
+
+
+def _read_rows(t2):
+    """(rows, row stride in elements) of a 2-D tensor as the kernels that read any row stride and any element alignment
+    take it: itself where the last dimension is contiguous, else a copy."""
+    if t2.shape[1] > 1 and t2.stride(1) != 1:
+        t2 = t2.contiguous()
+    row = t2.stride(0)
+    if t2.shape[0] <= 1:
+        row = t2.shape[1]
+    elif 0 < row < t2.shape[1]:   # overlapping windows
+        t2 = t2.contiguous()
+        row = t2.shape[1]
+    return t2, row
+
+
+def _apart(a, b):
+    """Whether two 2-D tensors of one shape and dtype with contiguous rows share no element, or are the same one."""
+    rows, width = a.shape
+    if rows == 0 or a.untyped_storage().data_ptr() != b.untyped_storage().data_ptr():
+        return True
+    sa, sb = (t.stride(0) if rows > 1 else width for t in (a, b))
+    lo, hi = sorted(((a.data_ptr(), sa), (b.data_ptr(), sb)))
+    if lo == hi or lo[0] + ((rows - 1) * lo[1] + width) * a.element_size() <= hi[0]:
+        return True
+    shift = (hi[0] - lo[0]) // a.element_size() % sa
+    return sa == sb and width <= shift <= sa - width   # column blocks of one buffer
+
+
+def embedding_fits(idx, table):
+    """Whether embedding() takes these tokens and table: int64 or int32 ids and a plain float32 or bfloat16 [vocab, d] table
+    on one GPU, inside the kernels' limits, outside forward-mode differentiation and function transforms."""
+    return (type(table) in (torch.Tensor, torch.nn.Parameter) and type(idx) is torch.Tensor
+            and torch.autograd.forward_ad._current_level < 0 and not torch._C._are_functorch_transforms_active()
+            and idx.is_cuda and table.is_cuda and idx.device == table.device and idx.dtype in (torch.int64, torch.int32)
+            and table.dtype in _DT and table.dim() == 2 and 0 < table.shape[0] <= 1 << 25 and 0 < table.shape[1] <= 1 << 20
+            and idx.numel() <= 1 << 30)
+
+
+def _embed(idx, table, scale):
+    d = table.shape[1]
+    ids = _ids("embedding", "idx", idx).reshape(-1).contiguous()
+    tab, stride = _read_rows(table.detach())
+    out = torch.empty(idx.shape + (d,), dtype=table.dtype, device=table.device)
+    lib = _lib.load()
+    with _on(table.device):
+        _lib.check(lib.sdm_rt_embed(_ptr(ids), ids.numel(), _ptr(tab), stride, _DT[table.dtype], table.shape[0], d,
+                                    float(scale), _ptr(out), d, _stream(table.device)), lib)
+    return out
+
+
+def embedding_backward(idx, dy, vocab, scale=1.0, padding_idx=None):
+    """The gradient [vocab, d] (in dy's dtype) of embedding's table for dy [..., d], the gradient of its output: each
+    row the scaled float32 sum over its tokens in their order (sdm_rt_embed_backward: deterministic), zeros for tokens that
+    do not occur and for padding_idx."""
+    d = dy.shape[-1]
+    if dy.device.type != "cuda":
+        raise RuntimeError("embedding_backward needs ROCm device tensors")
+    if dy.dtype not in _DT:
+        raise ValueError(f"embedding_backward: dtype {dy.dtype} is not float32 or bfloat16")
+    if tuple(dy.shape[:-1]) != tuple(idx.shape):
+        raise ValueError(f"embedding_backward: dy {tuple(dy.shape)} for ids {tuple(idx.shape)}")
+    _same_device("embedding_backward", dy.device, idx=idx)
+    ids = _ids("embedding_backward", "idx", idx).reshape(-1).contiguous()
+    dy2, stride = _read_rows(dy.reshape(-1, d))
+    out = torch.empty(vocab, d, dtype=dy.dtype, device=dy.device)
+    lib = _lib.load()
+    nbytes = lib.sdm_rt_embed_backward_workspace_bytes(ids.numel(), vocab, d)
+    ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=dy.device)
+    with _on(dy.device):
+        _lib.check(lib.sdm_rt_embed_backward(_ptr(ids), ids.numel(), _ptr(dy2), stride, _DT[dy.dtype], vocab, d,
+                                             float(scale), -1 if padding_idx is None else padding_idx, _ptr(out), d, _ptr(ws),
+                                             ws.numel(), _stream(dy.device)), lib)
+    return out
+
+
+class EmbeddingFunction(torch.autograd.Function):
+    """embedding() as an autograd function: the lookup kernel forward, embedding_backward backward, as torch ops where it is
+    to be differentiated again (create_graph).  apply(idx, table, scale, padding_idx) -> y."""
+
+    @staticmethod
+    def forward(ctx, idx, table, scale, padding_idx):
+        ctx.save_for_backward(idx)
+        ctx.vocab, ctx.scale, ctx.pad = table.shape[0], scale, padding_idx
+        return _embed(idx, table, scale)
+
+    @staticmethod
+    def backward(ctx, dy):
+        idx, = ctx.saved_tensors
+        if not torch.is_grad_enabled():
+            return None, embedding_backward(idx, dy, ctx.vocab, ctx.scale, ctx.pad), None, None
+        ids = idx.reshape(-1).long().clamp(0, ctx.vocab - 1)
+        g = dy.reshape(ids.numel(), -1).float()
+        if ctx.pad is not None:
+            g = g * (ids != ctx.pad)[:, None]
+        dt = torch.zeros(ctx.vocab, g.shape[1], dtype=torch.float32, device=g.device).index_add(0, ids, g) * ctx.scale
+        return None, dt.to(dy.dtype), None, None
+
+
+def embedding(idx, table, scale=1.0, padding_idx=None):
+    """The scaled embedding lookup: scale * table[idx] (float32 product, rounded once to table's dtype), differentiable in
+    table.  idx [...] int64 or int32, each in [0, vocab) (one outside is clamped into it, not reported); table [vocab, d]
+    float32 or bfloat16, any row stride.  Row padding_idx is read like any other and gets no gradient (F.embedding's).
+    The gradient is deterministic (embedding_backward)."""
+    if table.device.type != "cuda":
+        raise RuntimeError("embedding needs ROCm device tensors")
+    if table.dtype not in _DT:
+        raise ValueError(f"embedding: dtype {table.dtype} is not float32 or bfloat16")
+    if table.dim() != 2 or 0 in table.shape:
+        raise ValueError(f"embedding: table must be [vocab, d], got {tuple(table.shape)}")
+    if idx.dtype not in (torch.int64, torch.int32):
+        raise ValueError(f"embedding: idx must be int64 or int32, got {idx.dtype}")
+    _same_device("embedding", table.device, idx=idx)
+    if padding_idx is not None:
+        if not -table.shape[0] <= padding_idx < table.shape[0]:
+            raise ValueError(f"embedding: padding_idx {padding_idx} is outside the table of {table.shape[0]} rows")
+        padding_idx %= table.shape[0]
+    if torch.is_grad_enabled() and table.requires_grad:
+        return EmbeddingFunction.apply(idx, table, scale, padding_idx)
+    return _embed(idx, table, scale)
+
+
+_REDUCTION = {"none": _lib.SDM_RT_NONE, "mean": _lib.SDM_RT_MEAN, "sum": _lib.SDM_RT_SUM}
+
+
+class DistillFunction(torch.autograd.Function):
+    """distill_loss on rows as an autograd function (sdm_rt_distill_loss, sdm_rt_distill_grad); it cannot be
+    differentiated again.  apply(logits [rows, vocab], top_ids, top_logits [rows, k], labels [rows] or None, dims) -> loss,
+    dims an _lib.SdmRtDistill."""
+
+    @staticmethod
+    def forward(ctx, logits, ids, top, labels, dims):
+        dev = logits.device
+        z, zs = _read_rows(logits)
+        n = dims.rows
+        loss = torch.empty(n if dims.reduction == _lib.SDM_RT_NONE else (), dtype=torch.float32, device=dev)
+        stats = torch.empty(n, 4, dtype=torch.float32, device=dev) if ctx.needs_input_grad[0] else None
+        lib = _lib.load()
+        nbytes = lib.sdm_rt_distill_workspace_bytes(ctypes.byref(dims))
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        with _on(dev):
+            _lib.check(lib.sdm_rt_distill_loss(ctypes.byref(dims), _ptr(z), zs, _DT[z.dtype], _ptr(ids), dims.top_k,
+                                               _ptr(top), dims.top_k, _ptr(labels), _ptr(loss), _ptr(stats), _ptr(ws), nbytes,
+                                               _stream(dev)), lib)
+        if stats is not None:
+            ctx.dims = dims
+            ctx.save_for_backward(z, ids, top, labels, stats)
+        return loss
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dloss):
+        z, ids, top, labels, stats = ctx.saved_tensors
+        z, zs = _read_rows(z)
+        dims = ctx.dims
+        g = dloss.contiguous()
+        dz = torch.empty(z.shape, dtype=z.dtype, device=z.device)
+        lib = _lib.load()
+        with _on(z.device):
+            _lib.check(lib.sdm_rt_distill_grad(ctypes.byref(dims), _ptr(z), zs, _DT[z.dtype], _ptr(ids), dims.top_k,
+                                               _ptr(top), dims.top_k, _ptr(labels), _ptr(stats), _ptr(g), _ptr(dz), dims.vocab,
+                                               _stream(z.device)), lib)
+        return dz, None, None, None, None
+
+
+def distill_loss(logits, top_ids, top_logits, *, temperature=1.0, labels=None, alpha=1.0, ignore_index=-100,
+                 reduction="mean"):
+    """Distillation of a student's logits from a teacher's top logits, joined by the cross entropy of labels:
+
+        alpha * temperature^2 * KL(q || softmax(logits / temperature)) + (1 - alpha) * CE(logits, labels)
+
+    per position, q = softmax(top_logits / temperature) over the position's teacher entries.  logits [..., vocab] float32
+    or bfloat16; top_ids [..., k] int64 or int32 (an id outside the vocabulary, e.g. -1, is no entry; a repeated id's
+    shares add up) and top_logits [..., k], k at most 1,024; labels [...] int64 or int32 or None (ignore_index, or any id
+    outside the vocabulary: no label).  Positions may lack either part, or both: those have loss 0 and gradient 0 whatever
+    their logits hold.  reduction "mean" divides the sum by the number of positions with a target (0 if there is none),
+    "sum" does not, "none" gives float32 losses [...].  Differentiable in logits, once; the teacher gets no gradient."""
+    if logits.device.type != "cuda":
+        raise RuntimeError("distill_loss needs ROCm device tensors")
+    if logits.dtype not in _DT:
+        raise ValueError(f"distill_loss: dtype {logits.dtype} is not float32 or bfloat16")
+    if logits.dim() < 1 or logits.shape[-1] < 1:
+        raise ValueError(f"distill_loss: logits must be [..., vocab], got {tuple(logits.shape)}")
+    lead, V = tuple(logits.shape[:-1]), logits.shape[-1]
+    if top_ids.dim() < 1 or tuple(top_ids.shape[:-1]) != lead or top_ids.shape != top_logits.shape:
+        raise ValueError(f"distill_loss: top_ids {tuple(top_ids.shape)} and top_logits {tuple(top_logits.shape)} must be "
+                         f"{lead} + [k]")
+    if not top_logits.is_floating_point():
+        raise ValueError(f"distill_loss: top_logits must be floating point, got {top_logits.dtype}")
+    if labels is not None and tuple(labels.shape) != lead:
+        raise ValueError(f"distill_loss: labels {tuple(labels.shape)}, expected {lead}")
+    if reduction not in _REDUCTION:
+        raise ValueError(f"distill_loss: reduction {reduction!r} is not 'none', 'mean' or 'sum'")
+    if labels is None and alpha != 1.0:
+        raise ValueError("distill_loss: alpha below 1 needs labels")
+    _same_device("distill_loss", logits.device, top_ids=top_ids, top_logits=top_logits, labels=labels)
+    k = top_ids.shape[-1]
+    ids = _ids("distill_loss", "top_ids", top_ids).reshape(-1, k).contiguous() if k else None
+    top = top_logits.detach().to(torch.float32).reshape(-1, k).contiguous() if k else None
+    lab = None if labels is None else _ids("distill_loss", "labels", labels).reshape(-1).contiguous()
+    n = math.prod(lead)
+    dims = _lib.SdmRtDistill(n, V, k, float(temperature), float(alpha), int(ignore_index), _REDUCTION[reduction])
+    loss = DistillFunction.apply(logits.reshape(n, V), ids, top, lab, dims)
+    return loss.reshape(lead) if reduction == "none" else loss
+
+
+def _per_row(name, what, v, B, device):
+    """A penalty as (float32 [B] tensor or None, float)."""
+    if not torch.is_tensor(v):
+        v = float(v)
+        if not math.isfinite(v) or (what == "repetition" and v <= 0.0):
+            raise ValueError(f"{name}: {what} {v} must be finite" + (" and positive" if what == "repetition" else ""))
+        return None, v
+    if v.numel() not in (1, B) or v.dim() > 1 or not v.is_floating_point():
+        raise ValueError(f"{name}: {what} must be a number or a floating-point tensor [B={B}], got {v.dtype} {tuple(v.shape)}")
+    _same_device(name, device, **{what: v})
+    return v.detach().to(torch.float32).reshape(-1).expand(B).contiguous(), 0.0
+
+
+def _row_or_rows(name, what, t, B, width, dtype):
+    """A [width] or [B, width] tensor as (tensor, row stride; 0: one row for all)."""
+    if tuple(t.shape) not in ((width,), (B, width)) or t.dtype != dtype:
+        raise ValueError(f"{name}: {what} must be {dtype} [{width}] or [B={B}, {width}], got {t.dtype} {tuple(t.shape)}")
+    t = t.detach()
+    if t.dim() == 1:
+        return t.contiguous(), 0
+    return _read_rows(t)
+
+
+def pack_mask(allowed):
+    """A boolean mask of allowed tokens [..., vocab] as process_logits' words [..., ceil(vocab / 32)] int32: bit v mod 32 of
+    word v // 32 set where token v is allowed."""
+    if allowed.dtype != torch.bool or allowed.dim() < 1:
+        raise ValueError("pack_mask: expected a boolean tensor [..., vocab]")
+    pad = -allowed.shape[-1] % 32
+    bits = torch.nn.functional.pad(allowed, (0, pad)).unflatten(-1, (-1, 32)).long()
+    words = (bits << torch.arange(32, device=allowed.device)).sum(-1)
+    return torch.where(words >= 1 << 31, words - (1 << 32), words).to(torch.int32)
+
+
+def process_logits(logits, tokens=None, lengths=None, *, prompt=None, repetition=1.0, frequency=0.0, presence=0.0,
+                   bias=None, mask=None, out=None):
+    """The rules of a decode step on its logits [B, vocab] (float32 or bfloat16), in float32 and in this order:
+
+        a token of the stream's history                        x = x / repetition if x > 0 else x * repetition
+        one that occurred c > 0 times in it, at or after prompt    x -= c * frequency + presence
+        x += bias;  a token that the mask does not allow           x = -inf, whatever it was
+
+    tokens [B, width] int64, of which the first lengths [B] int64 are a stream's history (where lengths exceeds width: a
+    ring of its last width tokens, append_tokens); ids outside the vocabulary count nowhere.  prompt [B] int64: where the
+    stream's own tokens begin (0).  repetition, frequency, presence: numbers or [B] tensors.  bias [vocab] or [B, vocab]
+    float32.  mask [ceil(vocab / 32)] or [B, ceil(vocab / 32)] int32 words (pack_mask); a row that allows nothing becomes
+    -inf throughout.  Returns the logits in their dtype, in ``out`` if given (it may be logits itself; it must not overlap
+    them otherwise).  Inference only."""
+    name = "process_logits"
+    if logits.device.type != "cuda":
+        raise RuntimeError(f"{name} needs ROCm device tensors")
+    if logits.dtype not in _DT:
+        raise ValueError(f"{name}: dtype {logits.dtype} is not float32 or bfloat16")
+    if logits.dim() != 2 or logits.shape[1] < 1:
+        raise ValueError(f"{name}: logits must be [B, vocab], got {tuple(logits.shape)}")
+    if torch.is_grad_enabled() and logits.requires_grad:
+        raise RuntimeError(f"{name} is inference only: logits require a gradient")
+    B, V = logits.shape
+    dev = logits.device
+    _same_device(name, dev, tokens=tokens, lengths=lengths, prompt=prompt, bias=bias, mask=mask, out=out)
+    held = [_per_row(name, w, v, B, dev) for w, v in (("repetition", repetition), ("frequency", frequency),
+                                                      ("presence", presence))]
+    r = _lib.SdmRtRules()
+    r.repetition, r.frequency, r.presence = (_ptr(t) for t, _ in held)
+    r.repetition_all, r.frequency_all, r.presence_all = (v for _, v in held)
+    if tokens is not None:
+        if tokens.dtype != torch.int64 or tokens.dim() != 2 or tokens.shape[0] != B:
+            raise ValueError(f"{name}: tokens must be int64 [B={B}, width], got {tokens.dtype} {tuple(tokens.shape)}")
+        if lengths is None:
+            raise ValueError(f"{name}: tokens need lengths")
+        for what, t in (("lengths", lengths), ("prompt", prompt)):
+            if t is not None and (t.dtype != torch.int64 or tuple(t.shape) != (B,)):
+                raise ValueError(f"{name}: {what} must be int64 [B={B}], got {t.dtype} {tuple(t.shape)}")
+        if any(t is not None or v != w for (t, v), w in zip(held, (1.0, 0.0, 0.0))):
+            tokens, r.tokens_row_stride = _read_rows(tokens)
+            r.width = tokens.shape[1]
+            lengths = lengths.contiguous()
+            prompt = None if prompt is None else prompt.contiguous()
+            r.tokens, r.lengths, r.prompt = _ptr(tokens), _ptr(lengths), _ptr(prompt)
+    elif lengths is not None or prompt is not None:
+        raise ValueError(f"{name}: lengths and prompt need tokens")
+    if bias is not None:
+        bias, r.bias_row_stride = _row_or_rows(name, "bias", bias, B, V, torch.float32)
+        r.bias = _ptr(bias)
+    if mask is not None:
+        mask, r.mask_row_stride = _row_or_rows(name, "mask", mask, B, (V + 31) // 32, torch.int32)
+        r.mask = _ptr(mask)
+    src, ls = _read_rows(logits.detach())
+    if out is None:
+        out = torch.empty(B, V, dtype=logits.dtype, device=dev)
+    elif tuple(out.shape) != (B, V) or out.dtype != logits.dtype or (V > 1 and out.stride(1) != 1) or (
+            B > 1 and out.stride(0) < V):
+        raise ValueError(f"{name}: out must be {logits.dtype} [B={B}, {V}] with contiguous rows")
+    elif src.data_ptr() == logits.data_ptr() and not _apart(logits, out):
+        raise ValueError(f"{name}: out overlaps logits in part")
+    lib = _lib.load()
+    with _on(dev):
+        _lib.check(lib.sdm_rt_process_logits(ctypes.byref(r), _ptr(src), ls, _DT[logits.dtype], B, V, _ptr(out),
+                                             out.stride(0) if B > 1 else V, _stream(dev)), lib)
+    return out
+
+
+def append_tokens(tokens, lengths, new):
+    """One token more of each stream, in place: tokens[b, lengths[b] % width] = new[b], lengths[b] += 1 (tokens
+    [B, width], lengths and new [B], int64): the history that process_logits reads."""
+    if tokens.device.type != "cuda":
+        raise RuntimeError("append_tokens needs ROCm device tensors")
+    if tokens.dim() != 2 or tokens.shape[1] < 1:
+        raise ValueError(f"append_tokens: tokens must be [B, width], got {tuple(tokens.shape)}")
+    B, width = tokens.shape
+    _same_device("append_tokens", tokens.device, lengths=lengths, new=new)
+    for what, t in (("tokens", tokens), ("lengths", lengths), ("new", new)):
+        if t.dtype != torch.int64 or (what != "tokens" and tuple(t.shape) != (B,)):
+            raise ValueError(f"append_tokens: {what} must be int64" + ("" if what == "tokens" else f" [B={B}]"))
+    if (width > 1 and tokens.stride(1) != 1) or (B > 1 and tokens.stride(0) < width) or not lengths.is_contiguous():
+        raise ValueError("append_tokens: tokens must have contiguous rows, lengths must be contiguous")
+    new = new.contiguous()
+    lib = _lib.load()
+    with _on(tokens.device):
+        _lib.check(lib.sdm_rt_append_tokens(_ptr(tokens), tokens.stride(0) if B > 1 else width, width, _ptr(lengths),
+                                            _ptr(new), B, _stream(tokens.device)), lib)

@@ -1,0 +1,75 @@
+// sdm_vocab.h -- what the operators on token ids and vocabulary rows share (sdm_embed.hip, sdm_distill.hip,
+// sdm_rules.hip): 16-byte pieces of a row at any element alignment, and the sums and maxima of a workgroup.
+#pragma once
+#include "sdm_common.h"
+
+namespace sdmrt {
+
+// 16 bytes of a row: kN values of T.  A row of an odd vocabulary starts at any multiple of its element's size; gfx950
+// loads and stores 16 bytes at any address, so full pieces take the same instruction wherever the row starts, and only
+// a row's last, partial piece goes value by value.
+template <typename T>
+struct Piece {
+  static constexpr int kN = 16 / static_cast<int>(sizeof(T));
+  uint4 r;
+
+  __device__ __forceinline__ void load(const T* p) { __builtin_memcpy(&r, p, 16); }
+  // the first n (< kN) values at p, the rest `fill`
+  __device__ __forceinline__ void load_part(const T* p, int n, T fill) {
+    T v[kN];
+#pragma unroll
+    for (int e = 0; e < kN; ++e) {
+      v[e] = fill;
+      if (e < n) v[e] = p[e];
+    }
+    __builtin_memcpy(&r, v, 16);
+  }
+  __device__ __forceinline__ void store(T* p) const { __builtin_memcpy(p, &r, 16); }
+  __device__ __forceinline__ void store_part(T* p, int n) const {
+    T v[kN];
+    __builtin_memcpy(v, &r, 16);
+#pragma unroll
+    for (int e = 0; e < kN; ++e)
+      if (e < n) p[e] = v[e];
+  }
+  __device__ __forceinline__ float get(int e) const {
+    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+    if constexpr (sizeof(T) == 2)
+      return __uint_as_float(e & 1 ? w[e >> 1] & 0xffff0000u : w[e >> 1] << 16);
+    else
+      return __uint_as_float(w[e]);
+  }
+  // kN floats, each rounded once to T
+  __device__ __forceinline__ void set(const float (&v)[kN]) {
+    if constexpr (sizeof(T) == 2)
+      r = make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
+    else
+      r = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+  }
+};
+
+// rows that are only read may also be one row repeated (stride 0)
+inline bool bad_read_stride(int64_t stride, int64_t width) { return stride != 0 && stride < width; }
+
+// The row of a [vocab] table that a token id stands for: ids outside are clamped into it (the host reads none).
+__device__ __forceinline__ int clamp_token(int64_t id, int vocab) {
+  return static_cast<int>(min(max(id, int64_t{0}), static_cast<int64_t>(vocab) - 1));
+}
+
+__device__ __forceinline__ float wave_max(float v) {
+#pragma unroll
+  for (int j = 32; j > 0; j >>= 1) v = fmaxf(v, __shfl_xor(v, j));
+  return v;
+}
+__device__ __forceinline__ float wave_add(float v) {
+#pragma unroll
+  for (int j = 32; j > 0; j >>= 1) v += __shfl_xor(v, j);
+  return v;
+}
+__device__ __forceinline__ int wave_add(int v) {
+#pragma unroll
+  for (int j = 32; j > 0; j >>= 1) v += __shfl_xor(v, j);
+  return v;
+}
+
+}  // namespace sdmrt

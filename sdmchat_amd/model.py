@@ -98,6 +98,7 @@ class OneSdmLM(nn.Module):
     """Embedding, layers of [x + RunTimeSdm(x); x + FFN(x)], final RMSNorm, tied (or separate) head."""
 
     kind = "onesdm"
+    emb_scale = 1.0
 
     def __init__(self, V, d=256, layers=4, mlp_f=688, mem=True, heads=4, n_sub=32, d_a=32, k=16,
                  decays=(0.0, 0.8, 0.99, 1.0), learn_decay=False, write_gate=True, gate_bias=0.0, read_mode="mean",
@@ -105,7 +106,7 @@ class OneSdmLM(nn.Module):
                  read_eps=1e-3, addr_bias=0.0, archive=False,
                  arc_layers=None, arc_d_c=64, arc_n_sub=16, arc_k=4, arc_slot_keep=4, arc_window=16, arc_n_fetch=4,
                  arc_weighting="soft", tie=True, ffn="mlp", sdm_n_sub=0, sdm_heads=4, sdm_d_a=0, sdm_k=32,
-                 sdm_scale=8.0, sdm_learn_scale=True, reset_at_bos=False, bos_id=0, seed=0):
+                 sdm_scale=8.0, sdm_learn_scale=True, reset_at_bos=False, bos_id=0, seed=0, emb_scale=1.0):
         super().__init__()
         if ffn not in ("mlp", "sdm", "none"):
             raise ValueError("ffn must be 'mlp', 'sdm' or 'none'")
@@ -113,6 +114,7 @@ class OneSdmLM(nn.Module):
             raise NotImplementedError("OneSdmLM: the archive memory is a separate subsystem, not built here")
         self.V, self.d, self.n_layers, self.mlp_f, self.tie = V, d, layers, mlp_f, tie
         self.reset_at_bos, self.bos_id = reset_at_bos, bos_id
+        self.emb_scale = float(emb_scale)   # a factor on the embedded tokens (the tied head reads the table without it)
         self.ffn = ffn
         self.has_mem, self.has_arc = mem, False
         self.emb = nn.Embedding(V, d)
@@ -144,7 +146,14 @@ class OneSdmLM(nn.Module):
             s.reset_init()
 
     def enfold(self, idx):
-        return self.emb(idx)
+        """emb_scale * emb(idx): on core.embedding where emb is a plain nn.Embedding on the GPU (its gradient by sorted tokens,
+        deterministic; a token outside the table is clamped into it), else the module itself."""
+        e = self.emb
+        if (core.plain_module(e, nn.Embedding) and e.max_norm is None and not e.scale_grad_by_freq and not e.sparse
+                and core.embedding_fits(idx, e.weight)):
+            return core.embedding(idx, e.weight, self.emb_scale, e.padding_idx)
+        x = e(idx)
+        return x if self.emb_scale == 1.0 else x * self.emb_scale
 
     def project(self, h):
         if self.tie:
@@ -253,6 +262,14 @@ class OneSdmLM(nn.Module):
     def forward(self, idx, sequential=False):
         return self.project(self.hidden(idx, sequential))
 
+    def distill_loss(self, idx, top_ids, top_logits, labels=None, *, temperature=1.0, alpha=1.0, ignore_index=-100,
+                     reduction="mean"):
+        """The loss of forward(idx) against a teacher's top logits and, with alpha below 1, labels (core.distill_loss):
+        idx [B, T]; top_ids, top_logits [B, T, k]; labels [B, T] or None.  Position t's entries are the teacher's for
+        the token after t, as its label is."""
+        return core.distill_loss(self.forward(idx), top_ids, top_logits, temperature=temperature, labels=labels, alpha=alpha,
+                                 ignore_index=ignore_index, reduction=reduction)
+
     def memory_parameters(self):
         """Names of the memories' parameters (track4_onesdm_models.py:557-558): the mixers' (``mems.``); the
         reference also lists its archive's (``arcs.``), which this model does not build."""
@@ -289,10 +306,11 @@ class OneSdmLM(nn.Module):
                 m.keep_state = k
         return logits, ModelDecodeState(layers, idx.shape[1])
 
-    def step(self, idx_t, state):
+    def step(self, idx_t, state, rules=None):
         """One token for each of B streams: idx_t [B] int64 -> logits [B, V], the last position of
         forward(idx, sequential=True) (track4_onesdm_models.py:534-555), with every mixer's memory carried in
-        ``state`` (a ModelDecodeState, updated in place).  Inference only."""
+        ``state`` (a ModelDecodeState, updated in place).  rules: a TokenRules of B streams; idx_t joins its history and
+        the logits are returned with the rules applied.  Inference only."""
         reset = (idx_t == self.bos_id) if self.reset_at_bos else None
 
         def apply(kind, i, x, hx):
@@ -306,12 +324,72 @@ class OneSdmLM(nn.Module):
             return self.mems[i].step_residual(x, y, state.layers[i], reset)
         stages = self._stages()
         first = None   # a first mixer's step on the embedded tokens, the gather and its norm in the projection map
-        if (stages and stages[0][0] == "mem" and type(self).enfold is OneSdmLM.enfold
+        if (stages and stages[0][0] == "mem" and type(self).enfold is OneSdmLM.enfold and self.emb_scale == 1.0
                 and self.mems[stages[0][1]].embed_fits(idx_t, self.emb.weight)):
             first = self.mems[stages[0][1]].step_embed(idx_t, self.emb.weight, state.layers[stages[0][1]], reset)
         h = self._run(first[0] if first else self.enfold(idx_t), apply, apply_res, y0=first[1] if first else None)
         state.pos += 1
-        return self.project(h)
+        logits = self.project(h)
+        if rules is None:
+            return logits
+        rules.append(idx_t)
+        return rules.apply(logits, out=logits)
+
+
+class TokenRules:
+    """What a decode loop holds against its streams' logits (core.process_logits): penalties for tokens a stream has had,
+    a bias and a mask of the allowed tokens, and the history of B streams, the last ``window`` tokens of each.
+    repetition, frequency and presence are numbers or [B] tensors, bias [V] or [B, V] float32, mask int32 words
+    (core.pack_mask); they are read at every call, so a grammar writes its next mask into ``mask`` (in place where a
+    DecodeGraph replays).
+
+        logits, state = model.prefill(idx)
+        rules.start(idx)                                # the prompt: repetition counts it, frequency and presence do not
+        nxt = rules.apply(logits[:, -1]).argmax(-1)
+        while ...:
+            nxt = model.step(nxt, state, rules).argmax(-1)
+    """
+
+    def __init__(self, batch, window, device, *, repetition=1.0, frequency=0.0, presence=0.0, bias=None, mask=None):
+        if batch < 1 or window < 1:
+            raise ValueError("TokenRules: batch and window must be at least 1")
+        self.repetition, self.frequency, self.presence, self.bias, self.mask = repetition, frequency, presence, bias, mask
+        self.tokens = torch.zeros(batch, window, dtype=torch.long, device=device)
+        self.lengths = torch.zeros(batch, dtype=torch.long, device=device)
+        self.prompt = torch.zeros(batch, dtype=torch.long, device=device)
+
+    def start(self, idx, lengths=None):
+        """The streams begin anew after the prompts idx [B, T], of which the first lengths [B] (T) count."""
+        B, window = self.tokens.shape
+        if idx.dim() != 2 or idx.shape[0] != B:
+            raise ValueError(f"TokenRules.start: idx must be [B={B}, T], got {tuple(idx.shape)}")
+        T = idx.shape[1]
+        n = torch.full_like(self.lengths, T) if lengths is None else lengths.to(self.lengths).clamp(0, T)
+        if tuple(n.shape) != (B,):
+            raise ValueError(f"TokenRules.start: lengths must be [B={B}], got {tuple(n.shape)}")
+        # ring entry i holds the latest position p < n with p mod window = i
+        i = torch.arange(window, device=n.device)
+        p = n[:, None] - 1 - (n[:, None] - 1 - i) % window
+        kept = p >= 0
+        if T > 0:
+            self.tokens.copy_(torch.where(kept, idx.to(self.tokens).gather(1, p.clamp(0, T - 1)), 0))
+        self.lengths.copy_(n)
+        self.prompt.copy_(n)
+
+    def append(self, idx_t):
+        """One token more of each stream: idx_t [B]."""
+        core.append_tokens(self.tokens, self.lengths, idx_t.to(torch.long))
+
+    def apply(self, logits, out=None):
+        """The logits [B, V] with the rules applied, in ``out`` if given (core.process_logits)."""
+        return core.process_logits(logits, self.tokens, self.lengths, prompt=self.prompt, repetition=self.repetition,
+                                   frequency=self.frequency, presence=self.presence, bias=self.bias, mask=self.mask, out=out)
+
+    def scratch(self):
+        """The same rules on a history of their own."""
+        B, window = self.tokens.shape
+        return TokenRules(B, window, self.tokens.device, repetition=self.repetition, frequency=self.frequency,
+                          presence=self.presence, bias=self.bias, mask=self.mask)
 
 
 class DecodeGraph:
@@ -319,21 +397,23 @@ class DecodeGraph:
     the graph's input, replays it and returns the graph's logits tensor (overwritten by the next step).  ``steps``
     consecutive steps can be captured in one graph (``run(tokens [steps, B])``).  The state is the caller's
     ModelDecodeState, updated in place; capture first runs two steps on a scratch state of the same shapes, so that
-    every workspace and parameter cache exists before capture and nothing allocates inside the graph."""
+    every workspace and parameter cache exists before capture and nothing allocates inside the graph.  rules: a
+    TokenRules of the B streams that every step's logits pass (the graph reads its tensors where they are)."""
 
-    def __init__(self, model, state, steps=1):
+    def __init__(self, model, state, steps=1, rules=None):
         dev = model.emb.weight.device
         B = next(st.mem.shape[0] for st in state.layers if st is not None)
         self.model, self.state, self.steps = model, state, steps
         self.tokens = torch.zeros(steps, B, dtype=torch.long, device=dev)
         with torch.no_grad():
             scratch = model.decode_state(B, dev)
+            kw, spare = ({}, {}) if rules is None else ({"rules": rules}, {"rules": rules.scratch()})
             for _ in range(2):
-                model.step(self.tokens[0], scratch)
+                model.step(self.tokens[0], scratch, **spare)
             torch.cuda.synchronize(dev)
             self.graph = torch.cuda.CUDAGraph()
             with torch.cuda.graph(self.graph):
-                outs = [model.step(self.tokens[t], state) for t in range(steps)]
+                outs = [model.step(self.tokens[t], state, **kw) for t in range(steps)]
                 self.logits = torch.stack(outs) if steps > 1 else outs[0]
         state.pos -= steps   # capture ran no step
 
