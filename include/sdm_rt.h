@@ -448,8 +448,8 @@ int sdm_rt_table_backward(const sdm_rt_dims* dims, const sdm_rt_params* params,
 
 /* The scaled embedding lookup (OneSdmLM's emb, track4_onesdm_models.py:534-535, with a factor): out[i] =
  * round(scale * table[ids[i]]), n tokens.  ids int64, each in [0, vocab) (one outside is clamped into it: the host reads
- * none).  table [vocab][d], out [n][d] in dtype, row strides in elements, any alignment of an element.  At most 2^30
- * tokens, a vocabulary of 2^25 and rows of 2^20 values. */
+ * none).  table [vocab][d], out [n][d] in dtype, row strides in elements, any alignment of an element.  At most 2^27
+ * tokens, a vocabulary of 2^21 and rows of 2^20 values. */
 int sdm_rt_embed(const int64_t* ids, int64_t n, const void* table, int64_t table_row_stride, sdm_rt_dtype dtype,
                  int64_t vocab, int32_t d, float scale, void* out, int64_t out_row_stride, void* stream);
 

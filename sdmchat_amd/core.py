@@ -1298,8 +1298,8 @@ def embedding_fits(idx, table):
     return (type(table) in (torch.Tensor, torch.nn.Parameter) and type(idx) is torch.Tensor
             and torch.autograd.forward_ad._current_level < 0 and not torch._C._are_functorch_transforms_active()
             and idx.is_cuda and table.is_cuda and idx.device == table.device and idx.dtype in (torch.int64, torch.int32)
-            and table.dtype in _DT and table.dim() == 2 and 0 < table.shape[0] <= 1 << 25 and 0 < table.shape[1] <= 1 << 20
-            and idx.numel() <= 1 << 30)
+            and table.dtype in _DT and table.dim() == 2 and 0 < table.shape[0] <= 1 << 21 and 0 < table.shape[1] <= 1 << 20
+            and idx.numel() <= 1 << 27)
 
 
 def _embed(idx, table, scale):

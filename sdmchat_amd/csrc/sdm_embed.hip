@@ -15,23 +15,23 @@ __global__ void __launch_bounds__(256) embed_kernel(const int64_t* __restrict__ 
   for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * rows; r0 < n; r0 += static_cast<int64_t>(gridDim.x) * rows) {
     const int live = static_cast<int>(min(static_cast<int64_t>(rows), n - r0));
     for (int i = threadIdx.x; i < live * ppr; i += 256) {
-      const int r = i / ppr, c = (i - r * ppr) * kN;
+      // a row's last piece ends with the row: it may hold values of the piece before it once more
+      const int r = i / ppr, c = max(0, min((i - r * ppr) * kN, d - kN));
       const T* src = table + clamp_token(ids[r0 + r], vocab) * t_stride + c;
       T* dst = out + (r0 + r) * o_stride + c;
       Piece<T> p;
-      const bool full = c + kN <= d;
-      if (full)
+      if (d >= kN)
         p.load(src);
       else
-        p.load_part(src, d - c, T{});
+        p.load_part(src, d, T{});
       float v[kN];
 #pragma unroll
       for (int e = 0; e < kN; ++e) v[e] = p.get(e) * scale;
       p.set(v);
-      if (full)
+      if (d >= kN)
         p.store(dst);
       else
-        p.store_part(dst, d - c);
+        p.store_part(dst, d);
     }
   }
 }
@@ -40,62 +40,117 @@ __global__ void __launch_bounds__(256) embed_kernel(const int64_t* __restrict__ 
 // The gradient, d_table[v] = round(scale * sum over the tokens n of v of dy[n]), in the order of n: the tokens are put in
 // the order of their rows, then every row sums its own.
 //
-// embed_order_kernel: the stable order of the tokens by row, in one launch and without a float or a global atomic.  Row v
-// belongs to workgroup v mod G and is its row v / G: frequent tokens have low ids, so they are dealt out to all
-// workgroups.  Every workgroup reads all the ids twice (they stay in L2).  First it counts its own rows' tokens, each
-// wave its own stretch of the ids, and the tokens of the workgroups before it; that fixes where each of its (row, wave)
-// begins.  Then it reads them again and places its own, each wave in order: the lanes of one row find their ranks
-// among each other by ballot.
-// Slot b * R + i holds row i * G + b: offsets[slot] is where its tokens begin in order[], up to offsets[slot + 1].
-constexpr int kOrderWaves = 16;
-constexpr int kOrderMaxRows = 2048;   // rows of a workgroup: 16 counters of 4 bytes for each, 128 KiB of LDS
+// The stable order of the tokens by row, in two launches and without a global atomic.  Row v belongs to bucket v mod 256
+// and is its row v / 256: frequent tokens have low ids, so they are dealt out to all buckets.  embed_tiles_kernel orders
+// every tile of 1,024 tokens by bucket (lanes of one bucket find each other by ballots over its 8 bits, waves and buckets
+// by a prefix sum) and keeps where the buckets begin.  embed_order_kernel, a workgroup per bucket, reads its run of every
+// tile, each wave its own tiles: it counts its rows, and with the counts of the buckets before it (the sum over the tiles of
+// where it begins there) places its tokens in the rows' order.  Every token is read twice; one launch whose workgroups each
+// read all tokens was bound by its instructions (131,072 tokens: 106 us).
+// Slot b * R + i holds row 256 i + b: offsets[slot] is where its tokens begin in order[], up to offsets[slot + 1].
+constexpr int kTile = 1024, kBucketBits = 8, kBuckets = 1 << kBucketBits;
+constexpr int kOrderMaxRows = 8192;
 
-__global__ void __launch_bounds__(64 * kOrderWaves) embed_order_kernel(const int64_t* __restrict__ ids, int n, int vocab,
-                                                                       int pad, int lg, int R,
-                                                                       int32_t* __restrict__ offsets,
-                                                                       int32_t* __restrict__ order,
-                                                                       int32_t* __restrict__ row_of) {
-  extern __shared__ int32_t cnt[];   // [kOrderWaves][R]: tokens of a row in a wave's stretch, then where they go
-  __shared__ int32_t red[kOrderWaves];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int b = blockIdx.x, mask = (1 << lg) - 1;
-  for (int i = threadIdx.x; i < kOrderWaves * R; i += 64 * kOrderWaves) cnt[i] = 0;
+// the lanes of `live` whose `bits` low bits of v equal this lane's
+__device__ __forceinline__ uint64_t same_lanes(uint64_t live, int v, int bits) {
+  uint64_t m = live;
+  for (int k = 0; k < bits; ++k) {
+    const bool one = (v >> k) & 1;
+    const uint64_t ones = __ballot(one);
+    m &= one ? ones : ~ones;
+  }
+  return m;
+}
+__device__ __forceinline__ uint64_t lanes_below(int lane) { return (uint64_t{1} << lane) - 1; }
+
+// bucket_at[b][t] (b <= 256): where bucket b begins in tile t; packed[1024 t + ...]: its tokens' rows i and places in the
+// tile, i << 10 | place
+__global__ void __launch_bounds__(kTile) embed_tiles_kernel(const int64_t* __restrict__ ids, int n, int vocab, int pad,
+                                                            int tiles, int32_t* __restrict__ bucket_at,
+                                                            uint32_t* __restrict__ packed) {
+  __shared__ int32_t hist[kTile / 64][kBuckets];
+  __shared__ int32_t red[kBuckets / 64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, t = blockIdx.x;
+  const int i = t * kTile + static_cast<int>(threadIdx.x);
+  const int v = i < n ? clamp_token(ids[i], vocab) : pad;
+  for (int k = threadIdx.x; k < kTile / 64 * kBuckets; k += kTile) hist[k / kBuckets][k % kBuckets] = 0;
   __syncthreads();
-  const int seg = (n + 64 * kOrderWaves - 1) / (64 * kOrderWaves) * 64;
-  const int begin = min(n, wave * seg), end = min(n, begin + seg);
-  int32_t* mine = cnt + wave * R;
-  constexpr int kU = 8;
-  int below = 0;
-  for (int i0 = begin; i0 < end; i0 += 64 * kU) {
-    int v[kU];
+  const int b = v & (kBuckets - 1);
+  const bool live = i < n && v != pad;
+  const uint64_t group = same_lanes(__ballot(live), b, kBucketBits);
+  const int rank = __popcll(group & lanes_below(lane));
+  if (live && rank == 0) hist[wave][b] = __popcll(group);
+  __syncthreads();
+  int count = 0, inc = 0;
+  if (threadIdx.x < kBuckets) {
+    int32_t c[kTile / 64];
 #pragma unroll
-    for (int u = 0; u < kU; ++u) {
-      const int i = i0 + 64 * u + lane;
-      v[u] = i < end ? clamp_token(ids[i], vocab) : pad;
+    for (int w = 0; w < kTile / 64; ++w) c[w] = hist[w][threadIdx.x];
+#pragma unroll
+    for (int w = 0; w < kTile / 64; ++w) {
+      hist[w][threadIdx.x] = count;
+      count += c[w];
     }
+    inc = count;
 #pragma unroll
-    for (int u = 0; u < kU; ++u) {
-      const bool live = v[u] != pad && i0 + 64 * u + lane < end;
-      if (live && (v[u] & mask) < b) ++below;
-      if (live && (v[u] & mask) == b) atomicAdd(&mine[v[u] >> lg], 1);
+    for (int j = 1; j < 64; j <<= 1) {
+      const int u = __shfl_up(inc, j);
+      if (lane >= j) inc += u;
+    }
+    if (lane == 63) red[wave] = inc;
+  }
+  __syncthreads();
+  if (threadIdx.x < kBuckets) {
+    int start = inc - count;
+    for (int w = 0; w < wave; ++w) start += red[w];
+    for (int w = 0; w < kTile / 64; ++w) hist[w][threadIdx.x] += start;
+    bucket_at[static_cast<int64_t>(threadIdx.x) * tiles + t] = start;
+    if (threadIdx.x == kBuckets - 1) bucket_at[static_cast<int64_t>(kBuckets) * tiles + t] = start + count;
+  }
+  __syncthreads();
+  if (live) packed[static_cast<int64_t>(t) * kTile + hist[wave][b] + rank] =
+      static_cast<uint32_t>(v >> kBucketBits) << 10 | threadIdx.x;
+}
+
+__global__ void __launch_bounds__(1024) embed_order_kernel(const int32_t* __restrict__ bucket_at,
+                                                           const uint32_t* __restrict__ packed, int tiles, int R,
+                                                           int row_bits, int32_t* __restrict__ offsets,
+                                                           int32_t* __restrict__ order, int32_t* __restrict__ row_of) {
+  extern __shared__ int32_t cnt[];   // [waves][R]: tokens of a row in a wave's tiles, then where they go
+  __shared__ int32_t red[16];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+  const int b = blockIdx.x;
+  const int32_t* at = bucket_at + static_cast<int64_t>(b) * tiles;
+  int below = 0;
+  for (int t = threadIdx.x; t < tiles; t += blockDim.x) below += at[t];
+  for (int i = threadIdx.x; i < waves * R; i += blockDim.x) cnt[i] = 0;
+  __syncthreads();
+  const int per = (tiles + waves - 1) / waves;
+  const int t0 = min(tiles, wave * per), t1 = min(tiles, t0 + per);
+  int32_t* mine = cnt + wave * R;
+  // 64 tiles at a time: lane l holds the run of tile tb + l
+  for (int tb = t0; tb < t1; tb += 64) {
+    const int tl = min(tb + lane, t1 - 1);
+    const int from = at[tl], to = at[tiles + tl];
+    for (int q = 0; q < min(64, t1 - tb); ++q) {
+      const int end = __shfl(to, q);
+      for (int j = __shfl(from, q) + lane; j < end; j += 64)
+        atomicAdd(&mine[packed[static_cast<int64_t>(tb + q) * kTile + j] >> 10], 1);
     }
   }
   below = wave_add(below);
   if (lane == 0) red[wave] = below;
   __syncthreads();
   int base = 0;
-#pragma unroll
-  for (int w = 0; w < kOrderWaves; ++w) base += red[w];
+  for (int w = 0; w < waves; ++w) base += red[w];
   __syncthreads();
-  // where each row begins: thread t takes rows 2t and 2t + 1
-  int tot[2] = {0, 0};
-#pragma unroll
-  for (int q = 0; q < 2; ++q) {
-    const int r = 2 * static_cast<int>(threadIdx.x) + q;
-    if (r < R)
-      for (int w = 0; w < kOrderWaves; ++w) tot[q] += cnt[w * R + r];
-  }
-  int inc = tot[0] + tot[1];
+  // where each row begins: a thread takes a run of rows
+  const int rpt = (R + blockDim.x - 1) / blockDim.x;
+  const int r0 = min(R, static_cast<int>(threadIdx.x) * rpt), r1 = min(R, r0 + rpt);
+  int tot = 0;
+  for (int r = r0; r < r1; ++r)
+    for (int w = 0; w < waves; ++w) tot += cnt[w * R + r];
+  int inc = tot;
 #pragma unroll
   for (int j = 1; j < 64; j <<= 1) {
     const int u = __shfl_up(inc, j);
@@ -103,104 +158,380 @@ __global__ void __launch_bounds__(64 * kOrderWaves) embed_order_kernel(const int
   }
   if (lane == 63) red[wave] = inc;
   __syncthreads();
-  int at = base + inc - tot[0] - tot[1];
-  for (int w = 0; w < wave; ++w) at += red[w];
-#pragma unroll
-  for (int q = 0; q < 2; ++q) {
-    const int r = 2 * static_cast<int>(threadIdx.x) + q;
-    if (r >= R) continue;
-    offsets[b * R + r] = at;
-    for (int w = 0; w < kOrderWaves; ++w) {
+  int pos = base + inc - tot;
+  for (int w = 0; w < wave; ++w) pos += red[w];
+  for (int r = r0; r < r1; ++r) {
+    offsets[b * R + r] = pos;
+    for (int w = 0; w < waves; ++w) {
       const int c = cnt[w * R + r];
-      cnt[w * R + r] = at;
-      at += c;
+      cnt[w * R + r] = pos;
+      pos += c;
     }
   }
-  if (b == mask && threadIdx.x == 64 * kOrderWaves - 1) offsets[(b + 1) * R] = at;   // rows past R count nothing
+  if (b == kBuckets - 1 && threadIdx.x == blockDim.x - 1) offsets[kBuckets * R] = pos;   // rows past R count nothing
   __syncthreads();
-  for (int i0 = begin; i0 < end; i0 += 64 * kU) {
-    int v[kU];
-#pragma unroll
-    for (int u = 0; u < kU; ++u) {
-      const int i = i0 + 64 * u + lane;
-      v[u] = i < end ? clamp_token(ids[i], vocab) : pad;
-    }
-#pragma unroll
-    for (int u = 0; u < kU; ++u) {
-      const int i = i0 + 64 * u + lane;
-      uint64_t todo = __ballot(i < end && v[u] != pad && (v[u] & mask) == b);
-      while (todo) {   // one row of this workgroup at a time
-        const int row = __shfl(v[u], __ffsll(static_cast<unsigned long long>(todo)) - 1);
-        const bool same = ((todo >> lane) & 1) && v[u] == row;
-        const uint64_t group = __ballot(same);
-        const int start = mine[row >> lg];
-        if (same) {
-          const int pos = start + __popcll(group & ((1ull << lane) - 1));
-          order[pos] = i;
-          row_of[pos] = row;
+  for (int tb = t0; tb < t1; tb += 64) {
+    const int tl = min(tb + lane, t1 - 1);
+    const int from = at[tl], to = at[tiles + tl];
+    for (int q = 0; q < min(64, t1 - tb); ++q) {
+      const int begin = __shfl(from, q), end = __shfl(to, q);
+      for (int j0 = begin; j0 < end; j0 += 64) {
+        const bool live = j0 + lane < end;
+        const uint32_t e = live ? packed[static_cast<int64_t>(tb + q) * kTile + j0 + lane] : 0;
+        const int row = static_cast<int>(e >> 10);
+        const uint64_t group = same_lanes(__ballot(live), row, row_bits);
+        const int rank = __popcll(group & lanes_below(lane));
+        const int start = mine[row];
+        if (live) {
+          order[start + rank] = (tb + q) * kTile + static_cast<int>(e & 1023);
+          row_of[start + rank] = row << kBucketBits | b;
+          if (rank == 0) mine[row] = start + __popcll(group);
         }
-        if (lane == 0) mine[row >> lg] = start + __popcll(group);
-        todo &= ~group;
       }
     }
   }
 }
 
-// d_table: a wave per slot sums its tokens' rows in order
+// The rows' sums.  The ordered tokens are cut into pieces of `len`; a group of LANES lanes sums a piece's runs of equal rows
+// in order, lane l columns 4l ... 4l + 3 of every 4 LANES.  A run that is its whole row is scaled and stored; one that
+// crosses an edge of a workgroup's pieces leaves a float32 partial row: part[2 b] continues a row begun before workgroup b,
+// part[2 b + 1] begins one that goes on after it.  The work follows the tokens and not the rows: text repeats its tokens, and with a wave
+// per row the most frequent token's chain of loads was the kernel's time (16,384 tokens of 32,768 rows of 768, a Zipf
+// stream: 739 us).  The last workgroups clear the rows that have no token meanwhile.
 template <typename T>
-__global__ void __launch_bounds__(256) embed_rows_grad_kernel(const int32_t* __restrict__ offsets,
-                                                              const int32_t* __restrict__ order, const T* __restrict__ dy,
-                                                              int64_t dy_stride, int vocab, int d, float scale, int lg, int R,
-                                                              T* __restrict__ d_table, int64_t dt_stride) {
-  const int lane = threadIdx.x & 63;
-  const int slot = blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (slot >= (R << lg)) return;
-  const int row = ((slot % R) << lg) + slot / R;
-  if (row >= vocab) return;
-  const int begin = offsets[slot], end = offsets[slot + 1];
-  constexpr int kN = Piece<T>::kN;
-  for (int c = lane * kN; c < d; c += 64 * kN) {
-    float acc[kN] = {};
-    const bool full = c + kN <= d;
-    Piece<T> p;
-    for (int i = begin; i < end; ++i) {
-      const T* src = dy + order[i] * dy_stride + c;
-      if (full)
-        p.load(src);
-      else
-        p.load_part(src, d - c, T{});
+struct Quad4 {   // four values of a row at any element alignment
+  using Raw = typename std::conditional<sizeof(T) == 2, uint2, uint4>::type;
+  Raw r;
+  __device__ __forceinline__ void load(const T* p) { __builtin_memcpy(&r, p, sizeof(r)); }
+  __device__ __forceinline__ void load_part(const T* p, int n) {
+    T v[4];
 #pragma unroll
-      for (int e = 0; e < kN; ++e) acc[e] += p.get(e);
+    for (int e = 0; e < 4; ++e) {
+      v[e] = T{};
+      if (e < n) v[e] = p[e];
     }
-#pragma unroll
-    for (int e = 0; e < kN; ++e) acc[e] *= scale;
-    p.set(acc);
-    T* dst = d_table + static_cast<int64_t>(row) * dt_stride + c;
-    if (full)
-      p.store(dst);
+    __builtin_memcpy(&r, v, sizeof(r));
+  }
+  __device__ __forceinline__ float get(int e) const {
+    uint32_t w[sizeof(T)];
+    __builtin_memcpy(w, &r, sizeof(r));
+    if constexpr (sizeof(T) == 2)
+      return __uint_as_float(e & 1 ? w[e >> 1] & 0xffff0000u : w[e >> 1] << 16);
     else
-      p.store_part(dst, d - c);
+      return __uint_as_float(w[e]);
+  }
+  __device__ __forceinline__ void store(T* p, const float (&v)[4], int n) {
+    if constexpr (sizeof(T) == 2)
+      r = make_uint2(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]));
+    else
+      r = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+    if (n >= 4) {
+      __builtin_memcpy(p, &r, sizeof(r));
+      return;
+    }
+    T t[4];
+    __builtin_memcpy(t, &r, sizeof(r));
+#pragma unroll
+    for (int e = 0; e < 3; ++e)
+      if (e < n) p[e] = t[e];
+  }
+};
+
+// The four columns of a lane that would begin at column c: the row's last four where they would pass its end, so every load
+// and store is whole and none is behind a branch (two lanes then hold some columns, with the same sums).  Rows of less
+// than four values begin at 0.
+__device__ __forceinline__ int quad_column(int c, int d) { return max(0, min(c, d - 4)); }
+
+struct RowsGrad {
+  const int32_t* offsets;
+  const int32_t* order;
+  const int32_t* row_of;
+  float* part;        // [2 piece_blocks][pitch]
+  int pitch;          // d rounded up to 4
+  int n_slots;        // 256 R
+  int R, vocab, d;
+  int len;            // a piece's tokens
+  int piece_blocks;   // the most workgroups of pieces there can be
+  float scale;
+  const void* dy;
+  int64_t dy_stride;
+  void* d_table;
+  int64_t dt_stride;
+};
+
+constexpr int kZeroRows = 8;   // slots of a wave that clears rows
+
+template <typename T>
+__device__ __forceinline__ void clear_rows(const RowsGrad& a, int first) {
+  const int lane = threadIdx.x & 63;
+  const int mine = first + min(lane, kZeroRows);
+  const int off = mine <= a.n_slots ? a.offsets[mine] : -1;
+  for (int q = 0; q < kZeroRows; ++q) {
+    const int slot = first + q;
+    if (slot >= a.n_slots || __shfl(off, q) != __shfl(off, q + 1)) continue;
+    const int row = (slot % a.R) * kBuckets + slot / a.R;
+    if (row >= a.vocab) continue;
+    T* dst = static_cast<T*>(a.d_table) + static_cast<int64_t>(row) * a.dt_stride;
+    Piece<T> z;
+    z.r = make_uint4(0, 0, 0, 0);
+    constexpr int kN = Piece<T>::kN;
+    for (int c = lane * kN; c < a.d; c += 64 * kN) {
+      if (c + kN <= a.d)
+        z.store(dst + c);
+      else
+        z.store_part(dst + c, a.d - c);
+    }
   }
 }
 
-// the split of a vocabulary's rows over workgroups: 2^lg of them, R rows each
+// A workgroup of 256 threads takes 256 / LANES pieces side by side.  A group's cut runs go to LDS, head (a run begun before
+// its piece) and tail (one that goes on after it); a run cut inside the workgroup is then put together there by the group
+// it begins in, and only one that enters or leaves the workgroup becomes a partial row in memory: with a partial row for
+// every cut piece they were a sixth of the kernel's traffic and their join took as long again as the sums of 16,384
+// tokens (9.6 us).
+template <typename T, int LANES>
+__global__ void __launch_bounds__(256) embed_rows_grad_kernel(RowsGrad a) {
+  constexpr int CS = 4, QS = 8;   // column steps held in registers; rows in flight
+  constexpr int kGroups = 256 / LANES, kCols = 4 * LANES * CS;
+  __shared__ float heads[kGroups][kCols];
+  __shared__ float tails[kGroups][kCols];
+  __shared__ int through[kGroups];   // the group's head run goes on after its piece
+  if (static_cast<int>(blockIdx.x) >= a.piece_blocks) {
+    clear_rows<T>(a, ((blockIdx.x - a.piece_blocks) * 4 + (threadIdx.x >> 6)) * kZeroRows);
+    return;
+  }
+  const int lane = threadIdx.x % LANES, mine = threadIdx.x / LANES;
+  const int total = a.offsets[a.n_slots];
+  const int64_t block_begin = static_cast<int64_t>(blockIdx.x) * kGroups * a.len;
+  if (block_begin >= total) return;   // whole workgroups
+  const int begin = static_cast<int>(min(block_begin + mine * a.len, static_cast<int64_t>(total)));
+  const int n = min(a.len, total - begin);   // none for groups past the end
+  const int at0 = min(begin, total - 1);
+  const int before = begin > 0 ? a.row_of[begin - 1] : -1;
+  const int after = begin + n < total ? a.row_of[begin + n] : -1;
+  const int row0 = a.row_of[at0], row_last = a.row_of[min(begin + max(n, 1), total) - 1];
+  const bool head = n > 0 && row0 == before;               // its first run began before it
+  const bool whole = head && row0 == row_last && row0 == after;   // and goes on after it
+  const bool tail = n > 0 && row_last == after && !whole && !(head && row0 == row_last);   // its last begins here, goes on
+  if (lane == 0) through[mine] = whole;
+  const bool narrow = a.d < 4;
+  const int group = static_cast<int>(threadIdx.x & 63) & ~(LANES - 1);
+  float* part = a.part + 2 * static_cast<int64_t>(blockIdx.x) * a.pitch;
+  for (int cb = 0; cb < a.d; cb += kCols) {
+    float acc[CS][4] = {};
+    int cur = row0;
+    bool first = true;   // the run of cur is the piece's first
+    auto store_row = [&](int row, const float (&x)[CS][4]) {
+#pragma unroll
+      for (int t = 0; t < CS; ++t) {
+        const int col = cb + 4 * LANES * t + 4 * lane, c = quad_column(col, a.d);
+        if (col >= a.d) continue;
+        float v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = x[t][e] * a.scale;
+        Quad4<T> o;
+        o.store(static_cast<T*>(a.d_table) + static_cast<int64_t>(row) * a.dt_stride + c, v, a.d - c);
+      }
+    };
+    auto keep = [&](float* lds) {
+#pragma unroll
+      for (int t = 0; t < CS; ++t)
+        *reinterpret_cast<float4*>(lds + 4 * LANES * t + 4 * lane) = make_float4(acc[t][0], acc[t][1], acc[t][2], acc[t][3]);
+    };
+    auto flush = [&](bool last) {
+      if (first && head)
+        keep(heads[mine]);
+      else if (last && tail)
+        keep(tails[mine]);
+      else
+        store_row(cur, acc);
+#pragma unroll
+      for (int t = 0; t < CS; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[t][e] = 0.f;
+    };
+    if (n > 0) {
+      // lane q of a group's first QS holds token q of the batch; the next batch's are loaded ahead
+      int tok = a.order[begin + min(lane % QS, n - 1)], row = a.row_of[begin + min(lane % QS, n - 1)];
+      for (int i0 = 0; i0 < n; i0 += QS) {
+        Quad4<T> g[QS][CS];
+#pragma unroll
+        for (int q = 0; q < QS; ++q) {
+          const T* src = static_cast<const T*>(a.dy) + __shfl(tok, group + q) * a.dy_stride;
+#pragma unroll
+          for (int t = 0; t < CS; ++t) {
+            if (t > 0 && cb + 4 * LANES * t >= a.d) continue;   // the same for every lane
+            const int c = quad_column(cb + 4 * LANES * t + 4 * lane, a.d);
+            if (narrow)
+              g[q][t].load_part(src, a.d);
+            else
+              g[q][t].load(src + c);
+          }
+        }
+        const int rows = row;
+        const int nx = begin + min(i0 + QS + lane % QS, n - 1);
+        tok = a.order[nx];
+        row = a.row_of[nx];
+#pragma unroll
+        for (int q = 0; q < QS; ++q) {
+          const int r = __shfl(rows, group + q);
+          if (i0 + q < n) {   // past the piece's end nothing is added
+            if (r != cur) {
+              flush(false);
+              cur = r;
+              first = false;
+            }
+#pragma unroll
+            for (int t = 0; t < CS; ++t) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) acc[t][e] += g[q][t].get(e);
+            }
+          }
+        }
+      }
+      flush(true);
+    }
+    __syncthreads();
+    // the runs cut by the groups' edges: group 0 takes the one that enters the workgroup, every group the one it begins
+    const bool enters = mine == 0 && head;
+    if (enters || tail) {
+#pragma unroll 1
+      for (int which = enters ? 0 : 1; which < (tail ? 2 : 1); ++which) {
+        float x[CS][4];
+        const float* own = which ? tails[mine] : heads[0];
+#pragma unroll
+        for (int t = 0; t < CS; ++t) {
+          const float4 v = *reinterpret_cast<const float4*>(own + 4 * LANES * t + 4 * lane);
+          x[t][0] = v.x;
+          x[t][1] = v.y;
+          x[t][2] = v.z;
+          x[t][3] = v.w;
+        }
+        bool on = which ? true : through[0] != 0;   // the run goes on in group g
+        int g = which ? mine + 1 : 1;
+        for (; on && g < kGroups; ++g) {
+#pragma unroll
+          for (int t = 0; t < CS; ++t) {
+            const float4 v = *reinterpret_cast<const float4*>(heads[g] + 4 * LANES * t + 4 * lane);
+            x[t][0] += v.x;
+            x[t][1] += v.y;
+            x[t][2] += v.z;
+            x[t][3] += v.w;
+          }
+          on = through[g] != 0;
+        }
+        if (which && !on) {
+          store_row(row_last, x);   // begun and ended in this workgroup
+        } else {
+          float* dst = part + (which ? a.pitch : 0);
+#pragma unroll
+          for (int t = 0; t < CS; ++t) {
+            const int col = cb + 4 * LANES * t + 4 * lane;
+            if (col < a.d) __builtin_memcpy(dst + quad_column(col, a.d), x[t], 16);
+          }
+        }
+      }
+    }
+    __syncthreads();
+  }
+}
+
+// The rows cut over several workgroups: one workgroup per edge between them adds the row that begins before this edge and is
+// cut first by it, its four quarters of 256 threads a quarter of the partial rows each, in order.
+template <typename T>
+__global__ void __launch_bounds__(1024) embed_rows_join_kernel(RowsGrad a, int len) {
+  __shared__ float4 red[3][256];
+  const int s = blockIdx.x;
+  const int total = a.offsets[a.n_slots];
+  const int64_t edge = static_cast<int64_t>(s + 1) * len;
+  if (edge >= total) return;   // whole workgroups
+  const int row = a.row_of[edge];
+  if (a.row_of[edge - 1] != row) return;
+  if (s > 0 && a.row_of[edge - len - 1] == row) return;   // an earlier edge's
+  const int slot = (row & (kBuckets - 1)) * a.R + (row >> kBucketBits);
+  const int last = (a.offsets[slot + 1] - 1) / len;   // pieces s (its second partial row), s + 1 ... last (their first)
+  const int n = last - s + 1, quarter = threadIdx.x >> 8, per = (n + 3) / 4;
+  const int p0 = s + min(n, quarter * per), p1 = s + min(n, (quarter + 1) * per);
+  for (int cb = 0; cb < a.d; cb += 1024) {
+    const int col = cb + 4 * static_cast<int>(threadIdx.x & 255), c = quad_column(col, a.d);
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (col < a.d) {
+      constexpr int kB = 16;
+      for (int p = p0; p < p1; p += kB) {
+        float4 v[kB];
+#pragma unroll
+        for (int q = 0; q < kB; ++q) {
+          const int at = min(p + q, p1 - 1);
+          __builtin_memcpy(&v[q], a.part + (2 * static_cast<int64_t>(at) + (at == s)) * a.pitch + c, 16);
+        }
+#pragma unroll
+        for (int q = 0; q < kB; ++q) {
+          if (p + q < p1) {
+            acc.x += v[q].x;
+            acc.y += v[q].y;
+            acc.z += v[q].z;
+            acc.w += v[q].w;
+          }
+        }
+      }
+    }
+    if (quarter) red[quarter - 1][threadIdx.x & 255] = acc;
+    __syncthreads();
+    if (quarter == 0 && col < a.d) {
+#pragma unroll
+      for (int q = 0; q < 3; ++q) {
+        const float4 v = red[q][threadIdx.x];
+        acc.x += v.x;
+        acc.y += v.y;
+        acc.z += v.z;
+        acc.w += v.w;
+      }
+      const float v[4] = {acc.x * a.scale, acc.y * a.scale, acc.z * a.scale, acc.w * a.scale};
+      Quad4<T> o;
+      o.store(static_cast<T*>(a.d_table) + static_cast<int64_t>(row) * a.dt_stride + c, v, a.d - c);
+    }
+    __syncthreads();
+  }
+}
+
+// the shape of the order and the sums
 struct OrderPlan {
-  int lg, R;
-  size_t off_order, off_row, total;
+  int R, row_bits, waves, tiles;          // rows of a bucket, the bits of their numbers, waves that order them
+  int lanes, len, block, blocks, pitch;   // lanes of a piece, its tokens, those of a workgroup, workgroups
+  size_t off_bucket, off_packed, off_order, off_row, off_part, total;
 };
-inline OrderPlan order_plan(int64_t n, int64_t vocab) {
+inline OrderPlan order_plan(int64_t n, int64_t vocab, int d) {
   OrderPlan p;
-  p.lg = 8;   // a workgroup for every compute unit, until a workgroup's rows outgrow its counters
-  while (((vocab + (int64_t{1} << p.lg) - 1) >> p.lg) > kOrderMaxRows) ++p.lg;
-  p.R = static_cast<int>((vocab + (int64_t{1} << p.lg) - 1) >> p.lg);
-  const size_t offs = (static_cast<size_t>(p.R) << p.lg) + 1;
-  p.off_order = (offs * 4 + 255) / 256 * 256;
-  p.off_row = p.off_order + (static_cast<size_t>(n) * 4 + 255) / 256 * 256;
-  p.total = p.off_row + (static_cast<size_t>(n) * 4 + 255) / 256 * 256;
+  p.R = static_cast<int>((vocab + kBuckets - 1) / kBuckets);
+  p.row_bits = 0;
+  while ((p.R - 1) >> p.row_bits) ++p.row_bits;
+  p.waves = p.R <= 2048 ? 16 : 4;   // counters of 4 bytes per wave and row, 128 KiB of LDS
+  p.tiles = static_cast<int>((n + kTile - 1) / kTile);
+  p.lanes = d <= 64 ? 16 : d <= 128 ? 32 : 64;   // four columns a lane
+  // pieces of 16 tokens, two batches of rows in flight, for every SIMD; past 4,096 pieces longer ones, so that the partial
+  // rows of a frequent token stay few
+  p.len = 16;
+  while (p.len < 64 && n / p.len > 4096) p.len *= 2;
+  p.block = 256 / p.lanes * p.len;
+  p.blocks = static_cast<int>((n + p.block - 1) / p.block);
+  p.pitch = (d + 3) / 4 * 4;
+  size_t o = 0;
+  auto take = [&](size_t bytes) {
+    const size_t at = o;
+    o += (bytes + 255) / 256 * 256;
+    return at;
+  };
+  take((static_cast<size_t>(p.R) * kBuckets + 1) * 4);   // offsets
+  p.off_bucket = take((static_cast<size_t>(kBuckets) + 1) * p.tiles * 4);
+  p.off_packed = take(static_cast<size_t>(p.tiles) * kTile * 4);
+  p.off_order = take(static_cast<size_t>(n) * 4);
+  p.off_row = take(static_cast<size_t>(n) * 4);
+  p.off_part = take(2 * static_cast<size_t>(p.blocks) * p.pitch * 4);
+  p.total = o;
   return p;
 }
 
-constexpr int64_t kEmbedMaxTokens = int64_t{1} << 30, kEmbedMaxVocab = 1 << 25;   // positions in 32 bits, one launch
+constexpr int64_t kEmbedMaxTokens = 1 << 27, kEmbedMaxVocab = kOrderMaxRows * kBuckets;   // positions in 32 bits, one launch
 constexpr int kEmbedMaxWidth = 1 << 20;
 
 inline int check_embed(int64_t n, int64_t vocab, int32_t d, const void* ids, const void* a, const void* b,
@@ -209,7 +540,7 @@ inline int check_embed(int64_t n, int64_t vocab, int32_t d, const void* ids, con
   if ((rc = check_dtype(dtype, "dtype"))) return rc;
   if (n < 0 || vocab < 1 || d < 1) return set_err(SDM_RT_EINVAL, "n must be >= 0, vocab and d >= 1");
   if (n > kEmbedMaxTokens || vocab > kEmbedMaxVocab || d > kEmbedMaxWidth)
-    return set_err(SDM_RT_EUNSUPPORTED, "at most 2^30 tokens, a vocabulary of 2^25 and rows of 2^20 values");
+    return set_err(SDM_RT_EUNSUPPORTED, "at most 2^27 tokens, a vocabulary of 2^21 and rows of 2^20 values");
   if ((n > 0 && (!ids || !a)) || !b) return set_err(SDM_RT_EINVAL, "a tensor is NULL");
   if (n > 0 && bad_read_stride(a_stride, d)) return set_err(SDM_RT_EINVAL, "a read row stride must be 0 or >= d");
   if (b_stride < d) return set_err(SDM_RT_EINVAL, "the written rows' stride must be >= d");
@@ -246,7 +577,7 @@ int sdm_rt_embed(const int64_t* ids, int64_t n, const void* table, int64_t table
 
 size_t sdm_rt_embed_backward_workspace_bytes(int64_t n, int64_t vocab, int32_t d) {
   if (n < 0 || vocab < 1 || d < 1 || n > kEmbedMaxTokens || vocab > kEmbedMaxVocab || d > kEmbedMaxWidth) return 0;
-  return order_plan(n, vocab).total;
+  return order_plan(n, vocab, d).total;
 }
 
 int sdm_rt_embed_backward(const int64_t* ids, int64_t n, const void* dy, int64_t dy_row_stride, sdm_rt_dtype dtype,
@@ -255,7 +586,7 @@ int sdm_rt_embed_backward(const int64_t* ids, int64_t n, const void* dy, int64_t
   g_err[0] = 0;
   int rc = check_embed(n, vocab, d, ids, dy, d_table, dy_row_stride, d_table_row_stride, dtype);
   if (rc) return rc;
-  const OrderPlan p = order_plan(n, vocab);
+  const OrderPlan p = order_plan(n, vocab, d);
   if (!workspace) return set_err(SDM_RT_EINVAL, "workspace is NULL");
   if (workspace_bytes < p.total)
     return set_err(SDM_RT_ENOSPACE, "workspace of %zu bytes, %zu needed", workspace_bytes, p.total);
@@ -267,19 +598,49 @@ int sdm_rt_embed_backward(const int64_t* ids, int64_t n, const void* dy, int64_t
   int32_t* order = reinterpret_cast<int32_t*>(ws + p.off_order);
   int32_t* row_of = reinterpret_cast<int32_t*>(ws + p.off_row);
   const int pad = padding_idx >= 0 && padding_idx < vocab ? static_cast<int>(padding_idx) : -1;
-  hipLaunchKernelGGL(embed_order_kernel, dim3(1u << p.lg), dim3(64 * kOrderWaves),
-                     static_cast<size_t>(kOrderWaves) * p.R * 4, st, ids, static_cast<int>(n), static_cast<int>(vocab), pad,
-                     p.lg, p.R, offsets, order, row_of);
+  int32_t* bucket_at = reinterpret_cast<int32_t*>(ws + p.off_bucket);
+  uint32_t* packed = reinterpret_cast<uint32_t*>(ws + p.off_packed);
+  if (p.tiles > 0)
+    hipLaunchKernelGGL(embed_tiles_kernel, dim3(p.tiles), dim3(kTile), 0, st, ids, static_cast<int>(n),
+                       static_cast<int>(vocab), pad, p.tiles, bucket_at, packed);
+  hipLaunchKernelGGL(embed_order_kernel, dim3(kBuckets), dim3(64 * p.waves), static_cast<size_t>(p.waves) * p.R * 4, st,
+                     bucket_at, packed, p.tiles, p.R, p.row_bits, offsets, order, row_of);
   if ((rc = check_launch("embed_order"))) return rc;
-  const unsigned blocks = ((static_cast<unsigned>(p.R) << p.lg) + 3) / 4;
+  RowsGrad a{};
+  a.offsets = offsets;
+  a.order = order;
+  a.row_of = row_of;
+  a.part = reinterpret_cast<float*>(ws + p.off_part);
+  a.pitch = p.pitch;
+  a.n_slots = p.R * kBuckets;
+  a.R = p.R;
+  a.vocab = static_cast<int>(vocab);
+  a.d = d;
+  a.len = p.len;
+  a.piece_blocks = p.blocks;
+  a.scale = scale;
+  a.dy = dy;
+  a.dy_stride = dy_row_stride;
+  a.d_table = d_table;
+  a.dt_stride = d_table_row_stride;
+  const dim3 grid(static_cast<unsigned>(a.piece_blocks + (a.n_slots + 4 * kZeroRows - 1) / (4 * kZeroRows)));
+  const dim3 edges(static_cast<unsigned>(std::max(1, p.blocks - 1)));
+#define SDM_RT_ROWS_GRAD(T)                                                                          \
+  do {                                                                                               \
+    if (p.lanes == 16)                                                                                 \
+      hipLaunchKernelGGL((embed_rows_grad_kernel<T, 16>), grid, dim3(256), 0, st, a);                \
+    else if (p.lanes == 32)                                                                            \
+      hipLaunchKernelGGL((embed_rows_grad_kernel<T, 32>), grid, dim3(256), 0, st, a);                \
+    else                                                                                             \
+      hipLaunchKernelGGL((embed_rows_grad_kernel<T, 64>), grid, dim3(256), 0, st, a);                \
+    if (p.blocks > 1)                                                                                \
+      hipLaunchKernelGGL((embed_rows_join_kernel<T>), edges, dim3(1024), 0, st, a, p.block);         \
+  } while (0)
   if (dtype == SDM_RT_BF16)
-    hipLaunchKernelGGL((embed_rows_grad_kernel<bf16_t>), dim3(blocks), dim3(256), 0, st, offsets, order,
-                       static_cast<const bf16_t*>(dy), dy_row_stride, static_cast<int>(vocab), d, scale, p.lg, p.R,
-                       static_cast<bf16_t*>(d_table), d_table_row_stride);
+    SDM_RT_ROWS_GRAD(bf16_t);
   else
-    hipLaunchKernelGGL((embed_rows_grad_kernel<float>), dim3(blocks), dim3(256), 0, st, offsets, order,
-                       static_cast<const float*>(dy), dy_row_stride, static_cast<int>(vocab), d, scale, p.lg, p.R,
-                       static_cast<float*>(d_table), d_table_row_stride);
+    SDM_RT_ROWS_GRAD(float);
+#undef SDM_RT_ROWS_GRAD
   return check_launch("embed_rows_grad");
 }
 

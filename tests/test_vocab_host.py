@@ -19,8 +19,8 @@ def _fails(rc, code, text):
 @pytest.mark.parametrize("over,code,text", [
     (dict(dtype=7), -1, "dtype"), (dict(n=-1), -1, "n must"), (dict(vocab=0), -1, "vocab"), (dict(d=0), -1, "d >= 1"),
     (dict(ids=None), -1, "NULL"), (dict(table=None), -1, "NULL"), (dict(out=None), -1, "NULL"),
-    (dict(ts=7), -1, "stride"), (dict(os=7), -1, "stride"), (dict(vocab=1 << 26), -3, "2^25"),
-    (dict(n=(1 << 30) + 1), -3, "2^30"),
+    (dict(ts=7), -1, "stride"), (dict(os=7), -1, "stride"), (dict(vocab=(1 << 21) + 1), -3, "2^21"),
+    (dict(n=(1 << 27) + 1), -3, "2^27"),
 ])
 def test_embed_checks(over, code, text):
     a = dict(ids=P, n=4, table=P, ts=8, dtype=0, vocab=10, d=8, out=P, os=8)
