@@ -475,7 +475,7 @@ enum { SDM_RT_NONE = 0, SDM_RT_MEAN = 1, SDM_RT_SUM = 2 };
  * loss 0 and gradient 0 whatever its logits hold.  reduction: SDM_RT_NONE gives the rows' losses, SDM_RT_SUM their sum,
  * SDM_RT_MEAN that over the number of rows with a target (0 if there is none). */
 typedef struct {
-  int64_t rows;          /* at most 2^22 */
+  int64_t rows;          /* at most 2^21 */
   int32_t vocab;         /* at most 2^30 */
   int32_t top_k;         /* teacher entries per row, 0 to 1,024 */
   float temperature;     /* positive */
@@ -489,18 +489,21 @@ size_t sdm_rt_distill_workspace_bytes(const sdm_rt_distill* dims);
 
 /* loss: [rows] (SDM_RT_NONE) or [1] float32.
  *   logits [rows][vocab] in dtype, top_ids [rows][top_k] int64, top_logits [rows][top_k] float32, row strides in elements;
- *   labels [rows] int64 or NULL;  stats [rows][4] float32, 16-byte aligned, for sdm_rt_distill_grad, or NULL */
+ *   labels [rows] int64 or NULL;  stats [rows][4] float32, 16-byte aligned, for sdm_rt_distill_grad, or NULL;
+ *   d_logits [rows][vocab] in dtype or NULL: the gradient of loss (of the losses' sum for SDM_RT_NONE), from the same
+ *   pass over the logits; it must not overlap them */
 int sdm_rt_distill_loss(const sdm_rt_distill* dims, const void* logits, int64_t logits_row_stride, sdm_rt_dtype dtype,
                         const int64_t* top_ids, int64_t top_ids_row_stride, const float* top_logits,
-                        int64_t top_logits_row_stride, const int64_t* labels, float* loss, float* stats, void* workspace,
-                        size_t workspace_bytes, void* stream);
+                        int64_t top_logits_row_stride, const int64_t* labels, float* loss, float* stats, void* d_logits,
+                        int64_t d_logits_row_stride, void* workspace, size_t workspace_bytes, void* stream);
 
 /* d_logits [rows][vocab] in dtype: the gradient of sdm_rt_distill_loss of the same inputs (stats from that call) for
- * grad_out, the gradient of loss: float32 on the device, [rows] (SDM_RT_NONE) or [1]. */
+ * grad_out, the gradient of loss: float32 on the device, [rows] (SDM_RT_NONE) or [1].  unless_one (not with SDM_RT_NONE):
+ * d_logits is left as it is where grad_out is 1, for one that sdm_rt_distill_loss has filled. */
 int sdm_rt_distill_grad(const sdm_rt_distill* dims, const void* logits, int64_t logits_row_stride, sdm_rt_dtype dtype,
                         const int64_t* top_ids, int64_t top_ids_row_stride, const float* top_logits,
                         int64_t top_logits_row_stride, const int64_t* labels, const float* stats, const float* grad_out,
-                        void* d_logits, int64_t d_logits_row_stride, void* stream);
+                        int32_t unless_one, void* d_logits, int64_t d_logits_row_stride, void* stream);
 
 /* The rules of a decode step on its logits, in this order, in float32:
  *   a token of the stream's history        x = x > 0 ? x / repetition : x * repetition

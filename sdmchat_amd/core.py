@@ -1389,26 +1389,32 @@ _REDUCTION = {"none": _lib.SDM_RT_NONE, "mean": _lib.SDM_RT_MEAN, "sum": _lib.SD
 
 
 class DistillFunction(torch.autograd.Function):
-    """distill_loss on rows as an autograd function (sdm_rt_distill_loss, sdm_rt_distill_grad); it cannot be
-    differentiated again.  apply(logits [rows, vocab], top_ids, top_logits [rows, k], labels [rows] or None, dims) -> loss,
-    dims an _lib.SdmRtDistill."""
+    """distill_loss on rows as an autograd function; it cannot be differentiated again.  A loss of one value computes its
+    gradient with the loss (sdm_rt_distill_loss, one pass over the logits): the first backward hands it out, after
+    sdm_rt_distill_grad has put it right if the gradient that comes in is not 1.  "none", and a second backward, take
+    sdm_rt_distill_grad alone.  apply(logits [rows, vocab], top_ids, top_logits [rows, k], labels [rows] or None, dims) ->
+    loss, dims an _lib.SdmRtDistill."""
 
     @staticmethod
     def forward(ctx, logits, ids, top, labels, dims):
         dev = logits.device
         z, zs = _read_rows(logits)
-        n = dims.rows
-        loss = torch.empty(n if dims.reduction == _lib.SDM_RT_NONE else (), dtype=torch.float32, device=dev)
-        stats = torch.empty(n, 4, dtype=torch.float32, device=dev) if ctx.needs_input_grad[0] else None
+        n, V, none = dims.rows, dims.vocab, dims.reduction == _lib.SDM_RT_NONE
+        loss = torch.empty(n if none else (), dtype=torch.float32, device=dev)
+        stats = dz = None
+        if ctx.needs_input_grad[0]:
+            stats = torch.empty(n, 4, dtype=torch.float32, device=dev)
+            if not none:
+                dz = torch.empty(n, V, dtype=z.dtype, device=dev)
         lib = _lib.load()
         nbytes = lib.sdm_rt_distill_workspace_bytes(ctypes.byref(dims))
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
         with _on(dev):
             _lib.check(lib.sdm_rt_distill_loss(ctypes.byref(dims), _ptr(z), zs, _DT[z.dtype], _ptr(ids), dims.top_k,
-                                               _ptr(top), dims.top_k, _ptr(labels), _ptr(loss), _ptr(stats), _ptr(ws), nbytes,
-                                               _stream(dev)), lib)
+                                               _ptr(top), dims.top_k, _ptr(labels), _ptr(loss), _ptr(stats), _ptr(dz), V,
+                                               _ptr(ws), nbytes, _stream(dev)), lib)
         if stats is not None:
-            ctx.dims = dims
+            ctx.dims, ctx.dz = dims, dz
             ctx.save_for_backward(z, ids, top, labels, stats)
         return loss
 
@@ -1417,14 +1423,17 @@ class DistillFunction(torch.autograd.Function):
     def backward(ctx, dloss):
         z, ids, top, labels, stats = ctx.saved_tensors
         z, zs = _read_rows(z)
-        dims = ctx.dims
+        dims, dz = ctx.dims, ctx.dz
+        ctx.dz = None   # the caller's from here on
         g = dloss.contiguous()
-        dz = torch.empty(z.shape, dtype=z.dtype, device=z.device)
+        unless_one = dz is not None
+        if dz is None:
+            dz = torch.empty(z.shape, dtype=z.dtype, device=z.device)
         lib = _lib.load()
         with _on(z.device):
             _lib.check(lib.sdm_rt_distill_grad(ctypes.byref(dims), _ptr(z), zs, _DT[z.dtype], _ptr(ids), dims.top_k,
-                                               _ptr(top), dims.top_k, _ptr(labels), _ptr(stats), _ptr(g), _ptr(dz), dims.vocab,
-                                               _stream(z.device)), lib)
+                                               _ptr(top), dims.top_k, _ptr(labels), _ptr(stats), _ptr(g), unless_one, _ptr(dz),
+                                               dims.vocab, _stream(z.device)), lib)
         return dz, None, None, None, None
 
 
@@ -1439,7 +1448,8 @@ def distill_loss(logits, top_ids, top_logits, *, temperature=1.0, labels=None, a
     shares add up) and top_logits [..., k], k at most 1,024; labels [...] int64 or int32 or None (ignore_index, or any id
     outside the vocabulary: no label).  Positions may lack either part, or both: those have loss 0 and gradient 0 whatever
     their logits hold.  reduction "mean" divides the sum by the number of positions with a target (0 if there is none),
-    "sum" does not, "none" gives float32 losses [...].  Differentiable in logits, once; the teacher gets no gradient."""
+    "sum" does not, "none" gives float32 losses [...].  Differentiable in logits, once; the teacher gets no gradient.  With
+    autograd recording, "mean" and "sum" compute the gradient along with the loss, so it takes its memory from then on."""
     if logits.device.type != "cuda":
         raise RuntimeError("distill_loss needs ROCm device tensors")
     if logits.dtype not in _DT:

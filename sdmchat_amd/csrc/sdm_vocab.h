@@ -24,6 +24,11 @@ struct Piece {
     }
     __builtin_memcpy(&r, v, 16);
   }
+  // makes the compiler forget what it knows of the bits: values unpacked before are unpacked again after, instead of
+  // staying in twice the registers of the piece
+  __device__ __forceinline__ void forget() {
+    if constexpr (sizeof(T) == 2) asm volatile("" : "+v"(r.x), "+v"(r.y), "+v"(r.z), "+v"(r.w));
+  }
   __device__ __forceinline__ void store(T* p) const { __builtin_memcpy(p, &r, 16); }
   __device__ __forceinline__ void store_part(T* p, int n) const {
     T v[kN];
@@ -38,6 +43,12 @@ struct Piece {
       return __uint_as_float(e & 1 ? w[e >> 1] & 0xffff0000u : w[e >> 1] << 16);
     else
       return __uint_as_float(w[e]);
+  }
+  __device__ __forceinline__ void fill(float x) {
+    float v[kN];
+#pragma unroll
+    for (int e = 0; e < kN; ++e) v[e] = x;
+    set(v);
   }
   // kN floats, each rounded once to T
   __device__ __forceinline__ void set(const float (&v)[kN]) {
@@ -56,20 +67,40 @@ __device__ __forceinline__ int clamp_token(int64_t id, int vocab) {
   return static_cast<int>(min(max(id, int64_t{0}), static_cast<int64_t>(vocab) - 1));
 }
 
+// the maximum and the sum over a wave's 64 lanes, in every lane, by DPP: swap neighbours, swap pairs, mirror the halves and
+// the rows of 16, then the last lane of rows 0 and 2 into rows 1 and 3, and lane 31 into rows 2 and 3
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp_rows(int old, int v) {
+  return __builtin_amdgcn_update_dpp(old, v, CTRL, ROWS, 0xf, false);
+}
 __device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-  for (int j = 32; j > 0; j >>= 1) v = fmaxf(v, __shfl_xor(v, j));
-  return v;
+  auto step = [](float x, int y) { return fmaxf(x, __int_as_float(y)); };
+  v = step(v, dpp_rows<0xb1, 0xf>(0, __float_as_int(v)));
+  v = step(v, dpp_rows<0x4e, 0xf>(0, __float_as_int(v)));
+  v = step(v, dpp_rows<0x141, 0xf>(0, __float_as_int(v)));
+  v = step(v, dpp_rows<0x140, 0xf>(0, __float_as_int(v)));
+  v = step(v, dpp_rows<0x142, 0xa>(__float_as_int(v), __float_as_int(v)));
+  v = step(v, dpp_rows<0x143, 0xc>(__float_as_int(v), __float_as_int(v)));
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
 }
 __device__ __forceinline__ float wave_add(float v) {
-#pragma unroll
-  for (int j = 32; j > 0; j >>= 1) v += __shfl_xor(v, j);
-  return v;
+  auto step = [](float x, int y) { return x + __int_as_float(y); };
+  v = step(v, dpp_rows<0xb1, 0xf>(0, __float_as_int(v)));
+  v = step(v, dpp_rows<0x4e, 0xf>(0, __float_as_int(v)));
+  v = step(v, dpp_rows<0x141, 0xf>(0, __float_as_int(v)));
+  v = step(v, dpp_rows<0x140, 0xf>(0, __float_as_int(v)));
+  v = step(v, dpp_rows<0x142, 0xa>(0, __float_as_int(v)));
+  v = step(v, dpp_rows<0x143, 0xc>(0, __float_as_int(v)));
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
 }
 __device__ __forceinline__ int wave_add(int v) {
-#pragma unroll
-  for (int j = 32; j > 0; j >>= 1) v += __shfl_xor(v, j);
-  return v;
+  v += dpp_rows<0xb1, 0xf>(0, v);
+  v += dpp_rows<0x4e, 0xf>(0, v);
+  v += dpp_rows<0x141, 0xf>(0, v);
+  v += dpp_rows<0x140, 0xf>(0, v);
+  v += dpp_rows<0x142, 0xa>(0, v);
+  v += dpp_rows<0x143, 0xc>(0, v);
+  return __builtin_amdgcn_readlane(v, 63);
 }
 
 }  // namespace sdmrt

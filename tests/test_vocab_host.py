@@ -55,7 +55,7 @@ def _distill(**over):
 
 @pytest.mark.parametrize("over,code,text", [
     (dict(dtype=2), -1, "dtype"), (dict(rows=-1), -1, "rows"), (dict(vocab=0), -1, "vocab"), (dict(top_k=-1), -1, "top_k"),
-    (dict(top_k=1025, ids_s=1025, top_s=1025), -3, "1024"), (dict(rows=(1 << 22) + 1), -3, "2^22"),
+    (dict(top_k=1025, ids_s=1025, top_s=1025), -3, "1024"), (dict(rows=(1 << 21) + 1), -3, "2^21"),
     (dict(temperature=0.0), -1, "temperature"), (dict(temperature=-1.0), -1, "temperature"),
     (dict(temperature=float("inf")), -1, "temperature"), (dict(temperature=float("nan")), -1, "temperature"),
     (dict(temperature=1e-40), -1, "temperature"), (dict(alpha=1.5), -1, "alpha"), (dict(alpha=float("nan")), -1, "alpha"),
@@ -66,19 +66,22 @@ def _distill(**over):
 def test_distill_checks(over, code, text):
     lib = _lib.load()
     dims, a, head = _distill(**over)
-    _fails(lib.sdm_rt_distill_loss(*head, a["loss"], a["stats"], a["ws"], a["nws"], None), code, text)
-    _fails(lib.sdm_rt_distill_grad(*head, a["stats"], a["go"], a["dz"], a["dzs"], None), code, text)
+    _fails(lib.sdm_rt_distill_loss(*head, a["loss"], a["stats"], a["dz"], a["dzs"], a["ws"], a["nws"], None), code, text)
+    _fails(lib.sdm_rt_distill_grad(*head, a["stats"], a["go"], 1, a["dz"], a["dzs"], None), code, text)
 
 
 def test_distill_checks_of_outputs():
     lib = _lib.load()
     dims, a, head = _distill()
     need = lib.sdm_rt_distill_workspace_bytes(ctypes.byref(dims))
-    _fails(lib.sdm_rt_distill_loss(*head, None, P, P, need, None), -1, "loss")
-    _fails(lib.sdm_rt_distill_loss(*head, P, P, P, need - 1, None), -2, "needed")
-    _fails(lib.sdm_rt_distill_grad(*head, None, P, P, 100, None), -1, "stats")
-    _fails(lib.sdm_rt_distill_grad(*head, P, None, P, 100, None), -1, "grad_out")
-    _fails(lib.sdm_rt_distill_grad(*head, P, P, P, 99, None), -1, "d_logits_row_stride")
+    _fails(lib.sdm_rt_distill_loss(*head, None, P, P, 100, P, need, None), -1, "loss")
+    _fails(lib.sdm_rt_distill_loss(*head, P, P, P, 99, P, need, None), -1, "d_logits_row_stride")
+    _fails(lib.sdm_rt_distill_loss(*head, P, P, P, 100, P, need - 1, None), -2, "needed")
+    _fails(lib.sdm_rt_distill_grad(*head, None, P, 0, P, 100, None), -1, "stats")
+    _fails(lib.sdm_rt_distill_grad(*head, P, None, 0, P, 100, None), -1, "grad_out")
+    _fails(lib.sdm_rt_distill_grad(*head, P, P, 0, P, 99, None), -1, "d_logits_row_stride")
+    dims, a, head = _distill(reduction=0)
+    _fails(lib.sdm_rt_distill_grad(*head, P, P, 1, P, 100, None), -1, "unless_one")
 
 
 @pytest.mark.parametrize("over,call,code,text", [
