@@ -1247,9 +1247,12 @@ class TableSdmFunction(torch.autograd.Function):
 
 # -- the vocabulary's ends: embedding, distillation loss, rules on logits ------------------------------------------
 
+_HERE = contextlib.nullcontext()
+
+
 def _on(device):
     """The device as the current one, for a launch on a tensor of another device than the current one."""
-    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    return _HERE if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
 
 
 def _same_device(name, device, **tensors):
@@ -1259,23 +1262,25 @@ def _same_device(name, device, **tensors):
 
 
 def _ids(name, what, t):
-    """Token ids as int64 (int32 is widened)."""
-    if t.dtype not in (torch.int64, torch.int32):
-        raise ValueError(f"{name}: {what} must be int64 or int32, got {t.dtype}")
-    return t.to(torch.int64)
+    """Token ids as contiguous int64 (int32 is widened)."""
+    if t.dtype != torch.int64:
+        if t.dtype != torch.int32:
+            raise ValueError(f"{name}: {what} must be int64 or int32, got {t.dtype}")
+        t = t.to(torch.int64)
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def _read_rows(t2):
     """(rows, row stride in elements) of a 2-D tensor as the kernels that read any row stride and any element alignment
     take it: itself where the last dimension is contiguous, else a copy."""
-    if t2.shape[1] > 1 and t2.stride(1) != 1:
-        t2 = t2.contiguous()
-    row = t2.stride(0)
-    if t2.shape[0] <= 1:
-        row = t2.shape[1]
-    elif 0 < row < t2.shape[1]:   # overlapping windows
-        t2 = t2.contiguous()
-        row = t2.shape[1]
+    rows, width = t2.shape
+    row, step = t2.stride()
+    if step != 1 and width > 1:
+        return t2.contiguous(), width
+    if rows <= 1:
+        return t2, width
+    if 0 < row < width:   # overlapping windows
+        return t2.contiguous(), width
     return t2, row
 
 
@@ -1303,14 +1308,15 @@ def embedding_fits(idx, table):
 
 
 def _embed(idx, table, scale):
-    d = table.shape[1]
-    ids = _ids("embedding", "idx", idx).reshape(-1).contiguous()
-    tab, stride = _read_rows(table.detach())
-    out = torch.empty(idx.shape + (d,), dtype=table.dtype, device=table.device)
+    V, d = table.shape
+    dev = table.device
+    ids = _ids("embedding", "idx", idx)
+    tab, stride = _read_rows(table)
+    out = torch.empty(idx.shape + (d,), dtype=table.dtype, device=dev)
     lib = _lib.load()
-    with _on(table.device):
-        _lib.check(lib.sdm_rt_embed(_ptr(ids), ids.numel(), _ptr(tab), stride, _DT[table.dtype], table.shape[0], d,
-                                    float(scale), _ptr(out), d, _stream(table.device)), lib)
+    with _on(dev):
+        _lib.check(lib.sdm_rt_embed(ids.data_ptr(), ids.numel(), tab.data_ptr(), stride, _DT[table.dtype], V, d, scale,
+                                    out.data_ptr(), d, _stream(dev)), lib)
     return out
 
 
@@ -1323,19 +1329,21 @@ def embedding_backward(idx, dy, vocab, scale=1.0, padding_idx=None):
         raise RuntimeError("embedding_backward needs ROCm device tensors")
     if dy.dtype not in _DT:
         raise ValueError(f"embedding_backward: dtype {dy.dtype} is not float32 or bfloat16")
-    if tuple(dy.shape[:-1]) != tuple(idx.shape):
+    if dy.shape[:-1] != idx.shape:
         raise ValueError(f"embedding_backward: dy {tuple(dy.shape)} for ids {tuple(idx.shape)}")
-    _same_device("embedding_backward", dy.device, idx=idx)
-    ids = _ids("embedding_backward", "idx", idx).reshape(-1).contiguous()
-    dy2, stride = _read_rows(dy.reshape(-1, d))
-    out = torch.empty(vocab, d, dtype=dy.dtype, device=dy.device)
+    dev = dy.device
+    _same_device("embedding_backward", dev, idx=idx)
+    ids = _ids("embedding_backward", "idx", idx)
+    dy2, stride = _read_rows(dy if dy.dim() == 2 else dy.reshape(-1, d))
+    out = torch.empty(vocab, d, dtype=dy.dtype, device=dev)
     lib = _lib.load()
-    nbytes = lib.sdm_rt_embed_backward_workspace_bytes(ids.numel(), vocab, d)
-    ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=dy.device)
-    with _on(dy.device):
-        _lib.check(lib.sdm_rt_embed_backward(_ptr(ids), ids.numel(), _ptr(dy2), stride, _DT[dy.dtype], vocab, d,
-                                             float(scale), -1 if padding_idx is None else padding_idx, _ptr(out), d, _ptr(ws),
-                                             ws.numel(), _stream(dy.device)), lib)
+    n = ids.numel()
+    nbytes = lib.sdm_rt_embed_backward_workspace_bytes(n, vocab, d)   # 0 outside the limits: the call below reports why
+    ws = torch.empty(nbytes or 16, dtype=torch.uint8, device=dev)
+    with _on(dev):
+        _lib.check(lib.sdm_rt_embed_backward(ids.data_ptr(), n, dy2.data_ptr(), stride, _DT[dy.dtype], vocab, d, scale,
+                                             -1 if padding_idx is None else padding_idx, out.data_ptr(), d, ws.data_ptr(),
+                                             nbytes, _stream(dev)), lib)
     return out
 
 
@@ -1380,9 +1388,10 @@ def embedding(idx, table, scale=1.0, padding_idx=None):
         if not -table.shape[0] <= padding_idx < table.shape[0]:
             raise ValueError(f"embedding: padding_idx {padding_idx} is outside the table of {table.shape[0]} rows")
         padding_idx %= table.shape[0]
+    scale = float(scale)
     if torch.is_grad_enabled() and table.requires_grad:
         return EmbeddingFunction.apply(idx, table, scale, padding_idx)
-    return _embed(idx, table, scale)
+    return _embed(idx, table.detach(), scale)
 
 
 _REDUCTION = {"none": _lib.SDM_RT_NONE, "mean": _lib.SDM_RT_MEAN, "sum": _lib.SDM_RT_SUM}
@@ -1399,23 +1408,23 @@ class DistillFunction(torch.autograd.Function):
     def forward(ctx, logits, ids, top, labels, dims):
         dev = logits.device
         z, zs = _read_rows(logits)
-        n, V, none = dims.rows, dims.vocab, dims.reduction == _lib.SDM_RT_NONE
+        n, V, k, none = dims.rows, dims.vocab, dims.top_k, dims.reduction == _lib.SDM_RT_NONE
         loss = torch.empty(n if none else (), dtype=torch.float32, device=dev)
-        stats = dz = None
-        if ctx.needs_input_grad[0]:
-            stats = torch.empty(n, 4, dtype=torch.float32, device=dev)
-            if not none:
-                dz = torch.empty(n, V, dtype=z.dtype, device=dev)
         lib = _lib.load()
         nbytes = lib.sdm_rt_distill_workspace_bytes(ctypes.byref(dims))
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        grad = ctx.needs_input_grad[0]
+        # the rows' maxima and sums for the backward ([n, 4] float32), then the workspace
+        kept = 16 * n if grad else 0
+        buf = torch.empty(kept + nbytes, dtype=torch.uint8, device=dev)
+        dz = torch.empty(n, V, dtype=z.dtype, device=dev) if grad and not none else None
+        stats = buf.data_ptr()
         with _on(dev):
-            _lib.check(lib.sdm_rt_distill_loss(ctypes.byref(dims), _ptr(z), zs, _DT[z.dtype], _ptr(ids), dims.top_k,
-                                               _ptr(top), dims.top_k, _ptr(labels), _ptr(loss), _ptr(stats), _ptr(dz), V,
-                                               _ptr(ws), nbytes, _stream(dev)), lib)
-        if stats is not None:
+            _lib.check(lib.sdm_rt_distill_loss(ctypes.byref(dims), z.data_ptr(), zs, _DT[z.dtype], _ptr(ids), k, _ptr(top), k,
+                                               _ptr(labels), loss.data_ptr(), stats if grad else None, _ptr(dz), V,
+                                               stats + kept, nbytes, _stream(dev)), lib)
+        if grad:
             ctx.dims, ctx.dz = dims, dz
-            ctx.save_for_backward(z, ids, top, labels, stats)
+            ctx.save_for_backward(z, ids, top, labels, buf)
         return loss
 
     @staticmethod
@@ -1423,17 +1432,18 @@ class DistillFunction(torch.autograd.Function):
     def backward(ctx, dloss):
         z, ids, top, labels, stats = ctx.saved_tensors
         z, zs = _read_rows(z)
-        dims, dz = ctx.dims, ctx.dz
+        dims, dz, dev = ctx.dims, ctx.dz, z.device
         ctx.dz = None   # the caller's from here on
-        g = dloss.contiguous()
+        k, V = dims.top_k, dims.vocab
         unless_one = dz is not None
         if dz is None:
-            dz = torch.empty(z.shape, dtype=z.dtype, device=z.device)
+            dz = torch.empty(z.shape, dtype=z.dtype, device=dev)
+        g = dloss if dloss.is_contiguous() else dloss.contiguous()
         lib = _lib.load()
-        with _on(z.device):
-            _lib.check(lib.sdm_rt_distill_grad(ctypes.byref(dims), _ptr(z), zs, _DT[z.dtype], _ptr(ids), dims.top_k,
-                                               _ptr(top), dims.top_k, _ptr(labels), _ptr(stats), _ptr(g), unless_one, _ptr(dz),
-                                               dims.vocab, _stream(z.device)), lib)
+        with _on(dev):
+            _lib.check(lib.sdm_rt_distill_grad(ctypes.byref(dims), z.data_ptr(), zs, _DT[z.dtype], _ptr(ids), k, _ptr(top), k,
+                                               _ptr(labels), stats.data_ptr(), g.data_ptr(), unless_one, dz.data_ptr(), V,
+                                               _stream(dev)), lib)
         return dz, None, None, None, None
 
 
@@ -1450,33 +1460,38 @@ def distill_loss(logits, top_ids, top_logits, *, temperature=1.0, labels=None, a
     their logits hold.  reduction "mean" divides the sum by the number of positions with a target (0 if there is none),
     "sum" does not, "none" gives float32 losses [...].  Differentiable in logits, once; the teacher gets no gradient.  With
     autograd recording, "mean" and "sum" compute the gradient along with the loss, so it takes its memory from then on."""
-    if logits.device.type != "cuda":
+    dev = logits.device
+    if dev.type != "cuda":
         raise RuntimeError("distill_loss needs ROCm device tensors")
     if logits.dtype not in _DT:
         raise ValueError(f"distill_loss: dtype {logits.dtype} is not float32 or bfloat16")
-    if logits.dim() < 1 or logits.shape[-1] < 1:
-        raise ValueError(f"distill_loss: logits must be [..., vocab], got {tuple(logits.shape)}")
-    lead, V = tuple(logits.shape[:-1]), logits.shape[-1]
-    if top_ids.dim() < 1 or tuple(top_ids.shape[:-1]) != lead or top_ids.shape != top_logits.shape:
+    shape = logits.shape
+    if not shape or not shape[-1]:
+        raise ValueError(f"distill_loss: logits must be [..., vocab], got {tuple(shape)}")
+    lead, V = shape[:-1], shape[-1]
+    if top_ids.shape != top_logits.shape or top_ids.shape[:-1] != lead or not top_ids.shape:
         raise ValueError(f"distill_loss: top_ids {tuple(top_ids.shape)} and top_logits {tuple(top_logits.shape)} must be "
-                         f"{lead} + [k]")
+                         f"{tuple(lead)} + [k]")
     if not top_logits.is_floating_point():
         raise ValueError(f"distill_loss: top_logits must be floating point, got {top_logits.dtype}")
-    if labels is not None and tuple(labels.shape) != lead:
-        raise ValueError(f"distill_loss: labels {tuple(labels.shape)}, expected {lead}")
+    if labels is not None and labels.shape != lead:
+        raise ValueError(f"distill_loss: labels {tuple(labels.shape)}, expected {tuple(lead)}")
     if reduction not in _REDUCTION:
         raise ValueError(f"distill_loss: reduction {reduction!r} is not 'none', 'mean' or 'sum'")
     if labels is None and alpha != 1.0:
         raise ValueError("distill_loss: alpha below 1 needs labels")
-    _same_device("distill_loss", logits.device, top_ids=top_ids, top_logits=top_logits, labels=labels)
+    _same_device("distill_loss", dev, top_ids=top_ids, top_logits=top_logits, labels=labels)
     k = top_ids.shape[-1]
-    ids = _ids("distill_loss", "top_ids", top_ids).reshape(-1, k).contiguous() if k else None
-    top = top_logits.detach().to(torch.float32).reshape(-1, k).contiguous() if k else None
-    lab = None if labels is None else _ids("distill_loss", "labels", labels).reshape(-1).contiguous()
-    n = math.prod(lead)
-    dims = _lib.SdmRtDistill(n, V, k, float(temperature), float(alpha), int(ignore_index), _REDUCTION[reduction])
-    loss = DistillFunction.apply(logits.reshape(n, V), ids, top, lab, dims)
-    return loss.reshape(lead) if reduction == "none" else loss
+    ids = _ids("distill_loss", "top_ids", top_ids)
+    top = top_logits.detach() if top_logits.requires_grad else top_logits
+    if top.dtype != torch.float32 or not top.is_contiguous():
+        top = top.to(torch.float32).contiguous()
+    lab = None if labels is None else _ids("distill_loss", "labels", labels)
+    n = lead.numel()
+    dims = _lib.SdmRtDistill(n, V, k, temperature, alpha, ignore_index, _REDUCTION[reduction])
+    rows = logits if len(shape) == 2 else logits.reshape(n, V)
+    loss = DistillFunction.apply(rows, ids, top, lab, dims)
+    return loss.reshape(lead) if reduction == "none" and len(shape) != 2 else loss
 
 
 def _per_row(name, what, v, B, device):
@@ -1488,18 +1503,19 @@ def _per_row(name, what, v, B, device):
         return None, v
     if v.numel() not in (1, B) or v.dim() > 1 or not v.is_floating_point():
         raise ValueError(f"{name}: {what} must be a number or a floating-point tensor [B={B}], got {v.dtype} {tuple(v.shape)}")
-    _same_device(name, device, **{what: v})
+    if v.device != device:
+        raise ValueError(f"{name}: {what} is on {v.device}, expected {device}")
+    if v.dtype == torch.float32 and v.dim() == 1 and v.shape[0] == B and v.is_contiguous():
+        return v, 0.0
     return v.detach().to(torch.float32).reshape(-1).expand(B).contiguous(), 0.0
 
 
 def _row_or_rows(name, what, t, B, width, dtype):
     """A [width] or [B, width] tensor as (tensor, row stride; 0: one row for all)."""
-    if tuple(t.shape) not in ((width,), (B, width)) or t.dtype != dtype:
-        raise ValueError(f"{name}: {what} must be {dtype} [{width}] or [B={B}, {width}], got {t.dtype} {tuple(t.shape)}")
-    t = t.detach()
-    if t.dim() == 1:
-        return t.contiguous(), 0
-    return _read_rows(t)
+    shape = t.shape
+    if t.dtype != dtype or shape[-1:] != (width,) or len(shape) > 2 or (len(shape) == 2 and shape[0] != B):
+        raise ValueError(f"{name}: {what} must be {dtype} [{width}] or [B={B}, {width}], got {t.dtype} {tuple(shape)}")
+    return (t.contiguous(), 0) if len(shape) == 1 else _read_rows(t)
 
 
 def pack_mask(allowed):
@@ -1541,32 +1557,28 @@ def process_logits(logits, tokens=None, lengths=None, *, prompt=None, repetition
     _same_device(name, dev, tokens=tokens, lengths=lengths, prompt=prompt, bias=bias, mask=mask, out=out)
     held = [_per_row(name, w, v, B, dev) for w, v in (("repetition", repetition), ("frequency", frequency),
                                                       ("presence", presence))]
-    r = _lib.SdmRtRules()
-    r.repetition, r.frequency, r.presence = (_ptr(t) for t, _ in held)
-    r.repetition_all, r.frequency_all, r.presence_all = (v for _, v in held)
+    hist = (None, 0, 0, None, None)
     if tokens is not None:
         if tokens.dtype != torch.int64 or tokens.dim() != 2 or tokens.shape[0] != B:
             raise ValueError(f"{name}: tokens must be int64 [B={B}, width], got {tokens.dtype} {tuple(tokens.shape)}")
         if lengths is None:
             raise ValueError(f"{name}: tokens need lengths")
         for what, t in (("lengths", lengths), ("prompt", prompt)):
-            if t is not None and (t.dtype != torch.int64 or tuple(t.shape) != (B,)):
+            if t is not None and (t.dtype != torch.int64 or t.dim() != 1 or t.shape[0] != B):
                 raise ValueError(f"{name}: {what} must be int64 [B={B}], got {t.dtype} {tuple(t.shape)}")
         if any(t is not None or v != w for (t, v), w in zip(held, (1.0, 0.0, 0.0))):
-            tokens, r.tokens_row_stride = _read_rows(tokens)
-            r.width = tokens.shape[1]
+            tokens, ts = _read_rows(tokens)
             lengths = lengths.contiguous()
             prompt = None if prompt is None else prompt.contiguous()
-            r.tokens, r.lengths, r.prompt = _ptr(tokens), _ptr(lengths), _ptr(prompt)
+            hist = (tokens.data_ptr(), ts, tokens.shape[1], lengths.data_ptr(), _ptr(prompt))
     elif lengths is not None or prompt is not None:
         raise ValueError(f"{name}: lengths and prompt need tokens")
+    bs = ms = 0
     if bias is not None:
-        bias, r.bias_row_stride = _row_or_rows(name, "bias", bias, B, V, torch.float32)
-        r.bias = _ptr(bias)
+        bias, bs = _row_or_rows(name, "bias", bias, B, V, torch.float32)
     if mask is not None:
-        mask, r.mask_row_stride = _row_or_rows(name, "mask", mask, B, (V + 31) // 32, torch.int32)
-        r.mask = _ptr(mask)
-    src, ls = _read_rows(logits.detach())
+        mask, ms = _row_or_rows(name, "mask", mask, B, (V + 31) // 32, torch.int32)
+    src, ls = _read_rows(logits)
     if out is None:
         out = torch.empty(B, V, dtype=logits.dtype, device=dev)
     elif tuple(out.shape) != (B, V) or out.dtype != logits.dtype or (V > 1 and out.stride(1) != 1) or (
@@ -1574,9 +1586,11 @@ def process_logits(logits, tokens=None, lengths=None, *, prompt=None, repetition
         raise ValueError(f"{name}: out must be {logits.dtype} [B={B}, {V}] with contiguous rows")
     elif src.data_ptr() == logits.data_ptr() and not _apart(logits, out):
         raise ValueError(f"{name}: out overlaps logits in part")
+    (rep, rep_all), (freq, freq_all), (pres, pres_all) = held
+    r = _lib.SdmRtRules(*hist, _ptr(rep), _ptr(freq), _ptr(pres), rep_all, freq_all, pres_all, _ptr(bias), bs, _ptr(mask), ms)
     lib = _lib.load()
     with _on(dev):
-        _lib.check(lib.sdm_rt_process_logits(ctypes.byref(r), _ptr(src), ls, _DT[logits.dtype], B, V, _ptr(out),
+        _lib.check(lib.sdm_rt_process_logits(ctypes.byref(r), src.data_ptr(), ls, _DT[logits.dtype], B, V, out.data_ptr(),
                                              out.stride(0) if B > 1 else V, _stream(dev)), lib)
     return out
 
