@@ -25,92 +25,144 @@ struct RulesArgs {
   int64_t mask_stride;
 };
 
-// One workgroup per (row, slice of the vocabulary).  It counts the history's tokens that fall into its slice in LDS
-// (integer atomics: exact in any order), then passes over the slice once: in, rules, out.  Bit 31 of a counter says the
-// token was in the prompt, the rest counts its occurrences since.  A slice reads the row's whole history again, so
-// slices are as large as leaves every compute unit something to do (rules_slice).
-constexpr int kRulesThreads = 512;
+// One workgroup per (row, slice of the vocabulary): 512 threads, NP pieces of 16 bytes each.  The slice's logits and mask
+// words are loaded first; while they are on their way the workgroup counts the history's tokens that fall into the slice in
+// LDS (integer atomics: exact in any order); then rules, out.  Bit 31 of a counter says the token was in the prompt, the
+// rest counts its occurrences since.  Bound by memory, logits in and out, and by the history, which every slice of a row
+// reads again: so slices are as large as leaves every compute unit two workgroups, and a row's slices run on one XCD, whose
+// L2 then holds its history (workgroup i runs on XCD i mod 8).
+constexpr int kRulesThreads = 512, kXcds = 8;
 
-template <typename T>
-__global__ void __launch_bounds__(kRulesThreads) rules_kernel(RulesArgs a, int slice) {
-  extern __shared__ uint32_t cnt[];
-  constexpr int kN = Piece<T>::kN;
-  const int row = blockIdx.y;
-  const int v0 = blockIdx.x * slice;
-  const int nv = min(slice, a.vocab - v0);
+template <typename T, int NP>
+__global__ void __launch_bounds__(kRulesThreads) rules_kernel(RulesArgs a, int64_t rows, int slices) {
+  extern __shared__ uint4 lds[];
+  uint32_t* cnt = reinterpret_cast<uint32_t*>(lds);
+  constexpr int kN = Piece<T>::kN, kSlice = kRulesThreads * kN * NP;
+  const int64_t group = blockIdx.x / kXcds;
+  const int64_t row = group / slices * kXcds + blockIdx.x % kXcds;
+  if (row >= rows) return;   // whole workgroups
+  const int v0 = static_cast<int>(group % slices) * kSlice;
+  const int nv = min(kSlice, a.vocab - v0);
   const bool hist = a.tokens != nullptr;
+  const T* src = static_cast<const T*>(a.logits) + row * a.l_stride + v0;
+  const uint32_t* mask = a.mask ? a.mask + row * a.mask_stride + v0 / 32 : nullptr;   // slices are multiples of 32
+  Piece<T> p[NP];
+  uint32_t allowed[NP];
+#pragma unroll
+  for (int q = 0; q < NP; ++q) {
+    const int c = (q * kRulesThreads + static_cast<int>(threadIdx.x)) * kN;
+    allowed[q] = ~0u;
+    if (c + kN <= nv)
+      p[q].load(src + c);
+    else if (c < nv)
+      p[q].load_part(src + c, nv - c, T{});
+    if (mask && c < nv) allowed[q] = mask[c >> 5] >> (c & 31);   // a piece lies in one word
+  }
   if (hist) {
-    for (int i = threadIdx.x; i < slice; i += kRulesThreads) cnt[i] = 0;
-    __syncthreads();
+    for (int i = threadIdx.x; i < kSlice / 4; i += kRulesThreads) lds[i] = make_uint4(0, 0, 0, 0);
     const int64_t len = max(a.lengths[row], int64_t{0});
     const int64_t n = min(len, a.width);
     const int64_t prompt = a.prompt ? a.prompt[row] : 0;
     const int64_t* tk = a.tokens + row * a.t_stride;
     // the position of ring entry i: the latest one p < len with p mod width = i
     const int64_t last = len > a.width ? (len - 1) % a.width : len - 1;
-    for (int64_t i = threadIdx.x; i < n; i += kRulesThreads) {
-      const int64_t t = tk[i] - v0;
-      if (t < 0 || t >= nv) continue;
-      const int64_t pos = len - 1 - (i <= last ? last - i : last - i + a.width);
-      if (pos >= prompt)
-        atomicAdd(&cnt[t], 1u);
-      else
-        atomicOr(&cnt[t], 0x80000000u);
+    __syncthreads();
+    constexpr int kU = 8;   // tokens of a thread in flight
+    for (int64_t i0 = threadIdx.x; i0 < n; i0 += kU * kRulesThreads) {
+      int64_t t[kU];
+#pragma unroll
+      for (int u = 0; u < kU; ++u) t[u] = tk[min(i0 + u * kRulesThreads, n - 1)];
+#pragma unroll
+      for (int u = 0; u < kU; ++u) {
+        const int64_t i = i0 + u * kRulesThreads;
+        const uint64_t at = static_cast<uint64_t>(t[u]) - static_cast<uint64_t>(v0);   // below nv: in the slice
+        if (i < n && at < static_cast<uint64_t>(nv)) {
+          const int64_t pos = len - 1 - (i <= last ? last - i : last - i + a.width);
+          if (pos >= prompt)
+            atomicAdd(&cnt[at], 1u);
+          else
+            atomicOr(&cnt[at], 0x80000000u);
+        }
+      }
     }
     __syncthreads();
   }
-  const float rep = a.rep ? a.rep[row] : a.rep_all;
+  const float rep = a.rep ? a.rep[row] : a.rep_all, rep_inv = 1.f / rep;
   const float freq = a.freq ? a.freq[row] : a.freq_all;
   const float pres = a.pres ? a.pres[row] : a.pres_all;
-  const T* src = static_cast<const T*>(a.logits) + row * a.l_stride + v0;
   T* dst = static_cast<T*>(a.out) + row * a.o_stride + v0;
   const float* bias = a.bias ? a.bias + row * a.bias_stride + v0 : nullptr;
-  const uint32_t* mask = a.mask ? a.mask + row * a.mask_stride + v0 / 32 : nullptr;   // slices are multiples of 32
-  for (int c = static_cast<int>(threadIdx.x) * kN; c < nv; c += kRulesThreads * kN) {
+#pragma unroll
+  for (int q = 0; q < NP; ++q) {
+    const int c = (q * kRulesThreads + static_cast<int>(threadIdx.x)) * kN;
+    if (c >= nv) continue;
     const int live = min(kN, nv - c);
-    Piece<T> p;
-    if (live == kN)
-      p.load(src + c);
-    else
-      p.load_part(src + c, live, T{});
     float x[kN];
 #pragma unroll
-    for (int e = 0; e < kN; ++e) x[e] = p.get(e);
+    for (int e = 0; e < kN; ++e) x[e] = p[q].get(e);
     if (hist) {
+      uint32_t w[kN];
 #pragma unroll
-      for (int e = 0; e < kN; ++e) {
-        const uint32_t w = cnt[c + e];   // slices are multiples of kN
-        if (w) {
-          x[e] = x[e] > 0.f ? x[e] / rep : x[e] * rep;
-          const uint32_t k = w & 0x7fffffffu;
-          if (k) x[e] -= fmaf(static_cast<float>(k), freq, pres);
+      for (int e = 0; e < kN; e += 4) {
+        const uint4 u = lds[(c + e) / 4];
+        w[e] = u.x;
+        w[e + 1] = u.y;
+        w[e + 2] = u.z;
+        w[e + 3] = u.w;
+      }
+      uint32_t any = 0;
+#pragma unroll
+      for (int e = 0; e < kN; ++e) any |= w[e];
+      if (any) {
+#pragma unroll
+        for (int e = 0; e < kN; ++e) {
+          // x / rep: the product with the reciprocal, put right by its remainder (which is NaN for infinite x)
+          const float y0 = x[e] * rep_inv, y1 = fmaf(fmaf(-y0, rep, x[e]), rep_inv, y0);
+          const float y = x[e] > 0.f ? (y1 == y1 ? y1 : y0) : x[e] * rep;
+          const float k = static_cast<float>(w[e] & 0x7fffffffu);
+          const float z = k > 0.f ? y - fmaf(k, freq, pres) : y;
+          x[e] = w[e] ? z : x[e];
         }
       }
     }
     if (bias) {
+      if (live == kN) {
+        float b[kN];
+        __builtin_memcpy(b, bias + c, sizeof(b));
 #pragma unroll
-      for (int e = 0; e < kN; ++e)
-        if (e < live) x[e] += bias[c + e];
-    }
-    if (mask) {
-      const uint32_t w = mask[c >> 5] >> (c & 31);   // a piece lies in one word
+        for (int e = 0; e < kN; ++e) x[e] += b[e];
+      } else {
 #pragma unroll
-      for (int e = 0; e < kN; ++e)
-        if (!((w >> e) & 1)) x[e] = -INFINITY;
+        for (int e = 0; e < kN; ++e)
+          if (e < live) x[e] += bias[c + e];
+      }
     }
-    p.set(x);
+#pragma unroll
+    for (int e = 0; e < kN; ++e) x[e] = (allowed[q] >> e) & 1 ? x[e] : -INFINITY;
+    p[q].set(x);
     if (live == kN)
-      p.store(dst + c);
+      p[q].store(dst + c);
     else
-      p.store_part(dst + c, live);
+      p[q].store_part(dst + c, live);
   }
 }
 
-// the slice of the vocabulary of a workgroup
-inline int rules_slice(int64_t rows, int vocab, bool hist) {
-  int s = 2048;
-  while (s < 16384 && rows * ((vocab + 2 * s - 1) / (2 * s)) >= 512) s *= 2;
-  return s;
+template <typename T>
+void launch_rules(const RulesArgs& a, int64_t rows, hipStream_t st) {
+  constexpr int kPieces = kRulesThreads * Piece<T>::kN;
+  auto slices = [&](int np) { return (a.vocab + kPieces * np - 1) / (kPieces * np); };
+  const int64_t rows8 = (rows + kXcds - 1) / kXcds * kXcds;
+  auto launch = [&](auto np) {
+    constexpr int NP = decltype(np)::value;
+    hipLaunchKernelGGL((rules_kernel<T, NP>), dim3(static_cast<unsigned>(rows8 * slices(NP))), dim3(kRulesThreads),
+                       a.tokens ? static_cast<size_t>(kPieces) * NP * 4 : 0, st, a, rows, slices(NP));
+  };
+  if (rows * slices(4) >= 512)
+    launch(std::integral_constant<int, 4>{});
+  else if (rows * slices(2) >= 512)
+    launch(std::integral_constant<int, 2>{});
+  else
+    launch(std::integral_constant<int, 1>{});
 }
 
 // tokens[row][lengths[row] mod width] = new_ids[row], lengths[row] += 1
@@ -138,7 +190,7 @@ int sdm_rt_process_logits(const sdm_rt_rules* rules, const void* logits, int64_t
   if ((rc = check_dtype(dtype, "dtype"))) return rc;
   if (rows < 0 || vocab < 1) return set_err(SDM_RT_EINVAL, "rows must be >= 0 and vocab >= 1");
   if (rows > 65535) return set_err(SDM_RT_EUNSUPPORTED, "rows = %lld must be at most 65,535", (long long)rows);
-  if (vocab > (1 << 30)) return set_err(SDM_RT_EUNSUPPORTED, "vocab must be at most 2^30");
+  if (vocab > (1 << 21)) return set_err(SDM_RT_EUNSUPPORTED, "vocab must be at most 2^21");
   if (rows == 0) return SDM_RT_OK;
   if (!logits || !out) return set_err(SDM_RT_EINVAL, "logits and out must not be NULL");
   if (bad_read_stride(logits_row_stride, vocab) || out_row_stride < vocab)
@@ -173,14 +225,13 @@ int sdm_rt_process_logits(const sdm_rt_rules* rules, const void* logits, int64_t
   a.bias_stride = rules->bias_row_stride;
   a.mask = rules->mask;
   a.mask_stride = rules->mask_row_stride;
-  const int slice = rules_slice(rows, vocab, a.tokens != nullptr);
-  const dim3 grid(static_cast<unsigned>((vocab + slice - 1) / slice), static_cast<unsigned>(rows));
-  const size_t lds = a.tokens ? static_cast<size_t>(slice) * 4 : 0;
+  const int64_t groups = (rows + kXcds - 1) / kXcds * kXcds * ((vocab + 8191) / 8192);   // at most, in one launch
+  if (groups >= int64_t{1} << 23) return set_err(SDM_RT_EUNSUPPORTED, "too many rows of so large a vocabulary");
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (dtype == SDM_RT_BF16)
-    hipLaunchKernelGGL((rules_kernel<bf16_t>), grid, dim3(kRulesThreads), lds, st, a, slice);
+    launch_rules<bf16_t>(a, rows, st);
   else
-    hipLaunchKernelGGL((rules_kernel<float>), grid, dim3(kRulesThreads), lds, st, a, slice);
+    launch_rules<float>(a, rows, st);
   return check_launch("process_logits");
 }
 
