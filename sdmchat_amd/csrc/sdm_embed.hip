@@ -4,10 +4,11 @@
 namespace sdmrt {
 
 // out[n] = scale * table[ids[n]], rounded once.  A workgroup takes a run of whole rows and its threads their 16-byte
-// pieces in turn.  Bound by memory: the rows in, the rows out.
+// pieces in turn.  Bound by memory: the rows in, the rows out.  THROUGH: an output past kStreamBytes is stored past the
+// caches, which keep the table's frequent rows (131,072 tokens of rows of 2 KB: 90 -> 59 us, 268 MB out).
 constexpr int kEmbedPieces = 1024;   // pieces of a workgroup, about
 
-template <typename T>
+template <typename T, bool THROUGH>
 __global__ void __launch_bounds__(256) embed_kernel(const int64_t* __restrict__ ids, int64_t n, const T* __restrict__ table,
                                                     int64_t t_stride, int vocab, int d, float scale,
                                                     T* __restrict__ out, int64_t o_stride, int ppr, int rows) {
@@ -28,10 +29,12 @@ __global__ void __launch_bounds__(256) embed_kernel(const int64_t* __restrict__ 
 #pragma unroll
       for (int e = 0; e < kN; ++e) v[e] = p.get(e) * scale;
       p.set(v);
-      if (d >= kN)
-        p.store(dst);
-      else
+      if (d < kN)
         p.store_part(dst, d);
+      else if (THROUGH)
+        p.store_through(dst);
+      else
+        p.store(dst);
     }
   }
 }
@@ -112,10 +115,17 @@ __global__ void __launch_bounds__(kTile) embed_tiles_kernel(const int64_t* __res
       static_cast<uint32_t>(v >> kBucketBits) << 10 | threadIdx.x;
 }
 
+// The rows without a token are cleared here, between the two readings: the stores then drain while the workgroup goes on
+// (clearing them next to the sums, in workgroups of that kernel's size, ran at half the rate: 131,072 tokens of 131,072
+// rows of 2 KB, 46 us for 147 MB).
+constexpr int kTileBatch = 8;   // tiles of a wave whose tokens are loaded together
+
+template <typename T>
 __global__ void __launch_bounds__(1024) embed_order_kernel(const int32_t* __restrict__ bucket_at,
                                                            const uint32_t* __restrict__ packed, int tiles, int R,
                                                            int row_bits, int32_t* __restrict__ offsets,
-                                                           int32_t* __restrict__ order, int32_t* __restrict__ row_of) {
+                                                           int32_t* __restrict__ order, int32_t* __restrict__ row_of,
+                                                           int vocab, int d, T* __restrict__ d_table, int64_t dt_stride) {
   extern __shared__ int32_t cnt[];   // [waves][R]: tokens of a row in a wave's tiles, then where they go
   __shared__ int32_t red[16];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
@@ -128,16 +138,32 @@ __global__ void __launch_bounds__(1024) embed_order_kernel(const int32_t* __rest
   const int per = (tiles + waves - 1) / waves;
   const int t0 = min(tiles, wave * per), t1 = min(tiles, t0 + per);
   int32_t* mine = cnt + wave * R;
-  // 64 tiles at a time: lane l holds the run of tile tb + l
-  for (int tb = t0; tb < t1; tb += 64) {
-    const int tl = min(tb + lane, t1 - 1);
-    const int from = at[tl], to = at[tiles + tl];
-    for (int q = 0; q < min(64, t1 - tb); ++q) {
-      const int end = __shfl(to, q);
-      for (int j = __shfl(from, q) + lane; j < end; j += 64)
-        atomicAdd(&mine[packed[static_cast<int64_t>(tb + q) * kTile + j] >> 10], 1);
+  // a wave's tiles, kTileBatch at a time: lane q holds where the bucket's run of tile tb + q begins and ends
+  auto for_tokens = [&](auto use) {
+    for (int tb = t0; tb < t1; tb += kTileBatch) {
+      const int tl = min(tb + min(lane, kTileBatch - 1), t1 - 1);
+      const int from = at[tl], to = at[tiles + tl];
+      uint32_t e[kTileBatch];
+#pragma unroll
+      for (int q = 0; q < kTileBatch; ++q) {   // the first 64 tokens of every run, in flight together
+        const int tile = min(tb + q, t1 - 1);
+        e[q] = packed[static_cast<int64_t>(tile) * kTile + min(__shfl(from, q) + lane, kTile - 1)];
+      }
+#pragma unroll
+      for (int q = 0; q < kTileBatch; ++q) {
+        if (tb + q >= t1) continue;   // the same for the wave
+        const int begin = __shfl(from, q), end = __shfl(to, q);
+        use(tb + q, e[q], begin + lane < end);
+        for (int j = begin + 64; j < end; j += 64) {
+          const bool live = j + lane < end;
+          use(tb + q, live ? packed[static_cast<int64_t>(tb + q) * kTile + j + lane] : 0u, live);
+        }
+      }
     }
-  }
+  };
+  for_tokens([&](int, uint32_t e, bool live) {
+    if (live) atomicAdd(&mine[e >> 10], 1);
+  });
   below = wave_add(below);
   if (lane == 0) red[wave] = below;
   __syncthreads();
@@ -162,47 +188,59 @@ __global__ void __launch_bounds__(1024) embed_order_kernel(const int32_t* __rest
   for (int w = 0; w < wave; ++w) pos += red[w];
   for (int r = r0; r < r1; ++r) {
     offsets[b * R + r] = pos;
+    const int begin = pos;
     for (int w = 0; w < waves; ++w) {
       const int c = cnt[w * R + r];
       cnt[w * R + r] = pos;
       pos += c;
     }
+    if (pos == begin) cnt[r] = -1;   // wave 0's place of an empty row is not needed
   }
   if (b == kBuckets - 1 && threadIdx.x == blockDim.x - 1) offsets[kBuckets * R] = pos;   // rows past R count nothing
   __syncthreads();
-  for (int tb = t0; tb < t1; tb += 64) {
-    const int tl = min(tb + lane, t1 - 1);
-    const int from = at[tl], to = at[tiles + tl];
-    for (int q = 0; q < min(64, t1 - tb); ++q) {
-      const int begin = __shfl(from, q), end = __shfl(to, q);
-      for (int j0 = begin; j0 < end; j0 += 64) {
-        const bool live = j0 + lane < end;
-        const uint32_t e = live ? packed[static_cast<int64_t>(tb + q) * kTile + j0 + lane] : 0;
-        const int row = static_cast<int>(e >> 10);
-        const uint64_t group = same_lanes(__ballot(live), row, row_bits);
-        const int rank = __popcll(group & lanes_below(lane));
-        const int start = mine[row];
-        if (live) {
-          order[start + rank] = (tb + q) * kTile + static_cast<int>(e & 1023);
-          row_of[start + rank] = row << kBucketBits | b;
-          if (rank == 0) mine[row] = start + __popcll(group);
-        }
-      }
+  Piece<T> none;
+  none.r = make_uint4(0, 0, 0, 0);
+  constexpr int kN = Piece<T>::kN;
+  for (int r = wave; r < R; r += waves) {   // a wave per empty row
+    const int row = r * kBuckets + b;
+    if (row >= vocab || cnt[r] >= 0) continue;
+    T* dst = d_table + static_cast<int64_t>(row) * dt_stride;
+    for (int c = lane * kN; c < d; c += 64 * kN) {
+      if (c + kN <= d)
+        none.store(dst + c);
+      else
+        none.store_part(dst + c, d - c);
     }
   }
+  for_tokens([&](int tile, uint32_t e, bool live) {
+    const int row = live ? static_cast<int>(e >> 10) : 0;
+    const uint64_t group = same_lanes(__ballot(live), row, row_bits);
+    const int rank = __popcll(group & lanes_below(lane));
+    const int start = mine[row];
+    if (live) {
+      order[start + rank] = tile * kTile + static_cast<int>(e & 1023);
+      row_of[start + rank] = row << kBucketBits | b;
+      if (rank == 0) mine[row] = start + __popcll(group);
+    }
+  });
 }
 
 // The rows' sums.  The ordered tokens are cut into pieces of `len`; a group of LANES lanes sums a piece's runs of equal rows
-// in order, lane l columns 4l ... 4l + 3 of every 4 LANES.  A run that is its whole row is scaled and stored; one that
+// in order, lane l columns 4l ... 4l + 3 of its slice.  A run that is its whole row is scaled and stored; one that
 // crosses an edge of a workgroup's pieces leaves a float32 partial row: part[2 b] continues a row begun before workgroup b,
 // part[2 b + 1] begins one that goes on after it.  The work follows the tokens and not the rows: text repeats its tokens, and with a wave
 // per row the most frequent token's chain of loads was the kernel's time (16,384 tokens of 32,768 rows of 768, a Zipf
-// stream: 739 us).  The last workgroups clear the rows that have no token meanwhile.
+// stream: 739 us).
 template <typename T>
 struct Quad4 {   // four values of a row at any element alignment
   using Raw = typename std::conditional<sizeof(T) == 2, uint2, uint4>::type;
   Raw r;
   __device__ __forceinline__ void load(const T* p) { __builtin_memcpy(&r, p, sizeof(r)); }
+  __device__ __forceinline__ void load_through(const T* p) {
+    using W = typename std::conditional<sizeof(T) == 2, words2, words4>::type;
+    const W w = __builtin_nontemporal_load(reinterpret_cast<const W*>(p));
+    __builtin_memcpy(&r, &w, sizeof(r));
+  }
   __device__ __forceinline__ void load_part(const T* p, int n) {
     T v[4];
 #pragma unroll
@@ -246,12 +284,14 @@ struct RowsGrad {
   const int32_t* offsets;
   const int32_t* order;
   const int32_t* row_of;
-  float* part;        // [2 piece_blocks][pitch]
+  float* part;        // [2 blocks][pitch]
   int pitch;          // d rounded up to 4
+  int n_tokens;       // all of them, the padding's too
   int n_slots;        // 256 R
   int R, vocab, d;
+  int slices;         // workgroups on the columns of a row
   int len;            // a piece's tokens
-  int piece_blocks;   // the most workgroups of pieces there can be
+  int2* edge;         // [blocks] the row that leaves a workgroup and the last workgroup that has a part of it, or -1
   float scale;
   const void* dy;
   int64_t dy_stride;
@@ -259,197 +299,143 @@ struct RowsGrad {
   int64_t dt_stride;
 };
 
-constexpr int kZeroRows = 8;   // slots of a wave that clears rows
-
-template <typename T>
-__device__ __forceinline__ void clear_rows(const RowsGrad& a, int first) {
-  const int lane = threadIdx.x & 63;
-  const int mine = first + min(lane, kZeroRows);
-  const int off = mine <= a.n_slots ? a.offsets[mine] : -1;
-  for (int q = 0; q < kZeroRows; ++q) {
-    const int slot = first + q;
-    if (slot >= a.n_slots || __shfl(off, q) != __shfl(off, q + 1)) continue;
-    const int row = (slot % a.R) * kBuckets + slot / a.R;
-    if (row >= a.vocab) continue;
-    T* dst = static_cast<T*>(a.d_table) + static_cast<int64_t>(row) * a.dt_stride;
-    Piece<T> z;
-    z.r = make_uint4(0, 0, 0, 0);
-    constexpr int kN = Piece<T>::kN;
-    for (int c = lane * kN; c < a.d; c += 64 * kN) {
-      if (c + kN <= a.d)
-        z.store(dst + c);
-      else
-        z.store_part(dst + c, a.d - c);
-    }
-  }
-}
-
-// A workgroup of 256 threads takes 256 / LANES pieces side by side.  A group's cut runs go to LDS, head (a run begun before
-// its piece) and tail (one that goes on after it); a run cut inside the workgroup is then put together there by the group
-// it begins in, and only one that enters or leaves the workgroup becomes a partial row in memory: with a partial row for
-// every cut piece they were a sixth of the kernel's traffic and their join took as long again as the sums of 16,384
-// tokens (9.6 us).
-template <typename T, int LANES>
+// A workgroup of 256 threads takes 256 / LANES pieces side by side, and of their rows one slice of 4 LANES columns,
+// a lane four of them: the code that ends a run stands behind every row of a batch, and with a wave on 1,024
+// columns fetching it once each took a third of the kernel (16,384 tokens: 13 us).  A group's cut runs go to LDS, head (a run
+// begun before its piece) and tail (one that goes on after it); a run cut inside the workgroup is then put together there by
+// the group it begins in, and only one that enters or leaves the workgroup becomes a partial row in memory: with a
+// partial row for every cut piece they were a sixth of the kernel's traffic and their join took as long again as the sums
+// of 16,384 tokens (9.6 us).  THROUGH: gradients past kStreamBytes, each read once, are read past the caches (131,072 rows of
+// 2 KB: the backward 156 -> 125 us).
+template <typename T, int LANES, bool THROUGH>
 __global__ void __launch_bounds__(256) embed_rows_grad_kernel(RowsGrad a) {
-  constexpr int CS = 4, QS = 8;   // column steps held in registers; rows in flight
-  constexpr int kGroups = 256 / LANES, kCols = 4 * LANES * CS;
-  __shared__ float heads[kGroups][kCols];
-  __shared__ float tails[kGroups][kCols];
+  constexpr int QS = 16;   // rows in flight
+  constexpr int kGroups = 256 / LANES;
+  __shared__ float4 heads[kGroups][LANES];
+  __shared__ float4 tails[kGroups][LANES];
   __shared__ int through[kGroups];   // the group's head run goes on after its piece
-  if (static_cast<int>(blockIdx.x) >= a.piece_blocks) {
-    clear_rows<T>(a, ((blockIdx.x - a.piece_blocks) * 4 + (threadIdx.x >> 6)) * kZeroRows);
+  const int lane = threadIdx.x % LANES, mine = threadIdx.x / LANES;
+  const int block = blockIdx.x / a.slices, slice = blockIdx.x % a.slices;   // a row's slices side by side
+  const int group = static_cast<int>(threadIdx.x & 63) & ~(LANES - 1);
+  // one trip for everything the piece needs to know: lane l holds token l of the piece (len is at most LANES), the rows
+  // before and after it, and how many tokens there are (n_tokens but for the padding's; what lies past them is not used)
+  const int total = a.offsets[a.n_slots];
+  const int64_t block_begin = static_cast<int64_t>(block) * kGroups * a.len;
+  const int begin = static_cast<int>(min(block_begin + mine * a.len, static_cast<int64_t>(a.n_tokens)));
+  const int own_at = min(begin + min(lane, a.len - 1), a.n_tokens - 1);
+  const int tok = a.order[own_at], row = a.row_of[own_at];
+  const int row_before = a.row_of[max(begin - 1, 0)], row_after = a.row_of[min(begin + a.len, a.n_tokens - 1)];
+  const bool first_slice = slice == 0;
+  if (block_begin >= total) {   // whole workgroups
+    if (first_slice && threadIdx.x == 0) a.edge[block] = make_int2(-1, 0);
     return;
   }
-  const int lane = threadIdx.x % LANES, mine = threadIdx.x / LANES;
-  const int total = a.offsets[a.n_slots];
-  const int64_t block_begin = static_cast<int64_t>(blockIdx.x) * kGroups * a.len;
-  if (block_begin >= total) return;   // whole workgroups
-  const int begin = static_cast<int>(min(block_begin + mine * a.len, static_cast<int64_t>(total)));
-  const int n = min(a.len, total - begin);   // none for groups past the end
-  const int at0 = min(begin, total - 1);
-  const int before = begin > 0 ? a.row_of[begin - 1] : -1;
-  const int after = begin + n < total ? a.row_of[begin + n] : -1;
-  const int row0 = a.row_of[at0], row_last = a.row_of[min(begin + max(n, 1), total) - 1];
+  const int n = max(0, min(a.len, total - begin));   // none for groups past the end
+  const int before = begin > 0 && n > 0 ? row_before : -1;
+  const int after = begin + n < total ? row_after : -1;
+  const int row0 = __shfl(row, group), row_last = __shfl(row, group + max(n, 1) - 1);
   const bool head = n > 0 && row0 == before;               // its first run began before it
   const bool whole = head && row0 == row_last && row0 == after;   // and goes on after it
   const bool tail = n > 0 && row_last == after && !whole && !(head && row0 == row_last);   // its last begins here, goes on
   if (lane == 0) through[mine] = whole;
-  const bool narrow = a.d < 4;
-  const int group = static_cast<int>(threadIdx.x & 63) & ~(LANES - 1);
-  float* part = a.part + 2 * static_cast<int64_t>(blockIdx.x) * a.pitch;
-  for (int cb = 0; cb < a.d; cb += kCols) {
-    float acc[CS][4] = {};
-    int cur = row0;
-    bool first = true;   // the run of cur is the piece's first
-    auto store_row = [&](int row, const float (&x)[CS][4]) {
+  const int col = slice * 4 * LANES + 4 * lane, c = quad_column(col, a.d);
+  const bool live = col < a.d, narrow = a.d < 4;
+  auto store_row = [&](int to, float4 x) {
+    const float v[4] = {x.x * a.scale, x.y * a.scale, x.z * a.scale, x.w * a.scale};
+    Quad4<T> o;
+    if (live) o.store(static_cast<T*>(a.d_table) + static_cast<int64_t>(to) * a.dt_stride + c, v, a.d - c);
+  };
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  int cur = row0;
+  bool first = true;   // the run of cur is the piece's first
+  for (int i0 = 0; i0 < n; i0 += QS) {
+    Quad4<T> g[QS];
 #pragma unroll
-      for (int t = 0; t < CS; ++t) {
-        const int col = cb + 4 * LANES * t + 4 * lane, c = quad_column(col, a.d);
-        if (col >= a.d) continue;
-        float v[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = x[t][e] * a.scale;
-        Quad4<T> o;
-        o.store(static_cast<T*>(a.d_table) + static_cast<int64_t>(row) * a.dt_stride + c, v, a.d - c);
-      }
-    };
-    auto keep = [&](float* lds) {
-#pragma unroll
-      for (int t = 0; t < CS; ++t)
-        *reinterpret_cast<float4*>(lds + 4 * LANES * t + 4 * lane) = make_float4(acc[t][0], acc[t][1], acc[t][2], acc[t][3]);
-    };
-    auto flush = [&](bool last) {
-      if (first && head)
-        keep(heads[mine]);
-      else if (last && tail)
-        keep(tails[mine]);
+    for (int q = 0; q < QS; ++q) {
+      const T* src = static_cast<const T*>(a.dy) + __shfl(tok, group + min(i0 + q, n - 1)) * a.dy_stride;
+      if (narrow)
+        g[q].load_part(src, a.d);
+      else if (THROUGH)
+        g[q].load_through(src + c);
       else
-        store_row(cur, acc);
-#pragma unroll
-      for (int t = 0; t < CS; ++t)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[t][e] = 0.f;
-    };
-    if (n > 0) {
-      // lane q of a group's first QS holds token q of the batch; the next batch's are loaded ahead
-      int tok = a.order[begin + min(lane % QS, n - 1)], row = a.row_of[begin + min(lane % QS, n - 1)];
-      for (int i0 = 0; i0 < n; i0 += QS) {
-        Quad4<T> g[QS][CS];
-#pragma unroll
-        for (int q = 0; q < QS; ++q) {
-          const T* src = static_cast<const T*>(a.dy) + __shfl(tok, group + q) * a.dy_stride;
-#pragma unroll
-          for (int t = 0; t < CS; ++t) {
-            if (t > 0 && cb + 4 * LANES * t >= a.d) continue;   // the same for every lane
-            const int c = quad_column(cb + 4 * LANES * t + 4 * lane, a.d);
-            if (narrow)
-              g[q][t].load_part(src, a.d);
-            else
-              g[q][t].load(src + c);
-          }
-        }
-        const int rows = row;
-        const int nx = begin + min(i0 + QS + lane % QS, n - 1);
-        tok = a.order[nx];
-        row = a.row_of[nx];
-#pragma unroll
-        for (int q = 0; q < QS; ++q) {
-          const int r = __shfl(rows, group + q);
-          if (i0 + q < n) {   // past the piece's end nothing is added
-            if (r != cur) {
-              flush(false);
-              cur = r;
-              first = false;
-            }
-#pragma unroll
-            for (int t = 0; t < CS; ++t) {
-#pragma unroll
-              for (int e = 0; e < 4; ++e) acc[t][e] += g[q][t].get(e);
-            }
-          }
-        }
-      }
-      flush(true);
+        g[q].load(src + c);
     }
-    __syncthreads();
-    // the runs cut by the groups' edges: group 0 takes the one that enters the workgroup, every group the one it begins
-    const bool enters = mine == 0 && head;
-    if (enters || tail) {
-#pragma unroll 1
-      for (int which = enters ? 0 : 1; which < (tail ? 2 : 1); ++which) {
-        float x[CS][4];
-        const float* own = which ? tails[mine] : heads[0];
 #pragma unroll
-        for (int t = 0; t < CS; ++t) {
-          const float4 v = *reinterpret_cast<const float4*>(own + 4 * LANES * t + 4 * lane);
-          x[t][0] = v.x;
-          x[t][1] = v.y;
-          x[t][2] = v.z;
-          x[t][3] = v.w;
-        }
-        bool on = which ? true : through[0] != 0;   // the run goes on in group g
-        int g = which ? mine + 1 : 1;
-        for (; on && g < kGroups; ++g) {
-#pragma unroll
-          for (int t = 0; t < CS; ++t) {
-            const float4 v = *reinterpret_cast<const float4*>(heads[g] + 4 * LANES * t + 4 * lane);
-            x[t][0] += v.x;
-            x[t][1] += v.y;
-            x[t][2] += v.z;
-            x[t][3] += v.w;
-          }
-          on = through[g] != 0;
-        }
-        if (which && !on) {
-          store_row(row_last, x);   // begun and ended in this workgroup
-        } else {
-          float* dst = part + (which ? a.pitch : 0);
-#pragma unroll
-          for (int t = 0; t < CS; ++t) {
-            const int col = cb + 4 * LANES * t + 4 * lane;
-            if (col < a.d) __builtin_memcpy(dst + quad_column(col, a.d), x[t], 16);
-          }
-        }
+    for (int q = 0; q < QS; ++q) {
+      const int r = __shfl(row, group + min(i0 + q, n - 1));
+      if (r != cur) {
+        if (first && head)
+          heads[mine][lane] = acc;
+        else
+          store_row(cur, acc);
+        acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        cur = r;
+        first = false;
+      }
+      if (i0 + q < n) {   // past the piece's end nothing is added
+        acc.x += g[q].get(0);
+        acc.y += g[q].get(1);
+        acc.z += g[q].get(2);
+        acc.w += g[q].get(3);
       }
     }
-    __syncthreads();
+  }
+  if (n > 0) {
+    if (first && head)
+      heads[mine][lane] = acc;
+    else if (tail)
+      tails[mine][lane] = acc;
+    else
+      store_row(cur, acc);
+  }
+  __syncthreads();
+  // the runs cut by the groups' edges: group 0 takes the one that enters the workgroup, every group the one it begins
+  const bool enters = mine == 0 && head;
+  float* part = a.part + 2 * static_cast<int64_t>(block) * a.pitch;
+  auto join = [&](float4& x, int g, bool on) {   // adds the heads from group g while the run goes on; whether it leaves
+    for (; on && g < kGroups; ++g) {
+      const float4 v = heads[g][lane];
+      x.x += v.x;
+      x.y += v.y;
+      x.z += v.z;
+      x.w += v.w;
+      on = through[g] != 0;
+    }
+    return on;
+  };
+  if (enters) {
+    float4 x = heads[0][lane];
+    join(x, 1, through[0] != 0);
+    if (live) __builtin_memcpy(part + c, &x, 16);
+  }
+  bool leaves = false;
+  if (tail) {
+    float4 x = tails[mine][lane];
+    leaves = join(x, mine + 1, true);
+    if (!leaves)
+      store_row(row_last, x);   // begun and ended in this workgroup
+    else if (live)
+      __builtin_memcpy(part + a.pitch + c, &x, 16);
+  }
+  // the run that begins in this workgroup and leaves it, for the join: its row and the last workgroup it reaches
+  if (first_slice) {
+    if (leaves && lane == 0) {
+      const int slot = (row_last & (kBuckets - 1)) * a.R + (row_last >> kBucketBits);
+      a.edge[block] = make_int2(row_last, (a.offsets[slot + 1] - 1) / (kGroups * a.len));
+    }
+    if (!__syncthreads_or(leaves) && threadIdx.x == 0) a.edge[block] = make_int2(-1, 0);
   }
 }
 
-// The rows cut over several workgroups: one workgroup per edge between them adds the row that begins before this edge and is
-// cut first by it, its four quarters of 256 threads a quarter of the partial rows each, in order.
+// The rows cut over several workgroups: for each workgroup of the sums that one leaves, a workgroup adds that row's partial
+// rows, its four quarters of 256 threads a quarter of the partial rows each, in order.
 template <typename T>
-__global__ void __launch_bounds__(1024) embed_rows_join_kernel(RowsGrad a, int len) {
+__global__ void __launch_bounds__(1024) embed_rows_join_kernel(RowsGrad a) {
   __shared__ float4 red[3][256];
   const int s = blockIdx.x;
-  const int total = a.offsets[a.n_slots];
-  const int64_t edge = static_cast<int64_t>(s + 1) * len;
-  if (edge >= total) return;   // whole workgroups
-  const int row = a.row_of[edge];
-  if (a.row_of[edge - 1] != row) return;
-  if (s > 0 && a.row_of[edge - len - 1] == row) return;   // an earlier edge's
-  const int slot = (row & (kBuckets - 1)) * a.R + (row >> kBucketBits);
-  const int last = (a.offsets[slot + 1] - 1) / len;   // pieces s (its second partial row), s + 1 ... last (their first)
+  const int2 edge = a.edge[s];
+  if (edge.x < 0) return;   // whole workgroups
+  const int row = edge.x, last = edge.y;   // workgroups s (its second partial row), s + 1 ... last (their first)
   const int n = last - s + 1, quarter = threadIdx.x >> 8, per = (n + 3) / 4;
   const int p0 = s + min(n, quarter * per), p1 = s + min(n, (quarter + 1) * per);
   for (int cb = 0; cb < a.d; cb += 1024) {
@@ -498,7 +484,7 @@ __global__ void __launch_bounds__(1024) embed_rows_join_kernel(RowsGrad a, int l
 struct OrderPlan {
   int R, row_bits, waves, tiles;          // rows of a bucket, the bits of their numbers, waves that order them
   int lanes, len, block, blocks, pitch;   // lanes of a piece, its tokens, those of a workgroup, workgroups
-  size_t off_bucket, off_packed, off_order, off_row, off_part, total;
+  size_t off_bucket, off_packed, off_order, off_row, off_edge, off_part, total;
 };
 inline OrderPlan order_plan(int64_t n, int64_t vocab, int d) {
   OrderPlan p;
@@ -511,7 +497,7 @@ inline OrderPlan order_plan(int64_t n, int64_t vocab, int d) {
   // pieces of 16 tokens, two batches of rows in flight, for every SIMD; past 4,096 pieces longer ones, so that the partial
   // rows of a frequent token stay few
   p.len = 16;
-  while (p.len < 64 && n / p.len > 4096) p.len *= 2;
+  while (p.len < p.lanes && n / p.len > 4096) p.len *= 2;
   p.block = 256 / p.lanes * p.len;
   p.blocks = static_cast<int>((n + p.block - 1) / p.block);
   p.pitch = (d + 3) / 4 * 4;
@@ -526,6 +512,7 @@ inline OrderPlan order_plan(int64_t n, int64_t vocab, int d) {
   p.off_packed = take(static_cast<size_t>(p.tiles) * kTile * 4);
   p.off_order = take(static_cast<size_t>(n) * 4);
   p.off_row = take(static_cast<size_t>(n) * 4);
+  p.off_edge = take(static_cast<size_t>(p.blocks) * 8);
   p.off_part = take(2 * static_cast<size_t>(p.blocks) * p.pitch * 4);
   p.total = o;
   return p;
@@ -564,14 +551,18 @@ int sdm_rt_embed(const int64_t* ids, int64_t n, const void* table, int64_t table
   const int ppr = (d + kn - 1) / kn;
   const int rows = std::max(1, kEmbedPieces / ppr);
   const unsigned blocks = static_cast<unsigned>(std::min<int64_t>((n + rows - 1) / rows, 1 << 20));
-  if (dtype == SDM_RT_BF16)
-    hipLaunchKernelGGL((embed_kernel<bf16_t>), dim3(blocks), dim3(256), 0, st, ids, n, static_cast<const bf16_t*>(table),
-                       table_row_stride, static_cast<int>(vocab), d, scale, static_cast<bf16_t*>(out), out_row_stride, ppr,
-                       rows);
-  else
-    hipLaunchKernelGGL((embed_kernel<float>), dim3(blocks), dim3(256), 0, st, ids, n, static_cast<const float*>(table),
-                       table_row_stride, static_cast<int>(vocab), d, scale, static_cast<float*>(out), out_row_stride, ppr,
-                       rows);
+  const bool through = n * d * (dtype == SDM_RT_BF16 ? 2 : 4) > kStreamBytes;
+#define SDM_RT_EMBED(T, THROUGH)                                                                                            \
+  hipLaunchKernelGGL((embed_kernel<T, THROUGH>), dim3(blocks), dim3(256), 0, st, ids, n, static_cast<const T*>(table),      \
+                     table_row_stride, static_cast<int>(vocab), d, scale, static_cast<T*>(out), out_row_stride, ppr, rows)
+  if (dtype == SDM_RT_BF16) {
+    if (through) SDM_RT_EMBED(bf16_t, true);
+    else SDM_RT_EMBED(bf16_t, false);
+  } else {
+    if (through) SDM_RT_EMBED(float, true);
+    else SDM_RT_EMBED(float, false);
+  }
+#undef SDM_RT_EMBED
   return check_launch("embed");
 }
 
@@ -591,7 +582,8 @@ int sdm_rt_embed_backward(const int64_t* ids, int64_t n, const void* dy, int64_t
   if (workspace_bytes < p.total)
     return set_err(SDM_RT_ENOSPACE, "workspace of %zu bytes, %zu needed", workspace_bytes, p.total);
   hipStream_t st = static_cast<hipStream_t>(stream);
-  static const bool lds = allow_lds(reinterpret_cast<const void*>(embed_order_kernel));
+  static const bool lds = allow_lds(reinterpret_cast<const void*>(embed_order_kernel<bf16_t>)) &&
+                          allow_lds(reinterpret_cast<const void*>(embed_order_kernel<float>));
   if (!lds) return lds_err("embed_backward");
   char* ws = static_cast<char*>(workspace);
   int32_t* offsets = reinterpret_cast<int32_t*>(ws);
@@ -603,9 +595,17 @@ int sdm_rt_embed_backward(const int64_t* ids, int64_t n, const void* dy, int64_t
   if (p.tiles > 0)
     hipLaunchKernelGGL(embed_tiles_kernel, dim3(p.tiles), dim3(kTile), 0, st, ids, static_cast<int>(n),
                        static_cast<int>(vocab), pad, p.tiles, bucket_at, packed);
-  hipLaunchKernelGGL(embed_order_kernel, dim3(kBuckets), dim3(64 * p.waves), static_cast<size_t>(p.waves) * p.R * 4, st,
-                     bucket_at, packed, p.tiles, p.R, p.row_bits, offsets, order, row_of);
+  const size_t counters = static_cast<size_t>(p.waves) * p.R * 4;
+  if (dtype == SDM_RT_BF16)
+    hipLaunchKernelGGL((embed_order_kernel<bf16_t>), dim3(kBuckets), dim3(64 * p.waves), counters, st, bucket_at, packed,
+                       p.tiles, p.R, p.row_bits, offsets, order, row_of, static_cast<int>(vocab), d,
+                       static_cast<bf16_t*>(d_table), d_table_row_stride);
+  else
+    hipLaunchKernelGGL((embed_order_kernel<float>), dim3(kBuckets), dim3(64 * p.waves), counters, st, bucket_at, packed,
+                       p.tiles, p.R, p.row_bits, offsets, order, row_of, static_cast<int>(vocab), d,
+                       static_cast<float*>(d_table), d_table_row_stride);
   if ((rc = check_launch("embed_order"))) return rc;
+  if (n == 0) return SDM_RT_OK;
   RowsGrad a{};
   a.offsets = offsets;
   a.order = order;
@@ -617,30 +617,41 @@ int sdm_rt_embed_backward(const int64_t* ids, int64_t n, const void* dy, int64_t
   a.vocab = static_cast<int>(vocab);
   a.d = d;
   a.len = p.len;
-  a.piece_blocks = p.blocks;
+  a.n_tokens = static_cast<int>(n);
+  a.edge = reinterpret_cast<int2*>(ws + p.off_edge);
   a.scale = scale;
   a.dy = dy;
   a.dy_stride = dy_row_stride;
   a.d_table = d_table;
   a.dt_stride = d_table_row_stride;
-  const dim3 grid(static_cast<unsigned>(a.piece_blocks + (a.n_slots + 4 * kZeroRows - 1) / (4 * kZeroRows)));
+  a.slices = (d + 4 * p.lanes - 1) / (4 * p.lanes);
+  if (static_cast<int64_t>(p.blocks) * a.slices >= 1 << 24)
+    return set_err(SDM_RT_EUNSUPPORTED, "too many tokens of so wide rows for one launch");
+  const dim3 grid(static_cast<unsigned>(p.blocks * a.slices));
   const dim3 edges(static_cast<unsigned>(std::max(1, p.blocks - 1)));
-#define SDM_RT_ROWS_GRAD(T)                                                                          \
-  do {                                                                                               \
-    if (p.lanes == 16)                                                                                 \
-      hipLaunchKernelGGL((embed_rows_grad_kernel<T, 16>), grid, dim3(256), 0, st, a);                \
-    else if (p.lanes == 32)                                                                            \
-      hipLaunchKernelGGL((embed_rows_grad_kernel<T, 32>), grid, dim3(256), 0, st, a);                \
-    else                                                                                             \
-      hipLaunchKernelGGL((embed_rows_grad_kernel<T, 64>), grid, dim3(256), 0, st, a);                \
-    if (p.blocks > 1)                                                                                \
-      hipLaunchKernelGGL((embed_rows_join_kernel<T>), edges, dim3(1024), 0, st, a, p.block);         \
-  } while (0)
+  const bool through = n * d * (dtype == SDM_RT_BF16 ? 2 : 4) > kStreamBytes;
+  auto launch = [&](auto zero, auto lanes) {
+    using T = decltype(zero);
+    constexpr int LANES = decltype(lanes)::value;
+    if (through)
+      hipLaunchKernelGGL((embed_rows_grad_kernel<T, LANES, true>), grid, dim3(256), 0, st, a);
+    else
+      hipLaunchKernelGGL((embed_rows_grad_kernel<T, LANES, false>), grid, dim3(256), 0, st, a);
+  };
+  auto launch_type = [&](auto zero) {
+    using T = decltype(zero);
+    if (p.lanes == 16)
+      launch(zero, std::integral_constant<int, 16>{});
+    else if (p.lanes == 32)
+      launch(zero, std::integral_constant<int, 32>{});
+    else
+      launch(zero, std::integral_constant<int, 64>{});
+    if (p.blocks > 1) hipLaunchKernelGGL((embed_rows_join_kernel<T>), edges, dim3(1024), 0, st, a);
+  };
   if (dtype == SDM_RT_BF16)
-    SDM_RT_ROWS_GRAD(bf16_t);
+    launch_type(bf16_t{});
   else
-    SDM_RT_ROWS_GRAD(float);
-#undef SDM_RT_ROWS_GRAD
+    launch_type(float{});
   return check_launch("embed_rows_grad");
 }
 

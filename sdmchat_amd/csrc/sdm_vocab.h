@@ -5,6 +5,14 @@
 
 namespace sdmrt {
 
+// 8 and 16 bytes at any element's address, for loads and stores that leave the caches to others (nontemporal)
+typedef uint32_t words2 __attribute__((ext_vector_type(2), aligned(2)));
+typedef uint32_t words4 __attribute__((ext_vector_type(4), aligned(2)));
+
+// What passes once through a kernel and is larger than this does not stay in the 256 MB last-level cache until its next
+// reader anyway: then it should not drive out what the kernel reads again.
+constexpr int64_t kStreamBytes = int64_t{128} << 20;
+
 // 16 bytes of a row: kN values of T.  A row of an odd vocabulary starts at any multiple of its element's size; gfx950
 // loads and stores 16 bytes at any address, so full pieces take the same instruction wherever the row starts, and only
 // a row's last, partial piece goes value by value.
@@ -30,6 +38,10 @@ struct Piece {
     if constexpr (sizeof(T) == 2) asm volatile("" : "+v"(r.x), "+v"(r.y), "+v"(r.z), "+v"(r.w));
   }
   __device__ __forceinline__ void store(T* p) const { __builtin_memcpy(p, &r, 16); }
+  __device__ __forceinline__ void store_through(T* p) const {
+    const words4 w = {r.x, r.y, r.z, r.w};
+    __builtin_nontemporal_store(w, reinterpret_cast<words4*>(p));
+  }
   __device__ __forceinline__ void store_part(T* p, int n) const {
     T v[kN];
     __builtin_memcpy(v, &r, 16);
