@@ -1320,6 +1320,15 @@ def _embed(idx, table, scale):
     return out
 
 
+def _padding_row(name, padding_idx, vocab):
+    """A padding_idx, counted from the end where negative, as a row of the table."""
+    if padding_idx is None:
+        return None
+    if not -vocab <= padding_idx < vocab:
+        raise ValueError(f"{name}: padding_idx {padding_idx} is outside the table of {vocab} rows")
+    return padding_idx % vocab
+
+
 def embedding_backward(idx, dy, vocab, scale=1.0, padding_idx=None):
     """The gradient [vocab, d] (in dy's dtype) of embedding's table for dy [..., d], the gradient of its output: each
     row the scaled float32 sum over its tokens in their order (sdm_rt_embed_backward: deterministic), zeros for tokens that
@@ -1333,6 +1342,7 @@ def embedding_backward(idx, dy, vocab, scale=1.0, padding_idx=None):
         raise ValueError(f"embedding_backward: dy {tuple(dy.shape)} for ids {tuple(idx.shape)}")
     dev = dy.device
     _same_device("embedding_backward", dev, idx=idx)
+    padding_idx = _padding_row("embedding_backward", padding_idx, vocab)
     ids = _ids("embedding_backward", "idx", idx)
     dy2, stride = _read_rows(dy if dy.dim() == 2 else dy.reshape(-1, d))
     out = torch.empty(vocab, d, dtype=dy.dtype, device=dev)
@@ -1363,9 +1373,9 @@ class EmbeddingFunction(torch.autograd.Function):
         if not torch.is_grad_enabled():
             return None, embedding_backward(idx, dy, ctx.vocab, ctx.scale, ctx.pad), None, None
         ids = idx.reshape(-1).long().clamp(0, ctx.vocab - 1)
-        g = dy.reshape(ids.numel(), -1).float()
+        g = dy.reshape(ids.numel(), dy.shape[-1]).float()
         if ctx.pad is not None:
-            g = g * (ids != ctx.pad)[:, None]
+            g = g.masked_fill((ids == ctx.pad)[:, None], 0.0)
         dt = torch.zeros(ctx.vocab, g.shape[1], dtype=torch.float32, device=g.device).index_add(0, ids, g) * ctx.scale
         return None, dt.to(dy.dtype), None, None
 
@@ -1373,8 +1383,8 @@ class EmbeddingFunction(torch.autograd.Function):
 def embedding(idx, table, scale=1.0, padding_idx=None):
     """The scaled embedding lookup: scale * table[idx] (float32 product, rounded once to table's dtype), differentiable in
     table.  idx [...] int64 or int32, each in [0, vocab) (one outside is clamped into it, not reported); table [vocab, d]
-    float32 or bfloat16, any row stride.  Row padding_idx is read like any other and gets no gradient (F.embedding's).
-    The gradient is deterministic (embedding_backward)."""
+    float32 or bfloat16, any row stride, at most 2^21 rows.  Row padding_idx is read like any other and gets no gradient
+    (F.embedding's).  The gradient is deterministic (embedding_backward)."""
     if table.device.type != "cuda":
         raise RuntimeError("embedding needs ROCm device tensors")
     if table.dtype not in _DT:
@@ -1384,10 +1394,7 @@ def embedding(idx, table, scale=1.0, padding_idx=None):
     if idx.dtype not in (torch.int64, torch.int32):
         raise ValueError(f"embedding: idx must be int64 or int32, got {idx.dtype}")
     _same_device("embedding", table.device, idx=idx)
-    if padding_idx is not None:
-        if not -table.shape[0] <= padding_idx < table.shape[0]:
-            raise ValueError(f"embedding: padding_idx {padding_idx} is outside the table of {table.shape[0]} rows")
-        padding_idx %= table.shape[0]
+    padding_idx = _padding_row("embedding", padding_idx, table.shape[0])
     scale = float(scale)
     if torch.is_grad_enabled() and table.requires_grad:
         return EmbeddingFunction.apply(idx, table, scale, padding_idx)
@@ -1458,7 +1465,7 @@ def distill_loss(logits, top_ids, top_logits, *, temperature=1.0, labels=None, a
     shares add up) and top_logits [..., k], k at most 1,024; labels [...] int64 or int32 or None (ignore_index, or any id
     outside the vocabulary: no label).  Positions may lack either part, or both: those have loss 0 and gradient 0 whatever
     their logits hold.  reduction "mean" divides the sum by the number of positions with a target (0 if there is none),
-    "sum" does not, "none" gives float32 losses [...].  Differentiable in logits, once; the teacher gets no gradient.  With
+    "sum" does not, "none" gives float32 losses [...].  At most 2^21 positions.  Differentiable in logits, once; the teacher gets no gradient.  With
     autograd recording, "mean" and "sum" compute the gradient along with the loss, so it takes its memory from then on."""
     dev = logits.device
     if dev.type != "cuda":
@@ -1542,7 +1549,7 @@ def process_logits(logits, tokens=None, lengths=None, *, prompt=None, repetition
     stream's own tokens begin (0).  repetition, frequency, presence: numbers or [B] tensors.  bias [vocab] or [B, vocab]
     float32.  mask [ceil(vocab / 32)] or [B, ceil(vocab / 32)] int32 words (pack_mask); a row that allows nothing becomes
     -inf throughout.  Returns the logits in their dtype, in ``out`` if given (it may be logits itself; it must not overlap
-    them otherwise).  Inference only."""
+    them otherwise).  B at most 65,535, vocab at most 2^21.  Inference only."""
     name = "process_logits"
     if logits.device.type != "cuda":
         raise RuntimeError(f"{name} needs ROCm device tensors")

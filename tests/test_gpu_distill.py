@@ -106,6 +106,29 @@ def test_loss_and_gradient(N, V, K, tau, alpha, dtype):
     check(*make(N, V, K, dtype, N + V + K, labels=alpha < 1), tau, alpha)
 
 
+@pytest.mark.parametrize("N,V,K,dtype", [(530, 66001, 5, torch.bfloat16), (300, 100008, 70, torch.bfloat16),
+                                         (300, 34005, 20, torch.float32)])
+def test_rows_in_turn(N, V, K, dtype):
+    """More rows than compute units, each too long for several workgroups to a unit: a workgroup takes rows in turn, some of
+    them without a target and full of NaN."""
+    z, ids, top, lab = make(N, V, K, dtype, N)
+    gone = torch.rand(N, generator=torch.Generator().manual_seed(2)) < 0.2
+    gone[-3:] = True
+    ids[gone], lab[gone] = -1, -100
+    z[gone] = float("nan")
+    check(z, ids, top, lab, 2.0, 0.5)
+
+
+@pytest.mark.parametrize("K", [2, 63, 64, 65, 200, 1024])
+def test_repeated_ids(K):
+    """Ids that repeat, among few and many entries, with the label among them or not."""
+    z, ids, top, lab = make(24, 3001, K, torch.float32, K, empty=False)
+    ids[8:16, K // 2:] = ids[8:16, :K - K // 2]
+    ids[16:20] = 7
+    lab[::2] = ids[::2, 0]
+    check(z, ids, top, lab, 1.5, 0.5)
+
+
 @pytest.mark.parametrize("reduction", ["none", "sum", "mean"])
 @pytest.mark.parametrize("go", [1.0, 0.125, -3.3, 0.0])
 def test_reductions_and_outer_gradients(reduction, go):
@@ -141,7 +164,7 @@ def test_nothing_has_a_target():
     z0 = torch.zeros(0, 300, device="cuda", requires_grad=True)
     loss = core.distill_loss(z0, ids[:0].cuda(), top[:0].cuda(), labels=lab[:0].cuda(), alpha=0.5)
     loss.backward()
-    assert float(loss) == 0.0 and tuple(z0.grad.shape) == (0, 300)
+    assert float(loss.detach()) == 0.0 and tuple(z0.grad.shape) == (0, 300)
     assert tuple(core.distill_loss(z0, ids[:0].cuda(), top[:0].cuda(), reduction="none").shape) == (0,)
 
 

@@ -153,6 +153,47 @@ def test_twice_differentiable():
         assert float((a - b).abs().max()) <= 60 * U * float(b.abs().max())
 
 
+@pytest.mark.parametrize("again", [False, True])
+def test_nan_in_the_gradient_of_padding_is_not_read(again):
+    ids = torch.tensor([1, 2, 2, 0, 2], device="cuda")
+    table = torch.ones(4, 40, device="cuda", requires_grad=True)
+    dy = torch.ones(5, 40, device="cuda")
+    dy[[1, 2, 4]] = float("nan")
+    got, = torch.autograd.grad(core.embedding(ids, table, 1.0, padding_idx=2), table, dy, create_graph=again)
+    assert torch.equal(got.detach().cpu()[:, 0], torch.tensor([1.0, 1.0, 0.0, 0.0]))
+    assert torch.equal(core.embedding_backward(ids, dy, 4, padding_idx=-2), got.detach())
+
+
+@pytest.mark.parametrize("dtype,N,d", [(torch.bfloat16, 70001, 1024), (torch.float32, 66000, 514)])
+def test_streams_larger_than_the_caches(dtype, N, d):
+    """Outputs and gradients past 128 MiB take the kernels that pass the caches by."""
+    V = 3001
+    g = torch.Generator(device="cuda").manual_seed(4)
+    ids = torch.randint(0, V, (N,), generator=g, device="cuda")
+    ids[: N // 3] = 17
+    table = torch.randn(V, d, generator=g, device="cuda").to(dtype).requires_grad_(True)
+    dy = torch.randn(N, d, generator=g, device="cuda", dtype=dtype)
+    y = core.embedding(ids, table, 0.5)
+    assert torch.equal(y, (table.detach()[ids].float() * 0.5).to(dtype))
+    y.backward(dy)
+    want = torch.zeros(V, d, dtype=torch.float64, device="cuda").index_add_(0, ids, dy.double()) * 0.5
+    mag = torch.zeros_like(want).index_add_(0, ids, dy.double().abs()) * 0.5
+    c = torch.bincount(ids, minlength=V)[:, None]
+    half = torch.finfo(dtype).eps / 2
+    tol = (c + 2) * U * mag * (1 + half) + half * want.abs() + 1e-42
+    assert bool(((table.grad.double() - want).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("N", [255, 256, 257, 1023, 1024, 1025, 2049])
+@pytest.mark.parametrize("d", [64, 65, 128, 129, 256, 257])
+def test_sizes_around_tiles_and_slices(N, d):
+    g = torch.Generator().manual_seed(N * d)
+    for kind, V in (("zipf", 300), ("one", 9), ("bytes", 70000)):
+        ids = _ids(kind, N, V, g)
+        dy = torch.randn(N, d, generator=g)
+        _check_grad(core.embedding_backward(ids.cuda(), dy.cuda(), V, 1.0), ids, dy, V, 1.0)
+
+
 def test_refusals():
     table = torch.randn(10, 8, device="cuda")
     ids = torch.zeros(3, dtype=torch.long, device="cuda")
@@ -161,6 +202,8 @@ def test_refusals():
                        ((ids, table[:0]), "vocab")):
         with pytest.raises(ValueError, match=text):
             core.embedding(*args)
+    with pytest.raises(ValueError, match="padding_idx"):
+        core.embedding_backward(ids, table[:3], 10, padding_idx=10)
     with pytest.raises(ValueError, match="dy"):
         core.embedding_backward(ids, table, 10)
     with pytest.raises(ValueError, match="float32"):
