@@ -115,17 +115,12 @@ __global__ void __launch_bounds__(kTile) embed_tiles_kernel(const int64_t* __res
       static_cast<uint32_t>(v >> kBucketBits) << 10 | threadIdx.x;
 }
 
-// The rows without a token are cleared here, between the two readings: the stores then drain while the workgroup goes on
-// (clearing them next to the sums, in workgroups of that kernel's size, ran at half the rate: 131,072 tokens of 131,072
-// rows of 2 KB, 46 us for 147 MB).
 constexpr int kTileBatch = 8;   // tiles of a wave whose tokens are loaded together
 
-template <typename T>
 __global__ void __launch_bounds__(1024) embed_order_kernel(const int32_t* __restrict__ bucket_at,
                                                            const uint32_t* __restrict__ packed, int tiles, int R,
                                                            int row_bits, int32_t* __restrict__ offsets,
-                                                           int32_t* __restrict__ order, int32_t* __restrict__ row_of,
-                                                           int vocab, int d, T* __restrict__ d_table, int64_t dt_stride) {
+                                                           int32_t* __restrict__ order, int32_t* __restrict__ row_of) {
   extern __shared__ int32_t cnt[];   // [waves][R]: tokens of a row in a wave's tiles, then where they go
   __shared__ int32_t red[16];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
@@ -188,30 +183,14 @@ __global__ void __launch_bounds__(1024) embed_order_kernel(const int32_t* __rest
   for (int w = 0; w < wave; ++w) pos += red[w];
   for (int r = r0; r < r1; ++r) {
     offsets[b * R + r] = pos;
-    const int begin = pos;
     for (int w = 0; w < waves; ++w) {
       const int c = cnt[w * R + r];
       cnt[w * R + r] = pos;
       pos += c;
     }
-    if (pos == begin) cnt[r] = -1;   // wave 0's place of an empty row is not needed
   }
   if (b == kBuckets - 1 && threadIdx.x == blockDim.x - 1) offsets[kBuckets * R] = pos;   // rows past R count nothing
   __syncthreads();
-  Piece<T> none;
-  none.r = make_uint4(0, 0, 0, 0);
-  constexpr int kN = Piece<T>::kN;
-  for (int r = wave; r < R; r += waves) {   // a wave per empty row
-    const int row = r * kBuckets + b;
-    if (row >= vocab || cnt[r] >= 0) continue;
-    T* dst = d_table + static_cast<int64_t>(row) * dt_stride;
-    for (int c = lane * kN; c < d; c += 64 * kN) {
-      if (c + kN <= d)
-        none.store(dst + c);
-      else
-        none.store_part(dst + c, d - c);
-    }
-  }
   for_tokens([&](int tile, uint32_t e, bool live) {
     const int row = live ? static_cast<int>(e >> 10) : 0;
     const uint64_t group = same_lanes(__ballot(live), row, row_bits);
@@ -289,7 +268,7 @@ struct RowsGrad {
   int n_tokens;       // all of them, the padding's too
   int n_slots;        // 256 R
   int R, vocab, d;
-  int slices;         // workgroups on the columns of a row
+  int blocks, slices;   // workgroups on the pieces, on the columns of a row
   int len;            // a piece's tokens
   int2* edge;         // [blocks] the row that leaves a workgroup and the last workgroup that has a part of it, or -1
   float scale;
@@ -298,6 +277,31 @@ struct RowsGrad {
   void* d_table;
   int64_t dt_stride;
 };
+
+// Workgroups past the pieces' clear the rows without a token meanwhile, each wave those among kClearRows slots.
+constexpr int kClearRows = 8;
+
+template <typename T>
+__device__ __forceinline__ void clear_rows(const RowsGrad& a, int first) {
+  constexpr int kN = Piece<T>::kN;
+  const int lane = threadIdx.x & 63;
+  const int off = a.offsets[min(first + min(lane, kClearRows), a.n_slots)];
+  Piece<T> none;
+  none.r = make_uint4(0, 0, 0, 0);
+  for (int q = 0; q < kClearRows; ++q) {
+    const int slot = first + q;
+    if (slot >= a.n_slots || __shfl(off, q) != __shfl(off, q + 1)) continue;
+    const int row = slot % a.R * kBuckets + slot / a.R;
+    if (row >= a.vocab) continue;
+    T* dst = static_cast<T*>(a.d_table) + static_cast<int64_t>(row) * a.dt_stride;
+    for (int c = lane * kN; c < a.d; c += 64 * kN) {
+      if (c + kN <= a.d)
+        none.store(dst + c);
+      else
+        none.store_part(dst + c, a.d - c);
+    }
+  }
+}
 
 // A workgroup of 256 threads takes 256 / LANES pieces side by side, and of their rows one slice of 4 LANES columns,
 // a lane four of them: the code that ends a run stands behind every row of a batch, and with a wave on 1,024
@@ -315,6 +319,10 @@ __global__ void __launch_bounds__(256) embed_rows_grad_kernel(RowsGrad a) {
   __shared__ float4 tails[kGroups][LANES];
   __shared__ int through[kGroups];   // the group's head run goes on after its piece
   const int lane = threadIdx.x % LANES, mine = threadIdx.x / LANES;
+  if (static_cast<int>(blockIdx.x) >= a.blocks * a.slices) {
+    clear_rows<T>(a, ((blockIdx.x - a.blocks * a.slices) * 4 + (threadIdx.x >> 6)) * kClearRows);
+    return;
+  }
   const int block = blockIdx.x / a.slices, slice = blockIdx.x % a.slices;   // a row's slices side by side
   const int group = static_cast<int>(threadIdx.x & 63) & ~(LANES - 1);
   // one trip for everything the piece needs to know: lane l holds token l of the piece (len is at most LANES), the rows
@@ -582,8 +590,7 @@ int sdm_rt_embed_backward(const int64_t* ids, int64_t n, const void* dy, int64_t
   if (workspace_bytes < p.total)
     return set_err(SDM_RT_ENOSPACE, "workspace of %zu bytes, %zu needed", workspace_bytes, p.total);
   hipStream_t st = static_cast<hipStream_t>(stream);
-  static const bool lds = allow_lds(reinterpret_cast<const void*>(embed_order_kernel<bf16_t>)) &&
-                          allow_lds(reinterpret_cast<const void*>(embed_order_kernel<float>));
+  static const bool lds = allow_lds(reinterpret_cast<const void*>(embed_order_kernel));
   if (!lds) return lds_err("embed_backward");
   char* ws = static_cast<char*>(workspace);
   int32_t* offsets = reinterpret_cast<int32_t*>(ws);
@@ -595,17 +602,9 @@ int sdm_rt_embed_backward(const int64_t* ids, int64_t n, const void* dy, int64_t
   if (p.tiles > 0)
     hipLaunchKernelGGL(embed_tiles_kernel, dim3(p.tiles), dim3(kTile), 0, st, ids, static_cast<int>(n),
                        static_cast<int>(vocab), pad, p.tiles, bucket_at, packed);
-  const size_t counters = static_cast<size_t>(p.waves) * p.R * 4;
-  if (dtype == SDM_RT_BF16)
-    hipLaunchKernelGGL((embed_order_kernel<bf16_t>), dim3(kBuckets), dim3(64 * p.waves), counters, st, bucket_at, packed,
-                       p.tiles, p.R, p.row_bits, offsets, order, row_of, static_cast<int>(vocab), d,
-                       static_cast<bf16_t*>(d_table), d_table_row_stride);
-  else
-    hipLaunchKernelGGL((embed_order_kernel<float>), dim3(kBuckets), dim3(64 * p.waves), counters, st, bucket_at, packed,
-                       p.tiles, p.R, p.row_bits, offsets, order, row_of, static_cast<int>(vocab), d,
-                       static_cast<float*>(d_table), d_table_row_stride);
+  hipLaunchKernelGGL(embed_order_kernel, dim3(kBuckets), dim3(64 * p.waves), static_cast<size_t>(p.waves) * p.R * 4, st,
+                     bucket_at, packed, p.tiles, p.R, p.row_bits, offsets, order, row_of);
   if ((rc = check_launch("embed_order"))) return rc;
-  if (n == 0) return SDM_RT_OK;
   RowsGrad a{};
   a.offsets = offsets;
   a.order = order;
@@ -625,9 +624,11 @@ int sdm_rt_embed_backward(const int64_t* ids, int64_t n, const void* dy, int64_t
   a.d_table = d_table;
   a.dt_stride = d_table_row_stride;
   a.slices = (d + 4 * p.lanes - 1) / (4 * p.lanes);
-  if (static_cast<int64_t>(p.blocks) * a.slices >= 1 << 24)
+  a.blocks = p.blocks;
+  const int64_t groups = static_cast<int64_t>(p.blocks) * a.slices + (a.n_slots + 4 * kClearRows - 1) / (4 * kClearRows);
+  if (groups >= 1 << 24)
     return set_err(SDM_RT_EUNSUPPORTED, "too many tokens of so wide rows for one launch");
-  const dim3 grid(static_cast<unsigned>(p.blocks * a.slices));
+  const dim3 grid(static_cast<unsigned>(groups));
   const dim3 edges(static_cast<unsigned>(std::max(1, p.blocks - 1)));
   const bool through = n * d * (dtype == SDM_RT_BF16 ? 2 : 4) > kStreamBytes;
   auto launch = [&](auto zero, auto lanes) {
