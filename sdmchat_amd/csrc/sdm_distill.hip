@@ -36,22 +36,24 @@ __device__ __forceinline__ int has_label(const DistillArgs& a, int64_t r) {
 }
 
 // What a row aims at, found once: whether it has a teacher and whether that may repeat an id, its label or -1; counts[block]:
-// how many of the block's rows have either.  A wave takes four rows at a time.  Repeats are told by a table of 2^15 bits
+// how many of the block's rows have either.  A wave takes four rows at a time.  Repeats are told by a table of 2^14 bits
 // per row in LDS, each id one bit by its hash: an id that finds its bit set may be a repeat (of 32 distinct ids that happens
-// in 2 rows of 100, of 128 in 22), and only such rows compare their ids pair by pair.
+// in 3 rows of 100, of 128 in 39), and only such rows compare their ids pair by pair.
 struct Target {
   int flags;
   int label;
 };
 constexpr int kTaught = 1, kRepeats = 2;
-constexpr int kSeenBits = 15, kSeenWords = 1 << (kSeenBits - 5);
-constexpr int kTargetWaves = 4, kTargetRows = 4;
+constexpr int kSeenBits = 14, kSeenWords = 1 << (kSeenBits - 5);
+constexpr int kTargetWaves = 16, kTargetRows = 4;
+constexpr size_t kTargetLds = kTargetWaves * kTargetRows * kSeenWords * sizeof(uint32_t);   // 128 KiB
 
 __global__ void __launch_bounds__(64 * kTargetWaves) distill_targets_kernel(DistillArgs a, Target* __restrict__ targets,
                                                                             int* __restrict__ counts) {
-  __shared__ uint4 seen_all[kTargetWaves][kTargetRows][kSeenWords / 4];
+  extern __shared__ uint4 seen_lds[];
   __shared__ int red[kTargetWaves];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  uint4* seen_own = seen_lds + wave * (kTargetRows * kSeenWords / 4);
   const int64_t waves = static_cast<int64_t>(gridDim.x) * kTargetWaves;
   int n = 0;
   for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * kTargetWaves + wave; r0 < a.rows; r0 += waves * kTargetRows) {
@@ -63,7 +65,7 @@ __global__ void __launch_bounds__(64 * kTargetWaves) distill_targets_kernel(Dist
       label[q] = has_label(a, min(r0 + q * waves, a.rows - 1));
     }
     if (a.kd > 0.f && a.k > 0) {
-      for (int i = lane; i < kTargetRows * kSeenWords / 4; i += 64) seen_all[wave][0][i] = make_uint4(0, 0, 0, 0);
+      for (int i = lane; i < kTargetRows * kSeenWords / 4; i += 64) seen_own[i] = make_uint4(0, 0, 0, 0);
       for (int i0 = 0; i0 < a.k; i0 += 64) {
         const int i = min(i0 + lane, a.k - 1);
         int64_t id[kTargetRows];
@@ -80,7 +82,7 @@ __global__ void __launch_bounds__(64 * kTargetWaves) distill_targets_kernel(Dist
           any[q] |= live;
           if (live) {
             const uint32_t h = static_cast<uint32_t>(id[q]) * 2654435761u >> (32 - kSeenBits);
-            uint32_t* seen = reinterpret_cast<uint32_t*>(seen_all[wave][q]);
+            uint32_t* seen = reinterpret_cast<uint32_t*>(seen_own) + q * kSeenWords;
             twice[q] |= (atomicOr(&seen[h >> 5], 1u << (h & 31)) >> (h & 31)) & 1;
           }
         }
@@ -126,17 +128,6 @@ __device__ __forceinline__ float gradient_value(float x, float ct, float at, flo
   const float et = __builtin_amdgcn_exp2f(x * ct);
   if constexpr (S == kOneSum) return at * et;
   return fmaf(a1, second_exp<S>(et, x), at * et);
-}
-
-template <typename V>
-__device__ __forceinline__ V block_add(V v, V* red) {
-  v = wave_add(v);
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-  __syncthreads();
-  v = red[0];
-  for (int w = 1; w < static_cast<int>(blockDim.x >> 6); ++w) v += red[w];
-  __syncthreads();
-  return v;
 }
 
 // What a row's workgroup holds of its targets in LDS: k entries of the teacher and one of the label, their ids (-1: none),
@@ -437,25 +428,31 @@ __global__ void __launch_bounds__(NV > 8 ? kBigThreads : 1024, NV > 8 ? 3 : K ==
 // loss = the sum of the rows' losses (in float64, in a fixed order), divided by the rows with a target if `mean`
 __global__ void __launch_bounds__(1024) distill_sum_kernel(DistillArgs a, float* __restrict__ loss) {
   __shared__ double red[16];
-  __shared__ int redc[16];
-  int c = 0;
-  for (int i = threadIdx.x; i < a.n_counts; i += 1024) c += a.counts[i];
-  c = block_add(c, redc);   // a few hundred partial counts
+  __shared__ int red_count[16];
+  const int i0 = threadIdx.x;
+  int count = i0 < a.n_counts ? a.counts[i0] : 0;   // at most kCountBlocks of them
   double s = 0.0;
-  for (int64_t i0 = threadIdx.x; i0 < a.rows; i0 += 16 * 1024) {
+  for (int64_t i = i0; i < a.rows; i += 16 * 1024) {
     float v[16];
 #pragma unroll
-    for (int q = 0; q < 16; ++q) v[q] = i0 + q * 1024 < a.rows ? a.row_loss[i0 + q * 1024] : 0.f;
+    for (int q = 0; q < 16; ++q) v[q] = i + q * 1024 < a.rows ? a.row_loss[i + q * 1024] : 0.f;
 #pragma unroll
     for (int q = 0; q < 16; ++q) s += static_cast<double>(v[q]);
   }
 #pragma unroll
   for (int j = 32; j > 0; j >>= 1) s += __shfl_xor(s, j);
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+  count = wave_add(count);
+  if ((threadIdx.x & 63) == 0) {
+    red[threadIdx.x >> 6] = s;
+    red_count[threadIdx.x >> 6] = count;
+  }
   __syncthreads();
   if (threadIdx.x == 0) {
-    for (int w = 1; w < 16; ++w) s += red[w];
-    *loss = static_cast<float>(a.mean ? s / max(c, 1) : s);
+    for (int w = 1; w < 16; ++w) {
+      s += red[w];
+      count += red_count[w];
+    }
+    *loss = static_cast<float>(a.mean ? s / max(count, 1) : s);
   }
 }
 
@@ -511,7 +508,7 @@ __global__ void __launch_bounds__(kGradThreads) distill_grad_kernel(DistillArgs 
   }
 }
 
-constexpr int kCountBlocks = 512;   // two workgroups of the targets' LDS to a compute unit
+constexpr int kCountBlocks = 256;   // one workgroup of the targets' to a compute unit
 
 inline int fill_distill(const sdm_rt_distill* d, const void* logits, int64_t l_stride, sdm_rt_dtype dtype,
                         const int64_t* ids, int64_t i_stride, const float* top, int64_t t_stride, const int64_t* labels,
@@ -634,7 +631,9 @@ int sdm_rt_distill_loss(const sdm_rt_distill* dims, const void* logits, int64_t 
   a.counts = counts;
   a.n_counts = static_cast<int>(std::min<int64_t>(kCountBlocks, (a.rows + kTargetWaves - 1) / kTargetWaves));
   if (a.rows > 0) {
-    hipLaunchKernelGGL(distill_targets_kernel, dim3(a.n_counts), dim3(64 * kTargetWaves), 0, st, a, targets, counts);
+    static const bool lds = allow_lds(reinterpret_cast<const void*>(distill_targets_kernel));
+    if (!lds) return lds_err("distill_loss");
+    hipLaunchKernelGGL(distill_targets_kernel, dim3(a.n_counts), dim3(64 * kTargetWaves), kTargetLds, st, a, targets, counts);
     if (dtype == SDM_RT_BF16)
       launch_distill_rows<bf16_t>(a, targets, d_logits, d_logits_row_stride, st);
     else
