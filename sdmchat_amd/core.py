@@ -1312,7 +1312,7 @@ def _embed(idx, table, scale):
     dev = table.device
     ids = _ids("embedding", "idx", idx)
     tab, stride = _read_rows(table)
-    out = torch.empty(idx.shape + (d,), dtype=table.dtype, device=dev)
+    out = table.new_empty(idx.shape + (d,))
     lib = _lib.load()
     with _on(dev):
         _lib.check(lib.sdm_rt_embed(ids.data_ptr(), ids.numel(), tab.data_ptr(), stride, _DT[table.dtype], V, d, scale,
@@ -1340,20 +1340,24 @@ def embedding_backward(idx, dy, vocab, scale=1.0, padding_idx=None):
         raise ValueError(f"embedding_backward: dtype {dy.dtype} is not float32 or bfloat16")
     if dy.shape[:-1] != idx.shape:
         raise ValueError(f"embedding_backward: dy {tuple(dy.shape)} for ids {tuple(idx.shape)}")
-    dev = dy.device
-    _same_device("embedding_backward", dev, idx=idx)
+    _same_device("embedding_backward", dy.device, idx=idx)
     padding_idx = _padding_row("embedding_backward", padding_idx, vocab)
-    ids = _ids("embedding_backward", "idx", idx)
+    return _embed_backward(_ids("embedding_backward", "idx", idx), dy, vocab, float(scale),
+                           -1 if padding_idx is None else padding_idx)
+
+
+def _embed_backward(ids, dy, vocab, scale, pad):
+    d = dy.shape[-1]
+    dev = dy.device
     dy2, stride = _read_rows(dy if dy.dim() == 2 else dy.reshape(-1, d))
-    out = torch.empty(vocab, d, dtype=dy.dtype, device=dev)
+    out = dy.new_empty((vocab, d))
     lib = _lib.load()
     n = ids.numel()
     nbytes = lib.sdm_rt_embed_backward_workspace_bytes(n, vocab, d)   # 0 outside the limits: the call below reports why
     ws = torch.empty(nbytes or 16, dtype=torch.uint8, device=dev)
     with _on(dev):
-        _lib.check(lib.sdm_rt_embed_backward(ids.data_ptr(), n, dy2.data_ptr(), stride, _DT[dy.dtype], vocab, d, scale,
-                                             -1 if padding_idx is None else padding_idx, out.data_ptr(), d, ws.data_ptr(),
-                                             nbytes, _stream(dev)), lib)
+        _lib.check(lib.sdm_rt_embed_backward(ids.data_ptr(), n, dy2.data_ptr(), stride, _DT[dy.dtype], vocab, d, scale, pad,
+                                             out.data_ptr(), d, ws.data_ptr(), nbytes, _stream(dev)), lib)
     return out
 
 
@@ -1363,20 +1367,22 @@ class EmbeddingFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, idx, table, scale, padding_idx):
-        ctx.save_for_backward(idx)
-        ctx.vocab, ctx.scale, ctx.pad = table.shape[0], scale, padding_idx
-        return _embed(idx, table, scale)
+        ids = _ids("embedding", "idx", idx)
+        ctx.save_for_backward(ids)
+        ctx.call = (table.shape[0], scale, -1 if padding_idx is None else padding_idx)
+        return _embed(ids, table, scale)
 
     @staticmethod
     def backward(ctx, dy):
-        idx, = ctx.saved_tensors
+        ids, = ctx.saved_tensors
         if not torch.is_grad_enabled():
-            return None, embedding_backward(idx, dy, ctx.vocab, ctx.scale, ctx.pad), None, None
-        ids = idx.reshape(-1).long().clamp(0, ctx.vocab - 1)
+            return None, _embed_backward(ids, dy, *ctx.call), None, None
+        vocab, scale, pad = ctx.call
+        ids = ids.reshape(-1).clamp(0, vocab - 1)
         g = dy.reshape(ids.numel(), dy.shape[-1]).float()
-        if ctx.pad is not None:
-            g = g.masked_fill((ids == ctx.pad)[:, None], 0.0)
-        dt = torch.zeros(ctx.vocab, g.shape[1], dtype=torch.float32, device=g.device).index_add(0, ids, g) * ctx.scale
+        if pad >= 0:
+            g = g.masked_fill((ids == pad)[:, None], 0.0)
+        dt = torch.zeros(vocab, g.shape[1], dtype=torch.float32, device=g.device).index_add(0, ids, g) * scale
         return None, dt.to(dy.dtype), None, None
 
 
