@@ -151,8 +151,8 @@ __device__ __forceinline__ Entries entries_in(char* lds, int k) {
 inline size_t entries_bytes(int k) { return (static_cast<size_t>(k) + 1) * 16; }
 
 // One wave's part of it.  first_id, first_top: the lane's first entry, loaded by the caller (before the row, so that the
-// gathers below need not wait for it).  A label that the teacher names too has no entry of its own.  Returns the sum of the teacher's exponentials against their maximum, which t.q holds
-// the differences to.
+// gathers below need not wait for it).  A label that the teacher names too has no entry of its own.  Returns the sum of the
+// teacher's exponentials against their maximum, which t.q holds the differences to.
 template <typename T>
 __device__ __forceinline__ float load_entries(const DistillArgs& a, int64_t r, const T* z, bool taught, int label,
                                               int64_t first_id, float first_top, const Entries& t) {
@@ -200,20 +200,20 @@ __device__ __forceinline__ void sum_equal_ids(const DistillArgs& a, const Entrie
 }
 
 // The gradient at the entries' ids, put right after the pass over the row: base(z) less the shares (summed over equal ids)
-// and the label; a repeated id's lanes all write the same.  By the waves that wrote the pieces, each after its own stores, so that no wave waits for
-// another's: piece id / kN of a row was written by thread (id / kN) mod `threads`, a value past the last whole piece by
-// its own thread.
+// and the label; a repeated id's lanes all write the same.  By the waves that wrote the pieces, each after its own stores,
+// so that no wave waits for another's: the threads take the row's pieces in turn, beginning anew at first_end (where the
+// first chunk ends), and a thread each the values past the last whole piece.
 template <typename T, typename F>
 __device__ __forceinline__ void put_right(const DistillArgs& a, const Entries& t, const float* sums, int label, float kd,
-                                          float ce, T* dr, int threads, F base) {
+                                          float ce, T* dr, int threads, int first_end, F base) {
   constexpr int kN = Piece<T>::kN;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int whole = a.vocab / kN * kN;
-  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");   // the wave's stores are in memory
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");   // after the wave's stores
   __builtin_amdgcn_wave_barrier();
   for (int i = lane; i <= a.k; i += 64) {
     const int id = t.id[i];
-    const int owner = id < whole ? id / kN % threads : id - whole;
+    const int owner = id < whole ? (id < first_end ? id : id - first_end) / kN % threads : id - whole;
     if (id >= 0 && (owner >> 6) == wave)
       dr[id] = from_f32<T>(base(t.z[i]) - kd * sums[i] - (id == label ? ce : 0.f));
   }
@@ -221,10 +221,10 @@ __device__ __forceinline__ void put_right(const DistillArgs& a, const Entries& t
 
 // A row's loss and, with GRAD, its gradient for grad_out = 1, in one pass over the row by one workgroup.  A thread holds NV
 // 16-byte pieces of the row in registers, so it is read once, all loads at once; every wave takes its own maximum and sums
-// against it, and the workgroup joins them over LDS (one barrier that waits for stores); then the gradient comes from the
-// registers.  The first wave gathers the targets meanwhile and takes the loss.  Bound by memory, a row in and a row out:
-// what counts is that enough rows are under way on a compute unit while others wait for loads or stores (16,384 x 32,768
-// bf16, two sums: 8 waves to a SIMD by their registers 440 us, 6 waves 455, 5 waves 556; a copy of as many bytes 429).
+// against it, and the workgroup joins them over LDS; then the gradient comes from the registers, and no barrier waits for
+// stores.  The first wave gathers the targets meanwhile and takes the loss.  Bound by memory, a row in and a row out: what
+// counts is that enough rows are under way on a compute unit while others wait for loads or stores (16,384 x 32,768 bf16,
+// two sums: 8 waves to a SIMD by their registers 440 us, 6 waves 455, 5 waves 556; a copy of as many bytes 429).
 //   kOne   a workgroup per row, several to a compute unit
 //   kRoll  a workgroup holds a compute unit's registers: it takes rows in turn, and as a piece's gradient is stored its
 //          registers take the next row's piece, so loads and stores overlap all the same
@@ -297,7 +297,7 @@ __global__ void __launch_bounds__(NV > 8 ? kBigThreads : 1024, NV > 8 ? 3 : K ==
     const float z_tail = c_tail < a.vocab ? to_f32(z[c_tail]) : -INFINITY;
     if (GRAD && a.mean && wave == waves - 1) {   // the mean's divisor
       int count = 0;
-      #pragma unroll 8
+#pragma unroll 8
       for (int i = lane; i < a.n_counts; i += 64) count += a.counts[i];
       count = wave_add(count);
       if (lane == 0) shared_count = count;
@@ -419,7 +419,7 @@ __global__ void __launch_bounds__(NV > 8 ? kBigThreads : 1024, NV > 8 ? 3 : K ==
       sum_equal_ids(a, t);
       lds_barrier();
     }
-    put_right(a, t, repeats ? t.sum : t.q, target.label, kd, ce, dr, blockDim.x, value);
+    put_right(a, t, repeats ? t.sum : t.q, target.label, kd, ce, dr, blockDim.x, first_end, value);
     if (K != kRoll) return;
     lds_barrier();   // before the next row's entries
   }
@@ -503,7 +503,7 @@ __global__ void __launch_bounds__(kGradThreads) distill_grad_kernel(DistillArgs 
     lds_barrier();
     sum_equal_ids(a, t);
     lds_barrier();
-    put_right(a, t, t.sum, label, kd, ce, dr, kGradThreads, value);
+    put_right(a, t, t.sum, label, kd, ce, dr, kGradThreads, whole, value);
     lds_barrier();   // before the next row's entries
   }
 }

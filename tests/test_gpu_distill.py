@@ -119,6 +119,19 @@ def test_rows_in_turn(N, V, K, dtype):
     check(z, ids, top, lab, 2.0, 0.5)
 
 
+@pytest.mark.parametrize("V,dtype", [(98305, torch.float32), (200003, torch.bfloat16), (300001, torch.float32)])
+def test_many_targets_of_rows_in_chunks(V, dtype):
+    """Rows that pass in chunks, the first of them partial, with entries in all of them and around their edges."""
+    z, ids, top, lab = make(40, V, 1024, dtype, V, empty=False)
+    kn = 16 // z.element_size()
+    whole, chunk = V // kn * kn, 16 * 768 * kn
+    edges = torch.tensor([e + o for e in range(whole % chunk, V, chunk) for o in range(-kn, kn)] + [0, whole - 1, V - 1])
+    edges = edges[(edges >= 0) & (edges < V)].unique()
+    ids[:, :len(edges)] = edges
+    lab[:len(edges)] = edges[:len(lab)]
+    check(z, ids, top, lab, 2.0, 0.5)
+
+
 @pytest.mark.parametrize("K", [2, 63, 64, 65, 200, 1024])
 def test_repeated_ids(K):
     """Ids that repeat, among few and many entries, with the label among them or not."""
