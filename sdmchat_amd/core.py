@@ -1293,8 +1293,10 @@ def _apart(a, b):
     lo, hi = sorted(((a.data_ptr(), sa), (b.data_ptr(), sb)))
     if lo == hi or lo[0] + ((rows - 1) * lo[1] + width) * a.element_size() <= hi[0]:
         return True
+    if sa != sb or sa == 0:
+        return False
     shift = (hi[0] - lo[0]) // a.element_size() % sa
-    return sa == sb and width <= shift <= sa - width   # column blocks of one buffer
+    return width <= shift <= sa - width   # column blocks of one buffer
 
 
 def embedding_fits(idx, table):

@@ -125,6 +125,18 @@ def test_cpu_tensors_are_refused():
         core.append_tokens(torch.zeros(3, 8, dtype=torch.long), ids, ids)
 
 
+def test_apart():
+    """Which outputs share elements with their input in part."""
+    buf = torch.zeros(9, 24)
+    for a, b, want in ((buf, buf, True), (buf, torch.zeros(9, 24), True), (buf[:4], buf[4:8], True), (buf[:4], buf[1:5], False),
+                       (buf[:, :8], buf[:, 8:16], True), (buf[:, :8], buf[:, 16:], True), (buf[:, :8], buf[:, 7:15], False),
+                       (buf[0:1], buf[0:1], True), (buf[0:1, :8], buf[0:1, 4:12], False), (buf[:0], buf[:0], True),
+                       # one row repeated: before, at the beginning of, and inside the other
+                       (buf[:1].expand(4, 24), buf[1:5], True), (buf[:1].expand(4, 24), buf[:4], False),
+                       (buf[2:3].expand(4, 24), buf[:4], False)):
+        assert core._apart(a, b) is want and core._apart(b, a) is want
+
+
 @pytest.mark.parametrize("V", [1, 31, 32, 33, 100, 128])
 def test_pack_mask(V):
     allowed = torch.rand(3, V, generator=torch.Generator().manual_seed(V)) < 0.5
