@@ -1255,6 +1255,13 @@ def _on(device):
     return _HERE if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
 
 
+def _widths(name, **sizes):
+    """Sizes that the library takes in 32 bits and would otherwise see cut to them."""
+    for n, v in sizes.items():
+        if v >> 31:
+            raise ValueError(f"{name}: {n} = {v} is past the kernel's limits")
+
+
 def _same_device(name, device, **tensors):
     for n, t in tensors.items():
         if t is not None and t.device != device:
@@ -1343,6 +1350,7 @@ def embedding_backward(idx, dy, vocab, scale=1.0, padding_idx=None):
     if dy.shape[:-1] != idx.shape:
         raise ValueError(f"embedding_backward: dy {tuple(dy.shape)} for ids {tuple(idx.shape)}")
     _same_device("embedding_backward", dy.device, idx=idx)
+    _widths("embedding_backward", d=d)
     padding_idx = _padding_row("embedding_backward", padding_idx, vocab)
     return _embed_backward(_ids("embedding_backward", "idx", idx), dy, vocab, float(scale),
                            -1 if padding_idx is None else padding_idx)
@@ -1402,6 +1410,7 @@ def embedding(idx, table, scale=1.0, padding_idx=None):
     if idx.dtype not in (torch.int64, torch.int32):
         raise ValueError(f"embedding: idx must be int64 or int32, got {idx.dtype}")
     _same_device("embedding", table.device, idx=idx)
+    _widths("embedding", d=table.shape[1])
     padding_idx = _padding_row("embedding", padding_idx, table.shape[0])
     scale = float(scale)
     if torch.is_grad_enabled() and table.requires_grad:
@@ -1497,6 +1506,7 @@ def distill_loss(logits, top_ids, top_logits, *, temperature=1.0, labels=None, a
         raise ValueError("distill_loss: alpha below 1 needs labels")
     _same_device("distill_loss", dev, top_ids=top_ids, top_logits=top_logits, labels=labels)
     k = top_ids.shape[-1]
+    _widths("distill_loss", vocab=V, k=k)
     ids = _ids("distill_loss", "top_ids", top_ids)
     top = top_logits.detach() if top_logits.requires_grad else top_logits
     if top.dtype != torch.float32 or not top.is_contiguous():
@@ -1569,6 +1579,7 @@ def process_logits(logits, tokens=None, lengths=None, *, prompt=None, repetition
         raise RuntimeError(f"{name} is inference only: logits require a gradient")
     B, V = logits.shape
     dev = logits.device
+    _widths(name, vocab=V)
     _same_device(name, dev, tokens=tokens, lengths=lengths, prompt=prompt, bias=bias, mask=mask, out=out)
     held = [_per_row(name, w, v, B, dev) for w, v in (("repetition", repetition), ("frequency", frequency),
                                                       ("presence", presence))]

@@ -306,6 +306,16 @@ def test_refusals():
         core.distill_loss(z, ids.repeat(1, 300), top.repeat(1, 300))
 
 
+def test_widths_past_32_bits_are_refused():
+    """A vocabulary or a number of entries that 32 bits would cut to a small one is refused, not taken as that."""
+    wide = torch.zeros(1, 1, device="cuda").expand(2, 2 ** 32 + 1)
+    ids = torch.zeros(1, 1, dtype=torch.long, device="cuda")
+    with pytest.raises(ValueError, match="limits"):
+        core.distill_loss(wide, ids.expand(2, 3), torch.zeros(2, 3, device="cuda"))
+    with pytest.raises(ValueError, match="limits"):
+        core.distill_loss(torch.zeros(2, 9, device="cuda"), ids.expand(2, 2 ** 32 + 1), wide)
+
+
 @pytest.mark.parametrize("go", [1.0, 0.3])
 def test_captured_training_step_replays(go):
     z, ids, top, lab = (t.cuda() for t in make(70, 4099, 9, torch.bfloat16, 17))

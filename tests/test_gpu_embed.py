@@ -210,6 +210,16 @@ def test_refusals():
         core.embedding_backward(ids, table[:3].half(), 10)
 
 
+def test_widths_past_32_bits_are_refused():
+    """A width that 32 bits would cut to a small one is refused, not taken as that."""
+    wide = torch.zeros(1, 1, device="cuda").expand(3, 2 ** 32 + 1)
+    ids = torch.zeros(3, dtype=torch.long, device="cuda")
+    with pytest.raises(ValueError, match="limits"):
+        core.embedding(ids, wide)
+    with pytest.raises(ValueError, match="limits"):
+        core.embedding_backward(ids, wide, 4)
+
+
 def test_captured_training_step_replays():
     """Lookup and gradient in a captured graph, replayed on other tokens with eager work in between."""
     g = torch.Generator().manual_seed(5)

@@ -220,6 +220,11 @@ def test_refusals():
         core.append_tokens(a["tokens"].t().contiguous().t(), a["lengths"], a["lengths"])
 
 
+def test_a_vocabulary_past_32_bits_is_refused():
+    with pytest.raises(ValueError, match="limits"):
+        core.process_logits(torch.zeros(1, 1, device="cuda").expand(2, 2 ** 32 + 1))
+
+
 def test_append_tokens():
     B, width = 300, 5
     g = torch.Generator().manual_seed(11)
