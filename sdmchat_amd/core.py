@@ -1515,6 +1515,8 @@ def distill_loss(logits, top_ids, top_logits, *, temperature=1.0, labels=None, a
     n = lead.numel()
     dims = _lib.SdmRtDistill(n, V, k, temperature, alpha, ignore_index, _REDUCTION[reduction])
     rows = logits if len(shape) == 2 else logits.reshape(n, V)
+    if not torch.is_grad_enabled():
+        rows = rows.detach()   # no gradient along with the loss
     loss = DistillFunction.apply(rows, ids, top, lab, dims)
     return loss.reshape(lead) if reduction == "none" and len(shape) != 2 else loss
 

@@ -289,6 +289,18 @@ def test_no_gradient_asked_for():
     b.backward()
 
 
+def test_no_gradient_is_computed_where_none_is_recorded():
+    """Under no_grad logits that require a gradient cost no more memory than ones that do not."""
+    z, ids, top, lab = (t.cuda() for t in make(64, 32768, 5, torch.bfloat16, 18))
+    z.requires_grad_(True)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    with torch.no_grad():
+        core.distill_loss(z, ids, top, labels=lab, alpha=0.5)
+    assert torch.cuda.max_memory_allocated() - before < z.numel() * z.element_size()
+
+
 def test_refusals():
     z, ids, top, lab = (t.cuda() for t in make(6, 50, 4, torch.float32, 16))
     for args, kw, text in (((z.half(), ids, top), {}, "float32 or bfloat16"), ((z, ids[:5], top[:5]), {}, "top_ids"),
