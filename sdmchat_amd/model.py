@@ -311,6 +311,8 @@ class OneSdmLM(nn.Module):
         forward(idx, sequential=True) (track4_onesdm_models.py:534-555), with every mixer's memory carried in
         ``state`` (a ModelDecodeState, updated in place).  rules: a TokenRules of B streams; idx_t joins its history and
         the logits are returned with the rules applied.  Inference only."""
+        if rules is not None and rules.tokens.shape[0] != idx_t.shape[0]:
+            raise ValueError(f"OneSdmLM.step: rules of {rules.tokens.shape[0]} streams for {idx_t.shape[0]} tokens")
         reset = (idx_t == self.bos_id) if self.reset_at_bos else None
 
         def apply(kind, i, x, hx):
@@ -333,6 +335,7 @@ class OneSdmLM(nn.Module):
         if rules is None:
             return logits
         rules.append(idx_t)
+        logits = logits.detach()
         return rules.apply(logits, out=logits)
 
 

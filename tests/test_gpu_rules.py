@@ -278,6 +278,22 @@ def test_decode_loop_with_rules():
     assert rules.lengths.tolist() == [T + steps] * B and state.pos == T + steps
 
 
+def test_step_with_rules_of_another_batch_and_outside_no_grad():
+    """Rules of another batch are refused before the streams' state moves; a step does not need no_grad for them."""
+    m, B, V = _model(211), 3, 211
+    m.emb.weight.requires_grad_(True)
+    toks = torch.arange(B).cuda()
+    s1, s2 = m.decode_state(B, "cuda"), m.decode_state(B, "cuda")
+    r1, r2 = _rules(B, V), _rules(B, V)
+    with pytest.raises(ValueError, match="streams"):
+        m.step(toks, s1, _rules(B + 1, V))
+    assert s1.pos == 0
+    got = m.step(toks, s1, r1)
+    with torch.no_grad():
+        want = m.step(toks, s2, r2)
+    assert torch.equal(got, want) and not got.requires_grad
+
+
 @pytest.mark.parametrize("steps", [1, 3])
 def test_decode_graph_with_rules(steps):
     """The captured steps with rules equal the eager ones bit for bit, and read a mask that changes between replays."""
