@@ -66,6 +66,7 @@ __global__ void __launch_bounds__(64 * kTargetWaves) distill_targets_kernel(Dist
     }
     if (a.kd > 0.f && a.k > 0) {
       for (int i = lane; i < kTargetRows * kSeenWords / 4; i += 64) seen_own[i] = make_uint4(0, 0, 0, 0);
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");   // before the lanes' marks
       for (int i0 = 0; i0 < a.k; i0 += 64) {
         const int i = min(i0 + lane, a.k - 1);
         int64_t id[kTargetRows];

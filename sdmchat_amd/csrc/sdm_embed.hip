@@ -201,6 +201,7 @@ __global__ void __launch_bounds__(1024) embed_order_kernel(const int32_t* __rest
       row_of[start + rank] = row << kBucketBits | b;
       if (rank == 0) mine[row] = start + __popcll(group);
     }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");   // the next tokens' lanes read what these wrote
   });
 }
 
@@ -589,6 +590,10 @@ int sdm_rt_embed_backward(const int64_t* ids, int64_t n, const void* dy, int64_t
   if (!workspace) return set_err(SDM_RT_EINVAL, "workspace is NULL");
   if (workspace_bytes < p.total)
     return set_err(SDM_RT_ENOSPACE, "workspace of %zu bytes, %zu needed", workspace_bytes, p.total);
+  const int slices = (d + 4 * p.lanes - 1) / (4 * p.lanes);
+  const int64_t groups = static_cast<int64_t>(p.blocks) * slices + (p.R * kBuckets + 4 * kClearRows - 1) / (4 * kClearRows);
+  if (groups >= 1 << 24)
+    return set_err(SDM_RT_EUNSUPPORTED, "too many tokens of so wide rows for one launch");
   hipStream_t st = static_cast<hipStream_t>(stream);
   static const bool lds = allow_lds(reinterpret_cast<const void*>(embed_order_kernel));
   if (!lds) return lds_err("embed_backward");
@@ -623,11 +628,8 @@ int sdm_rt_embed_backward(const int64_t* ids, int64_t n, const void* dy, int64_t
   a.dy_stride = dy_row_stride;
   a.d_table = d_table;
   a.dt_stride = d_table_row_stride;
-  a.slices = (d + 4 * p.lanes - 1) / (4 * p.lanes);
+  a.slices = slices;
   a.blocks = p.blocks;
-  const int64_t groups = static_cast<int64_t>(p.blocks) * a.slices + (a.n_slots + 4 * kClearRows - 1) / (4 * kClearRows);
-  if (groups >= 1 << 24)
-    return set_err(SDM_RT_EUNSUPPORTED, "too many tokens of so wide rows for one launch");
   const dim3 grid(static_cast<unsigned>(groups));
   const dim3 edges(static_cast<unsigned>(std::max(1, p.blocks - 1)));
   const bool through = n * d * (dtype == SDM_RT_BF16 ? 2 : 4) > kStreamBytes;

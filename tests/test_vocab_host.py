@@ -41,6 +41,8 @@ def test_embed_backward_workspace():
     assert lib.sdm_rt_embed_backward_workspace_bytes(100, 0, 64) == 0
     _fails(lib.sdm_rt_embed_backward(P, 100, P, 64, 0, 1000, 64, 1.0, -1, P, 64, P, need - 1, None), -2, "needed")
     _fails(lib.sdm_rt_embed_backward(P, 100, P, 64, 0, 1000, 64, 1.0, -1, P, 64, None, need, None), -1, "workspace")
+    wide = 1 << 20
+    _fails(lib.sdm_rt_embed_backward(P, 1 << 27, P, wide, 0, 10, wide, 1.0, -1, P, wide, P, 1 << 60, None), -3, "one launch")
 
 
 def _distill(**over):
