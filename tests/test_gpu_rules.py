@@ -278,19 +278,22 @@ def test_decode_loop_with_rules():
     assert rules.lengths.tolist() == [T + steps] * B and state.pos == T + steps
 
 
-def test_step_with_rules_of_another_batch_and_outside_no_grad():
-    """Rules of another batch are refused before the streams' state moves; a step does not need no_grad for them."""
+def test_step_with_rules_of_another_batch_or_outside_no_grad():
+    """Rules of another batch are refused before the streams' state moves, and so is a step of the mixers outside no_grad;
+    a model without mixers steps there too, to logits without a gradient."""
     m, B, V = _model(211), 3, 211
-    m.emb.weight.requires_grad_(True)
     toks = torch.arange(B).cuda()
-    s1, s2 = m.decode_state(B, "cuda"), m.decode_state(B, "cuda")
-    r1, r2 = _rules(B, V), _rules(B, V)
-    with pytest.raises(ValueError, match="streams"):
-        m.step(toks, s1, _rules(B + 1, V))
-    assert s1.pos == 0
-    got = m.step(toks, s1, r1)
+    state, rules = m.decode_state(B, "cuda"), _rules(B, V)
+    with torch.no_grad(), pytest.raises(ValueError, match="streams"):
+        m.step(toks, state, _rules(B + 1, V))
+    with pytest.raises(RuntimeError, match="inference"):
+        m.step(toks, state, rules)
+    assert state.pos == 0 and rules.lengths.tolist() == [0] * B
+    torch.manual_seed(1)
+    m = OneSdmLM(V, d=64, layers=1, mlp_f=64, mem=False).cuda().eval()
+    got = m.step(toks, m.decode_state(B, "cuda"), rules)
     with torch.no_grad():
-        want = m.step(toks, s2, r2)
+        want = m.step(toks, m.decode_state(B, "cuda"), _rules(B, V))
     assert torch.equal(got, want) and not got.requires_grad
 
 
