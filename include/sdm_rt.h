@@ -530,7 +530,7 @@ typedef struct {
 } sdm_rt_rules;
 
 /* logits, out [rows][vocab] in dtype, each value rounded once; out may be logits itself.  At most 65,535 rows, a
- * vocabulary of 2^21, and fewer than 2^36 values (rows counted in eights, vocab in 8,192s). */
+ * vocabulary of 2^21, and fewer than 2^35 values (rows counted in eights, vocab in 8,192s). */
 int sdm_rt_process_logits(const sdm_rt_rules* rules, const void* logits, int64_t logits_row_stride, sdm_rt_dtype dtype,
                           int64_t rows, int32_t vocab, void* out, int64_t out_row_stride, void* stream);
 

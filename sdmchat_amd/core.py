@@ -1569,7 +1569,7 @@ def process_logits(logits, tokens=None, lengths=None, *, prompt=None, repetition
     stream's own tokens begin (0).  repetition, frequency, presence: numbers or [B] tensors.  bias [vocab] or [B, vocab]
     float32.  mask [ceil(vocab / 32)] or [B, ceil(vocab / 32)] int32 words (pack_mask); a row that allows nothing becomes
     -inf throughout.  Returns the logits in their dtype, in ``out`` if given (it may be logits itself; it must not overlap
-    them otherwise).  B at most 65,535, vocab at most 2^21, and fewer than 2^36 logits (B counted in eights, vocab in
+    them otherwise).  B at most 65,535, vocab at most 2^21, and fewer than 2^35 logits (B counted in eights, vocab in
     8,192s).  Inference only."""
     name = "process_logits"
     if logits.device.type != "cuda":

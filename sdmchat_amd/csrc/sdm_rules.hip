@@ -25,16 +25,19 @@ struct RulesArgs {
   int64_t mask_stride;
 };
 
-// One workgroup per (row, slice of the vocabulary): 512 threads, NP pieces of 16 bytes each.  The slice's logits and mask
+// One workgroup per (row, slice of the vocabulary): 1,024 threads, NP pieces of 16 bytes each.  The slice's logits and mask
 // words are loaded first; while they are on their way the workgroup counts the history's tokens that fall into the slice in
 // LDS (integer atomics: exact in any order); then rules, out.  Bit 31 of a counter says the token was in the prompt, the
 // rest counts its occurrences since.  Bound by memory, logits in and out, and by the history, which every slice of a row
 // reads again: so slices are as large as leaves every compute unit two workgroups, and a row's slices run on one XCD, whose
-// L2 then holds its history (workgroup i runs on XCD i mod 8).
-constexpr int kRulesThreads = 512, kXcds = 8;
+// L2 then holds its history (workgroup i runs on XCD i mod 8).  The loads of logits, those of the history and the counting
+// wait in turn, so every wave that fits is there to overlap them: 256 x 131,072 bf16 with histories of 8,192 take 36 us (a
+// copy of as many bytes 30), with slices of 512 threads x 4 pieces 40, and with 8 tokens of a thread in flight, whose
+// registers leave room for half the waves, 42.
+constexpr int kRulesThreads = 1024, kXcds = 8;
 
 template <typename T, int NP>
-__global__ void __launch_bounds__(kRulesThreads) rules_kernel(RulesArgs a, int64_t rows, int slices) {
+__global__ void __launch_bounds__(kRulesThreads, 8) rules_kernel(RulesArgs a, int64_t rows, int slices) {
   extern __shared__ uint4 lds[];
   uint32_t* cnt = reinterpret_cast<uint32_t*>(lds);
   constexpr int kN = Piece<T>::kN, kSlice = kRulesThreads * kN * NP;
@@ -67,7 +70,7 @@ __global__ void __launch_bounds__(kRulesThreads) rules_kernel(RulesArgs a, int64
     // the position of ring entry i: the latest one p < len with p mod width = i
     const int64_t last = len > a.width ? (len - 1) % a.width : len - 1;
     __syncthreads();
-    constexpr int kU = 8;   // tokens of a thread in flight
+    constexpr int kU = 4;   // tokens of a thread in flight
     for (int64_t i0 = threadIdx.x; i0 < n; i0 += kU * kRulesThreads) {
       int64_t t[kU];
 #pragma unroll
@@ -157,9 +160,7 @@ void launch_rules(const RulesArgs& a, int64_t rows, hipStream_t st) {
     hipLaunchKernelGGL((rules_kernel<T, NP>), dim3(static_cast<unsigned>(rows8 * slices(NP))), dim3(kRulesThreads),
                        a.tokens ? static_cast<size_t>(kPieces) * NP * 4 : 0, st, a, rows, slices(NP));
   };
-  if (rows * slices(4) >= 512)
-    launch(std::integral_constant<int, 4>{});
-  else if (rows * slices(2) >= 512)
+  if (rows * slices(2) >= 512)
     launch(std::integral_constant<int, 2>{});
   else
     launch(std::integral_constant<int, 1>{});
@@ -226,7 +227,7 @@ int sdm_rt_process_logits(const sdm_rt_rules* rules, const void* logits, int64_t
   a.mask = rules->mask;
   a.mask_stride = rules->mask_row_stride;
   const int64_t groups = (rows + kXcds - 1) / kXcds * kXcds * ((vocab + 8191) / 8192);   // at most, in one launch
-  if (groups >= int64_t{1} << 23) return set_err(SDM_RT_EUNSUPPORTED, "too many rows of so large a vocabulary");
+  if (groups >= int64_t{1} << 22) return set_err(SDM_RT_EUNSUPPORTED, "too many rows of so large a vocabulary");
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (dtype == SDM_RT_BF16)
     launch_rules<bf16_t>(a, rows, st);
