@@ -4,7 +4,6 @@ Tensors must live on a ROCm device.  Activations are [B, T, width] with unit str
 uniform row stride (a slice of a wider fused projection output is fine).  All work is queued on the current torch
 stream; nothing synchronises.
 """
-import contextlib
 import ctypes
 import math
 
@@ -1247,12 +1246,21 @@ class TableSdmFunction(torch.autograd.Function):
 
 # -- the vocabulary's ends: embedding, distillation loss, rules on logits ------------------------------------------
 
-_HERE = contextlib.nullcontext()
+# A training step's backward runs on a thread of torch's engine, where Python and the launches of a call take about twice
+# their time: these wrappers look up and build as little as they can.
+_current_device = getattr(torch._C, "_cuda_getDevice", None)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
-def _on(device):
-    """The device as the current one, for a launch on a tensor of another device than the current one."""
-    return _HERE if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
+def _launch(fn, index, *args):
+    """fn(*args, stream) on the current stream of GPU ``index``, with that GPU as the current one."""
+    if _current_device() == index:
+        rc = fn(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, _raw_stream(index))
+    if rc:
+        _lib.check(rc)
 
 
 def _widths(name, **sizes):
@@ -1280,6 +1288,8 @@ def _ids(name, what, t):
 def _read_rows(t2):
     """(rows, row stride in elements) of a 2-D tensor as the kernels that read any row stride and any element alignment
     take it: itself where the last dimension is contiguous, else a copy."""
+    if t2.is_contiguous():
+        return t2, t2.size(1)
     rows, width = t2.shape
     row, step = t2.stride()
     if step != 1 and width > 1:
@@ -1316,23 +1326,19 @@ def embedding_fits(idx, table):
             and idx.numel() <= 1 << 27)
 
 
-def _embed(idx, table, scale):
+def _embed(ids, table, scale):
     V, d = table.shape
-    dev = table.device
-    ids = _ids("embedding", "idx", idx)
     tab, stride = _read_rows(table)
-    out = table.new_empty(idx.shape + (d,))
-    lib = _lib.load()
-    with _on(dev):
-        _lib.check(lib.sdm_rt_embed(ids.data_ptr(), ids.numel(), tab.data_ptr(), stride, _DT[table.dtype], V, d, scale,
-                                    out.data_ptr(), d, _stream(dev)), lib)
+    out = table.new_empty(ids.shape + (d,))
+    _launch(_lib.load().sdm_rt_embed, table.get_device(), ids.data_ptr(), ids.numel(), tab.data_ptr(), stride,
+            _DT[table.dtype], V, d, scale, out.data_ptr(), d)
     return out
 
 
 def _padding_row(name, padding_idx, vocab):
-    """A padding_idx, counted from the end where negative, as a row of the table."""
+    """A padding_idx, counted from the end where negative, as a row of the table; -1 where there is none."""
     if padding_idx is None:
-        return None
+        return -1
     if not -vocab <= padding_idx < vocab:
         raise ValueError(f"{name}: padding_idx {padding_idx} is outside the table of {vocab} rows")
     return padding_idx % vocab
@@ -1351,35 +1357,33 @@ def embedding_backward(idx, dy, vocab, scale=1.0, padding_idx=None):
         raise ValueError(f"embedding_backward: dy {tuple(dy.shape)} for ids {tuple(idx.shape)}")
     _same_device("embedding_backward", dy.device, idx=idx)
     _widths("embedding_backward", d=d)
-    padding_idx = _padding_row("embedding_backward", padding_idx, vocab)
-    return _embed_backward(_ids("embedding_backward", "idx", idx), dy, vocab, float(scale),
-                           -1 if padding_idx is None else padding_idx)
+    return _embed_backward(_ids("embedding_backward", "idx", idx), dy, vocab, d, float(scale),
+                           _padding_row("embedding_backward", padding_idx, vocab))
 
 
-def _embed_backward(ids, dy, vocab, scale, pad):
-    d = dy.shape[-1]
-    dev = dy.device
-    dy2, stride = _read_rows(dy if dy.dim() == 2 else dy.reshape(-1, d))
+def _embed_backward(ids, dy, vocab, d, scale, pad):
+    if dy.is_contiguous():
+        stride = d
+    else:
+        dy, stride = _read_rows(dy if dy.dim() == 2 else dy.reshape(-1, d))
     out = dy.new_empty((vocab, d))
     lib = _lib.load()
     n = ids.numel()
     nbytes = lib.sdm_rt_embed_backward_workspace_bytes(n, vocab, d)   # 0 outside the limits: the call below reports why
-    ws = torch.empty(nbytes or 16, dtype=torch.uint8, device=dev)
-    with _on(dev):
-        _lib.check(lib.sdm_rt_embed_backward(ids.data_ptr(), n, dy2.data_ptr(), stride, _DT[dy.dtype], vocab, d, scale, pad,
-                                             out.data_ptr(), d, ws.data_ptr(), nbytes, _stream(dev)), lib)
+    ws = ids.new_empty(nbytes // 8 + 1)
+    _launch(lib.sdm_rt_embed_backward, dy.get_device(), ids.data_ptr(), n, dy.data_ptr(), stride, _DT[dy.dtype], vocab, d,
+            scale, pad, out.data_ptr(), d, ws.data_ptr(), nbytes)
     return out
 
 
 class EmbeddingFunction(torch.autograd.Function):
     """embedding() as an autograd function: the lookup kernel forward, embedding_backward backward, as torch ops where it is
-    to be differentiated again (create_graph).  apply(idx, table, scale, padding_idx) -> y."""
+    to be differentiated again (create_graph).  apply(ids contiguous int64, table, scale, padding row or -1) -> y."""
 
     @staticmethod
-    def forward(ctx, idx, table, scale, padding_idx):
-        ids = _ids("embedding", "idx", idx)
+    def forward(ctx, ids, table, scale, pad):
         ctx.save_for_backward(ids)
-        ctx.call = (table.shape[0], scale, -1 if padding_idx is None else padding_idx)
+        ctx.call = (*table.shape, scale, pad)
         return _embed(ids, table, scale)
 
     @staticmethod
@@ -1387,12 +1391,12 @@ class EmbeddingFunction(torch.autograd.Function):
         ids, = ctx.saved_tensors
         if not torch.is_grad_enabled():
             return None, _embed_backward(ids, dy, *ctx.call), None, None
-        vocab, scale, pad = ctx.call
+        vocab, d, scale, pad = ctx.call
         ids = ids.reshape(-1).clamp(0, vocab - 1)
-        g = dy.reshape(ids.numel(), dy.shape[-1]).float()
+        g = dy.reshape(ids.numel(), d).float()
         if pad >= 0:
             g = g.masked_fill((ids == pad)[:, None], 0.0)
-        dt = torch.zeros(vocab, g.shape[1], dtype=torch.float32, device=g.device).index_add(0, ids, g) * scale
+        dt = torch.zeros(vocab, d, dtype=torch.float32, device=g.device).index_add(0, ids, g) * scale
         return None, dt.to(dy.dtype), None, None
 
 
@@ -1401,21 +1405,22 @@ def embedding(idx, table, scale=1.0, padding_idx=None):
     table.  idx [...] int64 or int32, each in [0, vocab) (one outside is clamped into it, not reported); table [vocab, d]
     float32 or bfloat16, any row stride, at most 2^21 rows.  Row padding_idx is read like any other and gets no gradient
     (F.embedding's).  The gradient is deterministic (embedding_backward)."""
-    if table.device.type != "cuda":
+    dev, shape = table.device, table.shape
+    if dev.type != "cuda":
         raise RuntimeError("embedding needs ROCm device tensors")
     if table.dtype not in _DT:
         raise ValueError(f"embedding: dtype {table.dtype} is not float32 or bfloat16")
-    if table.dim() != 2 or 0 in table.shape:
-        raise ValueError(f"embedding: table must be [vocab, d], got {tuple(table.shape)}")
-    if idx.dtype not in (torch.int64, torch.int32):
-        raise ValueError(f"embedding: idx must be int64 or int32, got {idx.dtype}")
-    _same_device("embedding", table.device, idx=idx)
-    _widths("embedding", d=table.shape[1])
-    padding_idx = _padding_row("embedding", padding_idx, table.shape[0])
-    scale = float(scale)
-    if torch.is_grad_enabled() and table.requires_grad:
-        return EmbeddingFunction.apply(idx, table, scale, padding_idx)
-    return _embed(idx, table.detach(), scale)
+    if len(shape) != 2 or 0 in shape:
+        raise ValueError(f"embedding: table must be [vocab, d], got {tuple(shape)}")
+    ids = _ids("embedding", "idx", idx)
+    if ids.device != dev:
+        _same_device("embedding", dev, idx=idx)
+    if shape[1] >> 31:
+        _widths("embedding", d=shape[1])
+    pad = _padding_row("embedding", padding_idx, shape[0])
+    if table.requires_grad and torch.is_grad_enabled():
+        return EmbeddingFunction.apply(ids, table, float(scale), pad)
+    return _embed(ids, table, float(scale))
 
 
 _REDUCTION = {"none": _lib.SDM_RT_NONE, "mean": _lib.SDM_RT_MEAN, "sum": _lib.SDM_RT_SUM}
@@ -1430,24 +1435,22 @@ class DistillFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, logits, ids, top, labels, dims):
-        dev = logits.device
         z, zs = _read_rows(logits)
-        n, V, k, none = dims.rows, dims.vocab, dims.top_k, dims.reduction == _lib.SDM_RT_NONE
-        loss = torch.empty(n if none else (), dtype=torch.float32, device=dev)
+        n, V = z.shape
+        k, none, code, at = ids.size(-1), dims.reduction == _lib.SDM_RT_NONE, _DT[z.dtype], ctypes.byref(dims)
+        loss = top.new_empty((n,) if none else ())
         lib = _lib.load()
-        nbytes = lib.sdm_rt_distill_workspace_bytes(ctypes.byref(dims))
+        nbytes = lib.sdm_rt_distill_workspace_bytes(at)
         grad = ctx.needs_input_grad[0]
         # the rows' maxima and sums for the backward ([n, 4] float32), then the workspace
-        kept = 16 * n if grad else 0
-        buf = torch.empty(kept + nbytes, dtype=torch.uint8, device=dev)
-        dz = torch.empty(n, V, dtype=z.dtype, device=dev) if grad and not none else None
+        kept = 2 * n if grad else 0
+        buf = ids.new_empty(kept + nbytes // 8 + 1)
+        dz = z.new_empty((n, V)) if grad and not none else None
         stats = buf.data_ptr()
-        with _on(dev):
-            _lib.check(lib.sdm_rt_distill_loss(ctypes.byref(dims), z.data_ptr(), zs, _DT[z.dtype], _ptr(ids), k, _ptr(top), k,
-                                               _ptr(labels), loss.data_ptr(), stats if grad else None, _ptr(dz), V,
-                                               stats + kept, nbytes, _stream(dev)), lib)
+        _launch(lib.sdm_rt_distill_loss, z.get_device(), at, z.data_ptr(), zs, code, ids.data_ptr(), k, top.data_ptr(), k,
+                _ptr(labels), loss.data_ptr(), stats if grad else None, _ptr(dz), V, stats + 8 * kept, nbytes)
         if grad:
-            ctx.dims, ctx.dz = dims, dz
+            ctx.call, ctx.dz = (at, code, V, k), dz
             ctx.save_for_backward(z, ids, top, labels, buf)
         return loss
 
@@ -1455,19 +1458,15 @@ class DistillFunction(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dloss):
         z, ids, top, labels, stats = ctx.saved_tensors
-        z, zs = _read_rows(z)
-        dims, dz, dev = ctx.dims, ctx.dz, z.device
+        (at, code, V, k), dz = ctx.call, ctx.dz
         ctx.dz = None   # the caller's from here on
-        k, V = dims.top_k, dims.vocab
         unless_one = dz is not None
         if dz is None:
-            dz = torch.empty(z.shape, dtype=z.dtype, device=dev)
-        g = dloss if dloss.is_contiguous() else dloss.contiguous()
-        lib = _lib.load()
-        with _on(dev):
-            _lib.check(lib.sdm_rt_distill_grad(ctypes.byref(dims), z.data_ptr(), zs, _DT[z.dtype], _ptr(ids), k, _ptr(top), k,
-                                               _ptr(labels), stats.data_ptr(), g.data_ptr(), unless_one, dz.data_ptr(), V,
-                                               _stream(dev)), lib)
+            dz = z.new_empty(z.shape)
+        z, zs = _read_rows(z)
+        g = dloss.contiguous()
+        _launch(_lib.load().sdm_rt_distill_grad, z.get_device(), at, z.data_ptr(), zs, code, ids.data_ptr(), k, top.data_ptr(),
+                k, _ptr(labels), stats.data_ptr(), g.data_ptr(), unless_one, dz.data_ptr(), V)
         return dz, None, None, None, None
 
 
@@ -1504,9 +1503,11 @@ def distill_loss(logits, top_ids, top_logits, *, temperature=1.0, labels=None, a
         raise ValueError(f"distill_loss: reduction {reduction!r} is not 'none', 'mean' or 'sum'")
     if labels is None and alpha != 1.0:
         raise ValueError("distill_loss: alpha below 1 needs labels")
-    _same_device("distill_loss", dev, top_ids=top_ids, top_logits=top_logits, labels=labels)
-    k = top_ids.shape[-1]
-    _widths("distill_loss", vocab=V, k=k)
+    if top_ids.device != dev or top_logits.device != dev or (labels is not None and labels.device != dev):
+        _same_device("distill_loss", dev, top_ids=top_ids, top_logits=top_logits, labels=labels)
+    k = top_ids.size(-1)
+    if (V | k) >> 31:
+        _widths("distill_loss", vocab=V, k=k)
     ids = _ids("distill_loss", "top_ids", top_ids)
     top = top_logits.detach() if top_logits.requires_grad else top_logits
     if top.dtype != torch.float32 or not top.is_contiguous():
@@ -1617,10 +1618,8 @@ def process_logits(logits, tokens=None, lengths=None, *, prompt=None, repetition
         raise ValueError(f"{name}: out overlaps logits in part")
     (rep, rep_all), (freq, freq_all), (pres, pres_all) = held
     r = _lib.SdmRtRules(*hist, _ptr(rep), _ptr(freq), _ptr(pres), rep_all, freq_all, pres_all, _ptr(bias), bs, _ptr(mask), ms)
-    lib = _lib.load()
-    with _on(dev):
-        _lib.check(lib.sdm_rt_process_logits(ctypes.byref(r), src.data_ptr(), ls, _DT[logits.dtype], B, V, out.data_ptr(),
-                                             out.stride(0) if B > 1 else V, _stream(dev)), lib)
+    _launch(_lib.load().sdm_rt_process_logits, out.get_device(), ctypes.byref(r), src.data_ptr(), ls, _DT[logits.dtype], B, V,
+            out.data_ptr(), out.stride(0) if B > 1 else V)
     return out
 
 
@@ -1639,7 +1638,5 @@ def append_tokens(tokens, lengths, new):
     if (width > 1 and tokens.stride(1) != 1) or (B > 1 and tokens.stride(0) < width) or not lengths.is_contiguous():
         raise ValueError("append_tokens: tokens must have contiguous rows, lengths must be contiguous")
     new = new.contiguous()
-    lib = _lib.load()
-    with _on(tokens.device):
-        _lib.check(lib.sdm_rt_append_tokens(_ptr(tokens), tokens.stride(0) if B > 1 else width, width, _ptr(lengths),
-                                            _ptr(new), B, _stream(tokens.device)), lib)
+    _launch(_lib.load().sdm_rt_append_tokens, tokens.get_device(), tokens.data_ptr(), tokens.stride(0) if B > 1 else width,
+            width, lengths.data_ptr(), new.data_ptr(), B)
