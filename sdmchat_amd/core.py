@@ -1455,8 +1455,12 @@ class DistillFunction(torch.autograd.Function):
         return loss
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dloss):
+        # once_differentiable alone takes 4 us, which a backward that is not recorded need not pay
+        return (_distill_backward_recorded if torch.is_grad_enabled() else DistillFunction.gradients)(ctx, dloss)
+
+    @staticmethod
+    def gradients(ctx, dloss):
         z, ids, top, labels, stats = ctx.saved_tensors
         (at, code, V, k), dz = ctx.call, ctx.dz
         ctx.dz = None   # the caller's from here on
@@ -1468,6 +1472,9 @@ class DistillFunction(torch.autograd.Function):
         _launch(_lib.load().sdm_rt_distill_grad, z.get_device(), at, z.data_ptr(), zs, code, ids.data_ptr(), k, top.data_ptr(),
                 k, _ptr(labels), stats.data_ptr(), g.data_ptr(), unless_one, dz.data_ptr(), V)
         return dz, None, None, None, None
+
+
+_distill_backward_recorded = once_differentiable(DistillFunction.gradients)
 
 
 def distill_loss(logits, top_ids, top_logits, *, temperature=1.0, labels=None, alpha=1.0, ignore_index=-100,
