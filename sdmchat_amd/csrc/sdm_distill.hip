@@ -21,7 +21,7 @@ struct DistillArgs {
   const int* counts;    // partial counts of those rows
   int n_counts;
   float* row_loss;
-  float4* stats;        // per row: maximum, 1 / sum at the temperature, 1 / sum at 1, the row's weight
+  float4* stats;        // per row: maximum (or near it), 1 / sum at the temperature, 1 / sum at 1, the row's weight
 };
 
 // a row has a teacher: an entry in the vocabulary whose logit over the temperature is not -inf; a label: one in the
@@ -36,15 +36,16 @@ __device__ __forceinline__ int has_label(const DistillArgs& a, int64_t r) {
 }
 
 // What a row aims at, found once: whether it has a teacher and whether that may repeat an id, its label or -1; counts[block]:
-// how many of the block's rows have either.  A wave takes four rows at a time.  Repeats are told by a table of 2^14 bits
-// per row in LDS, each id one bit by its hash: an id that finds its bit set may be a repeat (of 32 distinct ids that happens
-// in 3 rows of 100, of 128 in 39), and only such rows compare their ids pair by pair.
+// how many of the block's rows have either.  A wave takes four rows at a time.  Repeats are told by a table of 512 words
+// per row in LDS: an id's hash picks a word and three of its bits, and one that finds them set may be a repeat (of 100
+// distinct ids that happens in 1 row of 100; with one bit of 2^14 it was 1 of 4).  Only such rows compare their ids pair by
+// pair, which they pay for at their end (512 x 151,936 with 100 entries: 96 us, now 90).
 struct Target {
   int flags;
   int label;
 };
 constexpr int kTaught = 1, kRepeats = 2;
-constexpr int kSeenBits = 14, kSeenWords = 1 << (kSeenBits - 5);
+constexpr int kSeenBits = 9, kSeenWords = 1 << kSeenBits;
 constexpr int kTargetWaves = 16, kTargetRows = 4;
 constexpr size_t kTargetLds = kTargetWaves * kTargetRows * kSeenWords * sizeof(uint32_t);   // 128 KiB
 
@@ -82,9 +83,10 @@ __global__ void __launch_bounds__(64 * kTargetWaves) distill_targets_kernel(Dist
           const bool live = i0 + lane < a.k && teacher_entry(id[q], t[q] * a.inv_tau, a.vocab);
           any[q] |= live;
           if (live) {
-            const uint32_t h = static_cast<uint32_t>(id[q]) * 2654435761u >> (32 - kSeenBits);
+            const uint32_t h = static_cast<uint32_t>(id[q]) * 2654435761u;
+            const uint32_t bits = 1u << (h >> 18 & 31) | 1u << (h >> 13 & 31) | 1u << (h >> 8 & 31);
             uint32_t* seen = reinterpret_cast<uint32_t*>(seen_own) + q * kSeenWords;
-            twice[q] |= (atomicOr(&seen[h >> 5], 1u << (h & 31)) >> (h & 31)) & 1;
+            twice[q] |= (bits & ~atomicOr(&seen[h >> (32 - kSeenBits)], bits)) == 0;
           }
         }
       }
@@ -229,8 +231,9 @@ __device__ __forceinline__ void put_right(const DistillArgs& a, const Entries& t
 //   kOne   a workgroup per row, several to a compute unit
 //   kRoll  a workgroup holds a compute unit's registers: it takes rows in turn, and as a piece's gradient is stored its
 //          registers take the next row's piece, so loads and stores overlap all the same
-//   kMulti rows past 1,024 threads of 20 pieces, or without a gradient, go by in chunks, with running maxima and sums; the
-//          last chunk stays in registers, the others are read again for the gradient
+//   kMulti longer rows, or rows without a gradient, go by in chunks, with running references and sums, piece after piece as
+//          they arrive (100 x 300,001: 104 us with a chunk's maximum first, now 73; of no use to a row held whole); the last
+//          chunk stays in registers, the others are read again for the gradient
 enum Kind { kOne, kRoll, kMulti };
 constexpr int kBigThreads = 768;   // 12 waves: 168 registers a thread
 
@@ -250,6 +253,7 @@ __global__ void __launch_bounds__(NV > 8 ? kBigThreads : 1024, NV > 8 ? 3 : K ==
   const int whole = a.vocab / kN * kN;
   const int c_tail = whole + static_cast<int>(threadIdx.x);   // the values past the last whole piece: a thread each
   const float ct = a.kd > 0.f ? a.inv_tau * kLog2e : kLog2e;
+  const float slack = 16.f / fmaxf(ct, kLog2e);   // kMulti: a factor of up to 2^16 in the sums
   const Entries t = entries_in(lds, a.k);
   // chunks of a row, the first of them the partial one
   const int n_chunks = K == kMulti ? max((whole + chunk - 1) / chunk, 1) : 1;
@@ -307,29 +311,36 @@ __global__ void __launch_bounds__(NV > 8 ? kBigThreads : 1024, NV > 8 ? 3 : K ==
       const float ts = load_entries(a, r, z, taught, target.label, first_id, first_top, t);
       if (lane == 0) shared_ts = ts;
     }
-    float m = -INFINITY, st = 0.f, s1 = 0.f;
-    for (int q = 0;;) {
-      float mm = q == 0 ? z_tail : m;
+    float m = z_tail, st, s1 = 0.f;
+    if (K != kMulti) {
 #pragma unroll
       for (int v = 0; v < NV; ++v)
 #pragma unroll
-        for (int e = 0; e < kN; ++e) mm = fmaxf(mm, p[v].get(e));
+        for (int e = 0; e < kN; ++e) m = fmaxf(m, p[v].get(e));
 #pragma unroll
       for (int v = 0; v < NV; ++v) p[v].forget();
-      if (K != kMulti) mm = wave_max(mm);
-      const float ref = mm == -INFINITY ? 0.f : mm;   // nothing but -inf so far: sums of 0
-      if (K == kMulti && m > -INFINITY) {
-        st *= __builtin_amdgcn_exp2f((m - mm) * ct);
-        if (BOTH) s1 *= __builtin_amdgcn_exp2f((m - mm) * kLog2e);
-      }
-      m = mm;
-      if (q == 0) {
-        const float x = z_tail - ref;
-        st = __builtin_amdgcn_exp2f(x * ct);
-        if (BOTH) s1 = second_exp<S>(st, x);
-      }
+      m = wave_max(m);
+    }
+    float ref = m == -INFINITY ? 0.f : m;   // nothing but -inf so far: sums of 0
+    st = __builtin_amdgcn_exp2f((z_tail - ref) * ct);
+    if (BOTH) s1 = second_exp<S>(st, z_tail - ref);
+    for (int q = 0;;) {
 #pragma unroll
       for (int v = 0; v < NV; ++v) {   // a piece's values at a time: those of all pieces would take the registers
+        if (K == kMulti) {   // the sums of a piece while the next ones load, against a reference of each lane's
+          float pm = p[v].get(0);
+#pragma unroll
+          for (int e = 1; e < kN; ++e) pm = fmaxf(pm, p[v].get(e));
+          if (__any(pm > m + slack)) {   // seldom: it follows a later maximum only past `slack`
+            const float to = fmaxf(m, pm);
+            if (m > -INFINITY) {
+              st *= __builtin_amdgcn_exp2f((m - to) * ct);
+              if (BOTH) s1 *= __builtin_amdgcn_exp2f((m - to) * kLog2e);
+            }
+            m = to;
+            ref = m == -INFINITY ? 0.f : m;
+          }
+        }
 #pragma unroll
         for (int e = 0; e < kN; ++e) {
           const float x = p[v].get(e) - ref;
@@ -337,14 +348,16 @@ __global__ void __launch_bounds__(NV > 8 ? kBigThreads : 1024, NV > 8 ? 3 : K ==
           st += et;
           if (BOTH) s1 += second_exp<S>(et, x);
         }
+        if (K == kMulti) p[v].forget();
         __builtin_amdgcn_sched_barrier(0);
       }
-#pragma unroll
-      for (int v = 0; v < NV; ++v) p[v].forget();
       if (K != kMulti || ++q == n_chunks) break;
       load(z, first_end + (q - 1) * chunk, first_end + q * chunk);
     }
-    if (K == kMulti) {
+    if (K != kMulti) {
+#pragma unroll
+      for (int v = 0; v < NV; ++v) p[v].forget();
+    } else {
       const float mw = wave_max(m);
       if (m > -INFINITY) {
         st *= __builtin_amdgcn_exp2f((m - mw) * ct);
@@ -576,7 +589,8 @@ void launch_distill(const DistillArgs& a, int64_t groups, int threads, const Tar
 }
 
 // Threads of a row's workgroup and pieces of a thread: few pieces while a few waves hold the row (a wave computes on all its
-// pieces, there or not), 8 up to 16 waves, then 16 and 20, where the registers of 16 waves end, then chunks.
+// pieces, there or not), 8 up to 16 waves, then 16 and 25 of 12 waves, where a compute unit's registers end, then chunks
+// (512 x 151,936 bf16 in chunks 1% slower, 1,200 rows 8%).
 template <typename T>
 void launch_distill_rows(const DistillArgs& a, const Target* targets, void* dz, int64_t d_stride, hipStream_t st) {
   const int pieces = a.vocab / Piece<T>::kN;
@@ -592,8 +606,8 @@ void launch_distill_rows(const DistillArgs& a, const Target* targets, void* dz, 
     launch_distill<T, 8, true, kOne>(a, a.rows, threads(8), targets, dz, d_stride, st);
   else if (pieces <= 16 * kBigThreads)
     launch_distill<T, 16, true, kRoll>(a, std::min(a.rows, units), kBigThreads, targets, dz, d_stride, st);
-  else if (pieces <= 26 * kBigThreads)
-    launch_distill<T, 26, true, kRoll>(a, std::min(a.rows, units), kBigThreads, targets, dz, d_stride, st);
+  else if (pieces <= 25 * kBigThreads)
+    launch_distill<T, 25, true, kRoll>(a, std::min(a.rows, units), kBigThreads, targets, dz, d_stride, st);
   else
     launch_distill<T, 16, true, kMulti>(a, a.rows, kBigThreads, targets, dz, d_stride, st);
 }
