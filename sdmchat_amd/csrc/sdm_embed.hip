@@ -489,6 +489,161 @@ __global__ void __launch_bounds__(1024) embed_rows_join_kernel(RowsGrad a) {
   }
 }
 
+// Few tokens: the whole gradient in one launch.  A workgroup per bucket and 256 columns reads all ids itself, every wave a run
+// of them, puts its own tokens in the order of their rows in LDS (counts per wave and row, their prefix sums, places by
+// ballots: the tokens of a row stay in their order), clears its rows without one and sums the others: rows of up to kAlone
+// tokens by a wave each, the frequent ones by all waves, which share a row's tokens and join over LDS.  What bounds it is
+// the table's gradient going out and one compute unit's loads of a frequent token's rows (410 of 5,003 in a Zipf stream: 9 us),
+// which the four launches share evenly: 64 tokens of 32,768 rows of 768 in bfloat16 take 13 us against their 18, 2,048 18
+// against 23, 4,096 22 against 23, 6,144 26 against 24.  A call that waits for the host also saves three launches.
+constexpr int kFewTokens = 5120, kFewRows = 1024, kFewWaves = 16, kAlone = 32;
+inline size_t few_lds(int R, int64_t n) {
+  return (static_cast<size_t>(kFewWaves) * R + R + 1 + kFewTokens / kAlone) * 4 + static_cast<size_t>(n) * 2;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(64 * kFewWaves, 8) embed_few_grad_kernel(const int64_t* __restrict__ ids, int n, int vocab,
+                                                                        int pad, int R, int row_bits,
+                                                                        const T* __restrict__ dy, int64_t dy_stride,
+                                                                        float scale, T* __restrict__ d_table,
+                                                                        int64_t dt_stride, int d) {
+  extern __shared__ int32_t cnt[];   // [waves][R]: tokens of a row in a wave's run, then where they go
+  __shared__ float4 part[kFewWaves][64];
+  __shared__ int32_t red[kFewWaves];
+  __shared__ int32_t n_many;
+  constexpr int kRun = kFewTokens / kFewWaves / 64;   // tokens of a lane, at most
+  int32_t* off = cnt + kFewWaves * R;                 // [R + 1]: where a row's tokens begin in list
+  int32_t* many = off + R + 1;                        // rows of more than kAlone
+  uint16_t* list = reinterpret_cast<uint16_t*>(many + kFewTokens / kAlone);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int b = blockIdx.x;
+  const int run = (n + 64 * kFewWaves - 1) / (64 * kFewWaves);   // 64 tokens each
+  int64_t id[kRun];
+  int row[kRun];   // of the bucket, or -1
+#pragma unroll
+  for (int k = 0; k < kRun; ++k)   // all on their way together
+    if (k < run) id[k] = ids[min((wave * run + k) * 64 + lane, n - 1)];
+#pragma unroll
+  for (int k = 0; k < kRun; ++k) {
+    row[k] = -1;
+    if (k >= run || (wave * run + k) * 64 + lane >= n) continue;
+    const int v = clamp_token(id[k], vocab);
+    if (v != pad && (v & (kBuckets - 1)) == b) row[k] = v >> kBucketBits;
+  }
+  for (int i = threadIdx.x; i < kFewWaves * R; i += 64 * kFewWaves) cnt[i] = 0;
+  if (threadIdx.x == 0) n_many = 0;
+  __syncthreads();
+  int32_t* mine = cnt + wave * R;
+#pragma unroll
+  for (int k = 0; k < kRun; ++k)
+    if (row[k] >= 0) atomicAdd(&mine[row[k]], 1);
+  __syncthreads();
+  {   // a thread per row (R is at most their number)
+    const int r = threadIdx.x;
+    int tot = 0;
+    if (r < R)
+      for (int w = 0; w < kFewWaves; ++w) tot += cnt[w * R + r];
+    int inc = tot;
+#pragma unroll
+    for (int j = 1; j < 64; j <<= 1) {
+      const int u = __shfl_up(inc, j);
+      if (lane >= j) inc += u;
+    }
+    if (lane == 63) red[wave] = inc;
+    __syncthreads();
+    int pos = inc - tot;
+    for (int w = 0; w < wave; ++w) pos += red[w];
+    if (r < R) {
+      off[r] = pos;
+      if (r == R - 1) off[R] = pos + tot;
+      if (tot > kAlone) many[atomicAdd(&n_many, 1)] = r;
+      for (int w = 0; w < kFewWaves; ++w) {
+        const int c = cnt[w * R + r];
+        cnt[w * R + r] = pos;
+        pos += c;
+      }
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < kRun; ++k) {
+    const bool live = row[k] >= 0;
+    const uint64_t all = __ballot(live);
+    if (!all) continue;   // the same for the wave
+    const int r = live ? row[k] : 0;
+    const uint64_t group = same_lanes(all, r, row_bits);
+    const int rank = __popcll(group & lanes_below(lane));
+    const int start = mine[r];
+    if (live) {
+      list[start + rank] = static_cast<uint16_t>((wave * run + k) * 64 + lane);
+      if (rank == 0) mine[r] = start + __popcll(group);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");   // the next tokens' lanes read what these wrote
+  }
+  __syncthreads();
+  const bool narrow = d < 4;
+  const int col = blockIdx.y * 256 + 4 * lane, c = quad_column(col, d);
+  // the sum of the rows of m tokens from list[first] on
+  auto sum = [&](int first, int m) {
+    constexpr int kB = 4;   // rows in flight (8: no gain, the waves are many)
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int j = 0; j < m; j += kB) {
+      const int t = list[first + min(j + min(lane, kB - 1), m - 1)];
+      Quad4<T> g[kB];
+#pragma unroll
+      for (int q = 0; q < kB; ++q) {
+        const T* src = dy + __builtin_amdgcn_readlane(t, q) * dy_stride;
+        if (narrow)
+          g[q].load_part(src, d);
+        else
+          g[q].load(src + c);
+      }
+#pragma unroll
+      for (int q = 0; q < kB; ++q) {
+        if (j + q < m) {
+          acc.x += g[q].get(0);
+          acc.y += g[q].get(1);
+          acc.z += g[q].get(2);
+          acc.w += g[q].get(3);
+        }
+      }
+    }
+    return acc;
+  };
+  auto store = [&](int r, float4 x) {
+    const float v[4] = {x.x * scale, x.y * scale, x.z * scale, x.w * scale};
+    Quad4<T> o;
+    if (col < d) o.store(d_table + (static_cast<int64_t>(r) << kBucketBits | b) * dt_stride + c, v, d - c);
+  };
+  const int r_own = kFewWaves * lane + wave;   // a wave's rows: 16 lane + wave
+  const bool there = r_own < R && (r_own << kBucketBits | b) < vocab;
+  const int first = there ? off[r_own] : 0, m = there ? off[r_own + 1] - first : -1;
+  for (uint64_t left = __ballot(m == 0); left; left &= left - 1)
+    store(kFewWaves * (__ffsll(static_cast<unsigned long long>(left)) - 1) + wave, make_float4(0.f, 0.f, 0.f, 0.f));
+  for (uint64_t left = __ballot(m > 0 && m <= kAlone); left; left &= left - 1) {
+    const int l = __ffsll(static_cast<unsigned long long>(left)) - 1;
+    store(kFewWaves * l + wave, sum(__builtin_amdgcn_readlane(first, l), __builtin_amdgcn_readlane(m, l)));
+  }
+  for (int e = 0; e < n_many; ++e) {
+    const int r = many[e], from = off[r], k = off[r + 1] - from, per = (k + kFewWaves - 1) / kFewWaves;
+    const int j0 = min(k, wave * per);
+    part[wave][lane] = sum(from + j0, min(k, j0 + per) - j0);
+    __syncthreads();
+    if (wave == 0) {
+      float4 x = part[0][lane];
+      for (int q = 1; q < kFewWaves; ++q) {
+        const float4 y = part[q][lane];
+        x.x += y.x;
+        x.y += y.y;
+        x.z += y.z;
+        x.w += y.w;
+      }
+      store(r, x);
+    }
+    __syncthreads();
+  }
+}
+
 // the shape of the order and the sums
 struct OrderPlan {
   int R, row_bits, waves, tiles;          // rows of a bucket, the bits of their numbers, waves that order them
@@ -595,13 +750,25 @@ int sdm_rt_embed_backward(const int64_t* ids, int64_t n, const void* dy, int64_t
   if (groups >= 1 << 24)
     return set_err(SDM_RT_EUNSUPPORTED, "too many tokens of so wide rows for one launch");
   hipStream_t st = static_cast<hipStream_t>(stream);
+  const int pad = padding_idx >= 0 && padding_idx < vocab ? static_cast<int>(padding_idx) : -1;
+  if (n <= kFewTokens && p.R <= kFewRows) {
+    auto few = [&](auto zero) -> int {
+      using T = decltype(zero);
+      static const bool lds = allow_lds(reinterpret_cast<const void*>(embed_few_grad_kernel<T>));
+      if (!lds) return lds_err("embed_backward");
+      hipLaunchKernelGGL((embed_few_grad_kernel<T>), dim3(kBuckets, (d + 255) / 256), dim3(64 * kFewWaves), few_lds(p.R, n), st, ids,
+                         static_cast<int>(n), static_cast<int>(vocab), pad, p.R, p.row_bits, static_cast<const T*>(dy),
+                         dy_row_stride, scale, static_cast<T*>(d_table), d_table_row_stride, d);
+      return check_launch("embed_few_grad");
+    };
+    return dtype == SDM_RT_BF16 ? few(bf16_t{}) : few(float{});
+  }
   static const bool lds = allow_lds(reinterpret_cast<const void*>(embed_order_kernel));
   if (!lds) return lds_err("embed_backward");
   char* ws = static_cast<char*>(workspace);
   int32_t* offsets = reinterpret_cast<int32_t*>(ws);
   int32_t* order = reinterpret_cast<int32_t*>(ws + p.off_order);
   int32_t* row_of = reinterpret_cast<int32_t*>(ws + p.off_row);
-  const int pad = padding_idx >= 0 && padding_idx < vocab ? static_cast<int>(padding_idx) : -1;
   int32_t* bucket_at = reinterpret_cast<int32_t*>(ws + p.off_bucket);
   uint32_t* packed = reinterpret_cast<uint32_t*>(ws + p.off_packed);
   if (p.tiles > 0)

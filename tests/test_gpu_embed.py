@@ -194,6 +194,33 @@ def test_sizes_around_tiles_and_slices(N, d):
         _check_grad(core.embedding_backward(ids.cuda(), dy.cuda(), V, 1.0), ids, dy, V, 1.0)
 
 
+@pytest.mark.parametrize("N,V,d", [
+    (5119, 300, 257), (5120, 9, 65), (5120, 300, 1028), (5121, 9, 65), (5121, 300, 257), (5121, 300, 3), (9217, 20000, 1),
+    (10240, 257, 130), (5000, 262144, 9), (5000, 262145, 9), (255, 262145, 65), (1025, 300000, 2), (1, 300000, 64),
+])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_sizes_around_one_launch(N, V, d, dtype):
+    """Tokens and vocabularies on both sides of what one launch takes, with padding."""
+    g = torch.Generator().manual_seed(N + V + d)
+    for kind in ("zipf", "one"):
+        ids = _ids(kind, N, V, g)
+        pad = int(ids[0]) if kind == "zipf" else (int(ids[0]) + 1) % V
+        dy = torch.randn(N, d, generator=g).to(dtype)
+        _check_grad(core.embedding_backward(ids.cuda(), dy.cuda(), V, 1.3, pad), ids, dy, V, 1.3, pad)
+
+
+@pytest.mark.parametrize("m", [1, 31, 32, 33, 64, 500])
+@pytest.mark.parametrize("d", [1, 2, 5, 255, 256, 260, 4100, 5000])
+def test_rows_of_few_and_many_tokens(m, d):
+    """Rows of m tokens each, summed by one wave or by all of them, of fewer and more column slices than those."""
+    g = torch.Generator().manual_seed(m + d)
+    V = 1030
+    rows = torch.tensor([0, 1, 255, 256, 257, 511, 512, 768, 1024])[:max(1, 4096 // m)]   # several of one bucket
+    ids = rows.repeat(m)[torch.randperm(len(rows) * m, generator=g)]
+    dy = torch.randn(len(ids), d, generator=g)
+    _check_grad(core.embedding_backward(ids.cuda(), dy.cuda(), V, 1.0), ids, dy, V, 1.0)
+
+
 def test_refusals():
     table = torch.randn(10, 8, device="cuda")
     ids = torch.zeros(3, dtype=torch.long, device="cuda")
