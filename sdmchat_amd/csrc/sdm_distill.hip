@@ -449,9 +449,9 @@ __global__ void __launch_bounds__(1024) distill_sum_kernel(DistillArgs a, float*
   for (int64_t i = i0; i < a.rows; i += 16 * 1024) {
     float v[16];
 #pragma unroll
-    for (int q = 0; q < 16; ++q) v[q] = i + q * 1024 < a.rows ? a.row_loss[i + q * 1024] : 0.f;
+    for (int q = 0; q < 16; ++q) v[q] = a.row_loss[min(i + q * 1024, a.rows - 1)];   // no load behind a branch
 #pragma unroll
-    for (int q = 0; q < 16; ++q) s += static_cast<double>(v[q]);
+    for (int q = 0; q < 16; ++q) s += i + q * 1024 < a.rows ? static_cast<double>(v[q]) : 0.0;
   }
 #pragma unroll
   for (int j = 32; j > 0; j >>= 1) s += __shfl_xor(s, j);
