@@ -388,6 +388,11 @@ class TokenRules:
         return core.process_logits(logits, self.tokens, self.lengths, prompt=self.prompt, repetition=self.repetition,
                                    frequency=self.frequency, presence=self.presence, bias=self.bias, mask=self.mask, out=out)
 
+    def tensors(self):
+        """The tensors that a call reads or writes now."""
+        return [t for t in (self.tokens, self.lengths, self.prompt, self.repetition, self.frequency, self.presence, self.bias,
+                            self.mask) if torch.is_tensor(t)]
+
     def scratch(self):
         """The same rules on a history of their own."""
         B, window = self.tokens.shape
@@ -401,12 +406,15 @@ class DecodeGraph:
     consecutive steps can be captured in one graph (``run(tokens [steps, B])``).  The state is the caller's
     ModelDecodeState, updated in place; capture first runs two steps on a scratch state of the same shapes, so that
     every workspace and parameter cache exists before capture and nothing allocates inside the graph.  rules: a
-    TokenRules of the B streams that every step's logits pass (the graph reads its tensors where they are)."""
+    TokenRules of the B streams that every step's logits pass.  The graph reads and writes the tensors that rules had at
+    capture where they are, and keeps them: what is written into them reaches the next replay, another tensor or number put
+    in their place does not."""
 
     def __init__(self, model, state, steps=1, rules=None):
         dev = model.emb.weight.device
         B = next(st.mem.shape[0] for st in state.layers if st is not None)
         self.model, self.state, self.steps = model, state, steps
+        self.rules, self._rules_held = rules, None if rules is None else rules.tensors()
         self.tokens = torch.zeros(steps, B, dtype=torch.long, device=dev)
         with torch.no_grad():
             scratch = model.decode_state(B, dev)
