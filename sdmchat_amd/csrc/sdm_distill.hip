@@ -253,6 +253,7 @@ __global__ void __launch_bounds__(NV > 8 ? kBigThreads : 1024, NV > 8 ? 3 : K ==
   const int whole = a.vocab / kN * kN;
   const int c_tail = whole + static_cast<int>(threadIdx.x);   // the values past the last whole piece: a thread each
   const float ct = a.kd > 0.f ? a.inv_tau * kLog2e : kLog2e;
+  const bool weighted = a.mean && (GRAD || a.stats);   // a row's weight in the gradient, made here or from the stats
   const float slack = 16.f / fmaxf(ct, kLog2e);   // kMulti: a factor of up to 2^16 in the sums
   const Entries t = entries_in(lds, a.k);
   // chunks of a row, the first of them the partial one
@@ -300,7 +301,7 @@ __global__ void __launch_bounds__(NV > 8 ? kBigThreads : 1024, NV > 8 ? 3 : K ==
     }
     if (K != kRoll) load(z, 0, first_end);
     const float z_tail = c_tail < a.vocab ? to_f32(z[c_tail]) : -INFINITY;
-    if (GRAD && a.mean && wave == waves - 1) {   // the mean's divisor
+    if (weighted && wave == waves - 1) {   // the mean's divisor
       int count = 0;
 #pragma unroll 8
       for (int i = lane; i < a.n_counts; i += 64) count += a.counts[i];
@@ -385,7 +386,7 @@ __global__ void __launch_bounds__(NV > 8 ? kBigThreads : 1024, NV > 8 ? 3 : K ==
     }
     if (!BOTH) s1 = st;
     const float inv_t = taught ? 1.f / st : 0.f, inv_1 = target.label >= 0 ? 1.f / s1 : 0.f;
-    const float w = GRAD && a.mean ? 1.f / static_cast<float>(max(shared_count, 1)) : 1.f;
+    const float w = weighted ? 1.f / static_cast<float>(max(shared_count, 1)) : 1.f;
     if (wave == 0) {
       float loss = 0.f;
       const float ts = shared_ts, lt = logf(ts), ls = logf(st);
