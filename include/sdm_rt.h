@@ -534,6 +534,10 @@ typedef struct {
 int sdm_rt_process_logits(const sdm_rt_rules* rules, const void* logits, int64_t logits_row_stride, sdm_rt_dtype dtype,
                           int64_t rows, int32_t vocab, void* out, int64_t out_row_stride, void* stream);
 
+/* The capture into a graph that the stream is in, 0 outside one: what a call made along with another one (the gradient of
+ * sdm_rt_distill_loss) is made again by every replay only if both belong to the same capture. */
+uint64_t sdm_rt_capture_id(void* stream);
+
 /* One token more of each stream: tokens[row][lengths[row] mod width] = new_ids[row], lengths[row] += 1. */
 int sdm_rt_append_tokens(int64_t* tokens, int64_t tokens_row_stride, int64_t width, int64_t* lengths,
                          const int64_t* new_ids, int64_t rows, void* stream);

@@ -217,6 +217,7 @@ SIGNATURES = {
     "sdm_rt_distill_grad": (ctypes.c_int, [ctypes.POINTER(SdmRtDistill), c_void_p, c_i64, ctypes.c_int, c_void_p, c_i64,
                                            c_void_p, c_i64, c_void_p, c_void_p, c_void_p, ctypes.c_int32, c_void_p, c_i64,
                                            c_void_p]),
+    "sdm_rt_capture_id": (ctypes.c_uint64, [c_void_p]),
     "sdm_rt_process_logits": (ctypes.c_int, [ctypes.POINTER(SdmRtRules), c_void_p, c_i64, ctypes.c_int, c_i64,
                                              ctypes.c_int32, c_void_p, c_i64, c_void_p]),
     "sdm_rt_append_tokens": (ctypes.c_int, [c_void_p, c_i64, c_i64, c_void_p, c_void_p, c_i64, c_void_p]),

@@ -1429,8 +1429,8 @@ _REDUCTION = {"none": _lib.SDM_RT_NONE, "mean": _lib.SDM_RT_MEAN, "sum": _lib.SD
 class DistillFunction(torch.autograd.Function):
     """distill_loss on rows as an autograd function; it cannot be differentiated again.  A loss of one value computes its
     gradient with the loss (sdm_rt_distill_loss, one pass over the logits): the first backward hands it out, after
-    sdm_rt_distill_grad has put it right if the gradient that comes in is not 1.  "none", and a second backward, take
-    sdm_rt_distill_grad alone.  apply(logits [rows, vocab], top_ids, top_logits [rows, k], labels [rows] or None, dims) ->
+    sdm_rt_distill_grad has put it right if the gradient that comes in is not 1.  "none", a second backward, and one that is
+    captured into another graph than the loss (or that alone), take sdm_rt_distill_grad alone.  apply(logits [rows, vocab], top_ids, top_logits [rows, k], labels [rows] or None, dims) ->
     loss, dims an _lib.SdmRtDistill."""
 
     @staticmethod
@@ -1442,6 +1442,8 @@ class DistillFunction(torch.autograd.Function):
         lib = _lib.load()
         nbytes = lib.sdm_rt_distill_workspace_bytes(at)
         grad = ctx.needs_input_grad[0]
+        if grad and not none:
+            ctx.capture = lib.sdm_rt_capture_id(_raw_stream(z.get_device()))
         # the rows' maxima and sums for the backward ([n, 4] float32), then the workspace
         kept = 2 * n if grad else 0
         buf = ids.new_empty(kept + nbytes // 8 + 1)
@@ -1462,14 +1464,16 @@ class DistillFunction(torch.autograd.Function):
     @staticmethod
     def gradients(ctx, dloss):
         z, ids, top, labels, stats = ctx.saved_tensors
-        (at, code, V, k), dz = ctx.call, ctx.dz
-        ctx.dz = None   # the caller's from here on
-        unless_one = dz is not None
-        if dz is None:
+        (at, code, V, k), dz, lib = ctx.call, ctx.dz, _lib.load()
+        # replays of a capture that holds this pass alone find in dz what the caller has made of it since
+        unless_one = dz is not None and lib.sdm_rt_capture_id(_raw_stream(z.get_device())) == ctx.capture
+        if unless_one:
+            ctx.dz = None   # the caller's from here on
+        else:
             dz = z.new_empty(z.shape)
         z, zs = _read_rows(z)
         g = dloss.contiguous()
-        _launch(_lib.load().sdm_rt_distill_grad, z.get_device(), at, z.data_ptr(), zs, code, ids.data_ptr(), k, top.data_ptr(),
+        _launch(lib.sdm_rt_distill_grad, z.get_device(), at, z.data_ptr(), zs, code, ids.data_ptr(), k, top.data_ptr(),
                 k, _ptr(labels), stats.data_ptr(), g.data_ptr(), unless_one, dz.data_ptr(), V)
         return dz, None, None, None, None
 

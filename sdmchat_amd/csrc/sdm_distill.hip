@@ -619,6 +619,16 @@ using namespace sdmrt;
 
 extern "C" {
 
+uint64_t sdm_rt_capture_id(void* stream) {
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  if (hipStreamGetCaptureInfo(static_cast<hipStream_t>(stream), &status, &id) != hipSuccess) {
+    (void)hipGetLastError();   // the null stream while another one is captured: not captured itself
+    return 0;
+  }
+  return status == hipStreamCaptureStatusActive ? id : 0;
+}
+
 size_t sdm_rt_distill_workspace_bytes(const sdm_rt_distill* dims) {
   return dims && dims->rows >= 0 ? distill_bytes(dims) : 0;
 }

@@ -50,3 +50,69 @@ def test_loss_then_gradient(reduction, along, N, V, K, dtype):
         err = (first.double().cpu() * 0.7 - grad).abs()
         # 0.7 times a rounded value, against the value for float32's 0.7 (off by 2^-25 of it)
         assert bool((err <= gb * (1 + half) + (half + U) * grad.abs() + 2.0 ** -126).all())
+
+
+def _setup(seed=31):
+    z, ids, top, lab = make(20, 700, 6, torch.float32, seed)
+    return z, ids, top, lab, tuple(t.cuda() for t in (z, ids, top, lab))
+
+
+def _want(z, ids, top, lab, go):
+    _, grad, _, gb, _, _ = reference(z, ids, top, lab, 2.0, 0.5, grad_out=torch.tensor(go))
+    return grad, gb + U * grad.abs() + 2.0 ** -126
+
+
+def test_a_backward_captured_alone_replays_whatever_became_of_its_gradient():
+    """The loss eager, its backward in a graph: every replay gives the gradient for what comes in then, also where the caller
+    has written into the last one."""
+    z, ids, top, lab, (zd, idd, td, ld) = _setup()
+    go, stream = torch.ones((), device="cuda"), torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        zz = zd.detach().requires_grad_(True)
+        loss = core.distill_loss(zz, idd, td, labels=ld, alpha=0.5, temperature=2.0)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        dz, = torch.autograd.grad(loss, zz, go, retain_graph=True)
+    for x in (1.0, 3.0, 1.0, 0.0, 1.0):
+        go.fill_(x)
+        graph.replay()
+        torch.cuda.synchronize()
+        want, tol = _want(z, ids, top, lab, x)
+        assert bool(((dz.double().cpu() - want).abs() <= tol).all()), x
+        dz.fill_(5.0)   # the caller owns it between the replays
+    with torch.cuda.stream(stream):   # the graph of the eager loss is whole
+        eager, = torch.autograd.grad(loss, zz, torch.ones((), device="cuda"))
+    torch.cuda.synchronize()
+    want, tol = _want(z, ids, top, lab, 1.0)
+    assert bool(((eager.double().cpu() - want).abs() <= tol).all())
+
+
+def test_loss_and_backward_in_graphs_of_their_own():
+    """Two backward replays after one of the loss, with other gradients coming in and the last result overwritten."""
+    z, ids, top, lab, (zd, idd, td, ld) = _setup(32)
+    go, stream = torch.ones((), device="cuda"), torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    args = dict(labels=ld, alpha=0.5, temperature=2.0)
+    with torch.cuda.stream(stream):
+        zz = zd.detach().requires_grad_(True)
+        torch.autograd.grad(core.distill_loss(zz, idd, td, **args), zz, go)
+    torch.cuda.synchronize()
+    first, second = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(first, stream=stream):
+        loss = core.distill_loss(zz, idd, td, **args)
+    with torch.cuda.graph(second, stream=stream, pool=first.pool()):
+        dz, = torch.autograd.grad(loss, zz, go, retain_graph=True)
+    for r in range(3):
+        z, ids, top, lab = make(20, 700, 6, torch.float32, 40 + r)
+        for old, new in zip((zd, idd, td, ld), (z, ids, top, lab)):
+            old.copy_(new)
+        first.replay()
+        for x in (1.0, -2.0, 1.0):
+            go.fill_(x)
+            second.replay()
+            torch.cuda.synchronize()
+            want, tol = _want(z, ids, top, lab, x)
+            assert bool(((dz.double().cpu() - want).abs() <= tol).all()), (r, x)
+            dz.zero_()
