@@ -1568,6 +1568,42 @@ def pack_mask(allowed):
     return torch.where(words >= 1 << 31, words - (1 << 32), words).to(torch.int32)
 
 
+def prepare_rules(name, B, V, dev, tokens=None, lengths=None, prompt=None, repetition=1.0, frequency=0.0, presence=0.0,
+                  bias=None, mask=None, limits=False):
+    """process_logits' rules for logits [B, V] on dev, checked: (SdmRtRules, the tensors it points to).  limits: those of the
+    kernel too, which sdm_rt_process_logits reports when it is called."""
+    _widths(name, vocab=V)
+    if limits and (B > 65535 or V > 1 << 21 or (B + 7) // 8 * 8 * ((V + 8191) // 8192) >= 1 << 22):
+        raise ValueError(f"{name}: {B} rows of {V} logits are past the kernel's limits")
+    _same_device(name, dev, tokens=tokens, lengths=lengths, prompt=prompt, bias=bias, mask=mask)
+    held = [_per_row(name, w, v, B, dev) for w, v in (("repetition", repetition), ("frequency", frequency),
+                                                      ("presence", presence))]
+    hist = (None, 0, 0, None, None)
+    if tokens is not None:
+        if tokens.dtype != torch.int64 or tokens.dim() != 2 or tokens.shape[0] != B:
+            raise ValueError(f"{name}: tokens must be int64 [B={B}, width], got {tokens.dtype} {tuple(tokens.shape)}")
+        if lengths is None:
+            raise ValueError(f"{name}: tokens need lengths")
+        for what, t in (("lengths", lengths), ("prompt", prompt)):
+            if t is not None and (t.dtype != torch.int64 or t.dim() != 1 or t.shape[0] != B):
+                raise ValueError(f"{name}: {what} must be int64 [B={B}], got {t.dtype} {tuple(t.shape)}")
+        if any(t is not None or v != w for (t, v), w in zip(held, (1.0, 0.0, 0.0))):
+            tokens, ts = _read_rows(tokens)
+            lengths = lengths.contiguous()
+            prompt = None if prompt is None else prompt.contiguous()
+            hist = (tokens.data_ptr(), ts, tokens.shape[1], lengths.data_ptr(), _ptr(prompt))
+    elif lengths is not None or prompt is not None:
+        raise ValueError(f"{name}: lengths and prompt need tokens")
+    bs = ms = 0
+    if bias is not None:
+        bias, bs = _row_or_rows(name, "bias", bias, B, V, torch.float32)
+    if mask is not None:
+        mask, ms = _row_or_rows(name, "mask", mask, B, (V + 31) // 32, torch.int32)
+    (rep, rep_all), (freq, freq_all), (pres, pres_all) = held
+    return (_lib.SdmRtRules(*hist, _ptr(rep), _ptr(freq), _ptr(pres), rep_all, freq_all, pres_all, _ptr(bias), bs, _ptr(mask),
+                            ms), (tokens, lengths, prompt, rep, freq, pres, bias, mask))
+
+
 def process_logits(logits, tokens=None, lengths=None, *, prompt=None, repetition=1.0, frequency=0.0, presence=0.0,
                    bias=None, mask=None, out=None):
     """The rules of a decode step on its logits [B, vocab] (float32 or bfloat16), in float32 and in this order:
@@ -1594,49 +1630,29 @@ def process_logits(logits, tokens=None, lengths=None, *, prompt=None, repetition
         raise RuntimeError(f"{name} is inference only: logits require a gradient")
     B, V = logits.shape
     dev = logits.device
-    _widths(name, vocab=V)
-    _same_device(name, dev, tokens=tokens, lengths=lengths, prompt=prompt, bias=bias, mask=mask, out=out)
-    held = [_per_row(name, w, v, B, dev) for w, v in (("repetition", repetition), ("frequency", frequency),
-                                                      ("presence", presence))]
-    hist = (None, 0, 0, None, None)
-    if tokens is not None:
-        if tokens.dtype != torch.int64 or tokens.dim() != 2 or tokens.shape[0] != B:
-            raise ValueError(f"{name}: tokens must be int64 [B={B}, width], got {tokens.dtype} {tuple(tokens.shape)}")
-        if lengths is None:
-            raise ValueError(f"{name}: tokens need lengths")
-        for what, t in (("lengths", lengths), ("prompt", prompt)):
-            if t is not None and (t.dtype != torch.int64 or t.dim() != 1 or t.shape[0] != B):
-                raise ValueError(f"{name}: {what} must be int64 [B={B}], got {t.dtype} {tuple(t.shape)}")
-        if any(t is not None or v != w for (t, v), w in zip(held, (1.0, 0.0, 0.0))):
-            tokens, ts = _read_rows(tokens)
-            lengths = lengths.contiguous()
-            prompt = None if prompt is None else prompt.contiguous()
-            hist = (tokens.data_ptr(), ts, tokens.shape[1], lengths.data_ptr(), _ptr(prompt))
-    elif lengths is not None or prompt is not None:
-        raise ValueError(f"{name}: lengths and prompt need tokens")
-    bs = ms = 0
-    if bias is not None:
-        bias, bs = _row_or_rows(name, "bias", bias, B, V, torch.float32)
-    if mask is not None:
-        mask, ms = _row_or_rows(name, "mask", mask, B, (V + 31) // 32, torch.int32)
+    _same_device(name, dev, out=out)
+    rules = prepare_rules(name, B, V, dev, tokens, lengths, prompt, repetition, frequency, presence, bias, mask)
+    return apply_rules(name, rules, logits, out)
+
+
+def apply_rules(name, rules, logits, out):
+    """process_logits with prepare_rules' rules."""
+    B, V = logits.shape
     src, ls = _read_rows(logits)
     if out is None:
-        out = torch.empty(B, V, dtype=logits.dtype, device=dev)
+        out = torch.empty(B, V, dtype=logits.dtype, device=logits.device)
     elif tuple(out.shape) != (B, V) or out.dtype != logits.dtype or (V > 1 and out.stride(1) != 1) or (
             B > 1 and out.stride(0) < V):
         raise ValueError(f"{name}: out must be {logits.dtype} [B={B}, {V}] with contiguous rows")
     elif src.data_ptr() == logits.data_ptr() and not _apart(logits, out):
         raise ValueError(f"{name}: out overlaps logits in part")
-    (rep, rep_all), (freq, freq_all), (pres, pres_all) = held
-    r = _lib.SdmRtRules(*hist, _ptr(rep), _ptr(freq), _ptr(pres), rep_all, freq_all, pres_all, _ptr(bias), bs, _ptr(mask), ms)
-    _launch(_lib.load().sdm_rt_process_logits, out.get_device(), ctypes.byref(r), src.data_ptr(), ls, _DT[logits.dtype], B, V,
-            out.data_ptr(), out.stride(0) if B > 1 else V)
+    _launch(_lib.load().sdm_rt_process_logits, out.get_device(), ctypes.byref(rules[0]), src.data_ptr(), ls, _DT[logits.dtype],
+            B, V, out.data_ptr(), out.stride(0) if B > 1 else V)
     return out
 
 
-def append_tokens(tokens, lengths, new):
-    """One token more of each stream, in place: tokens[b, lengths[b] % width] = new[b], lengths[b] += 1 (tokens
-    [B, width], lengths and new [B], int64): the history that process_logits reads."""
+def check_append(tokens, lengths, new):
+    """What append_tokens refuses."""
     if tokens.device.type != "cuda":
         raise RuntimeError("append_tokens needs ROCm device tensors")
     if tokens.dim() != 2 or tokens.shape[1] < 1:
@@ -1648,6 +1664,18 @@ def append_tokens(tokens, lengths, new):
             raise ValueError(f"append_tokens: {what} must be int64" + ("" if what == "tokens" else f" [B={B}]"))
     if (width > 1 and tokens.stride(1) != 1) or (B > 1 and tokens.stride(0) < width) or not lengths.is_contiguous():
         raise ValueError("append_tokens: tokens must have contiguous rows, lengths must be contiguous")
+
+
+def append_tokens(tokens, lengths, new):
+    """One token more of each stream, in place: tokens[b, lengths[b] % width] = new[b], lengths[b] += 1 (tokens
+    [B, width], lengths and new [B], int64): the history that process_logits reads."""
+    check_append(tokens, lengths, new)
+    append_checked(tokens, lengths, new)
+
+
+def append_checked(tokens, lengths, new):
+    """append_tokens without its checks."""
+    B, width = tokens.shape
     new = new.contiguous()
     _launch(_lib.load().sdm_rt_append_tokens, tokens.get_device(), tokens.data_ptr(), tokens.stride(0) if B > 1 else width,
             width, lengths.data_ptr(), new.data_ptr(), B)

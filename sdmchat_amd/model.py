@@ -310,9 +310,16 @@ class OneSdmLM(nn.Module):
         """One token for each of B streams: idx_t [B] int64 -> logits [B, V], the last position of
         forward(idx, sequential=True) (track4_onesdm_models.py:534-555), with every mixer's memory carried in
         ``state`` (a ModelDecodeState, updated in place).  rules: a TokenRules of B streams; idx_t joins its history and
-        the logits are returned with the rules applied.  Inference only."""
-        if rules is not None and rules.tokens.shape[0] != idx_t.shape[0]:
-            raise ValueError(f"OneSdmLM.step: rules of {rules.tokens.shape[0]} streams for {idx_t.shape[0]} tokens")
+        the logits are returned with the rules applied; rules that it cannot apply are refused before the state or the
+        history moves.  Inference only."""
+        if rules is not None:
+            if rules.tokens.shape[0] != idx_t.shape[0]:
+                raise ValueError(f"OneSdmLM.step: rules of {rules.tokens.shape[0]} streams for {idx_t.shape[0]} tokens")
+            table = self.emb.weight if self.tie else self.head.weight
+            if table.dtype == torch.float64:
+                raise ValueError("OneSdmLM.step: rules take no float64 logits")
+            # a projection that is not this class's may give any number of logits
+            ready = rules.prepare(idx_t, table.shape[0] if type(self).project is OneSdmLM.project else None)
         reset = (idx_t == self.bos_id) if self.reset_at_bos else None
 
         def apply(kind, i, x, hx):
@@ -334,9 +341,7 @@ class OneSdmLM(nn.Module):
         logits = self.project(h)
         if rules is None:
             return logits
-        rules.append(idx_t)
-        logits = logits.detach()
-        return rules.apply(logits, out=logits)
+        return rules.apply_prepared(ready, logits.detach())
 
 
 class TokenRules:
@@ -387,6 +392,25 @@ class TokenRules:
         """The logits [B, V] with the rules applied, in ``out`` if given (core.process_logits)."""
         return core.process_logits(logits, self.tokens, self.lengths, prompt=self.prompt, repetition=self.repetition,
                                    frequency=self.frequency, presence=self.presence, bias=self.bias, mask=self.mask, out=out)
+
+    def prepare(self, idx_t, vocab):
+        """The tokens idx_t [B] that a step is about to append and the rules for its logits [B, vocab] (None: not known yet),
+        refused here where append or apply would refuse them."""
+        new = idx_t.to(torch.long)
+        core.check_append(self.tokens, self.lengths, new)
+        return new, None if vocab is None else core.prepare_rules(
+            "TokenRules", self.tokens.shape[0], vocab, new.device, self.tokens, self.lengths, self.prompt, self.repetition,
+            self.frequency, self.presence, self.bias, self.mask, limits=True)
+
+    def apply_prepared(self, ready, logits):
+        """append(idx_t), then apply(logits, out=logits), both checked before (prepare)."""
+        new, rules = ready
+        core.append_checked(self.tokens, self.lengths, new)
+        if rules is None:
+            return self.apply(logits, out=logits)
+        if logits.dtype == torch.float16:   # a projection under autocast: the rules in float32, rounded once more
+            return logits.copy_(core.apply_rules("TokenRules", rules, logits.float(), None))
+        return core.apply_rules("TokenRules", rules, logits, logits)
 
     def tensors(self):
         """The tensors that a call reads or writes now."""

@@ -7,7 +7,7 @@ import weakref
 import pytest
 import torch
 
-from sdmchat_amd import DecodeGraph, TokenRules
+from sdmchat_amd import DecodeGraph, OneSdmLM, TokenRules
 
 B, V = 3, 40
 
@@ -61,3 +61,12 @@ def test_a_decode_graph_keeps_the_rules_and_the_tensors_it_captured(no_gpu, repl
 def test_a_decode_graph_without_rules(no_gpu):
     m = _Model()
     assert DecodeGraph(m, m.decode_state(B)).rules is None
+
+
+def test_rules_that_cannot_be_applied_are_refused_before_a_step_moves():
+    """Rules on the CPU, where the kernels do not run: the state has not taken the token."""
+    m = OneSdmLM(V, d=16, layers=1, mlp_f=16, mem=False, ffn="none", heads=4, n_sub=4, d_a=4, k=2)
+    state = m.decode_state(B)
+    with torch.no_grad(), pytest.raises(RuntimeError, match="ROCm"):
+        m.step(torch.zeros(B, dtype=torch.long), state, TokenRules(B, 4, "cpu"))
+    assert state.pos == 0
