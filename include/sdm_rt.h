@@ -453,6 +453,13 @@ int sdm_rt_table_backward(const sdm_rt_dims* dims, const sdm_rt_params* params,
 int sdm_rt_embed(const int64_t* ids, int64_t n, const void* table, int64_t table_row_stride, sdm_rt_dtype dtype,
                  int64_t vocab, int32_t d, float scale, void* out, int64_t out_row_stride, void* stream);
 
+/* sdm_rt_embed that also tells of ids outside the table: the last one found is written to *outside, a word that host and
+ * device both reach (hipHostMalloc), which is left alone otherwise.  0 is inside every table, so a word that the caller
+ * keeps at 0 says by itself whether any call so far met one; NULL: not told. */
+int sdm_rt_embed_checked(const int64_t* ids, int64_t n, const void* table, int64_t table_row_stride, sdm_rt_dtype dtype,
+                         int64_t vocab, int32_t d, float scale, void* out, int64_t out_row_stride, int64_t* outside,
+                         void* stream);
+
 /* Bytes of workspace sdm_rt_embed_backward needs (0 on sizes outside its limits). */
 size_t sdm_rt_embed_backward_workspace_bytes(int64_t n, int64_t vocab, int32_t d);
 

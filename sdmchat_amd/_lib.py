@@ -206,6 +206,8 @@ SIGNATURES = {
                                              c_void_p, ctypes.c_size_t, c_void_p]),
     "sdm_rt_embed": (ctypes.c_int, [c_void_p, c_i64, c_void_p, c_i64, ctypes.c_int, c_i64, ctypes.c_int32, ctypes.c_float,
                                     c_void_p, c_i64, c_void_p]),
+    "sdm_rt_embed_checked": (ctypes.c_int, [c_void_p, c_i64, c_void_p, c_i64, ctypes.c_int, c_i64, ctypes.c_int32,
+                                            ctypes.c_float, c_void_p, c_i64, c_void_p, c_void_p]),
     "sdm_rt_embed_backward_workspace_bytes": (ctypes.c_size_t, [c_i64, c_i64, ctypes.c_int32]),
     "sdm_rt_embed_backward": (ctypes.c_int, [c_void_p, c_i64, c_void_p, c_i64, ctypes.c_int, c_i64, ctypes.c_int32,
                                              ctypes.c_float, c_i64, c_void_p, c_i64, c_void_p, ctypes.c_size_t,

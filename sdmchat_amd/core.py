@@ -1326,12 +1326,45 @@ def embedding_fits(idx, table):
             and idx.numel() <= 1 << 27)
 
 
-def _embed(ids, table, scale):
+# per GPU, the last id that embedding(check=True) found outside its table: a word of pinned memory that the kernels write
+# and nothing frees, as (tensor, ctypes view)
+_OUTSIDE = {}
+
+
+def _outside_word(index):
+    """The word's address; None in a capture before there is one (nothing is allocated there)."""
+    held = _OUTSIDE.get(index)
+    if held is None:
+        if _lib.load().sdm_rt_capture_id(_raw_stream(index)):
+            return None
+        t = torch.zeros(1, dtype=torch.int64, pin_memory=True)
+        held = _OUTSIDE[index] = t, ctypes.c_int64.from_address(t.data_ptr())
+    return ctypes.addressof(held[1])
+
+
+def report_outside_ids(index):
+    """Raises IndexError if an embedding(check=True) of GPU ``index`` that has run met an id outside its table; does not
+    wait."""
+    held = _OUTSIDE.get(index)
+    if held is not None and held[1].value:
+        bad, held[1].value = held[1].value, 0
+        raise IndexError(f"token id {bad} is outside the embedding's table (looked up in an earlier call on GPU {index})")
+
+
+def check_token_ids(device=None):
+    """Waits for the device and raises IndexError if a token id outside the table was looked up on it by
+    embedding(check=True), OneSdmLM's embedding among them, since the last report."""
+    torch.cuda.synchronize(device)
+    index = None if device is None else torch.device(device).index
+    report_outside_ids(torch.cuda.current_device() if index is None else index)
+
+
+def _embed(ids, table, scale, outside=None):
     V, d = table.shape
     tab, stride = _read_rows(table)
     out = table.new_empty(ids.shape + (d,))
-    _launch(_lib.load().sdm_rt_embed, table.get_device(), ids.data_ptr(), ids.numel(), tab.data_ptr(), stride,
-            _DT[table.dtype], V, d, scale, out.data_ptr(), d)
+    _launch(_lib.load().sdm_rt_embed_checked, table.get_device(), ids.data_ptr(), ids.numel(), tab.data_ptr(), stride,
+            _DT[table.dtype], V, d, scale, out.data_ptr(), d, outside)
     return out
 
 
@@ -1378,33 +1411,36 @@ def _embed_backward(ids, dy, vocab, d, scale, pad):
 
 class EmbeddingFunction(torch.autograd.Function):
     """embedding() as an autograd function: the lookup kernel forward, embedding_backward backward, as torch ops where it is
-    to be differentiated again (create_graph).  apply(ids contiguous int64, table, scale, padding row or -1) -> y."""
+    to be differentiated again (create_graph).  apply(ids contiguous int64, table, scale, padding row or -1, address of the
+    word for ids outside or None) -> y."""
 
     @staticmethod
-    def forward(ctx, ids, table, scale, pad):
+    def forward(ctx, ids, table, scale, pad, outside):
         ctx.save_for_backward(ids)
         ctx.call = (*table.shape, scale, pad)
-        return _embed(ids, table, scale)
+        return _embed(ids, table, scale, outside)
 
     @staticmethod
     def backward(ctx, dy):
         ids, = ctx.saved_tensors
         if not torch.is_grad_enabled():
-            return None, _embed_backward(ids, dy, *ctx.call), None, None
+            return None, _embed_backward(ids, dy, *ctx.call), None, None, None
         vocab, d, scale, pad = ctx.call
         ids = ids.reshape(-1).clamp(0, vocab - 1)
         g = dy.reshape(ids.numel(), d).float()
         if pad >= 0:
             g = g.masked_fill((ids == pad)[:, None], 0.0)
         dt = torch.zeros(vocab, d, dtype=torch.float32, device=g.device).index_add(0, ids, g) * scale
-        return None, dt.to(dy.dtype), None, None
+        return None, dt.to(dy.dtype), None, None, None
 
 
-def embedding(idx, table, scale=1.0, padding_idx=None):
+def embedding(idx, table, scale=1.0, padding_idx=None, check=False):
     """The scaled embedding lookup: scale * table[idx] (float32 product, rounded once to table's dtype), differentiable in
-    table.  idx [...] int64 or int32, each in [0, vocab) (one outside is clamped into it, not reported); table [vocab, d]
-    float32 or bfloat16, any row stride, at most 2^21 rows.  Row padding_idx is read like any other and gets no gradient
-    (F.embedding's).  The gradient is deterministic (embedding_backward)."""
+    table.  idx [...] int64 or int32, each in [0, vocab) (one outside is clamped into it); table [vocab, d] float32 or
+    bfloat16, any row stride, at most 2^21 rows.  Row padding_idx is read like any other and gets no gradient
+    (F.embedding's).  The gradient is deterministic (embedding_backward).  check: the kernel tells of ids outside the table,
+    and an IndexError follows in the first call with check on this GPU after that kernel has run, or in check_token_ids();
+    nothing waits for it here."""
     dev, shape = table.device, table.shape
     if dev.type != "cuda":
         raise RuntimeError("embedding needs ROCm device tensors")
@@ -1418,9 +1454,13 @@ def embedding(idx, table, scale=1.0, padding_idx=None):
     if shape[1] >> 31:
         _widths("embedding", d=shape[1])
     pad = _padding_row("embedding", padding_idx, shape[0])
+    outside = None
+    if check:
+        report_outside_ids(dev.index)
+        outside = _outside_word(dev.index)
     if table.requires_grad and torch.is_grad_enabled():
-        return EmbeddingFunction.apply(ids, table, float(scale), pad)
-    return _embed(ids, table, float(scale))
+        return EmbeddingFunction.apply(ids, table, float(scale), pad, outside)
+    return _embed(ids, table, float(scale), outside)
 
 
 _REDUCTION = {"none": _lib.SDM_RT_NONE, "mean": _lib.SDM_RT_MEAN, "sum": _lib.SDM_RT_SUM}

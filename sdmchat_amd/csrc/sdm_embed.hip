@@ -1,24 +1,28 @@
-// sdm_embed.hip -- the scaled embedding lookup (sdm_rt_embed) and its gradient by sorted tokens (sdm_rt_embed_backward).
+// sdm_embed.hip -- the scaled embedding lookup (sdm_rt_embed, sdm_rt_embed_checked) and its gradient by sorted tokens (sdm_rt_embed_backward).
 #include "sdm_vocab.h"
 
 namespace sdmrt {
 
 // out[n] = scale * table[ids[n]], rounded once.  A workgroup takes a run of whole rows and its threads their 16-byte
 // pieces in turn.  Bound by memory: the rows in, the rows out.  THROUGH: an output past kStreamBytes is stored past the
-// caches, which keep the table's frequent rows (131,072 tokens of rows of 2 KB: 90 -> 59 us, 268 MB out).
+// caches, which keep the table's frequent rows (131,072 tokens of rows of 2 KB: 90 -> 59 us, 268 MB out).  outside: where
+// not nullptr, the last id found outside the table (a word of host memory, written only then).
 constexpr int kEmbedPieces = 1024;   // pieces of a workgroup, about
 
 template <typename T, bool THROUGH>
 __global__ void __launch_bounds__(256) embed_kernel(const int64_t* __restrict__ ids, int64_t n, const T* __restrict__ table,
                                                     int64_t t_stride, int vocab, int d, float scale,
-                                                    T* __restrict__ out, int64_t o_stride, int ppr, int rows) {
+                                                    T* __restrict__ out, int64_t o_stride, int ppr, int rows,
+                                                    int64_t* outside) {
   constexpr int kN = Piece<T>::kN;
   for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * rows; r0 < n; r0 += static_cast<int64_t>(gridDim.x) * rows) {
     const int live = static_cast<int>(min(static_cast<int64_t>(rows), n - r0));
     for (int i = threadIdx.x; i < live * ppr; i += 256) {
       // a row's last piece ends with the row: it may hold values of the piece before it once more
       const int r = i / ppr, c = max(0, min((i - r * ppr) * kN, d - kN));
-      const T* src = table + clamp_token(ids[r0 + r], vocab) * t_stride + c;
+      const int64_t id = ids[r0 + r];
+      if (outside && (id < 0 || id >= vocab)) __hip_atomic_store(outside, id, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+      const T* src = table + clamp_token(id, vocab) * t_stride + c;
       T* dst = out + (r0 + r) * o_stride + c;
       Piece<T> p;
       if (d >= kN)
@@ -704,8 +708,9 @@ using namespace sdmrt;
 
 extern "C" {
 
-int sdm_rt_embed(const int64_t* ids, int64_t n, const void* table, int64_t table_row_stride, sdm_rt_dtype dtype,
-                 int64_t vocab, int32_t d, float scale, void* out, int64_t out_row_stride, void* stream) {
+int sdm_rt_embed_checked(const int64_t* ids, int64_t n, const void* table, int64_t table_row_stride, sdm_rt_dtype dtype,
+                         int64_t vocab, int32_t d, float scale, void* out, int64_t out_row_stride, int64_t* outside,
+                         void* stream) {
   g_err[0] = 0;
   if (n == 0) return SDM_RT_OK;
   int rc = check_embed(n, vocab, d, ids, table, out, table_row_stride, out_row_stride, dtype);
@@ -718,7 +723,8 @@ int sdm_rt_embed(const int64_t* ids, int64_t n, const void* table, int64_t table
   const bool through = n * d * (dtype == SDM_RT_BF16 ? 2 : 4) > kStreamBytes;
 #define SDM_RT_EMBED(T, THROUGH)                                                                                            \
   hipLaunchKernelGGL((embed_kernel<T, THROUGH>), dim3(blocks), dim3(256), 0, st, ids, n, static_cast<const T*>(table),      \
-                     table_row_stride, static_cast<int>(vocab), d, scale, static_cast<T*>(out), out_row_stride, ppr, rows)
+                     table_row_stride, static_cast<int>(vocab), d, scale, static_cast<T*>(out), out_row_stride, ppr, rows, \
+                     outside)
   if (dtype == SDM_RT_BF16) {
     if (through) SDM_RT_EMBED(bf16_t, true);
     else SDM_RT_EMBED(bf16_t, false);
@@ -728,6 +734,11 @@ int sdm_rt_embed(const int64_t* ids, int64_t n, const void* table, int64_t table
   }
 #undef SDM_RT_EMBED
   return check_launch("embed");
+}
+
+int sdm_rt_embed(const int64_t* ids, int64_t n, const void* table, int64_t table_row_stride, sdm_rt_dtype dtype,
+                 int64_t vocab, int32_t d, float scale, void* out, int64_t out_row_stride, void* stream) {
+  return sdm_rt_embed_checked(ids, n, table, table_row_stride, dtype, vocab, d, scale, out, out_row_stride, nullptr, stream);
 }
 
 size_t sdm_rt_embed_backward_workspace_bytes(int64_t n, int64_t vocab, int32_t d) {

@@ -99,6 +99,7 @@ class OneSdmLM(nn.Module):
 
     kind = "onesdm"
     emb_scale = 1.0
+    check_ids = True   # token ids outside the table are an error (enfold); False: they are clamped into it without a word
 
     def __init__(self, V, d=256, layers=4, mlp_f=688, mem=True, heads=4, n_sub=32, d_a=32, k=16,
                  decays=(0.0, 0.8, 0.99, 1.0), learn_decay=False, write_gate=True, gate_bias=0.0, read_mode="mean",
@@ -147,11 +148,13 @@ class OneSdmLM(nn.Module):
 
     def enfold(self, idx):
         """emb_scale * emb(idx): on core.embedding where emb is a plain nn.Embedding on the GPU (its gradient by sorted tokens,
-        deterministic; a token outside the table is clamped into it), else the module itself."""
+        deterministic), else the module itself.  There a token outside the table is clamped into it and, with check_ids,
+        raises IndexError: in the model's next call after the kernel has run, in the next replay of a graph, or in
+        core.check_token_ids(), which waits."""
         e = self.emb
         if (core.plain_module(e, nn.Embedding) and e.max_norm is None and not e.scale_grad_by_freq and not e.sparse
                 and core.embedding_fits(idx, e.weight)):
-            return core.embedding(idx, e.weight, self.emb_scale, e.padding_idx)
+            return core.embedding(idx, e.weight, self.emb_scale, e.padding_idx, self.check_ids)
         x = e(idx)
         return x if self.emb_scale == 1.0 else x * self.emb_scale
 
@@ -454,6 +457,7 @@ class DecodeGraph:
 
     def run(self, tokens):
         """tokens [steps, B] (or [B] for one step) -> logits [steps, B, V] (or [B, V])."""
+        core.report_outside_ids(self.tokens.get_device())
         self.tokens.copy_(tokens.reshape(self.tokens.shape))
         self.graph.replay()
         self.state.pos += self.steps
@@ -487,6 +491,7 @@ class ForwardGraph:
 
     def run(self, idx):
         """idx [B, T] int64 -> logits [B, T, V]."""
+        core.report_outside_ids(self.idx.get_device())
         self.idx.copy_(idx)
         self.graph.replay()
         return self.logits
