@@ -500,7 +500,11 @@ __global__ void __launch_bounds__(1024) embed_rows_join_kernel(RowsGrad a) {
 // the table's gradient going out and one compute unit's loads of a frequent token's rows (410 of 5,003 in a Zipf stream: 9 us),
 // which the four launches share evenly: 64 tokens of 32,768 rows of 768 in bfloat16 take 13 us against their 18, 2,048 18
 // against 23, 4,096 22 against 23, 6,144 26 against 24.  A call that waits for the host also saves three launches.
-constexpr int kFewTokens = 5120, kFewRows = 1024, kFewWaves = 16, kAlone = 32;
+// Every slice of 256 columns orders the tokens anew, so wide rows are left to the four launches: Zipf streams of 640 and
+// 5,120 tokens of 8,192 float32 rows take 8 and 14 us against 19 and 21 with 256 columns, 20 and 26 against 21 and 26 with
+// 1,024, but 29 and 41 against 27 and 36 with 2,048, 45 and 76 against 39 and 57 with 4,096.  One token all along is the
+// worst stream for one launch: 5,120 times 131 us against 40 with 1,024 columns, 188 against 77 with 4,096.
+constexpr int kFewTokens = 5120, kFewRows = 1024, kFewWidth = 1024, kFewWaves = 16, kAlone = 32;
 inline size_t few_lds(int R, int64_t n) {
   return (static_cast<size_t>(kFewWaves) * R + R + 1 + kFewTokens / kAlone) * 4 + static_cast<size_t>(n) * 2;
 }
@@ -762,7 +766,7 @@ int sdm_rt_embed_backward(const int64_t* ids, int64_t n, const void* dy, int64_t
     return set_err(SDM_RT_EUNSUPPORTED, "too many tokens of so wide rows for one launch");
   hipStream_t st = static_cast<hipStream_t>(stream);
   const int pad = padding_idx >= 0 && padding_idx < vocab ? static_cast<int>(padding_idx) : -1;
-  if (n <= kFewTokens && p.R <= kFewRows) {
+  if (n <= kFewTokens && p.R <= kFewRows && d <= kFewWidth) {
     auto few = [&](auto zero) -> int {
       using T = decltype(zero);
       static const bool lds = allow_lds(reinterpret_cast<const void*>(embed_few_grad_kernel<T>));
