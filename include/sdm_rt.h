@@ -485,7 +485,7 @@ typedef struct {
   int64_t rows;          /* at most 2^21 */
   int32_t vocab;         /* at most 2^30 */
   int32_t top_k;         /* teacher entries per row, 0 to 1,024 */
-  float temperature;     /* positive */
+  float temperature;     /* 1e-18 to 1e18: it and its square are ordinary float32 values */
   float alpha;           /* in [0, 1] */
   int64_t ignore_index;
   int32_t reduction;

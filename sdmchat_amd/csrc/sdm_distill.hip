@@ -535,8 +535,9 @@ inline int fill_distill(const sdm_rt_distill* d, const void* logits, int64_t l_s
   if (d->rows > (1 << 21)) return set_err(SDM_RT_EUNSUPPORTED, "rows must be at most 2^21");
   if (d->vocab > (1 << 30)) return set_err(SDM_RT_EUNSUPPORTED, "vocab must be at most 2^30");
   if (d->top_k > kMaxTop) return set_err(SDM_RT_EUNSUPPORTED, "top_k = %d must be at most %d", d->top_k, kMaxTop);
-  if (!(d->temperature > 0.f) || !(d->temperature < INFINITY) || !(1.f / d->temperature < INFINITY))
-    return set_err(SDM_RT_EINVAL, "temperature must be positive and finite");
+  // its square weighs the teacher's part (0 would say that there is none), its reciprocal times log2(e) the exponents
+  if (!(d->temperature >= 1e-18f) || !(d->temperature <= 1e18f))
+    return set_err(SDM_RT_EINVAL, "temperature must be positive and finite, from 1e-18 to 1e18");
   if (!(d->alpha >= 0.f && d->alpha <= 1.f)) return set_err(SDM_RT_EINVAL, "alpha must be in [0, 1]");
   if (d->reduction < 0 || d->reduction > 2) return set_err(SDM_RT_EINVAL, "unknown reduction %d", d->reduction);
   if (d->rows > 0) {
