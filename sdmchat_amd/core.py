@@ -1458,8 +1458,8 @@ def embedding(idx, table, scale=1.0, padding_idx=None, check=False):
     if check:
         report_outside_ids(dev.index)
         outside = _outside_word(dev.index)
-    if table.requires_grad and torch.is_grad_enabled():
-        return EmbeddingFunction.apply(ids, table, float(scale), pad, outside)
+    if (table.requires_grad and torch.is_grad_enabled()) or torch.autograd.forward_ad._current_level >= 0:
+        return EmbeddingFunction.apply(ids, table, float(scale), pad, outside)   # which refuses a tangent
     return _embed(ids, table, float(scale), outside)
 
 
