@@ -1410,8 +1410,8 @@ def _embed_backward(ids, dy, vocab, d, scale, pad):
 
 
 class EmbeddingFunction(torch.autograd.Function):
-    """embedding() as an autograd function: the lookup kernel forward, embedding_backward backward, as torch ops where it is
-    to be differentiated again (create_graph).  apply(ids contiguous int64, table, scale, padding row or -1, address of the
+    """embedding() as an autograd function: the lookup kernel forward, embedding_backward backward, differentiable in its
+    turn where that is recorded (create_graph).  apply(ids contiguous int64, table, scale, padding row or -1, address of the
     word for ids outside or None) -> y."""
 
     @staticmethod
@@ -1423,15 +1423,28 @@ class EmbeddingFunction(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dy):
         ids, = ctx.saved_tensors
-        if not torch.is_grad_enabled():
-            return None, _embed_backward(ids, dy, *ctx.call), None, None, None
-        vocab, d, scale, pad = ctx.call
-        ids = ids.reshape(-1).clamp(0, vocab - 1)
-        g = dy.reshape(ids.numel(), d).float()
+        grad = EmbeddingGradFunction.apply if torch.is_grad_enabled() else _embed_backward
+        return None, grad(ids, dy, *ctx.call), None, None, None
+
+
+class EmbeddingGradFunction(torch.autograd.Function):
+    """embedding_backward as an autograd function: linear in dy, so that its own gradient is the lookup of the rows that come
+    in, zeros for padding.  apply(ids, dy, vocab, d, scale, padding row or -1) -> the table's gradient."""
+
+    @staticmethod
+    def forward(ctx, ids, dy, vocab, d, scale, pad):
+        ctx.save_for_backward(ids)
+        ctx.call = (scale, pad)
+        return _embed_backward(ids, dy, vocab, d, scale, pad)
+
+    @staticmethod
+    def backward(ctx, g):
+        ids, = ctx.saved_tensors
+        scale, pad = ctx.call
         if pad >= 0:
-            g = g.masked_fill((ids == pad)[:, None], 0.0)
-        dt = torch.zeros(vocab, d, dtype=torch.float32, device=g.device).index_add(0, ids, g) * scale
-        return None, dt.to(dy.dtype), None, None, None
+            g = g.masked_fill((torch.arange(g.shape[0], device=g.device) == pad)[:, None], 0.0)
+        dy = EmbeddingFunction.apply(ids, g, scale, pad, None) if torch.is_grad_enabled() else _embed(ids, g, scale)
+        return None, dy, None, None, None, None
 
 
 def embedding(idx, table, scale=1.0, padding_idx=None, check=False):
