@@ -1683,7 +1683,12 @@ def process_logits(logits, tokens=None, lengths=None, *, prompt=None, repetition
         raise RuntimeError(f"{name} is inference only: logits require a gradient")
     B, V = logits.shape
     dev = logits.device
-    _same_device(name, dev, out=out)
+    if out is not None:
+        _same_device(name, dev, out=out)
+        if torch.is_grad_enabled() and out.requires_grad:
+            raise RuntimeError(f"{name} is inference only: out requires a gradient")
+        if not out.is_inference():
+            torch.autograd.graph.increment_version(out)   # written in place: a graph that saved it must not read it again
     rules = prepare_rules(name, B, V, dev, tokens, lengths, prompt, repetition, frequency, presence, bias, mask)
     return apply_rules(name, rules, logits, out)
 
