@@ -31,3 +31,11 @@ def test_inference_tensors():
         z = torch.randn(2, 50, device="cuda")
         want = z + 1
         assert torch.equal(core.process_logits(z, bias=torch.ones(50, device="cuda"), out=z), want)
+
+
+def test_logits_shared_by_another_allocation_record():
+    """A tensor that shares the logits' memory without sharing their storage object (through dlpack) overlaps all the same."""
+    z = torch.randn(6, 50, device="cuda")
+    other = torch.utils.dlpack.from_dlpack(torch.utils.dlpack.to_dlpack(z[1:]))
+    with pytest.raises(ValueError, match="overlaps"):
+        core.process_logits(z[:5], bias=torch.ones(50, device="cuda"), out=other)
