@@ -1337,7 +1337,7 @@ def _outside_word(index):
     if held is None:
         if _lib.load().sdm_rt_capture_id(_raw_stream(index)):
             return None
-        t = torch.zeros(1, dtype=torch.int64, pin_memory=True)
+        t = torch.zeros(1, dtype=torch.int64, device="cpu", pin_memory=True)
         held = _OUTSIDE[index] = t, ctypes.c_int64.from_address(t.data_ptr())
     return ctypes.addressof(held[1])
 
@@ -1415,7 +1415,7 @@ class EmbeddingFunction(torch.autograd.Function):
     word for ids outside or None) -> y."""
 
     @staticmethod
-    def forward(ctx, ids, table, scale, pad, outside):
+    def forward(ctx, ids, table, scale, pad, outside=None):
         ctx.save_for_backward(ids)
         ctx.call = (*table.shape, scale, pad)
         return _embed(ids, table, scale, outside)
@@ -1689,22 +1689,16 @@ def process_logits(logits, tokens=None, lengths=None, *, prompt=None, repetition
             raise RuntimeError(f"{name} is inference only: out requires a gradient")
         if not out.is_inference():
             torch.autograd.graph.increment_version(out)   # written in place: a graph that saved it must not read it again
-    rules = prepare_rules(name, B, V, dev, tokens, lengths, prompt, repetition, frequency, presence, bias, mask)
-    return apply_rules(name, rules, logits, out)
-
-
-def apply_rules(name, rules, logits, out):
-    """process_logits with prepare_rules' rules."""
-    B, V = logits.shape
+    rules, held = prepare_rules(name, B, V, dev, tokens, lengths, prompt, repetition, frequency, presence, bias, mask)
     src, ls = _read_rows(logits)
     if out is None:
-        out = torch.empty(B, V, dtype=logits.dtype, device=logits.device)
+        out = torch.empty(B, V, dtype=logits.dtype, device=dev)
     elif tuple(out.shape) != (B, V) or out.dtype != logits.dtype or (V > 1 and out.stride(1) != 1) or (
             B > 1 and out.stride(0) < V):
         raise ValueError(f"{name}: out must be {logits.dtype} [B={B}, {V}] with contiguous rows")
     elif src.data_ptr() == logits.data_ptr() and not _apart(logits, out):
         raise ValueError(f"{name}: out overlaps logits in part")
-    _launch(_lib.load().sdm_rt_process_logits, out.get_device(), ctypes.byref(rules[0]), src.data_ptr(), ls, _DT[logits.dtype],
+    _launch(_lib.load().sdm_rt_process_logits, out.get_device(), ctypes.byref(rules), src.data_ptr(), ls, _DT[logits.dtype],
             B, V, out.data_ptr(), out.stride(0) if B > 1 else V)
     return out
 
@@ -1728,11 +1722,6 @@ def append_tokens(tokens, lengths, new):
     """One token more of each stream, in place: tokens[b, lengths[b] % width] = new[b], lengths[b] += 1 (tokens
     [B, width], lengths and new [B], int64): the history that process_logits reads."""
     check_append(tokens, lengths, new)
-    append_checked(tokens, lengths, new)
-
-
-def append_checked(tokens, lengths, new):
-    """append_tokens without its checks."""
     B, width = tokens.shape
     new = new.contiguous()
     _launch(_lib.load().sdm_rt_append_tokens, tokens.get_device(), tokens.data_ptr(), tokens.stride(0) if B > 1 else width,

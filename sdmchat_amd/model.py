@@ -321,8 +321,8 @@ class OneSdmLM(nn.Module):
             table = self.emb.weight if self.tie else self.head.weight
             if table.dtype == torch.float64:
                 raise ValueError("OneSdmLM.step: rules take no float64 logits")
-            # a projection that is not this class's may give any number of logits
-            ready = rules.prepare(idx_t, table.shape[0] if type(self).project is OneSdmLM.project else None)
+            if isinstance(rules, TokenRules):   # a projection that is not this class's may give any number of logits
+                rules.check(idx_t, table.shape[0] if type(self).project is OneSdmLM.project else None)
         reset = (idx_t == self.bos_id) if self.reset_at_bos else None
 
         def apply(kind, i, x, hx):
@@ -344,7 +344,11 @@ class OneSdmLM(nn.Module):
         logits = self.project(h)
         if rules is None:
             return logits
-        return rules.apply_prepared(ready, logits.detach())
+        rules.append(idx_t)
+        logits = logits.detach()
+        if logits.dtype == torch.float16:   # a projection under autocast: the rules in float32, rounded once more
+            return logits.copy_(rules.apply(logits.float()))
+        return rules.apply(logits, out=logits)
 
 
 class TokenRules:
@@ -396,29 +400,14 @@ class TokenRules:
         return core.process_logits(logits, self.tokens, self.lengths, prompt=self.prompt, repetition=self.repetition,
                                    frequency=self.frequency, presence=self.presence, bias=self.bias, mask=self.mask, out=out)
 
-    def prepare(self, idx_t, vocab):
-        """The tokens idx_t [B] that a step is about to append and the rules for its logits [B, vocab] (None: not known yet),
-        refused here where append or apply would refuse them."""
-        new = idx_t.to(torch.long)
-        core.check_append(self.tokens, self.lengths, new)
-        return new, None if vocab is None else core.prepare_rules(
-            "TokenRules", self.tokens.shape[0], vocab, new.device, self.tokens, self.lengths, self.prompt, self.repetition,
-            self.frequency, self.presence, self.bias, self.mask, limits=True)
-
-    def apply_prepared(self, ready, logits):
-        """append(idx_t), then apply(logits, out=logits), both checked before (prepare)."""
-        new, rules = ready
-        core.append_checked(self.tokens, self.lengths, new)
-        if rules is None:
-            return self.apply(logits, out=logits)
-        if logits.dtype == torch.float16:   # a projection under autocast: the rules in float32, rounded once more
-            return logits.copy_(core.apply_rules("TokenRules", rules, logits.float(), None))
-        return core.apply_rules("TokenRules", rules, logits, logits)
-
-    def tensors(self):
-        """The tensors that a call reads or writes now."""
-        return [t for t in (self.tokens, self.lengths, self.prompt, self.repetition, self.frequency, self.presence, self.bias,
-                            self.mask) if torch.is_tensor(t)]
+    def check(self, idx_t, vocab):
+        """Raises where append(idx_t) or apply to logits [B, vocab] (None: not known yet) would, as far as they are this class's,
+        and for the kernel's limits; nothing moves."""
+        if type(self).append is TokenRules.append:
+            core.check_append(self.tokens, self.lengths, idx_t.to(torch.long))
+        if type(self).apply is TokenRules.apply and vocab is not None:
+            core.prepare_rules("TokenRules", self.tokens.shape[0], vocab, idx_t.device, self.tokens, self.lengths, self.prompt,
+                               self.repetition, self.frequency, self.presence, self.bias, self.mask, limits=True)
 
     def scratch(self):
         """The same rules on a history of their own."""
@@ -441,7 +430,8 @@ class DecodeGraph:
         dev = model.emb.weight.device
         B = next(st.mem.shape[0] for st in state.layers if st is not None)
         self.model, self.state, self.steps = model, state, steps
-        self.rules, self._rules_held = rules, None if rules is None else rules.tensors()
+        self.rules = rules
+        self._rules_held = [t for t in getattr(rules, "__dict__", {}).values() if torch.is_tensor(t)]
         self.tokens = torch.zeros(steps, B, dtype=torch.long, device=dev)
         with torch.no_grad():
             scratch = model.decode_state(B, dev)

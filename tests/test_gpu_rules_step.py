@@ -103,3 +103,29 @@ def test_float16_logits_of_an_autocast_step():
     assert raw.dtype == got.dtype == torch.float16
     check(dict(logits=raw.cpu(), tokens=idx.cpu()[:, None], lengths=torch.ones(B, dtype=torch.long), repetition=rules.repetition.cpu(),
                frequency=0.3, presence=0.2, bias=rules.bias.cpu()), got)
+
+
+def test_rules_of_a_class_of_ones_own():
+    """append and apply of a subclass, or of any object with them, are the ones that step calls."""
+    class Loud(TokenRules):
+        def append(self, idx_t):
+            super().append(idx_t + 1)
+
+        def apply(self, logits, out=None):
+            return super().apply(logits, out=out).neg_()
+
+    class Other:
+        tokens = torch.zeros(B, 1)
+
+        def append(self, idx_t):
+            self.seen = idx_t
+
+        def apply(self, logits, out=None):
+            return logits + 1
+    m, idx = _model(), torch.arange(B, device="cuda")
+    with torch.no_grad():
+        raw = m.step(idx, m.decode_state(B, "cuda"))
+        rules = Loud(B, 4, "cuda", bias=torch.ones(V, device="cuda"))
+        assert torch.equal(m.step(idx, m.decode_state(B, "cuda"), rules), -(raw + 1)) and rules.tokens[:, 0].tolist() == [1, 2, 3]
+        other = Other()
+        assert torch.equal(m.step(idx, m.decode_state(B, "cuda"), other), raw + 1) and other.seen is idx
