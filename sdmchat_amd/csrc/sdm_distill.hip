@@ -38,8 +38,9 @@ __device__ __forceinline__ int has_label(const DistillArgs& a, int64_t r) {
 // What a row aims at, found once: whether it has a teacher and whether that may repeat an id, its label or -1; counts[block]:
 // how many of the block's rows have either.  A wave takes four rows at a time.  Repeats are told by a table of 512 words
 // per row in LDS: an id's hash picks a word and three of its bits, and one that finds them set may be a repeat (of 100
-// distinct ids that happens in 1 row of 100; with one bit of 2^14 it was 1 of 4).  Only such rows compare their ids pair by
-// pair, which they pay for at their end (512 x 151,936 with 100 entries: 96 us, now 90).
+// distinct ids that happens in 1 row of 100; with one bit of 2^14 it was 1 of 4).  In the loss and the gradient made along with
+// it only such rows compare their ids pair by pair, which they pay for at their end (512 x 151,936 with 100 entries: 93 us, 100
+// if all rows did); sdm_rt_distill_grad does not know them and compares every row's.
 struct Target {
   int flags;
   int label;

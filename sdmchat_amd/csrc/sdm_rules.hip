@@ -31,9 +31,9 @@ struct RulesArgs {
 // rest counts its occurrences since.  Bound by memory, logits in and out, and by the history, which every slice of a row
 // reads again: so slices are as large as leaves every compute unit two workgroups, and a row's slices run on one XCD, whose
 // L2 then holds its history (workgroup i runs on XCD i mod 8).  The loads of logits, those of the history and the counting
-// wait in turn, so every wave that fits is there to overlap them: 256 x 131,072 bf16 with histories of 8,192 take 36 us (a
-// copy of as many bytes 30), with slices of 512 threads x 4 pieces 40, and with 8 tokens of a thread in flight, whose
-// registers leave room for half the waves, 42.
+// wait in turn, so every wave that fits is there to overlap them: 256 x 131,072 bf16 with histories of 8,192 take 36-38 us
+// (a copy of as many bytes 30; rows of 131,071, which begin at any element, 40), with slices of 512 threads x 4 pieces 40, and
+// with 8 tokens of a thread in flight, whose registers leave room for half the waves, 42.
 constexpr int kRulesThreads = 1024, kXcds = 8;
 
 template <typename T, int NP>
