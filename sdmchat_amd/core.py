@@ -1483,8 +1483,8 @@ class DistillFunction(torch.autograd.Function):
     """distill_loss on rows as an autograd function; it cannot be differentiated again.  A loss of one value computes its
     gradient with the loss (sdm_rt_distill_loss, one pass over the logits): the first backward hands it out, after
     sdm_rt_distill_grad has put it right if the gradient that comes in is not 1.  "none", a second backward, and one that is
-    captured into another graph than the loss (or that alone), take sdm_rt_distill_grad alone.  apply(logits [rows, vocab], top_ids, top_logits [rows, k], labels [rows] or None, dims) ->
-    loss, dims an _lib.SdmRtDistill."""
+    captured into another graph than the loss (or that alone), take sdm_rt_distill_grad alone.  apply(logits [rows, vocab],
+    top_ids, top_logits [rows, k], labels [rows] or None, dims) -> loss, dims an _lib.SdmRtDistill."""
 
     @staticmethod
     def forward(ctx, logits, ids, top, labels, dims):
@@ -1545,8 +1545,8 @@ def distill_loss(logits, top_ids, top_logits, *, temperature=1.0, labels=None, a
     shares add up) and top_logits [..., k], k at most 1,024; labels [...] int64 or int32 or None (ignore_index, or any id
     outside the vocabulary: no label).  Positions may lack either part, or both: those have loss 0 and gradient 0 whatever
     their logits hold.  reduction "mean" divides the sum by the number of positions with a target (0 if there is none),
-    "sum" does not, "none" gives float32 losses [...].  At most 2^21 positions.  Differentiable in logits, once; the teacher gets no gradient.  With
-    autograd recording, "mean" and "sum" compute the gradient along with the loss, so it takes its memory from then on."""
+    "sum" does not, "none" gives float32 losses [...].  At most 2^21 positions, temperature from 1e-18 to 1e18.
+    Differentiable in logits, once; the teacher gets no gradient.  With autograd recording, "mean" and "sum" compute the gradient along with the loss, so it takes its memory from then on."""
     dev = logits.device
     if dev.type != "cuda":
         raise RuntimeError("distill_loss needs ROCm device tensors")
