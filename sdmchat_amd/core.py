@@ -1546,7 +1546,8 @@ def distill_loss(logits, top_ids, top_logits, *, temperature=1.0, labels=None, a
     outside the vocabulary: no label).  Positions may lack either part, or both: those have loss 0 and gradient 0 whatever
     their logits hold.  reduction "mean" divides the sum by the number of positions with a target (0 if there is none),
     "sum" does not, "none" gives float32 losses [...].  At most 2^21 positions, temperature from 1e-18 to 1e18.
-    Differentiable in logits, once; the teacher gets no gradient.  With autograd recording, "mean" and "sum" compute the gradient along with the loss, so it takes its memory from then on."""
+    Differentiable in logits, once; the teacher gets no gradient.  With autograd recording, "mean" and "sum" compute the
+    gradient along with the loss, so it takes its memory from then on."""
     dev = logits.device
     if dev.type != "cuda":
         raise RuntimeError("distill_loss needs ROCm device tensors")
