@@ -549,6 +549,96 @@ uint64_t sdm_rt_capture_id(void* stream);
 int sdm_rt_append_tokens(int64_t* tokens, int64_t tokens_row_stride, int64_t width, int64_t* lengths,
                          const int64_t* new_ids, int64_t rows, void* stream);
 
+/* ---- a scored token, and the end of a training step: log probabilities, the gradients' norm, AdamW --------------- */
+
+/* Log probabilities of given tokens.  With l = z / temperature - log sum exp(z / temperature) over a row of logits z and
+ * p = exp(l):  logprob = l_target,  entropy = -sum p l,  and the top_k largest logits of the row (at equal logits the lower
+ * id first) with their l.  A target outside [0, vocab), or ignore_index, is none: logprob 0.  A logit of -inf has p = 0, is
+ * no alternative, and as a target gives -inf; a row has no more alternatives than other logits: the ids behind them are -1,
+ * their l -inf.  A row of nothing but -inf has entropy 0.  One with a NaN or +inf has NaN throughout (but for a target that
+ * is none) and ids -1. */
+typedef struct {
+  int64_t rows;          /* at most 2^21 */
+  int32_t vocab;         /* at most 2^24 */
+  int32_t top_k;         /* 0 to 256 */
+  float temperature;     /* 1e-18 to 1e18 */
+  int64_t ignore_index;
+} sdm_rt_logprob;
+
+/* Bytes of workspace sdm_rt_token_logprobs needs for logits of this type. */
+size_t sdm_rt_token_logprobs_workspace_bytes(const sdm_rt_logprob* dims, sdm_rt_dtype dtype);
+
+/* logits [rows][vocab] in dtype, any alignment of an element, row stride in elements (0: one row for all).  targets [rows]
+ * int64, or NULL: then logprobs is NULL.  Each of logprobs, entropy [rows] float32 is written where it is not NULL;
+ * top_ids [rows][top_k] int64 and top_logprobs [rows][top_k] float32 with top_k above 0; stats [rows][4] float32, 16-byte
+ * aligned, for sdm_rt_token_logprobs_grad, or NULL. */
+int sdm_rt_token_logprobs(const sdm_rt_logprob* dims, const void* logits, int64_t logits_row_stride, sdm_rt_dtype dtype,
+                          const int64_t* targets, float* logprobs, float* entropy, int64_t* top_ids, float* top_logprobs,
+                          float* stats, void* workspace, size_t workspace_bytes, void* stream);
+
+/* d_logits [rows][vocab] in dtype, every row written: the gradient of logprobs and entropy for d_logprobs and d_entropy,
+ * float32 on the device, [rows] with a stride in elements (0: one value for all), or NULL:
+ *   d z_j = (d_logprob (1[j = target] - p_j) - d_entropy p_j (l_j + entropy)) / temperature
+ * A row whose two gradients are 0 (d_logprob counts as 0 without a target) has gradient 0 whatever its logits hold.  It must
+ * not overlap the logits. */
+int sdm_rt_token_logprobs_grad(const sdm_rt_logprob* dims, const void* logits, int64_t logits_row_stride,
+                               sdm_rt_dtype dtype, const int64_t* targets, const float* stats, const float* d_logprobs,
+                               int64_t d_logprobs_stride, const float* d_entropy, int64_t d_entropy_stride,
+                               void* d_logits, int64_t d_logits_row_stride, void* stream);
+
+/* A tensor of a training step: n values of dtype at each of param and grad, dense and in the same order, any alignment of an
+ * element.  exp_avg, exp_avg_sq: float32 [n] each; or exp_avg the 8-bit moments of sdm_rt_moments_bytes(n) bytes, 8-byte
+ * aligned, and exp_avg_sq NULL.  All fields are 64 bits wide. */
+typedef struct {
+  void* param;
+  const void* grad;
+  void* exp_avg;
+  void* exp_avg_sq;
+  int64_t n;
+  int64_t dtype;
+} sdm_rt_tensor;
+
+/* Bytes of workspace sdm_rt_grad_norm needs (0 on sizes outside its limits). */
+size_t sdm_rt_grad_norm_workspace_bytes(const sdm_rt_tensor* tensors, int32_t count);
+
+/* norm[0] (float32, on the device) = the square root of the sum over all tensors of grad^2, in float64, in a fixed order.
+ * Reads grad, n and dtype of the tensors, an array on the host. */
+int sdm_rt_grad_norm(const sdm_rt_tensor* tensors, int32_t count, float* norm, void* workspace, size_t workspace_bytes,
+                     void* stream);
+
+/* One AdamW step on all tensors (an array on the host), in float32, rounded once to the parameter's dtype:
+ *   g = grad * min(1, max_norm / (norm + 1e-6))                     with norm; else g = grad
+ *   m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2
+ *   param = param (1 - lr weight_decay) - lr / (1 - beta1^t) m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
+ * The tensors must not overlap each other.
+ *
+ * Moments in 8 bits (state_bits 8): ceil(n / 128) blocks of 264 bytes, each the codes of 128 consecutive values of m, those
+ * of v, an exponent E of each, 6 bytes unused.  2^(E - 127) is the block's largest magnitude without its mantissa (twice that
+ * where the mantissa is over 1.875; E = 0: all zero).  A code of m is a sign bit, 4 bits e of exponent and 3 bits f of
+ * mantissa, of v 5 and 3: value = 2^(E - 127) (1 + f / 8) 2^(e - 15), of v 2^(e - 31), and with e = 0 that of e = 1 without
+ * the 1.  A new value between two codes takes the upper one with the probability that its place between them says, by a hash
+ * of its position in the list of tensors, seed and t; a v above 0 has no code 0.  A block with a value that is not finite (or
+ * from 2^127 on) reads as NaN. */
+typedef struct {
+  double lr, beta1, beta2, eps, weight_decay;
+  int64_t t;             /* the step's number, from 1 on; ignored with t_device */
+  int64_t* t_device;     /* NULL, or the number of steps so far on the device: one more is written before the step */
+  const float* lr_device;   /* NULL, or the learning rate on the device (with t_device) */
+  const float* norm;     /* NULL, or the gradients' norm on the device (sdm_rt_grad_norm) */
+  float max_norm;        /* with norm */
+  int32_t state_bits;    /* 32 or 8 */
+  uint32_t seed;         /* of the 8-bit moments' rounding */
+} sdm_rt_adamw_options;
+
+int sdm_rt_adamw(const sdm_rt_adamw_options* options, const sdm_rt_tensor* tensors, int32_t count, void* stream);
+
+/* Bytes of the 8-bit moments of n values. */
+int64_t sdm_rt_moments_bytes(int64_t n);
+
+/* The values that 8-bit moments stand for: n values of m and of v in dtype (bfloat16 holds them exactly).  tensors: exp_avg
+ * the moments, param where m goes, exp_avg_sq where v goes, n, and their dtype. */
+int sdm_rt_read_moments(const sdm_rt_tensor* tensors, int32_t count, void* stream);
+
 /* Description of the last failure on the calling thread ("" if none). */
 const char* sdm_rt_last_error(void);
 

@@ -94,6 +94,36 @@ class SdmRtRules(ctypes.Structure):
     ]
 
 
+class SdmRtLogprob(ctypes.Structure):
+    _fields_ = [
+        ("rows", c_i64),
+        ("vocab", ctypes.c_int32),
+        ("top_k", ctypes.c_int32),
+        ("temperature", ctypes.c_float),
+        ("ignore_index", c_i64),
+    ]
+
+
+TENSOR_FIELDS = 6   # sdm_rt_tensor: param, grad, exp_avg, exp_avg_sq, n, dtype, 64 bits each
+
+
+class SdmRtAdamwOptions(ctypes.Structure):
+    _fields_ = [
+        ("lr", ctypes.c_double),
+        ("beta1", ctypes.c_double),
+        ("beta2", ctypes.c_double),
+        ("eps", ctypes.c_double),
+        ("weight_decay", ctypes.c_double),
+        ("t", c_i64),
+        ("t_device", c_void_p),
+        ("lr_device", c_void_p),
+        ("norm", c_void_p),
+        ("max_norm", ctypes.c_float),
+        ("state_bits", ctypes.c_int32),
+        ("seed", ctypes.c_uint32),
+    ]
+
+
 class SdmRtGrads(ctypes.Structure):
     _fields_ = [
         ("d_kz", c_void_p),
@@ -223,6 +253,16 @@ SIGNATURES = {
     "sdm_rt_process_logits": (ctypes.c_int, [ctypes.POINTER(SdmRtRules), c_void_p, c_i64, ctypes.c_int, c_i64,
                                              ctypes.c_int32, c_void_p, c_i64, c_void_p]),
     "sdm_rt_append_tokens": (ctypes.c_int, [c_void_p, c_i64, c_i64, c_void_p, c_void_p, c_i64, c_void_p]),
+    "sdm_rt_token_logprobs_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(SdmRtLogprob), ctypes.c_int]),
+    "sdm_rt_token_logprobs": (ctypes.c_int, [ctypes.POINTER(SdmRtLogprob), c_void_p, c_i64, ctypes.c_int, c_void_p, c_void_p,
+                                             c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, ctypes.c_size_t, c_void_p]),
+    "sdm_rt_token_logprobs_grad": (ctypes.c_int, [ctypes.POINTER(SdmRtLogprob), c_void_p, c_i64, ctypes.c_int, c_void_p,
+                                                  c_void_p, c_void_p, c_i64, c_void_p, c_i64, c_void_p, c_i64, c_void_p]),
+    "sdm_rt_grad_norm_workspace_bytes": (ctypes.c_size_t, [c_void_p, ctypes.c_int32]),
+    "sdm_rt_grad_norm": (ctypes.c_int, [c_void_p, ctypes.c_int32, c_void_p, c_void_p, ctypes.c_size_t, c_void_p]),
+    "sdm_rt_adamw": (ctypes.c_int, [ctypes.POINTER(SdmRtAdamwOptions), c_void_p, ctypes.c_int32, c_void_p]),
+    "sdm_rt_moments_bytes": (c_i64, [c_i64]),
+    "sdm_rt_read_moments": (ctypes.c_int, [c_void_p, ctypes.c_int32, c_void_p]),
     "sdm_rt_status": (ctypes.c_int, [ctypes.POINTER(SdmRtDims), c_void_p, c_void_p]),
     "sdm_rt_set_wait_limit": (None, [c_i64]),
     "sdm_rt_set_crowded_threshold": (None, [ctypes.c_int32]),

@@ -4,8 +4,10 @@ Tensors must live on a ROCm device.  Activations are [B, T, width] with unit str
 uniform row stride (a slice of a wider fused projection output is fine).  All work is queued on the current torch
 stream; nothing synchronises.
 """
+import array
 import ctypes
 import math
+import typing
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -1727,3 +1729,286 @@ def append_tokens(tokens, lengths, new):
     new = new.contiguous()
     _launch(_lib.load().sdm_rt_append_tokens, tokens.get_device(), tokens.data_ptr(), tokens.stride(0) if B > 1 else width,
             width, lengths.data_ptr(), new.data_ptr(), B)
+
+
+class TokenLogprobs(typing.NamedTuple):
+    """What token_logprobs returns; None for what was not asked."""
+    logprobs: typing.Optional[torch.Tensor]       # [...] float32
+    entropy: typing.Optional[torch.Tensor]        # [...] float32
+    top_ids: typing.Optional[torch.Tensor]        # [..., top] int64
+    top_logprobs: typing.Optional[torch.Tensor]   # [..., top] float32
+
+
+def _logprobs(z, zs, targets, dims, entropy, stats):
+    n, k, at, lib = z.size(0), dims.top_k, ctypes.byref(dims), _lib.load()
+    empty = torch.empty
+    dev, code = z.device, _DT[z.dtype]
+    lp = None if targets is None else empty(n, dtype=torch.float32, device=dev)
+    h = empty(n, dtype=torch.float32, device=dev) if entropy else None
+    ids = empty((n, k), dtype=torch.int64, device=dev) if k else None
+    tops = empty((n, k), dtype=torch.float32, device=dev) if k else None
+    nbytes = lib.sdm_rt_token_logprobs_workspace_bytes(at, code)
+    ws = empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    _launch(lib.sdm_rt_token_logprobs, z.get_device(), at, z.data_ptr(), zs, code, _ptr(targets), _ptr(lp), _ptr(h), _ptr(ids),
+            _ptr(tops), _ptr(stats), _ptr(ws), nbytes)
+    return lp, h, ids, tops
+
+
+class LogprobFunction(torch.autograd.Function):
+    """token_logprobs on rows as an autograd function: differentiable in logits through the log probabilities and the entropy,
+    once.  apply(logits [rows, vocab], targets [rows] or None, dims, entropy) -> (logprobs, entropy, top_ids, top_logprobs),
+    dims an _lib.SdmRtLogprob."""
+
+    @staticmethod
+    def forward(ctx, logits, targets, dims, entropy):
+        z, zs = _read_rows(logits)
+        stats = torch.empty((z.size(0), 4), dtype=torch.float32, device=z.device)
+        out = _logprobs(z, zs, targets, dims, entropy, stats)
+        ctx.dims = dims
+        ctx.set_materialize_grads(False)
+        ctx.mark_non_differentiable(*(t for t in out[2:] if t is not None))
+        ctx.save_for_backward(z, targets, stats)
+        return out
+
+    @staticmethod
+    def backward(ctx, dlp, dh, dids, dtops):
+        return (_logprob_backward_recorded if torch.is_grad_enabled() else LogprobFunction.gradients)(ctx, dlp, dh, dids, dtops)
+
+    @staticmethod
+    def gradients(ctx, dlp, dh, dids, dtops):
+        z, targets, stats = ctx.saved_tensors
+        if dlp is None and dh is None:
+            return None, None, None, None
+        dz = z.new_empty(z.shape)
+        z, zs = _read_rows(z)
+        _launch(_lib.load().sdm_rt_token_logprobs_grad, z.get_device(), ctypes.byref(ctx.dims), z.data_ptr(), zs, _DT[z.dtype],
+                _ptr(targets), stats.data_ptr(), _ptr(dlp), 0 if dlp is None else dlp.stride(0), _ptr(dh),
+                0 if dh is None else dh.stride(0), dz.data_ptr(), z.size(1))
+        return dz, None, None, None
+
+
+_logprob_backward_recorded = once_differentiable(LogprobFunction.gradients)
+
+
+def token_logprobs(logits, targets=None, *, temperature=1.0, entropy=False, top=0, ignore_index=-100):
+    """Log probabilities of given tokens under softmax(logits / temperature), with the rows' entropies and top alternatives
+    where asked: a TokenLogprobs.
+
+    logits [..., vocab] float32 or bfloat16.  targets [...] int64 or int32, or None: logprobs [...] float32 are those of the
+    targets, 0 for ignore_index or any id outside the vocabulary.  entropy: [...] float32 in nats.  top: the row's top (at
+    most 256) tokens by falling logit, at equal logits the lower id first: top_ids [..., top] int64, top_logprobs [..., top]
+    float32 (distill_loss takes the two as a teacher's).
+
+    A logit of -inf is a token that cannot come: it is no alternative (the ids behind a row's last one are -1, their log
+    probabilities -inf), and as a target has -inf.  A row of nothing else has entropy 0 and gradient 0, one with a NaN or
+    +inf is NaN throughout with ids -1.  At most 2^21 rows, a vocabulary of 2^24, temperature from 1e-18 to 1e18.
+
+    Differentiable in logits through logprobs and entropy, once; the alternatives carry no gradient.  A row whose gradients
+    are all 0 has gradient 0 whatever its logits hold."""
+    name = "token_logprobs"
+    dev, shape = logits.device, logits.shape
+    if dev.type != "cuda":
+        raise RuntimeError(f"{name} needs ROCm device tensors")
+    if logits.dtype not in _DT:
+        raise ValueError(f"{name}: dtype {logits.dtype} is not float32 or bfloat16")
+    if not shape or not shape[-1]:
+        raise ValueError(f"{name}: logits must be [..., vocab], got {tuple(shape)}")
+    lead, V = shape[:-1], shape[-1]
+    if targets is None:
+        if not entropy and not top:
+            raise ValueError(f"{name}: neither targets, entropy nor top alternatives asked")
+    else:
+        if targets.shape != lead:
+            raise ValueError(f"{name}: targets {tuple(targets.shape)}, expected {tuple(lead)}")
+        if targets.device != dev:
+            _same_device(name, dev, targets=targets)
+        targets = _ids(name, "targets", targets)
+    if (V | top) >> 31:
+        _widths(name, vocab=V, top=top)
+    n = lead.numel()
+    flat = len(shape) == 2
+    rows = logits if flat else logits.reshape(n, V)
+    if not flat and targets is not None:
+        targets = targets.reshape(n)
+    dims = _lib.SdmRtLogprob(n, V, top, temperature, ignore_index)
+    if (logits.requires_grad and torch.is_grad_enabled()) or torch.autograd.forward_ad._current_level >= 0:
+        out = LogprobFunction.apply(rows, targets, dims, bool(entropy))
+    else:
+        rows, zs = _read_rows(rows)
+        out = _logprobs(rows, zs, targets, dims, entropy, None)
+    if flat:
+        return TokenLogprobs(*out)
+    return TokenLogprobs(*(None if t is None else t.reshape(lead + t.shape[1:]) for t in out))
+
+
+MOMENT_BLOCK, MOMENT_BYTES = 128, 264   # values that share the exponents of their 8-bit moments, a block's bytes
+
+
+def new_moments(t):
+    """The 8-bit moments of a parameter before its first step: zeros, uint8 [ceil(numel / 128), 264] (sdm_rt_adamw has the
+    layout)."""
+    return torch.zeros(-(-t.numel() // MOMENT_BLOCK), MOMENT_BYTES, dtype=torch.uint8, device=t.device)
+
+
+def _dense(t):
+    """Whether a tensor's values fill a stretch of memory, each once, whatever the order of its dimensions."""
+    if t.layout is not torch.strided:
+        return False
+    if t.is_contiguous():
+        return True
+    step = 1
+    for stride, size in sorted((st, n) for st, n in zip(t.stride(), t.shape) if n != 1):
+        if stride != step:
+            return False
+        step *= size
+    return True
+
+
+def _listed(name, **lists):
+    """Lists of equal length, not empty, on one GPU: (lists, device)."""
+    lists = {k: list(v) for k, v in lists.items()}
+    first = next(iter(lists.values()))
+    if not first:
+        raise ValueError(f"{name}: no tensors")
+    dev = first[0].device
+    if dev.type != "cuda":
+        raise RuntimeError(f"{name} needs ROCm device tensors")
+    for what, ts in lists.items():
+        if len(ts) != len(first):
+            raise ValueError(f"{name}: {len(ts)} {what} for {len(first)} {next(iter(lists))}")
+        for t in ts:
+            if t.device != dev:
+                raise ValueError(f"{name}: one of the {what} is on {t.device}, expected {dev}")
+    return list(lists.values()), dev
+
+
+def _float_code(name, what, t):
+    code = _DT.get(t.dtype)
+    if code is None:
+        raise ValueError(f"{name}: one of the {what} has dtype {t.dtype}, not float32 or bfloat16")
+    return code
+
+
+def _written(tensors):
+    """Tensors that a kernel has written in place: a graph that saved one must not read it again, and what is derived from one
+    is derived anew."""
+    torch.autograd.graph.increment_version([t for t in tensors if not t.is_inference()])
+
+
+def grad_norm(tensors):
+    """The norm of all of these tensors' values together, sqrt(sum of squares): a float32 scalar on their GPU.  float32 or
+    bfloat16 tensors, mixed; the squares are summed in float64 in a fixed order (deterministic)."""
+    (ts,), dev = _listed("grad_norm", tensors=tensors)
+    rows, held = [], []
+    for t in ts:
+        if not _dense(t):
+            if t.layout is not torch.strided:
+                raise ValueError(f"grad_norm: a tensor of layout {t.layout}")
+            t = t.contiguous()
+            held.append(t)
+        rows += (0, t.data_ptr(), 0, 0, t.numel(), _float_code("grad_norm", "tensors", t))
+    table = array.array("q", rows)
+    at, lib = table.buffer_info()[0], _lib.load()
+    out = torch.empty((), dtype=torch.float32, device=dev)
+    nbytes = lib.sdm_rt_grad_norm_workspace_bytes(at, len(ts))   # 0 outside the limits: the call below reports why
+    ws = torch.empty(nbytes // 8, dtype=torch.float64, device=dev)
+    _launch(lib.sdm_rt_grad_norm, out.get_device(), at, len(ts), out.data_ptr(), ws.data_ptr(), nbytes)
+    return out
+
+
+def adamw(params, grads, exp_avgs, exp_avg_sqs=None, *, step, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2,
+          max_norm=None, norm=None, seed=0):
+    """One AdamW step on all params in place (float32 arithmetic, each rounded once to its dtype):
+
+        g = grad * min(1, max_norm / (norm + 1e-6))        with max_norm; norm: that of all grads (grad_norm), or the one given
+        exp_avg = b1 exp_avg + (1 - b1) g;  exp_avg_sq = b2 exp_avg_sq + (1 - b2) g^2
+        param = param (1 - lr weight_decay) - lr / (1 - b1^t) exp_avg / (sqrt(exp_avg_sq) / sqrt(1 - b2^t) + eps)
+
+    params and grads: float32 or bfloat16 tensors (mixed in a list, a grad of its param's dtype and shape), dense, on one GPU.
+    The moments: exp_avgs and exp_avg_sqs float32 like the params; or exp_avgs alone, the uint8 tensors of new_moments that
+    hold both in 8 bits (rounded by chance, by a hash of position, seed and step: the same inputs give the same bits).  None
+    of the tensors may overlap another that is written.  step: t, an int from 1 on; or an int64 tensor of one element on the
+    GPU with the number of steps so far, which is counted up (a step that a graph captures); then lr may be a float32 tensor of one
+    element too.  Returns the norm (float32 scalar on the GPU) with max_norm, else None."""
+    name = "adamw"
+    eight = exp_avg_sqs is None
+    if eight:
+        (ps, gs, ms), dev = _listed(name, params=params, grads=grads, exp_avgs=exp_avgs)
+        vs = ms
+    else:
+        (ps, gs, ms, vs), dev = _listed(name, params=params, grads=grads, exp_avgs=exp_avgs, exp_avg_sqs=exp_avg_sqs)
+    rows, held, count = [], [], len(ps)
+    for i in range(count):
+        p, g, m, v = ps[i], gs[i], ms[i], vs[i]
+        n = p.numel()
+        if g.dtype != p.dtype or g.shape != p.shape:
+            raise ValueError(f"{name}: a grad of {g.dtype} {tuple(g.shape)} for a param of {p.dtype} {tuple(p.shape)}")
+        if not _dense(p):
+            raise ValueError(f"{name}: a param {tuple(p.shape)} of strides {tuple(p.stride())}: its values must be dense")
+        if g.layout is not torch.strided:
+            raise ValueError(f"{name}: a grad of layout {g.layout}")
+        if not p.is_contiguous() or not g.is_contiguous():
+            if g.stride() != p.stride():
+                g = torch.empty_like(p).copy_(g)
+                held.append(g)
+        if eight:
+            if m.dtype != torch.uint8 or tuple(m.shape) != (-(-n // MOMENT_BLOCK), MOMENT_BYTES) or not m.is_contiguous():
+                raise ValueError(f"{name}: 8-bit moments must be contiguous uint8 {(-(-n // MOMENT_BLOCK), MOMENT_BYTES)} for "
+                                 f"a param {tuple(p.shape)}, got {m.dtype} {tuple(m.shape)}")
+        else:
+            for t in (m, v):
+                if t.dtype != torch.float32 or t.shape != p.shape or (t.stride() != p.stride() and not (
+                        t.is_contiguous() and p.is_contiguous())):
+                    raise ValueError(f"{name}: moments must be float32 {tuple(p.shape)} of the param's strides "
+                                     f"{tuple(p.stride())}, got {t.dtype} {tuple(t.shape)} of {tuple(t.stride())}")
+        rows += (p.data_ptr(), g.data_ptr(), m.data_ptr(), 0 if eight else v.data_ptr(), n, _float_code(name, "params", p))
+    table = array.array("q", rows)
+    written = [a for k in ((0, 2) if eight else (0, 2, 3)) for a, n in zip(rows[k::6], rows[4::6]) if n]
+    if len(set(written)) != len(written) or not set(written).isdisjoint(rows[1::6]):
+        raise ValueError(f"{name}: a tensor occurs twice")
+    t_dev, lr_dev = None, None
+    if torch.is_tensor(step):
+        if step.dtype != torch.int64 or step.numel() != 1 or step.device != dev:
+            raise ValueError(f"{name}: a step on the device must be int64 with one element on {dev}")
+        t_dev, step = step, 0
+    if torch.is_tensor(lr):
+        if lr.dtype != torch.float32 or lr.numel() != 1 or lr.device != dev or t_dev is None:
+            raise ValueError(f"{name}: an lr on the device must be float32 with one element on {dev}, beside a step there")
+        lr_dev, lr = lr, 0.0
+    if max_norm is None:
+        if norm is not None:
+            raise ValueError(f"{name}: norm needs max_norm")
+    elif norm is None:
+        norm = grad_norm(gs)
+    elif norm.dtype != torch.float32 or norm.numel() != 1 or norm.device != dev:
+        raise ValueError(f"{name}: norm must be float32 with one element on {dev}")
+    options = _lib.SdmRtAdamwOptions(lr, betas[0], betas[1], eps, weight_decay, step, _ptr(t_dev), _ptr(lr_dev), _ptr(norm),
+                                     1.0 if max_norm is None else max_norm, 8 if eight else 32, seed & 0xffffffff)
+    _launch(_lib.load().sdm_rt_adamw, ps[0].get_device(), ctypes.byref(options), table.buffer_info()[0], count)
+    _written(ps)
+    _written(ms)
+    if not eight:
+        _written(vs)
+    if t_dev is not None:
+        _written([t_dev])
+    return norm
+
+
+def read_moments(moments, exp_avgs, exp_avg_sqs):
+    """Writes the values that 8-bit moments (new_moments) stand for into exp_avgs and exp_avg_sqs: tensors of the params'
+    sizes, contiguous, bfloat16 (which holds them exactly) or float32."""
+    name = "read_moments"
+    (ss, ms, vs), dev = _listed(name, moments=moments, exp_avgs=exp_avgs, exp_avg_sqs=exp_avg_sqs)
+    rows = []
+    for s, m, v in zip(ss, ms, vs):
+        n = m.numel()
+        if s.dtype != torch.uint8 or tuple(s.shape) != (-(-n // MOMENT_BLOCK), MOMENT_BYTES) or not s.is_contiguous():
+            raise ValueError(f"{name}: moments must be contiguous uint8 {(-(-n // MOMENT_BLOCK), MOMENT_BYTES)} for {n} values, "
+                             f"got {s.dtype} {tuple(s.shape)}")
+        if v.numel() != n or v.dtype != m.dtype or not m.is_contiguous() or not v.is_contiguous():
+            raise ValueError(f"{name}: exp_avgs and exp_avg_sqs must be contiguous and alike in size and dtype")
+        rows += (m.data_ptr(), 0, s.data_ptr(), v.data_ptr(), n, _float_code(name, "exp_avgs", m))
+    table = array.array("q", rows)
+    _launch(_lib.load().sdm_rt_read_moments, ss[0].get_device(), table.buffer_info()[0], len(ss))
+    _written(ms)
+    _written(vs)

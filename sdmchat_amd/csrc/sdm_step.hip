@@ -1,0 +1,502 @@
+// sdm_step.hip -- the end of a training step over a whole model's tensors: the norm of the gradients (sdm_rt_grad_norm), the
+// AdamW step with its moments in 32 or in 8 bits (sdm_rt_adamw), and the values of 8-bit moments (sdm_rt_read_moments).
+//
+// A call takes a list of tensors.  Their addresses and sizes ride in the kernel's arguments (4 KB of them at most), some 80
+// to a launch: nothing is copied to the device, a captured launch holds all it needs, and no list has to outlive the call.
+// A tensor is cut into chunks, one a workgroup; a workgroup finds its tensor by its index in the chunks of the launch.
+#include "sdm_vocab.h"
+
+namespace sdmrt {
+
+constexpr int kStepThreads = 256;
+constexpr int kBlock = 128;                       // values of a block of 8-bit moments
+constexpr int kBlockBytes = 2 * kBlock + 8;       // codes of m, codes of v, two exponents, 6 unused
+
+// -- lists of tensors in kernel arguments -----------------------------------------------------------------------------
+struct StepTensor {
+  char* p;
+  const char* g;
+  char* m;
+  char* v;
+  int64_t n;
+  uint32_t chunk;   // its first chunk in this launch
+  uint32_t flags;   // bit 0: bfloat16
+  uint32_t block;   // the blocks of the tensors before it in the call
+  uint32_t pad;
+};
+template <int N>
+struct StepTable {
+  StepTensor t[N];
+  int count;
+};
+constexpr int kStepTensors = 68;   // 56 bytes each and the options: under 4 KB
+
+// the tensor of a chunk: the last one that begins at or before it
+template <int N>
+__device__ __forceinline__ int tensor_of(const StepTable<N>& table, uint32_t chunk) {
+  int lo = 0, hi = table.count - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) / 2;
+    if (table.t[mid].chunk <= chunk)
+      lo = mid;
+    else
+      hi = mid - 1;
+  }
+  return lo;
+}
+
+// N values of T at p, of which the first n are there (the others 0)
+template <typename T, int N>
+__device__ __forceinline__ void load_values(const T* p, int64_t n, float (&v)[N]) {
+  if (n >= N) {
+    T x[N];
+    __builtin_memcpy(x, p, sizeof(x));
+#pragma unroll
+    for (int e = 0; e < N; ++e) v[e] = to_f32(x[e]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; ++e) v[e] = e < n ? to_f32(p[e]) : 0.f;
+  }
+}
+template <typename T, int N>
+__device__ __forceinline__ void store_values(T* p, int64_t n, const float (&v)[N]) {
+  if (n >= N) {
+    if constexpr (sizeof(T) == 2) {
+      uint32_t w[N / 2];
+#pragma unroll
+      for (int e = 0; e < N / 2; ++e) w[e] = pack_bf16(v[2 * e], v[2 * e + 1]);
+      __builtin_memcpy(p, w, sizeof(w));
+    } else {
+      __builtin_memcpy(p, v, sizeof(v));
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; ++e)
+      if (e < n) p[e] = from_f32<T>(v[e]);
+  }
+}
+
+// -- the gradients' norm ----------------------------------------------------------------------------------------------
+constexpr int kNormChunk = 16384;
+
+__device__ __forceinline__ double wave_add(double v) {
+  for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d);
+  return v;
+}
+
+template <typename T>
+__device__ __forceinline__ double sum_squares(const T* g, int64_t n) {
+  constexpr int kN = 16 / static_cast<int>(sizeof(T));
+  double s = 0.0;
+  for (int64_t i = threadIdx.x * kN; i < n; i += kStepThreads * kN) {
+    float v[kN];
+    load_values(g + i, n - i, v);
+#pragma unroll
+    for (int e = 0; e < kN; ++e) s = fma(static_cast<double>(v[e]), static_cast<double>(v[e]), s);
+  }
+  return s;
+}
+
+// Each chunk's sum of squares in float64: no gradient is too large or too small for its square, and the order is fixed.
+__global__ void __launch_bounds__(kStepThreads) norm_kernel(StepTable<kStepTensors> table, double* __restrict__ partial) {
+  __shared__ double red[kStepThreads / 64];
+  const StepTensor& t = table.t[tensor_of(table, blockIdx.x)];
+  const int64_t begin = static_cast<int64_t>(blockIdx.x - t.chunk) * kNormChunk;
+  const int64_t n = min(t.n - begin, static_cast<int64_t>(kNormChunk));
+  double s = t.flags & 1 ? sum_squares(reinterpret_cast<const bf16_t*>(t.g) + begin, n)
+                         : sum_squares(reinterpret_cast<const float*>(t.g) + begin, n);
+  s = wave_add(s);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < kStepThreads / 64; ++w) s += red[w];
+    partial[blockIdx.x] = s;
+  }
+}
+
+__global__ void __launch_bounds__(1024) norm_join_kernel(const double* __restrict__ partial, int n, float* __restrict__ norm) {
+  __shared__ double red[16];
+  double s = 0.0;
+  for (int i = threadIdx.x; i < n; i += 1024) s += partial[i];
+  s = wave_add(s);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < 16; ++w) s += red[w];
+    *norm = static_cast<float>(sqrt(s));
+  }
+}
+
+// -- moments in 8 bits ------------------------------------------------------------------------------------------------
+// The hash that decides the rounding of a value at position i in step t: two multiplications by odd numbers (from the golden
+// ratio and the square root of 3) with shifts between them.  Its upper half is for m, its lower half for v.
+__host__ __device__ __forceinline__ uint32_t mix(uint32_t x) {
+  x = (x ^ (x >> 16)) * 2654435761u;
+  x = (x ^ (x >> 15)) * 3144134277u;
+  return x ^ (x >> 16);
+}
+__host__ __device__ __forceinline__ uint32_t step_key(uint32_t seed, int64_t t) {
+  return mix(seed + static_cast<uint32_t>(t) * 2654435761u);
+}
+
+// the exponent of a block whose largest magnitude has these bits: 255 where it is not finite or from 2^127 on
+__device__ __forceinline__ uint32_t block_exponent(uint32_t bits) {
+  const uint32_t e = (bits + 0xfffffu) >> 23;
+  return e >= 254 ? 255 : e;
+}
+__device__ __forceinline__ float block_scale(uint32_t e) { return __uint_as_float(e == 255 ? 0x7fc00000u : e << 23); }
+
+// A code's bits, put where float32 has its exponent and mantissa, are the value times a power of two: float32's own values
+// below its least normal one do for e = 0.  So decoding is a shift and two products, and encoding two products, the addition
+// of the random bits below the code's last place, and a shift, whatever the value's size.  TOP: the code's largest exponent.
+template <int TOP>
+__device__ __forceinline__ float decode(uint32_t magnitude, uint32_t sign, float scale) {
+  constexpr float up = TOP == 15 ? 0x1p112f : 0x1p96f;   // 2^(127 - TOP)
+  return __uint_as_float(magnitude << 20 | sign) * up * scale;
+}
+template <int TOP>
+__device__ __forceinline__ uint32_t encode(float x, float inv_scale, uint32_t random16) {
+  constexpr float down = TOP == 15 ? 0x1p-112f : 0x1p-96f;
+  return (__float_as_uint(fabsf(x) * inv_scale * down) + (random16 << 4)) >> 20;
+}
+
+// the maximum over a row of 16 lanes, in each of them
+__device__ __forceinline__ uint32_t row16_max(uint32_t v) {
+  v = max(v, static_cast<uint32_t>(dpp_rows<0xb1, 0xf>(0, static_cast<int>(v))));
+  v = max(v, static_cast<uint32_t>(dpp_rows<0x4e, 0xf>(0, static_cast<int>(v))));
+  v = max(v, static_cast<uint32_t>(dpp_rows<0x141, 0xf>(0, static_cast<int>(v))));
+  return max(v, static_cast<uint32_t>(dpp_rows<0x140, 0xf>(0, static_cast<int>(v))));
+}
+
+// -- the step ---------------------------------------------------------------------------------------------------------
+struct StepArgs {
+  float b1, c1, b2, c2, eps;      // c: 1 - b
+  float decay, size, r2;          // 1 - lr weight_decay, lr / (1 - beta1^t), 1 / sqrt(1 - beta2^t)
+  float max_norm;
+  uint32_t key, seed;
+  const float* norm;
+  const int64_t* t_device;
+  const float* lr_device;
+  double lr, weight_decay, log_b1, log_b2;
+};
+
+__global__ void count_step_kernel(int64_t* t) { *t += 1; }
+
+// What of the arguments depends on the device's step and learning rate.
+__device__ __forceinline__ void read_step(StepArgs& a) {
+  const int64_t t = *a.t_device;
+  const double lr = a.lr_device ? static_cast<double>(*a.lr_device) : a.lr;
+  a.decay = static_cast<float>(1.0 - lr * a.weight_decay);
+  a.size = static_cast<float>(lr / -expm1(static_cast<double>(t) * a.log_b1));
+  a.r2 = static_cast<float>(1.0 / sqrt(-expm1(static_cast<double>(t) * a.log_b2)));
+  a.key = step_key(a.seed, t);
+}
+
+// One value's new moments and parameter.  Every product and sum of the moments is rounded by itself, as the formula is
+// written: their codes in 8 bits then do not hang on what a compiler fuses.
+__device__ __forceinline__ void step_value(const StepArgs& a, float clip, float g, float& p, float& m, float& v) {
+#pragma clang fp contract(off)
+  g = g * clip;
+  m = m * a.b1 + g * a.c1;
+  v = v * a.b2 + g * g * a.c2;
+  const float d = __builtin_amdgcn_sqrtf(v) * a.r2 + a.eps;
+  p = p * a.decay - m * a.size * __builtin_amdgcn_rcpf(d);
+}
+
+constexpr int kStepChunk = 4096;
+
+template <typename T>
+__device__ __forceinline__ void step_chunk32(const StepArgs& a, float clip, const StepTensor& t, int64_t begin, int64_t n) {
+  T* p = reinterpret_cast<T*>(t.p) + begin;
+  const T* g = reinterpret_cast<const T*>(t.g) + begin;
+  float* m = reinterpret_cast<float*>(t.m) + begin;
+  float* v = reinterpret_cast<float*>(t.v) + begin;
+  for (int64_t i = threadIdx.x * 4; i < n; i += kStepThreads * 4) {
+    float pv[4], gv[4], mv[4], vv[4];
+    load_values(p + i, n - i, pv);
+    load_values(g + i, n - i, gv);
+    load_values(m + i, n - i, mv);
+    load_values(v + i, n - i, vv);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) step_value(a, clip, gv[e], pv[e], mv[e], vv[e]);
+    store_values(p + i, n - i, pv);
+    store_values(m + i, n - i, mv);
+    store_values(v + i, n - i, vv);
+  }
+}
+
+// Sixteen lanes hold a block, 8 values each: its maxima come from four DPP steps.
+template <typename T>
+__device__ __forceinline__ void step_chunk8(const StepArgs& a, float clip, const StepTensor& t, int64_t begin, int64_t n) {
+  T* p = reinterpret_cast<T*>(t.p) + begin;
+  const T* g = reinterpret_cast<const T*>(t.g) + begin;
+  const int64_t whole = (n + kBlock - 1) / kBlock * kBlock;
+  for (int64_t i = threadIdx.x * 8; i < whole; i += kStepThreads * 8) {
+    const int64_t block = (begin + i) / kBlock;
+    char* state = t.m + block * kBlockBytes;
+    const int at = static_cast<int>(i % kBlock);
+    const uint2 cm = *reinterpret_cast<const uint2*>(state + at), cv = *reinterpret_cast<const uint2*>(state + kBlock + at);
+    const uint32_t e = *reinterpret_cast<const uint16_t*>(state + 2 * kBlock);
+    float pv[8], gv[8], mv[8], vv[8];
+    load_values(p + i, n - i, pv);
+    load_values(g + i, n - i, gv);
+    const float sm = block_scale(e & 255), sv = block_scale(e >> 8);
+    const uint32_t counter = t.block * static_cast<uint32_t>(kBlock) + static_cast<uint32_t>(begin + i) + a.key;
+    uint32_t am = 0, av = 0;
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      const uint32_t wm = (q < 4 ? cm.x : cm.y) >> (8 * (q & 3)), wv = (q < 4 ? cv.x : cv.y) >> (8 * (q & 3));
+      mv[q] = decode<15>(wm & 127, (wm & 128) << 24, sm);
+      vv[q] = decode<31>(wv & 255, 0, sv);
+      step_value(a, clip, gv[q], pv[q], mv[q], vv[q]);
+      if (i + q >= n) mv[q] = vv[q] = 0.f;
+      am = max(am, __float_as_uint(mv[q]) & 0x7fffffffu);
+      av = max(av, __float_as_uint(vv[q]) & 0x7fffffffu);
+    }
+    store_values(p + i, n - i, pv);
+    const uint32_t em = block_exponent(row16_max(am)), ev = block_exponent(row16_max(av));
+    const float im = __uint_as_float((254 - min(em, 254u)) << 23), iv = __uint_as_float((254 - min(ev, 254u)) << 23);
+    uint2 nm = make_uint2(0, 0), nv = make_uint2(0, 0);
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      const uint32_t u = mix(counter + q);
+      uint32_t c = encode<15>(mv[q], im, u >> 16) | (__float_as_uint(mv[q]) >> 24 & 128);
+      uint32_t d = max(encode<31>(vv[q], iv, u & 0xffff), vv[q] > 0.f ? 1u : 0u);
+      if (em == 0 || em == 255) c = 0;
+      if (ev == 0 || ev == 255) d = 0;
+      (q < 4 ? nm.x : nm.y) |= c << (8 * (q & 3));
+      (q < 4 ? nv.x : nv.y) |= d << (8 * (q & 3));
+    }
+    *reinterpret_cast<uint2*>(state + at) = nm;
+    *reinterpret_cast<uint2*>(state + kBlock + at) = nv;
+    if (at == 0) *reinterpret_cast<uint16_t*>(state + 2 * kBlock) = static_cast<uint16_t>(em | ev << 8);
+  }
+}
+
+template <int BITS, bool DEVICE>
+__global__ void __launch_bounds__(kStepThreads) adamw_kernel(StepTable<kStepTensors> table, StepArgs a) {
+  if constexpr (DEVICE) read_step(a);
+  const StepTensor& t = table.t[tensor_of(table, blockIdx.x)];
+  const int64_t begin = static_cast<int64_t>(blockIdx.x - t.chunk) * kStepChunk;
+  const int64_t n = min(t.n - begin, static_cast<int64_t>(kStepChunk));
+  // a norm that is NaN makes the gradients NaN, as a product with it would
+  float clip = 1.f;
+  if (a.norm) {
+    clip = a.max_norm / (*a.norm + 1e-6f);
+    clip = clip > 1.f ? 1.f : clip;
+  }
+  if constexpr (BITS == 32) {
+    if (t.flags & 1)
+      step_chunk32<bf16_t>(a, clip, t, begin, n);
+    else
+      step_chunk32<float>(a, clip, t, begin, n);
+  } else {
+    if (t.flags & 1)
+      step_chunk8<bf16_t>(a, clip, t, begin, n);
+    else
+      step_chunk8<float>(a, clip, t, begin, n);
+  }
+}
+
+// -- the values of 8-bit moments --------------------------------------------------------------------------------------
+template <typename T>
+__device__ __forceinline__ void read_chunk(const StepTensor& t, int64_t begin, int64_t n) {
+  T* m = reinterpret_cast<T*>(t.p) + begin;
+  T* v = reinterpret_cast<T*>(t.v) + begin;
+  for (int64_t i = threadIdx.x * 8; i < n; i += kStepThreads * 8) {
+    const char* state = t.m + (begin + i) / kBlock * kBlockBytes;
+    const int at = static_cast<int>(i % kBlock);
+    const uint2 cm = *reinterpret_cast<const uint2*>(state + at), cv = *reinterpret_cast<const uint2*>(state + kBlock + at);
+    const uint32_t e = *reinterpret_cast<const uint16_t*>(state + 2 * kBlock);
+    const float sm = block_scale(e & 255), sv = block_scale(e >> 8);
+    float mv[8], vv[8];
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      const uint32_t wm = (q < 4 ? cm.x : cm.y) >> (8 * (q & 3)), wv = (q < 4 ? cv.x : cv.y) >> (8 * (q & 3));
+      mv[q] = decode<15>(wm & 127, (wm & 128) << 24, sm);
+      vv[q] = decode<31>(wv & 255, 0, sv);
+    }
+    store_values(m + i, n - i, mv);
+    store_values(v + i, n - i, vv);
+  }
+}
+
+__global__ void __launch_bounds__(kStepThreads) read_moments_kernel(StepTable<kStepTensors> table) {
+  const StepTensor& t = table.t[tensor_of(table, blockIdx.x)];
+  const int64_t begin = static_cast<int64_t>(blockIdx.x - t.chunk) * kStepChunk;
+  const int64_t n = min(t.n - begin, static_cast<int64_t>(kStepChunk));
+  if (t.flags & 1)
+    read_chunk<bf16_t>(t, begin, n);
+  else
+    read_chunk<float>(t, begin, n);
+}
+
+// -- host -------------------------------------------------------------------------------------------------------------
+static_assert(sizeof(StepTable<kStepTensors>) + sizeof(StepArgs) + 16 <= 4096, "kernel arguments");
+
+inline int64_t chunks_of(int64_t n, int chunk) { return (n + chunk - 1) / chunk; }
+
+// Every check that needs no device; total: the chunks of all tensors.
+inline int check_tensors(const sdm_rt_tensor* t, int32_t count, int chunk, int64_t* total) {
+  if (count < 0 || (count > 0 && !t)) return set_err(SDM_RT_EINVAL, "count must be >= 0, tensors not NULL");
+  *total = 0;
+  for (int32_t i = 0; i < count; ++i) {
+    if (t[i].n < 0) return set_err(SDM_RT_EINVAL, "tensor %d: n must be >= 0", i);
+    if (t[i].dtype != SDM_RT_F32 && t[i].dtype != SDM_RT_BF16)
+      return set_err(SDM_RT_EINVAL, "tensor %d: unknown dtype %lld", i, (long long)t[i].dtype);
+    if (t[i].n > (int64_t{1} << 38)) return set_err(SDM_RT_EUNSUPPORTED, "tensor %d: n must be at most 2^38", i);
+    *total += chunks_of(t[i].n, chunk);
+  }
+  if (*total > (int64_t{1} << 23)) return set_err(SDM_RT_EUNSUPPORTED, "too many values in one call");
+  return SDM_RT_OK;
+}
+
+// launch(table, chunks of the launch, chunks before it) over the list, as many tensors at a time as a launch takes
+template <typename F>
+void for_tables(const sdm_rt_tensor* t, int32_t count, int chunk, F launch) {
+  StepTable<kStepTensors> table;
+  table.count = 0;
+  int64_t chunks = 0, before = 0, blocks = 0;
+  auto flush = [&] {
+    if (table.count) launch(table, static_cast<unsigned>(chunks), before);
+    before += chunks;
+    chunks = table.count = 0;
+  };
+  for (int32_t i = 0; i < count; ++i) {
+    if (t[i].n == 0) continue;
+    if (table.count == kStepTensors) flush();
+    StepTensor& s = table.t[table.count++];
+    s.p = static_cast<char*>(t[i].param);
+    s.g = static_cast<const char*>(t[i].grad);
+    s.m = static_cast<char*>(t[i].exp_avg);
+    s.v = static_cast<char*>(t[i].exp_avg_sq);
+    s.n = t[i].n;
+    s.chunk = static_cast<uint32_t>(chunks);
+    s.flags = t[i].dtype == SDM_RT_BF16;
+    s.block = static_cast<uint32_t>(blocks);
+    chunks += chunks_of(t[i].n, chunk);
+    blocks += chunks_of(t[i].n, kBlock);
+  }
+  flush();
+}
+
+}  // namespace sdmrt
+
+using namespace sdmrt;
+
+extern "C" {
+
+size_t sdm_rt_grad_norm_workspace_bytes(const sdm_rt_tensor* tensors, int32_t count) {
+  int64_t total;
+  return check_tensors(tensors, count, kNormChunk, &total) ? 0 : static_cast<size_t>(total) * sizeof(double);
+}
+
+int sdm_rt_grad_norm(const sdm_rt_tensor* tensors, int32_t count, float* norm, void* workspace, size_t workspace_bytes,
+                     void* stream) {
+  g_err[0] = 0;
+  int64_t total;
+  if (int rc = check_tensors(tensors, count, kNormChunk, &total)) return rc;
+  for (int32_t i = 0; i < count; ++i)
+    if (tensors[i].n && !tensors[i].grad) return set_err(SDM_RT_EINVAL, "tensor %d: grad is NULL", i);
+  if (!norm) return set_err(SDM_RT_EINVAL, "norm is NULL");
+  const size_t need = static_cast<size_t>(total) * sizeof(double);
+  if (need && (!workspace || workspace_bytes < need))
+    return set_err(SDM_RT_ENOSPACE, "workspace of %zu bytes, %zu needed", workspace ? workspace_bytes : 0, need);
+  if (reinterpret_cast<uintptr_t>(workspace) % 8) return set_err(SDM_RT_EINVAL, "workspace must be 8-byte aligned");
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  double* partial = static_cast<double*>(workspace);
+  for_tables(tensors, count, kNormChunk, [&](const StepTable<kStepTensors>& table, unsigned chunks, int64_t before) {
+    hipLaunchKernelGGL(norm_kernel, dim3(chunks), dim3(kStepThreads), 0, st, table, partial + before);
+  });
+  hipLaunchKernelGGL(norm_join_kernel, dim3(1), dim3(1024), 0, st, partial, static_cast<int>(total), norm);
+  return check_launch("grad_norm");
+}
+
+int sdm_rt_adamw(const sdm_rt_adamw_options* o, const sdm_rt_tensor* tensors, int32_t count, void* stream) {
+  g_err[0] = 0;
+  if (!o) return set_err(SDM_RT_EINVAL, "options is NULL");
+  if (!(o->beta1 >= 0.0 && o->beta1 < 1.0) || !(o->beta2 >= 0.0 && o->beta2 < 1.0))
+    return set_err(SDM_RT_EINVAL, "beta1 and beta2 must be in [0, 1)");
+  if (!(o->eps >= 0.0) || !std::isfinite(o->eps) || !(o->weight_decay >= 0.0) || !std::isfinite(o->weight_decay))
+    return set_err(SDM_RT_EINVAL, "eps and weight_decay must be finite and >= 0");
+  if (!(o->lr_device && o->t_device) && (!(o->lr >= 0.0) || !std::isfinite(o->lr)))
+    return set_err(SDM_RT_EINVAL, "lr must be finite and >= 0");
+  if (o->lr_device && !o->t_device) return set_err(SDM_RT_EINVAL, "lr_device needs t_device");
+  if (!o->t_device && o->t < 1) return set_err(SDM_RT_EINVAL, "t must be >= 1");
+  if (o->norm && !(o->max_norm > 0.f)) return set_err(SDM_RT_EINVAL, "max_norm must be positive");
+  if (o->state_bits != 32 && o->state_bits != 8) return set_err(SDM_RT_EINVAL, "state_bits must be 32 or 8");
+  int64_t total;
+  if (int rc = check_tensors(tensors, count, kStepChunk, &total)) return rc;
+  for (int32_t i = 0; i < count; ++i) {
+    const sdm_rt_tensor& t = tensors[i];
+    if (t.n == 0) continue;
+    if (!t.param || !t.grad || !t.exp_avg || (o->state_bits == 32) != (t.exp_avg_sq != nullptr))
+      return set_err(SDM_RT_EINVAL, "tensor %d: param, grad and exp_avg must not be NULL, exp_avg_sq NULL for 8 bits alone", i);
+    if (o->state_bits == 8 && reinterpret_cast<uintptr_t>(t.exp_avg) % 8)
+      return set_err(SDM_RT_EINVAL, "tensor %d: 8-bit moments must be 8-byte aligned", i);
+  }
+  if (total == 0 && !o->t_device) return SDM_RT_OK;
+  StepArgs a{};
+  a.b1 = static_cast<float>(o->beta1);
+  a.c1 = static_cast<float>(1.0 - o->beta1);
+  a.b2 = static_cast<float>(o->beta2);
+  a.c2 = static_cast<float>(1.0 - o->beta2);
+  a.eps = static_cast<float>(o->eps);
+  a.max_norm = o->max_norm;
+  a.norm = o->norm;
+  a.seed = o->seed;
+  a.lr = o->lr;
+  a.weight_decay = o->weight_decay;
+  if (o->t_device) {
+    a.t_device = o->t_device;
+    a.lr_device = o->lr_device;
+    a.log_b1 = std::log(o->beta1);
+    a.log_b2 = std::log(o->beta2);
+  } else {
+    const double t = static_cast<double>(o->t);
+    a.decay = static_cast<float>(1.0 - o->lr * o->weight_decay);
+    a.size = static_cast<float>(o->lr / (1.0 - std::pow(o->beta1, t)));
+    a.r2 = static_cast<float>(1.0 / std::sqrt(1.0 - std::pow(o->beta2, t)));
+    a.key = step_key(o->seed, o->t);
+  }
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (o->t_device) hipLaunchKernelGGL(count_step_kernel, dim3(1), dim3(1), 0, st, o->t_device);
+  for_tables(tensors, count, kStepChunk, [&](const StepTable<kStepTensors>& table, unsigned chunks, int64_t) {
+    const dim3 grid(chunks), threads(kStepThreads);
+    if (o->state_bits == 32) {
+      if (o->t_device)
+        hipLaunchKernelGGL((adamw_kernel<32, true>), grid, threads, 0, st, table, a);
+      else
+        hipLaunchKernelGGL((adamw_kernel<32, false>), grid, threads, 0, st, table, a);
+    } else {
+      if (o->t_device)
+        hipLaunchKernelGGL((adamw_kernel<8, true>), grid, threads, 0, st, table, a);
+      else
+        hipLaunchKernelGGL((adamw_kernel<8, false>), grid, threads, 0, st, table, a);
+    }
+  });
+  return check_launch("adamw");
+}
+
+int64_t sdm_rt_moments_bytes(int64_t n) { return n > 0 ? (n + kBlock - 1) / kBlock * kBlockBytes : 0; }
+
+int sdm_rt_read_moments(const sdm_rt_tensor* tensors, int32_t count, void* stream) {
+  g_err[0] = 0;
+  int64_t total;
+  if (int rc = check_tensors(tensors, count, kStepChunk, &total)) return rc;
+  for (int32_t i = 0; i < count; ++i) {
+    const sdm_rt_tensor& t = tensors[i];
+    if (t.n == 0) continue;
+    if (!t.param || !t.exp_avg || !t.exp_avg_sq) return set_err(SDM_RT_EINVAL, "tensor %d: a NULL pointer", i);
+    if (reinterpret_cast<uintptr_t>(t.exp_avg) % 8)
+      return set_err(SDM_RT_EINVAL, "tensor %d: 8-bit moments must be 8-byte aligned", i);
+  }
+  if (total == 0) return SDM_RT_OK;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  for_tables(tensors, count, kStepChunk, [&](const StepTable<kStepTensors>& table, unsigned chunks, int64_t) {
+    hipLaunchKernelGGL(read_moments_kernel, dim3(chunks), dim3(kStepThreads), 0, st, table);
+  });
+  return check_launch("read_moments");
+}
+
+}  // extern "C"

@@ -19,6 +19,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from . import core
+from .optim import AdamW
 from .runtime_sdm import RMSNorm, RunTimeSdm
 from .trained_sdm import TrainedSdm
 
@@ -272,6 +273,24 @@ class OneSdmLM(nn.Module):
         the token after t, as its label is."""
         return core.distill_loss(self.forward(idx), top_ids, top_logits, temperature=temperature, labels=labels, alpha=alpha,
                                  ignore_index=ignore_index, reduction=reduction)
+
+    def token_logprobs(self, idx, targets=None, *, temperature=1.0, entropy=False, top=0, ignore_index=-100):
+        """Log probabilities of targets [B, T] under forward(idx), idx [B, T], with the positions' entropies and top
+        alternatives where asked (core.token_logprobs).  Without targets position t's is the next token, idx[:, t + 1]; the last
+        position has none (log probability 0)."""
+        if targets is None:
+            targets = torch.nn.functional.pad(idx[:, 1:], (0, 1), value=ignore_index)
+        return core.token_logprobs(self.forward(idx), targets, temperature=temperature, entropy=entropy, top=top,
+                                   ignore_index=ignore_index)
+
+    def optimizer(self, lr, weight_decay=0.1, **options):
+        """An AdamW (optim.AdamW, which takes the options) of this model's parameters: the embedding and the dense maps decay,
+        norms, biases and the memories' addresses, scales and value tables do not."""
+        named = [(n, p) for n, p in self.named_parameters() if p.requires_grad]
+        dense = [p.dim() == 2 and "onorm_w" not in n and "addr_b" not in n for n, p in named]
+        groups = [dict(params=[p for (_, p), d in zip(named, dense) if d == kind], weight_decay=weight_decay * kind)
+                  for kind in (True, False)]
+        return AdamW([g for g in groups if g["params"]], lr=lr, **options)
 
     def memory_parameters(self):
         """Names of the memories' parameters (track4_onesdm_models.py:557-558): the mixers' (``mems.``); the
