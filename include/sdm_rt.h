@@ -559,7 +559,7 @@ int sdm_rt_append_tokens(int64_t* tokens, int64_t tokens_row_stride, int64_t wid
  * is none) and ids -1. */
 typedef struct {
   int64_t rows;          /* at most 2^21 */
-  int32_t vocab;         /* at most 2^24 */
+  int32_t vocab;         /* at most 2^21 */
   int32_t top_k;         /* 0 to 256 */
   float temperature;     /* 1e-18 to 1e18 */
   int64_t ignore_index;

@@ -1801,7 +1801,7 @@ def token_logprobs(logits, targets=None, *, temperature=1.0, entropy=False, top=
 
     A logit of -inf is a token that cannot come: it is no alternative (the ids behind a row's last one are -1, their log
     probabilities -inf), and as a target has -inf.  A row of nothing else has entropy 0 and gradient 0, one with a NaN or
-    +inf is NaN throughout with ids -1.  At most 2^21 rows, a vocabulary of 2^24, temperature from 1e-18 to 1e18.
+    +inf is NaN throughout with ids -1.  At most 2^21 rows, a vocabulary of 2^21, temperature from 1e-18 to 1e18.
 
     Differentiable in logits through logprobs and entropy, once; the alternatives carry no gradient.  A row whose gradients
     are all 0 has gradient 0 whatever its logits hold."""

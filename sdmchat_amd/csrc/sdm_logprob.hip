@@ -67,65 +67,314 @@ __device__ __forceinline__ void write_row(const LogprobArgs& a, int64_t r, const
   if (a.stats) a.stats[r] = bad ? make_float4(NAN, NAN, NAN, 0.f) : none ? make_float4(0.f, INFINITY, 0.f, 0.f) : make_float4(s.m, g.l2, h, 0.f);
 }
 
-constexpr int kRowThreads = 256;
+// -- a row, or a slice of one, by one workgroup -------------------------------------------------------------------------
+// The slice is in registers, NV 16-byte pieces a thread, so the row is read once: its maximum, its sums against that, and its
+// alternatives all come from there.
+constexpr int kCandidates = 1024;   // keys that are ranked against each other
+constexpr uint32_t kLowest = 0x00800000u;   // the key of the least finite number
 
-// One workgroup per row: its maximum, its sums, then its alternatives one by one, each the greatest below the last.
-template <typename T>
-__global__ void __launch_bounds__(kRowThreads) logprob_kernel(LogprobArgs a) {
-  __shared__ float red[3][kRowThreads / 64];
-  __shared__ uint64_t best[kRowThreads / 64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t r = blockIdx.x;
-  const T* z = static_cast<const T*>(a.logits) + r * a.l_stride;
-  float m = -INFINITY;
-  for (int i = threadIdx.x; i < a.vocab; i += kRowThreads) m = fmaxf(m, to_f32(z[i]));
-  m = wave_max(m);
-  if (lane == 0) red[0][wave] = m;
-  __syncthreads();
-  for (int w = 0; w < kRowThreads / 64; ++w) m = fmaxf(m, red[0][w]);
-  __syncthreads();
-  float count = 0.f, rest = 0.f, u = 0.f;
-  for (int i = threadIdx.x; i < a.vocab; i += kRowThreads) {
-    const float x = to_f32(z[i]);
-    if (x == m) {
-      count += 1.f;
+// What of a row's slices is joined later (slices > 1): their sums, and their alternatives' keys, falling, 0 behind the last.
+struct Partial {
+  RowSums* sums;    // [rows][slices]
+  uint64_t* keys;   // [rows][slices][k]
+};
+
+struct RowLds {
+  uint64_t keys[kCandidates];
+  uint32_t top[1024];   // the threads' maxima
+  float red[4][16];
+  int count[16];
+  uint32_t threshold;
+  int n;
+};
+
+// The greatest t for which about k of the P values have key >= t (k to k + k / 4, where no tie forbids it), by one wave that
+// halves the range of keys: those of k threads' maxima are k logits of the row, so all alternatives have keys >= t.  The key of the least
+// finite number if fewer than k have that.
+template <int PER>
+__device__ __forceinline__ uint32_t near_kth(const uint32_t* top, int threads, int k, uint32_t largest) {
+  uint32_t v[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int at = i * 64 + static_cast<int>(threadIdx.x & 63);
+    v[i] = at < threads ? top[at] : 0;
+  }
+  uint32_t lo = kLowest, hi = max(largest, kLowest);   // count(lo) >= k or lo = kLowest, count(hi + 1) = 0
+  while (lo < hi) {
+    const uint32_t mid = lo + (hi - lo + 1) / 2;
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) n += __popcll(__ballot(v[i] >= mid));
+    if (n >= k) {
+      lo = mid;
+      if (n <= k + k / 4) break;
     } else {
-      const float e = (x - m) * a.c, w = exp2f(e);
-      rest += w;
-      u = fmaf(w, fmaxf(e, -1000.f), u);
+      hi = mid - 1;
+    }
+  }
+  return lo;
+}
+
+// Keeps the work on a piece where it is written, so that the registers of one piece's values serve the next one's.
+template <typename T>
+__device__ __forceinline__ void in_turn(Piece<T>& p) {
+  asm volatile("" : "+v"(p.r.x), "+v"(p.r.y), "+v"(p.r.z), "+v"(p.r.w));
+}
+
+// Ties in great number, or the best logits in a few threads' pieces: more than kCandidates logits at or above the threshold.
+// The workgroup halves the range of keys, then that of the ids that have the key, until the logits taken are at least k and
+// at most kCandidates, and collects them anew.  It reads the slice each time (from the caches: it has just passed), and all its
+// threads get here together.  Returns how many were taken.
+template <typename T>
+__device__ __noinline__ int crowded(int k, const T* z, int n, int first, uint32_t lo, uint32_t hi, RowLds& lds) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, threads = blockDim.x, waves = threads >> 6;
+  auto taken = [&](uint32_t key, int id) {
+    int c = 0;
+    for (int i = threadIdx.x; i < n; i += threads) {
+      const uint32_t o = ordered(to_f32(z[i]));
+      c += o > key || (o == key && i <= id);
+    }
+    c = wave_add(c);
+    __syncthreads();   // the counts before this one are read
+    if (lane == 0) lds.count[wave] = c;
+    __syncthreads();
+    c = 0;
+    for (int w = 0; w < waves; ++w) c += lds.count[w];
+    return c;
+  };
+  bool done = false;
+  while (lo < hi && !done) {
+    const uint32_t mid = lo + (hi - lo + 1) / 2;
+    const int c = taken(mid, n);
+    if (c >= k)
+      lo = mid, done = c <= kCandidates;
+    else
+      hi = mid - 1;
+  }
+  int last = n;
+  if (!done) {   // fewer than k have a greater key, more than kCandidates this one or a greater
+    int from = 0, to = n - 1;
+    while (from < to && !done) {
+      const int mid = (from + to) / 2;
+      const int c = taken(lo, mid);
+      if (c >= k)
+        to = mid, done = c <= kCandidates;
+      else
+        from = mid + 1;
+    }
+    last = to;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) lds.n = 0;
+  __syncthreads();
+  for (int i = threadIdx.x; i < n; i += threads) {
+    const float x = to_f32(z[i]);
+    const uint32_t o = ordered(x);
+    if (o > lo || (o == lo && i <= last)) {
+      const int at = atomicAdd(&lds.n, 1);
+      if (at < kCandidates) lds.keys[at] = logit_key(x, first + i);
+    }
+  }
+  __syncthreads();
+  return min(lds.n, kCandidates);
+}
+
+template <typename T, int NV, bool TOP>
+__global__ void __launch_bounds__(1024, 8) logprob_kernel(LogprobArgs a, int slices, int pieces_per_slice, Partial part) {
+  constexpr int kN = Piece<T>::kN;
+  __shared__ typename std::conditional<TOP, RowLds, float[4][16]>::type lds_;
+  float(*red)[16];
+  if constexpr (TOP)
+    red = lds_.red;
+  else
+    red = lds_;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, threads = blockDim.x, waves = threads >> 6;
+  const int64_t r = slices == 1 ? blockIdx.x : blockIdx.x / slices;
+  const int slice = slices == 1 ? 0 : static_cast<int>(blockIdx.x - r * slices);
+  const int first = slice * pieces_per_slice;
+  const T* z = static_cast<const T*>(a.logits) + r * a.l_stride + static_cast<int64_t>(first) * kN;
+  const int n = min(a.vocab - first * kN, pieces_per_slice * kN);   // logits of the slice
+  Piece<T> p[NV];
+#pragma unroll
+  for (int v = 0; v < NV; ++v) {
+    const int at = (v * threads + static_cast<int>(threadIdx.x)) * kN;
+    if (at + kN <= n)
+      p[v].load(z + at);
+    else if (at < n)
+      p[v].load_part(z + at, n - at, from_f32<T>(-INFINITY));
+    else
+      p[v].fill(-INFINITY);
+  }
+  float mine = -INFINITY;
+#pragma unroll
+  for (int v = 0; v < NV; ++v)
+#pragma unroll
+    for (int e = 0; e < kN; ++e) mine = fmaxf(mine, p[v].get(e));
+#pragma unroll
+  for (int v = 0; v < NV; ++v) p[v].forget();
+  float m = wave_max(mine);
+  if (lane == 0) red[0][wave] = m;
+  if constexpr (TOP) {
+    lds_.top[threadIdx.x] = ordered(mine);
+    if (threadIdx.x == 0) lds_.n = 0;
+  }
+  __syncthreads();
+#pragma unroll 4
+  for (int w = 0; w < waves; ++w) m = fmaxf(m, red[0][w]);
+  if constexpr (TOP) {
+    if (wave == 0) {
+      const uint32_t t = threads <= 512 ? near_kth<8>(lds_.top, threads, a.k, ordered(m))
+                                        : near_kth<16>(lds_.top, threads, a.k, ordered(m));
+      if (lane == 0) lds_.threshold = t;
+    }
+  }
+  const float ref = m == -INFINITY ? 0.f : m;
+  float count = 0.f, rest = 0.f, u = 0.f;
+  if (__ballot(mine == m)) {   // a wave that holds the maximum counts it apart
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      in_turn(p[v]);
+#pragma unroll
+      for (int e = 0; e < kN; ++e) {
+        const float x = p[v].get(e), t = fmaxf((x - ref) * a.c, -1000.f);
+        const bool top = x == m;
+        const float w = __builtin_amdgcn_exp2f(t);
+        count += top ? 1.f : 0.f;
+        rest += top ? 0.f : (x != x ? x : w);
+        u = fmaf(w, t, u);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      in_turn(p[v]);
+#pragma unroll
+      for (int e = 0; e < kN; ++e) {
+        const float x = p[v].get(e), t = (x - ref) * a.c, w = __builtin_amdgcn_exp2f(t);
+        rest += w;
+        u = fmaf(w, fmaxf(t, -1000.f), u);
+      }
     }
   }
   count = wave_add(count);
   rest = wave_add(rest);
   u = wave_add(u);
-  if (lane == 0) red[0][wave] = count, red[1][wave] = rest, red[2][wave] = u;
+  if (lane == 0) red[1][wave] = count, red[2][wave] = rest, red[3][wave] = u;
   __syncthreads();
   RowSums s{m, 0.f, 0.f, 0.f};
-  for (int w = 0; w < kRowThreads / 64; ++w) s.count += red[0][w], s.rest += red[1][w], s.u += red[2][w];
+#pragma unroll 4
+  for (int w = 0; w < waves; ++w) s.count += red[1][w], s.rest += red[2][w], s.u += red[3][w];
+  RowLogs g{};
+  if (slices == 1) {
+    g = row_logs(s);
+    if (threadIdx.x == 0) write_row<T>(a, r, s, g);
+  } else if (threadIdx.x == 0) {
+    part.sums[r * slices + slice] = s;
+  }
+  if constexpr (TOP) {
+    // the logits at or above the threshold, in any order
+    const uint32_t threshold = lds_.threshold;
+    const float from = unordered(threshold);
+    if (mine >= from) {
+#pragma unroll
+      for (int v = 0; v < NV; ++v) {
+        in_turn(p[v]);
+#pragma unroll
+        for (int e = 0; e < kN; ++e) {
+          const float x = p[v].get(e);
+          if (x >= from) {
+            const int at = atomicAdd(&lds_.n, 1);
+            if (at < kCandidates) lds_.keys[at] = logit_key(x, first * kN + (v * threads + static_cast<int>(threadIdx.x)) * kN + e);
+          }
+        }
+      }
+    }
+    __syncthreads();
+    int found = lds_.n;
+    if (found > kCandidates) {
+      found = crowded<T>(a.k, z, n, first * kN, threshold, ordered(m), lds_);
+    }
+    // each key's place among them: how many are greater
+    const bool bad = m == INFINITY || s.rest != s.rest;
+    for (int i = threadIdx.x; i < max(found, a.k); i += threads) {
+      const uint64_t key = i < found ? lds_.keys[i] : 0;
+      int place = i < found ? 0 : i;
+      if (i < found)
+        for (int j = 0; j < found; ++j) place += lds_.keys[j] > key;
+      if (place >= a.k) continue;
+      if (slices > 1) {
+        part.keys[(r * slices + slice) * a.k + place] = key;
+      } else {
+        a.top_ids[r * a.k + place] = key && !bad ? static_cast<int64_t>(~static_cast<uint32_t>(key)) : -1;
+        a.top_logprobs[r * a.k + place] = bad ? NAN : key ? (unordered(static_cast<uint32_t>(key >> 32)) - m) * a.inv_tau - g.l : -INFINITY;
+      }
+    }
+  }
+}
+
+// -- a row's slices joined ----------------------------------------------------------------------------------------------
+constexpr int kJoinThreads = 256;
+
+template <typename T>
+__global__ void __launch_bounds__(kJoinThreads) logprob_join_kernel(LogprobArgs a, int slices, Partial part) {
+  const int64_t r = blockIdx.x;
+  const RowSums* sums = part.sums + r * slices;
+  RowSums s{-INFINITY, 0.f, 0.f, 0.f};
+  bool bad = false;
+  for (int i = 0; i < slices; ++i) {
+    s.m = fmaxf(s.m, sums[i].m);
+    bad |= sums[i].rest != sums[i].rest || sums[i].m == INFINITY;
+  }
+  for (int i = 0; i < slices; ++i) {
+    const RowSums q = sums[i];
+    if (q.m == s.m) {
+      s.count += q.count;
+      s.rest += q.rest;
+      s.u += q.u;
+    } else if (q.m > -INFINITY) {
+      const float t = fmaxf((q.m - s.m) * a.c, -1000.f), w = exp2f(t);
+      s.rest += w * (q.count + q.rest);
+      s.u += w * fmaf(t, q.count + q.rest, q.u);
+    }
+  }
+  if (bad) s.rest = NAN;
   const RowLogs g = row_logs(s);
   if (threadIdx.x == 0) write_row<T>(a, r, s, g);
-  const bool bad = m == INFINITY || s.rest != s.rest;
-  uint64_t last = ~uint64_t{0};
-  for (int q = 0; q < a.k; ++q) {
-    uint64_t k = 0;
-    for (int i = threadIdx.x; i < a.vocab; i += kRowThreads) {
-      const uint64_t x = logit_key(to_f32(z[i]), i);
-      if (x < last && x > k) k = x;
+  // a key's place: its place in its slice's list and, by halving, in each of the others
+  const uint64_t* keys = part.keys + r * slices * a.k;
+  int there = 0;
+  for (int i = threadIdx.x; i < slices * a.k; i += blockDim.x) {
+    const int own = i / a.k;
+    const uint64_t key = keys[i];
+    int place = i - own * a.k;
+    if (key == 0) continue;
+    for (int q = 0; q < slices && place < a.k; ++q) {
+      if (q == own) continue;
+      int lo = 0, hi = a.k;   // how many of this list are greater
+      while (lo < hi) {
+        const int mid = (lo + hi) / 2;
+        if (keys[q * a.k + mid] > key)
+          lo = mid + 1;
+        else
+          hi = mid;
+      }
+      place += lo;
     }
-    for (int d = 32; d > 0; d >>= 1) {
-      const uint64_t o = __shfl_xor(static_cast<unsigned long long>(k), d);
-      k = o > k ? o : k;
-    }
-    __syncthreads();
-    if (lane == 0) best[wave] = k;
-    __syncthreads();
-    for (int w = 0; w < kRowThreads / 64; ++w) k = best[w] > k ? best[w] : k;
-    last = k;
-    if (threadIdx.x == 0) {
-      const bool there = !bad && (k >> 32) != 0;
-      a.top_ids[r * a.k + q] = there ? static_cast<int64_t>(~static_cast<uint32_t>(k)) : -1;
-      a.top_logprobs[r * a.k + q] = bad ? NAN : there ? (unordered(static_cast<uint32_t>(k >> 32)) - m) * a.inv_tau - g.l : -INFINITY;
-    }
+    if (place >= a.k) continue;
+    ++there;
+    a.top_ids[r * a.k + place] = bad ? -1 : static_cast<int64_t>(~static_cast<uint32_t>(key));
+    a.top_logprobs[r * a.k + place] = bad ? NAN : (unordered(static_cast<uint32_t>(key >> 32)) - s.m) * a.inv_tau - g.l;
+  }
+  if (a.k == 0) return;
+  there = wave_add(there);
+  __shared__ int red[kJoinThreads / 64];
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = there;
+  __syncthreads();
+  there = 0;
+  for (int w = 0; w < static_cast<int>(blockDim.x) / 64; ++w) there += red[w];
+  for (int i = there + threadIdx.x; i < a.k; i += blockDim.x) {
+    a.top_ids[r * a.k + i] = -1;
+    a.top_logprobs[r * a.k + i] = bad ? NAN : -INFINITY;
   }
 }
 
@@ -146,25 +395,57 @@ struct LogprobGradArgs {
   int64_t d_stride;
 };
 
+// -- the gradient -------------------------------------------------------------------------------------------------------
+// One workgroup per segment of a row, kGradPieces pieces a thread: a logit in, its gradient out.
+constexpr int kGradThreads = 256, kGradPieces = 4;
+
 template <typename T>
-__global__ void __launch_bounds__(kRowThreads) logprob_grad_kernel(LogprobGradArgs a) {
-  const int64_t r = blockIdx.x;
-  const T* z = static_cast<const T*>(a.logits) + r * a.l_stride;
-  T* d = static_cast<T*>(a.dz) + r * a.d_stride;
-  const int64_t y64 = a.targets && a.dlp ? a.targets[r] : -1;
-  const bool given = y64 >= 0 && y64 < a.vocab && y64 != a.ignore;
-  const float ga = given ? a.dlp[r * a.dlp_stride] * a.inv_tau : 0.f;
-  const float gb = a.dh ? a.dh[r * a.dh_stride] * a.inv_tau : 0.f;
-  if (ga == 0.f && gb == 0.f) {
-    for (int i = threadIdx.x; i < a.vocab; i += kRowThreads) d[i] = T{};
-    return;
-  }
-  const float4 s = a.stats[r];
-  const int y = given && s.y != INFINITY ? static_cast<int>(y64) : -1;
-  for (int i = threadIdx.x; i < a.vocab; i += kRowThreads) {
-    const float e = (to_f32(z[i]) - s.x) * a.c - s.y, p = exp2f(e);
-    const float t = fmaf(gb, fmaf(fmaxf(e, -1000.f), kLn2, s.z), ga);
-    d[i] = from_f32<T>((i == y ? ga : 0.f) - p * t);
+__global__ void __launch_bounds__(kGradThreads) logprob_grad_kernel(LogprobGradArgs a, int segments, int64_t groups) {
+  constexpr int kN = Piece<T>::kN;
+  const int threads = blockDim.x;
+  for (int64_t b = blockIdx.x; b < groups; b += gridDim.x) {
+    const int64_t r = segments == 1 ? b : b / segments;
+    const int first = static_cast<int>(b - r * segments) * kGradPieces * threads * kN;
+    const T* z = static_cast<const T*>(a.logits) + r * a.l_stride;
+    T* d = static_cast<T*>(a.dz) + r * a.d_stride;
+    const int64_t y64 = a.targets && a.dlp ? a.targets[r] : -1;
+    const bool given = y64 >= 0 && y64 < a.vocab && y64 != a.ignore;
+    const float ga = given ? a.dlp[r * a.dlp_stride] * a.inv_tau : 0.f;
+    const float gb = a.dh ? a.dh[r * a.dh_stride] * a.inv_tau : 0.f;
+    const bool live = !(ga == 0.f && gb == 0.f);
+    const float4 s = a.stats[r];
+    const int y = given && s.y != INFINITY ? static_cast<int>(y64) : -1;
+    Piece<T> p[kGradPieces];
+    if (live) {
+#pragma unroll
+      for (int v = 0; v < kGradPieces; ++v) {
+        const int at = first + (v * threads + static_cast<int>(threadIdx.x)) * kN;
+        if (at + kN <= a.vocab)
+          p[v].load(z + at);
+        else if (at < a.vocab)
+          p[v].load_part(z + at, a.vocab - at, from_f32<T>(-INFINITY));
+      }
+    }
+#pragma unroll
+    for (int v = 0; v < kGradPieces; ++v) {
+      const int at = first + (v * threads + static_cast<int>(threadIdx.x)) * kN;
+      if (at >= a.vocab) break;
+      float o[kN];
+#pragma unroll
+      for (int e = 0; e < kN; ++e) {
+        const float t = (p[v].get(e) - s.x) * a.c - s.y, w = __builtin_amdgcn_exp2f(t);
+        o[e] = live ? -w * fmaf(gb, fmaf(fmaxf(t, -1000.f), kLn2, s.z), ga) : 0.f;
+      }
+      if (static_cast<unsigned>(y - at) < static_cast<unsigned>(kN)) {
+#pragma unroll
+        for (int e = 0; e < kN; ++e) o[e] += y - at == e ? ga : 0.f;
+      }
+      p[v].set(o);
+      if (at + kN <= a.vocab)
+        p[v].store(d + at);
+      else
+        p[v].store_part(d + at, a.vocab - at);
+    }
   }
 }
 
@@ -174,13 +455,61 @@ inline int check_logprob(const sdm_rt_logprob* d, const void* logits, int64_t l_
   if ((rc = check_dtype(dtype, "dtype"))) return rc;
   if (d->rows < 0 || d->vocab < 1 || d->top_k < 0) return set_err(SDM_RT_EINVAL, "rows and top_k must be >= 0, vocab >= 1");
   if (d->rows > (1 << 21)) return set_err(SDM_RT_EUNSUPPORTED, "rows must be at most 2^21");
-  if (d->vocab > (1 << 24)) return set_err(SDM_RT_EUNSUPPORTED, "vocab must be at most 2^24");
+  if (d->vocab > (1 << 21)) return set_err(SDM_RT_EUNSUPPORTED, "vocab must be at most 2^21");
   if (d->top_k > kMaxAlternatives) return set_err(SDM_RT_EUNSUPPORTED, "top_k = %d must be at most %d", d->top_k, kMaxAlternatives);
   if (!(d->temperature >= 1e-18f) || !(d->temperature <= 1e18f))
     return set_err(SDM_RT_EINVAL, "temperature must be positive and finite, from 1e-18 to 1e18");
   if (d->rows > 0 && (!logits || bad_read_stride(l_stride, d->vocab)))
     return set_err(SDM_RT_EINVAL, "logits must not be NULL, their row stride 0 or >= vocab");
   return SDM_RT_OK;
+}
+
+// How a row is cut: at most 32,768 logits to a slice, 8 pieces a thread (2 in rows that a few waves hold).
+struct RowShape {
+  int slices, pieces, nv, threads;   // pieces: of a slice
+};
+inline RowShape row_shape(int64_t rows, int vocab, sdm_rt_dtype dtype) {
+  const int kN = dtype == SDM_RT_BF16 ? 8 : 4, most = 32768 / kN;
+  const int pieces = (vocab + kN - 1) / kN;
+  RowShape s;
+  s.slices = (pieces + most - 1) / most;
+  s.pieces = (pieces + s.slices - 1) / s.slices;
+  s.nv = s.pieces <= 512 ? 2 : 8;
+  s.threads = std::max(64, (s.pieces + 64 * s.nv - 1) / (64 * s.nv) * 64);
+  (void)rows;
+  return s;
+}
+inline size_t logprob_bytes(int64_t rows, int k, int slices) {
+  return slices == 1 ? 0 : static_cast<size_t>(rows) * slices * (static_cast<size_t>(k) * sizeof(uint64_t) + sizeof(RowSums));
+}
+
+template <typename T>
+void launch_logprob(const LogprobArgs& a, const RowShape& s, const Partial& part, hipStream_t st) {
+  const dim3 grid(static_cast<unsigned>(a.rows * s.slices)), threads(s.threads);
+  if (s.nv == 2) {
+    if (a.k)
+      hipLaunchKernelGGL((logprob_kernel<T, 2, true>), grid, threads, 0, st, a, s.slices, s.pieces, part);
+    else
+      hipLaunchKernelGGL((logprob_kernel<T, 2, false>), grid, threads, 0, st, a, s.slices, s.pieces, part);
+  } else {
+    if (a.k)
+      hipLaunchKernelGGL((logprob_kernel<T, 8, true>), grid, threads, 0, st, a, s.slices, s.pieces, part);
+    else
+      hipLaunchKernelGGL((logprob_kernel<T, 8, false>), grid, threads, 0, st, a, s.slices, s.pieces, part);
+  }
+  if (s.slices > 1)
+    hipLaunchKernelGGL(logprob_join_kernel<T>, dim3(static_cast<unsigned>(a.rows)), dim3(a.k ? kJoinThreads : 64), 0, st, a,
+                       s.slices, part);
+}
+
+template <typename T>
+void launch_logprob_grad(const LogprobGradArgs& a, hipStream_t st) {
+  const int pieces = (a.vocab + Piece<T>::kN - 1) / Piece<T>::kN;
+  const int threads = std::min(kGradThreads, (pieces + 64 * kGradPieces - 1) / (64 * kGradPieces) * 64);
+  const int segments = (pieces + threads * kGradPieces - 1) / (threads * kGradPieces);
+  const int64_t groups = a.rows * segments;
+  hipLaunchKernelGGL(logprob_grad_kernel<T>, dim3(static_cast<unsigned>(std::min<int64_t>(groups, 1 << 22))), dim3(threads), 0,
+                     st, a, segments, groups);
 }
 
 }  // namespace sdmrt
@@ -190,9 +519,8 @@ using namespace sdmrt;
 extern "C" {
 
 size_t sdm_rt_token_logprobs_workspace_bytes(const sdm_rt_logprob* dims, sdm_rt_dtype dtype) {
-  (void)dims;
-  (void)dtype;
-  return 0;
+  if (!dims || dims->rows < 0 || dims->vocab < 1 || dims->top_k < 0) return 0;
+  return logprob_bytes(dims->rows, dims->top_k, row_shape(dims->rows, dims->vocab, dtype).slices);
 }
 
 int sdm_rt_token_logprobs(const sdm_rt_logprob* dims, const void* logits, int64_t logits_row_stride, sdm_rt_dtype dtype,
@@ -223,12 +551,19 @@ int sdm_rt_token_logprobs(const sdm_rt_logprob* dims, const void* logits, int64_
   a.top_ids = top_ids;
   a.top_logprobs = top_logprobs;
   a.stats = reinterpret_cast<float4*>(stats);
+  const RowShape shape = row_shape(a.rows, a.vocab, dtype);
+  if (a.rows * shape.slices >= int64_t{1} << 22) return set_err(SDM_RT_EUNSUPPORTED, "too many rows of so large a vocabulary");
+  Partial part{};
+  if (shape.slices > 1) {
+    if (reinterpret_cast<uintptr_t>(workspace) % 8) return set_err(SDM_RT_EINVAL, "workspace must be 8-byte aligned");
+    part.keys = static_cast<uint64_t*>(workspace);
+    part.sums = reinterpret_cast<RowSums*>(part.keys + a.rows * shape.slices * a.k);
+  }
   hipStream_t st = static_cast<hipStream_t>(stream);
-  const dim3 grid(static_cast<unsigned>(a.rows));
   if (dtype == SDM_RT_BF16)
-    hipLaunchKernelGGL(logprob_kernel<bf16_t>, grid, dim3(kRowThreads), 0, st, a);
+    launch_logprob<bf16_t>(a, shape, part, st);
   else
-    hipLaunchKernelGGL(logprob_kernel<float>, grid, dim3(kRowThreads), 0, st, a);
+    launch_logprob<float>(a, shape, part, st);
   return check_launch("token_logprobs");
 }
 
@@ -260,11 +595,10 @@ int sdm_rt_token_logprobs_grad(const sdm_rt_logprob* dims, const void* logits, i
   a.dz = d_logits;
   a.d_stride = d_logits_row_stride;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  const dim3 grid(static_cast<unsigned>(a.rows));
   if (dtype == SDM_RT_BF16)
-    hipLaunchKernelGGL(logprob_grad_kernel<bf16_t>, grid, dim3(kRowThreads), 0, st, a);
+    launch_logprob_grad<bf16_t>(a, st);
   else
-    hipLaunchKernelGGL(logprob_grad_kernel<float>, grid, dim3(kRowThreads), 0, st, a);
+    launch_logprob_grad<float>(a, st);
   return check_launch("token_logprobs_grad");
 }
 

@@ -27,7 +27,7 @@ def _logprob(**over):
 
 BAD = [(dict(dtype=2), -1, "dtype"), (dict(rows=-1), -1, "rows"), (dict(vocab=0), -1, "vocab"), (dict(top_k=-1), -1, "top_k"),
        (dict(top_k=257), -3, "256"), (dict(rows=(1 << 21) + 1), -3, "2^21"),
-       (dict(vocab=(1 << 24) + 1, ls=(1 << 24) + 1, dzs=(1 << 24) + 1), -3, "2^24"),
+       (dict(vocab=(1 << 21) + 1, ls=(1 << 21) + 1, dzs=(1 << 21) + 1), -3, "2^21"),
        (dict(temperature=0.0), -1, "temperature"), (dict(temperature=-1.0), -1, "temperature"),
        (dict(temperature=math.nan), -1, "temperature"), (dict(temperature=math.inf), -1, "temperature"),
        (dict(logits=None), -1, "logits"), (dict(ls=99), -1, "stride"), (dict(ls=-100), -1, "stride"),
