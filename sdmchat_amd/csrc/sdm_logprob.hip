@@ -81,28 +81,37 @@ struct Partial {
 
 struct RowLds {
   uint64_t keys[kCandidates];
-  uint32_t top[1024];   // the threads' maxima
+  float top[1024];   // the threads' maxima
   float red[4][16];
   int count[16];
   uint32_t threshold;
-  int n;
+  float log;
+  int n, n_hot;
+  uint16_t hot[1024];   // threads with a logit at or above the threshold
 };
 
-// The greatest t for which about k of the P values have key >= t (k to k + k / 4, where no tie forbids it), by one wave that
-// halves the range of keys: those of k threads' maxima are k logits of the row, so all alternatives have keys >= t.  The key of the least
-// finite number if fewer than k have that.
+// The key t for which k to 5/4 k of the threads' maxima have key >= t (k or more, where ties forbid that), by one wave that
+// halves the range of keys: those maxima are k logits of the row, so all alternatives have keys >= t.  The key of the least
+// finite number if fewer than k maxima are finite.
 template <int PER>
-__device__ __forceinline__ uint32_t near_kth(const uint32_t* top, int threads, int k, uint32_t largest) {
+__device__ __forceinline__ uint32_t near_kth(const float* top, int threads, int k, float largest) {
+  const int lane = threadIdx.x & 63;
   uint32_t v[PER];
+  float least = INFINITY;
+  int n = 0;
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
-    const int at = i * 64 + static_cast<int>(threadIdx.x & 63);
-    v[i] = at < threads ? top[at] : 0;
+    const float x = i * 64 + lane < threads ? top[i * 64 + lane] : -INFINITY;
+    v[i] = ordered(x);
+    const bool there = v[i] != 0;
+    least = fminf(least, there ? x : INFINITY);
+    n += __popcll(__ballot(there));
   }
-  uint32_t lo = kLowest, hi = max(largest, kLowest);   // count(lo) >= k or lo = kLowest, count(hi + 1) = 0
+  if (n < k) return kLowest;
+  uint32_t lo = ordered(-wave_max(-least)), hi = max(ordered(largest), lo);   // k or more from lo on, none past hi
   while (lo < hi) {
     const uint32_t mid = lo + (hi - lo + 1) / 2;
-    int n = 0;
+    n = 0;
 #pragma unroll
     for (int i = 0; i < PER; ++i) n += __popcll(__ballot(v[i] >= mid));
     if (n >= k) {
@@ -114,6 +123,41 @@ __device__ __forceinline__ uint32_t near_kth(const uint32_t* top, int threads, i
   }
   return lo;
 }
+
+// A thread's maximum over its pieces.  Bfloat16 values are ordered as whole numbers, two at a time: among those of the positive
+// sign the signed maximum, where there are none the unsigned minimum (one instruction a value, unpacking and comparing floats
+// two).  A NaN may be taken for the maximum, or passed over: the sums find it.
+typedef short short2_t __attribute__((ext_vector_type(2)));
+typedef unsigned short ushort2_t __attribute__((ext_vector_type(2)));
+template <typename T>
+struct RunningMax;
+template <>
+struct RunningMax<bf16_t> {
+  short2_t most = {-32768, -32768};
+  ushort2_t least = {0xffff, 0xffff};
+  __device__ __forceinline__ void add(const Piece<bf16_t>& p) {
+    const uint32_t w[4] = {p.r.x, p.r.y, p.r.z, p.r.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      most = __builtin_elementwise_max(most, __builtin_bit_cast(short2_t, w[i]));
+      least = __builtin_elementwise_min(least, __builtin_bit_cast(ushort2_t, w[i]));
+    }
+  }
+  __device__ __forceinline__ float get() const {
+    const int a = max(most.x, most.y);
+    const uint32_t b = min(least.x, least.y);
+    return __uint_as_float((a >= 0 ? static_cast<uint32_t>(a) : b) << 16);
+  }
+};
+template <>
+struct RunningMax<float> {
+  float most = -INFINITY;
+  __device__ __forceinline__ void add(const Piece<float>& p) {
+    most = fmaxf(fmaxf(most, p.get(0)), p.get(1));
+    most = fmaxf(fmaxf(most, p.get(2)), p.get(3));
+  }
+  __device__ __forceinline__ float get() const { return most; }
+};
 
 // Keeps the work on a piece where it is written, so that the registers of one piece's values serve the next one's.
 template <typename T>
@@ -179,7 +223,7 @@ __device__ __noinline__ int crowded(int k, const T* z, int n, int first, uint32_
   return min(lds.n, kCandidates);
 }
 
-template <typename T, int NV, bool TOP>
+template <typename T, int NV, bool TOP, bool ENT>
 __global__ void __launch_bounds__(1024, 8) logprob_kernel(LogprobArgs a, int slices, int pieces_per_slice, Partial part) {
   constexpr int kN = Piece<T>::kN;
   __shared__ typename std::conditional<TOP, RowLds, float[4][16]>::type lds_;
@@ -205,87 +249,114 @@ __global__ void __launch_bounds__(1024, 8) logprob_kernel(LogprobArgs a, int sli
     else
       p[v].fill(-INFINITY);
   }
-  float mine = -INFINITY;
+  RunningMax<T> running;
 #pragma unroll
-  for (int v = 0; v < NV; ++v)
-#pragma unroll
-    for (int e = 0; e < kN; ++e) mine = fmaxf(mine, p[v].get(e));
-#pragma unroll
-  for (int v = 0; v < NV; ++v) p[v].forget();
+  for (int v = 0; v < NV; ++v) running.add(p[v]);
+  const float mine = running.get();
   float m = wave_max(mine);
   if (lane == 0) red[0][wave] = m;
   if constexpr (TOP) {
-    lds_.top[threadIdx.x] = ordered(mine);
-    if (threadIdx.x == 0) lds_.n = 0;
+    lds_.top[threadIdx.x] = mine;
+    if (threadIdx.x == 0) lds_.n = lds_.n_hot = 0;
   }
   __syncthreads();
 #pragma unroll 4
   for (int w = 0; w < waves; ++w) m = fmaxf(m, red[0][w]);
-  if constexpr (TOP) {
-    if (wave == 0) {
-      const uint32_t t = threads <= 512 ? near_kth<8>(lds_.top, threads, a.k, ordered(m))
-                                        : near_kth<16>(lds_.top, threads, a.k, ordered(m));
-      if (lane == 0) lds_.threshold = t;
-    }
-  }
   const float ref = m == -INFINITY ? 0.f : m;
   float count = 0.f, rest = 0.f, u = 0.f;
-  if (__ballot(mine == m)) {   // a wave that holds the maximum counts it apart
+  const bool holds = __ballot(mine == m) != 0;
+  // t = z c - m c in one rounding, where m c is small enough for its own rounding (that all of them share) to be taken back after
+  const float mc = ref * a.c;
+  bool plain = !holds && fabsf(mc) < 256.f;
+  if (plain) {
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
       in_turn(p[v]);
 #pragma unroll
       for (int e = 0; e < kN; ++e) {
-        const float x = p[v].get(e), t = fmaxf((x - ref) * a.c, -1000.f);
-        const bool top = x == m;
-        const float w = __builtin_amdgcn_exp2f(t);
-        count += top ? 1.f : 0.f;
-        rest += top ? 0.f : (x != x ? x : w);
-        u = fmaf(w, t, u);
+        const float t = fmaf(p[v].get(e), a.c, -mc), w = __builtin_amdgcn_exp2f(t);
+        rest += w;
+        if constexpr (ENT) u = fmaf(w, t, u);
       }
     }
-  } else {
+    const float off = fmaf(ref, a.c, -mc), scale = __builtin_amdgcn_exp2f(-off);
+    if constexpr (ENT) {
+      u = scale * fmaf(-off, rest, u);
+      plain = __ballot(u != u) == 0;   // 0 times -inf, if there is no NaN
+    }
+    rest *= scale;
+  }
+  if (!plain) {   // a wave that holds the maximum counts it apart
+    count = rest = u = 0.f;
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
       in_turn(p[v]);
 #pragma unroll
       for (int e = 0; e < kN; ++e) {
         const float x = p[v].get(e), t = (x - ref) * a.c, w = __builtin_amdgcn_exp2f(t);
-        rest += w;
-        u = fmaf(w, fmaxf(t, -1000.f), u);
+        const bool top = x == m;
+        count += top ? 1.f : 0.f;
+        rest += top ? 0.f : w;
+        if constexpr (ENT) u = fmaf(w, fmaxf(t, -1000.f), u);
       }
     }
   }
-  count = wave_add(count);
+  if (holds) count = wave_add(count);
   rest = wave_add(rest);
-  u = wave_add(u);
+  if constexpr (ENT) u = wave_add(u);
   if (lane == 0) red[1][wave] = count, red[2][wave] = rest, red[3][wave] = u;
+  if constexpr (TOP) {
+    if (wave == 0) {   // its pieces' registers are free by now
+      const uint32_t t = threads <= 512 ? near_kth<8>(lds_.top, threads, a.k, m) : near_kth<16>(lds_.top, threads, a.k, m);
+      if (lane == 0) lds_.threshold = t;
+    }
+  }
   __syncthreads();
-  RowSums s{m, 0.f, 0.f, 0.f};
-#pragma unroll 4
-  for (int w = 0; w < waves; ++w) s.count += red[1][w], s.rest += red[2][w], s.u += red[3][w];
-  RowLogs g{};
-  if (slices == 1) {
-    g = row_logs(s);
-    if (threadIdx.x == 0) write_row<T>(a, r, s, g);
-  } else if (threadIdx.x == 0) {
-    part.sums[r * slices + slice] = s;
+  if (wave == 0) {   // the slice's sums, by the first wave
+    const bool there = lane < waves;
+    const RowSums s{m, wave_add(there ? red[1][lane] : 0.f), wave_add(there ? red[2][lane] : 0.f),
+                    ENT ? wave_add(there ? red[3][lane] : 0.f) : 0.f};
+    if (slices > 1) {
+      if (lane == 0) part.sums[r * slices + slice] = s;
+    } else {
+      const RowLogs g = row_logs(s);
+      if (lane == 0) write_row<T>(a, r, s, g);
+      if constexpr (TOP) {
+        if (lane == 0) lds_.log = m == INFINITY || s.rest != s.rest ? NAN : g.l;   // NaN: a row without alternatives
+      }
+    }
   }
   if constexpr (TOP) {
-    // the logits at or above the threshold, in any order
+    // The threads with a logit at or above the threshold are few (k to 5/4 k of them): their pieces are dealt out to all threads,
+    // which read them again from the caches, and the logits found are listed in any order.
     const uint32_t threshold = lds_.threshold;
     const float from = unordered(threshold);
-    if (mine >= from) {
+    const uint64_t hot = __ballot(mine >= from);
+    if (hot) {
+      int at = 0;
+      if (lane == 0) at = atomicAdd(&lds_.n_hot, __popcll(hot));
+      at = __builtin_amdgcn_readfirstlane(at) + __popcll(hot & ((uint64_t{1} << lane) - 1));
+      if (hot >> lane & 1) lds_.hot[at] = static_cast<uint16_t>(threadIdx.x);
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < lds_.n_hot * NV; i += threads) {
+      const int at = ((i % NV) * threads + lds_.hot[i / NV]) * kN;
+      Piece<T> q;
+      if (at + kN <= n)
+        q.load(z + at);
+      else if (at < n)
+        q.load_part(z + at, n - at, from_f32<T>(-INFINITY));
+      else
+        continue;
+      RunningMax<T> most;
+      most.add(q);
+      if (!(most.get() >= from)) continue;
 #pragma unroll
-      for (int v = 0; v < NV; ++v) {
-        in_turn(p[v]);
-#pragma unroll
-        for (int e = 0; e < kN; ++e) {
-          const float x = p[v].get(e);
-          if (x >= from) {
-            const int at = atomicAdd(&lds_.n, 1);
-            if (at < kCandidates) lds_.keys[at] = logit_key(x, first * kN + (v * threads + static_cast<int>(threadIdx.x)) * kN + e);
-          }
+      for (int e = 0; e < kN; ++e) {
+        const float x = q.get(e);
+        if (x >= from) {
+          const int to = atomicAdd(&lds_.n, 1);
+          if (to < kCandidates) lds_.keys[to] = logit_key(x, first * kN + at + e);
         }
       }
     }
@@ -295,25 +366,27 @@ __global__ void __launch_bounds__(1024, 8) logprob_kernel(LogprobArgs a, int sli
       found = crowded<T>(a.k, z, n, first * kN, threshold, ordered(m), lds_);
     }
     // each key's place among them: how many are greater
-    const bool bad = m == INFINITY || s.rest != s.rest;
+    const float log = lds_.log;
+    const bool bad = log != log;
     for (int i = threadIdx.x; i < max(found, a.k); i += threads) {
       const uint64_t key = i < found ? lds_.keys[i] : 0;
       int place = i < found ? 0 : i;
       if (i < found)
+#pragma unroll 8
         for (int j = 0; j < found; ++j) place += lds_.keys[j] > key;
       if (place >= a.k) continue;
       if (slices > 1) {
         part.keys[(r * slices + slice) * a.k + place] = key;
       } else {
         a.top_ids[r * a.k + place] = key && !bad ? static_cast<int64_t>(~static_cast<uint32_t>(key)) : -1;
-        a.top_logprobs[r * a.k + place] = bad ? NAN : key ? (unordered(static_cast<uint32_t>(key >> 32)) - m) * a.inv_tau - g.l : -INFINITY;
+        a.top_logprobs[r * a.k + place] = bad ? NAN : key ? (unordered(static_cast<uint32_t>(key >> 32)) - m) * a.inv_tau - log : -INFINITY;
       }
     }
   }
 }
 
 // -- a row's slices joined ----------------------------------------------------------------------------------------------
-constexpr int kJoinThreads = 256;
+constexpr int kJoinThreads = 256, kJoinKeys = 2048;
 
 template <typename T>
 __global__ void __launch_bounds__(kJoinThreads) logprob_join_kernel(LogprobArgs a, int slices, Partial part) {
@@ -341,11 +414,18 @@ __global__ void __launch_bounds__(kJoinThreads) logprob_join_kernel(LogprobArgs 
   const RowLogs g = row_logs(s);
   if (threadIdx.x == 0) write_row<T>(a, r, s, g);
   // a key's place: its place in its slice's list and, by halving, in each of the others
+  __shared__ uint64_t held[kJoinKeys];
   const uint64_t* keys = part.keys + r * slices * a.k;
+  const bool few = slices * a.k <= kJoinKeys;
+  if (few) {
+    for (int i = threadIdx.x; i < slices * a.k; i += blockDim.x) held[i] = keys[i];
+    __syncthreads();
+  }
+  auto key_at = [&](int i) { return few ? held[i] : keys[i]; };
   int there = 0;
   for (int i = threadIdx.x; i < slices * a.k; i += blockDim.x) {
     const int own = i / a.k;
-    const uint64_t key = keys[i];
+    const uint64_t key = key_at(i);
     int place = i - own * a.k;
     if (key == 0) continue;
     for (int q = 0; q < slices && place < a.k; ++q) {
@@ -353,7 +433,7 @@ __global__ void __launch_bounds__(kJoinThreads) logprob_join_kernel(LogprobArgs 
       int lo = 0, hi = a.k;   // how many of this list are greater
       while (lo < hi) {
         const int mid = (lo + hi) / 2;
-        if (keys[q * a.k + mid] > key)
+        if (key_at(q * a.k + mid) > key)
           lo = mid + 1;
         else
           hi = mid;
@@ -486,17 +566,26 @@ inline size_t logprob_bytes(int64_t rows, int k, int slices) {
 template <typename T>
 void launch_logprob(const LogprobArgs& a, const RowShape& s, const Partial& part, hipStream_t st) {
   const dim3 grid(static_cast<unsigned>(a.rows * s.slices)), threads(s.threads);
-  if (s.nv == 2) {
-    if (a.k)
-      hipLaunchKernelGGL((logprob_kernel<T, 2, true>), grid, threads, 0, st, a, s.slices, s.pieces, part);
+  auto launch = [&](auto nv, auto top, auto ent) {
+    hipLaunchKernelGGL((logprob_kernel<T, decltype(nv)::value, decltype(top)::value, decltype(ent)::value>), grid, threads, 0,
+                       st, a, s.slices, s.pieces, part);
+  };
+  auto with_nv = [&](auto top, auto ent) {
+    if (s.nv == 2)
+      launch(std::integral_constant<int, 2>{}, top, ent);
     else
-      hipLaunchKernelGGL((logprob_kernel<T, 2, false>), grid, threads, 0, st, a, s.slices, s.pieces, part);
-  } else {
+      launch(std::integral_constant<int, 8>{}, top, ent);
+  };
+  auto with_top = [&](auto ent) {
     if (a.k)
-      hipLaunchKernelGGL((logprob_kernel<T, 8, true>), grid, threads, 0, st, a, s.slices, s.pieces, part);
+      with_nv(std::true_type{}, ent);
     else
-      hipLaunchKernelGGL((logprob_kernel<T, 8, false>), grid, threads, 0, st, a, s.slices, s.pieces, part);
-  }
+      with_nv(std::false_type{}, ent);
+  };
+  if (a.entropy)
+    with_top(std::true_type{});
+  else
+    with_top(std::false_type{});
   if (s.slices > 1)
     hipLaunchKernelGGL(logprob_join_kernel<T>, dim3(static_cast<unsigned>(a.rows)), dim3(a.k ? kJoinThreads : 64), 0, st, a,
                        s.slices, part);
