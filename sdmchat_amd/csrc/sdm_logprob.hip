@@ -48,23 +48,26 @@ __device__ __forceinline__ uint64_t logit_key(float z, int id) {
   return static_cast<uint64_t>(ordered(z)) << 32 | ~static_cast<uint32_t>(id);
 }
 
+// A row's target (-1: none) and its logit, loaded ahead.
+struct RowTarget {
+  int64_t id;
+  float z;
+};
+__device__ __forceinline__ int64_t row_target(const LogprobArgs& a, int64_t r) {
+  if (!a.logprobs) return -1;
+  const int64_t y = a.targets[r];
+  return y >= 0 && y < a.vocab && y != a.ignore ? y : -1;
+}
+
 // What becomes of a row's sums, by one thread.
-template <typename T>
-__device__ __forceinline__ void write_row(const LogprobArgs& a, int64_t r, const RowSums& s, const RowLogs& g) {
+__device__ __forceinline__ void write_row(const LogprobArgs& a, int64_t r, const RowTarget& y, const RowSums& s, const RowLogs& g) {
   const bool bad = s.m == INFINITY || s.rest != s.rest, none = !bad && s.m == -INFINITY;
-  if (a.logprobs) {
-    const int64_t y = a.targets[r];
-    float lp = 0.f;
-    if (y >= 0 && y < a.vocab && y != a.ignore) {
-      const float z = to_f32(static_cast<const T*>(a.logits)[r * a.l_stride + y]);
-      lp = bad ? NAN : none ? -INFINITY : (z - s.m) * a.inv_tau - g.l;
-    }
-    a.logprobs[r] = lp;
-  }
+  if (a.logprobs) a.logprobs[r] = y.id < 0 ? 0.f : bad ? NAN : none ? -INFINITY : (y.z - s.m) * a.inv_tau - g.l;
   const float h = bad ? NAN : none ? 0.f : g.h;
   if (a.entropy) a.entropy[r] = h;
   // a row of -inf: sums that make every p 0
-  if (a.stats) a.stats[r] = bad ? make_float4(NAN, NAN, NAN, 0.f) : none ? make_float4(0.f, INFINITY, 0.f, 0.f) : make_float4(s.m, g.l2, h, 0.f);
+  if (a.stats)
+    a.stats[r] = bad ? make_float4(NAN, NAN, NAN, 0.f) : none ? make_float4(0.f, INFINITY, 0.f, 0.f) : make_float4(s.m, g.l2, h, 0.f);
 }
 
 // -- a row, or a slice of one, by one workgroup -------------------------------------------------------------------------
@@ -238,17 +241,22 @@ __global__ void __launch_bounds__(1024, 8) logprob_kernel(LogprobArgs a, int sli
   const int first = slice * pieces_per_slice;
   const T* z = static_cast<const T*>(a.logits) + r * a.l_stride + static_cast<int64_t>(first) * kN;
   const int n = min(a.vocab - first * kN, pieces_per_slice * kN);   // logits of the slice
+  RowTarget target{-1, 0.f};
+  if (wave == 0 && slices == 1) target.id = row_target(a, r);
   Piece<T> p[NV];
 #pragma unroll
   for (int v = 0; v < NV; ++v) {
     const int at = (v * threads + static_cast<int>(threadIdx.x)) * kN;
-    if (at + kN <= n)
+    if ((v + 1) * threads * kN <= n)   // all threads
+      p[v].load(z + at);
+    else if (at + kN <= n)
       p[v].load(z + at);
     else if (at < n)
       p[v].load_part(z + at, n - at, from_f32<T>(-INFINITY));
     else
       p[v].fill(-INFINITY);
   }
+  if (target.id >= 0) target.z = to_f32(z[target.id]);
   RunningMax<T> running;
 #pragma unroll
   for (int v = 0; v < NV; ++v) running.add(p[v]);
@@ -320,7 +328,7 @@ __global__ void __launch_bounds__(1024, 8) logprob_kernel(LogprobArgs a, int sli
       if (lane == 0) part.sums[r * slices + slice] = s;
     } else {
       const RowLogs g = row_logs(s);
-      if (lane == 0) write_row<T>(a, r, s, g);
+      if (lane == 0) write_row(a, r, target, s, g);
       if constexpr (TOP) {
         if (lane == 0) lds_.log = m == INFINITY || s.rest != s.rest ? NAN : g.l;   // NaN: a row without alternatives
       }
@@ -390,37 +398,32 @@ constexpr int kJoinThreads = 256, kJoinKeys = 2048;
 
 template <typename T>
 __global__ void __launch_bounds__(kJoinThreads) logprob_join_kernel(LogprobArgs a, int slices, Partial part) {
-  const int64_t r = blockIdx.x;
-  const RowSums* sums = part.sums + r * slices;
-  RowSums s{-INFINITY, 0.f, 0.f, 0.f};
-  bool bad = false;
-  for (int i = 0; i < slices; ++i) {
-    s.m = fmaxf(s.m, sums[i].m);
-    bad |= sums[i].rest != sums[i].rest || sums[i].m == INFINITY;
-  }
-  for (int i = 0; i < slices; ++i) {
-    const RowSums q = sums[i];
-    if (q.m == s.m) {
-      s.count += q.count;
-      s.rest += q.rest;
-      s.u += q.u;
-    } else if (q.m > -INFINITY) {
-      const float t = fmaxf((q.m - s.m) * a.c, -1000.f), w = exp2f(t);
-      s.rest += w * (q.count + q.rest);
-      s.u += w * fmaf(t, q.count + q.rest, q.u);
-    }
-  }
-  if (bad) s.rest = NAN;
-  const RowLogs g = row_logs(s);
-  if (threadIdx.x == 0) write_row<T>(a, r, s, g);
-  // a key's place: its place in its slice's list and, by halving, in each of the others
   __shared__ uint64_t held[kJoinKeys];
+  const int64_t r = blockIdx.x;
+  const int lane = threadIdx.x & 63;
+  RowTarget target{-1, 0.f};
+  if (threadIdx.x == 0) target.id = row_target(a, r);
   const uint64_t* keys = part.keys + r * slices * a.k;
   const bool few = slices * a.k <= kJoinKeys;
-  if (few) {
+  if (few)
     for (int i = threadIdx.x; i < slices * a.k; i += blockDim.x) held[i] = keys[i];
-    __syncthreads();
-  }
+  // a lane a slice: at most 64
+  const RowSums q = lane < slices ? part.sums[r * slices + lane] : RowSums{-INFINITY, 0.f, 0.f, 0.f};
+  if (target.id >= 0) target.z = to_f32(static_cast<const T*>(a.logits)[r * a.l_stride + target.id]);
+  const bool bad = __ballot(q.rest != q.rest || q.m == INFINITY) != 0;
+  RowSums s;
+  s.m = wave_max(q.m);
+  const float ref = s.m == -INFINITY ? 0.f : s.m, t = fmaxf((q.m - ref) * a.c, -1000.f), w = __builtin_amdgcn_exp2f(t);
+  const bool top = q.m == s.m;
+  s.count = wave_add(top ? q.count : 0.f);
+  s.rest = wave_add(top ? q.rest : w * (q.count + q.rest));
+  s.u = wave_add(top ? q.u : w * fmaf(t, q.count + q.rest, q.u));
+  if (bad) s.rest = NAN;
+  const RowLogs g = row_logs(s);
+  if (threadIdx.x == 0) write_row(a, r, target, s, g);
+  if (a.k == 0) return;
+  __syncthreads();
+  // a key's place: its place in its slice's list and, by halving, in each of the others
   auto key_at = [&](int i) { return few ? held[i] : keys[i]; };
   int there = 0;
   for (int i = threadIdx.x; i < slices * a.k; i += blockDim.x) {
@@ -445,7 +448,6 @@ __global__ void __launch_bounds__(kJoinThreads) logprob_join_kernel(LogprobArgs 
     a.top_ids[r * a.k + place] = bad ? -1 : static_cast<int64_t>(~static_cast<uint32_t>(key));
     a.top_logprobs[r * a.k + place] = bad ? NAN : (unordered(static_cast<uint32_t>(key >> 32)) - s.m) * a.inv_tau - g.l;
   }
-  if (a.k == 0) return;
   there = wave_add(there);
   __shared__ int red[kJoinThreads / 64];
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = there;
@@ -552,6 +554,7 @@ inline RowShape row_shape(int64_t rows, int vocab, sdm_rt_dtype dtype) {
   const int kN = dtype == SDM_RT_BF16 ? 8 : 4, most = 32768 / kN;
   const int pieces = (vocab + kN - 1) / kN;
   RowShape s;
+  static_assert(((1 << 21) + 32767) / 32768 <= 64, "a lane a slice");
   s.slices = (pieces + most - 1) / most;
   s.pieces = (pieces + s.slices - 1) / s.slices;
   s.nv = s.pieces <= 512 ? 2 : 8;
