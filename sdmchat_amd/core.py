@@ -7,6 +7,7 @@ stream; nothing synchronises.
 import array
 import ctypes
 import math
+import operator
 import typing
 
 import torch
@@ -1864,56 +1865,104 @@ def _dense(t):
     return True
 
 
-def _listed(name, **lists):
-    """Lists of equal length, not empty, on one GPU: (lists, device)."""
-    lists = {k: list(v) for k, v in lists.items()}
-    first = next(iter(lists.values()))
+_T = torch.Tensor
+_dtype_of, _shape_of = operator.attrgetter("dtype"), operator.attrgetter("shape")
+
+
+def _lists(name, **lists):
+    """Lists of equal length, not empty, on one GPU: (lists, its index)."""
+    out = [v if type(v) is list else list(v) for v in lists.values()]
+    first = out[0]
     if not first:
         raise ValueError(f"{name}: no tensors")
-    dev = first[0].device
-    if dev.type != "cuda":
+    index = first[0].get_device()
+    if index < 0:
         raise RuntimeError(f"{name} needs ROCm device tensors")
-    for what, ts in lists.items():
+    for what, ts in zip(lists, out):
         if len(ts) != len(first):
             raise ValueError(f"{name}: {len(ts)} {what} for {len(first)} {next(iter(lists))}")
-        for t in ts:
-            if t.device != dev:
-                raise ValueError(f"{name}: one of the {what} is on {t.device}, expected {dev}")
-    return list(lists.values()), dev
+        if set(map(_T.get_device, ts)) != {index}:
+            other = next(t for t in ts if t.get_device() != index)
+            raise ValueError(f"{name}: one of the {what} is on {other.device}, expected {first[0].device}")
+    return out, index
 
 
-def _float_code(name, what, t):
-    code = _DT.get(t.dtype)
-    if code is None:
-        raise ValueError(f"{name}: one of the {what} has dtype {t.dtype}, not float32 or bfloat16")
-    return code
+def _contiguous(ts):
+    """Whether all are strided and contiguous (a tensor of another layout cannot be asked)."""
+    try:
+        return all(map(_T.is_contiguous, ts))
+    except RuntimeError:
+        return False
+
+
+def _codes(name, what, ts):
+    """The library's codes of the tensors' dtypes."""
+    try:
+        return [_DT[d] for d in map(_dtype_of, ts)]
+    except KeyError as e:
+        raise ValueError(f"{name}: one of the {what} has dtype {e.args[0]}, not float32 or bfloat16") from None
+
+
+def _table(n, *columns):
+    """The sdm_rt_tensor array of n tensors from its columns: param, grad, exp_avg, exp_avg_sq, n, dtype."""
+    rows = [0] * (_lib.TENSOR_FIELDS * n)
+    for i, c in enumerate(columns):
+        if c is not None:
+            rows[i::_lib.TENSOR_FIELDS] = c if type(c) is list else list(c)
+    return array.array("q", rows)
 
 
 def _written(tensors):
     """Tensors that a kernel has written in place: a graph that saved one must not read it again, and what is derived from one
     is derived anew."""
-    torch.autograd.graph.increment_version([t for t in tensors if not t.is_inference()])
+    try:
+        torch.autograd.graph.increment_version(tensors)
+    except RuntimeError:   # inference tensors count no versions
+        torch.autograd.graph.increment_version([t for t in tensors if not t.is_inference()])
 
 
 def grad_norm(tensors):
     """The norm of all of these tensors' values together, sqrt(sum of squares): a float32 scalar on their GPU.  float32 or
     bfloat16 tensors, mixed; the squares are summed in float64 in a fixed order (deterministic)."""
-    (ts,), dev = _listed("grad_norm", tensors=tensors)
-    rows, held = [], []
-    for t in ts:
-        if not _dense(t):
-            if t.layout is not torch.strided:
-                raise ValueError(f"grad_norm: a tensor of layout {t.layout}")
-            t = t.contiguous()
-            held.append(t)
-        rows += (0, t.data_ptr(), 0, 0, t.numel(), _float_code("grad_norm", "tensors", t))
-    table = array.array("q", rows)
+    (ts,), index = _lists("grad_norm", tensors=tensors)
+    codes = _codes("grad_norm", "tensors", ts)
+    if not _contiguous(ts):
+        other = {t.layout for t in ts} - {torch.strided}
+        if other:
+            raise ValueError(f"grad_norm: a tensor of layout {other.pop()}")
+        ts = [t if _dense(t) else t.contiguous() for t in ts]
+    n = len(ts)
+    table = _table(n, None, map(_T.data_ptr, ts), None, None, map(_T.numel, ts), codes)
     at, lib = table.buffer_info()[0], _lib.load()
-    out = torch.empty((), dtype=torch.float32, device=dev)
-    nbytes = lib.sdm_rt_grad_norm_workspace_bytes(at, len(ts))   # 0 outside the limits: the call below reports why
-    ws = torch.empty(nbytes // 8, dtype=torch.float64, device=dev)
-    _launch(lib.sdm_rt_grad_norm, out.get_device(), at, len(ts), out.data_ptr(), ws.data_ptr(), nbytes)
+    out = ts[0].new_empty((), dtype=torch.float32)
+    nbytes = lib.sdm_rt_grad_norm_workspace_bytes(at, n)   # 0 outside the limits: the call below reports why
+    ws = out.new_empty(nbytes // 8, dtype=torch.float64)
+    _launch(lib.sdm_rt_grad_norm, index, at, n, out.data_ptr(), ws.data_ptr(), nbytes)
     return out
+
+
+def _ordered_grads(name, ps, gs):
+    """The grads in the order of their params' values in memory: a grad of other strides is copied."""
+    out = []
+    for p, g in zip(ps, gs):
+        if not _dense(p):
+            raise ValueError(f"{name}: a param {tuple(p.shape)} of strides {tuple(p.stride())}: its values must be dense")
+        if g.layout is not torch.strided:
+            raise ValueError(f"{name}: a grad of layout {g.layout}")
+        out.append(g if g.stride() == p.stride() or (p.is_contiguous() and g.is_contiguous()) else torch.empty_like(p).copy_(g))
+    return out
+
+
+def _check_moments8(name, what, ms, sizes):
+    """8-bit moments (new_moments) for these numbers of values."""
+    if {m.dtype for m in ms} == {torch.uint8} and _contiguous(ms) and list(map(_shape_of, ms)) == [
+            (-(-n // MOMENT_BLOCK), MOMENT_BYTES) for n in sizes]:
+        return
+    for m, n in zip(ms, sizes):
+        want = (-(-n // MOMENT_BLOCK), MOMENT_BYTES)
+        if m.dtype != torch.uint8 or tuple(m.shape) != want or not m.is_contiguous():
+            raise ValueError(f"{name}: 8-bit moments must be contiguous uint8 {want} for {n} values, got {m.dtype} "
+                             f"{tuple(m.shape)}")
 
 
 def adamw(params, grads, exp_avgs, exp_avg_sqs=None, *, step, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2,
@@ -1933,38 +1982,34 @@ def adamw(params, grads, exp_avgs, exp_avg_sqs=None, *, step, lr=1e-3, betas=(0.
     name = "adamw"
     eight = exp_avg_sqs is None
     if eight:
-        (ps, gs, ms), dev = _listed(name, params=params, grads=grads, exp_avgs=exp_avgs)
-        vs = ms
+        (ps, gs, ms), index = _lists(name, params=params, grads=grads, exp_avgs=exp_avgs)
     else:
-        (ps, gs, ms, vs), dev = _listed(name, params=params, grads=grads, exp_avgs=exp_avgs, exp_avg_sqs=exp_avg_sqs)
-    rows, held, count = [], [], len(ps)
-    for i in range(count):
-        p, g, m, v = ps[i], gs[i], ms[i], vs[i]
-        n = p.numel()
-        if g.dtype != p.dtype or g.shape != p.shape:
-            raise ValueError(f"{name}: a grad of {g.dtype} {tuple(g.shape)} for a param of {p.dtype} {tuple(p.shape)}")
-        if not _dense(p):
-            raise ValueError(f"{name}: a param {tuple(p.shape)} of strides {tuple(p.stride())}: its values must be dense")
-        if g.layout is not torch.strided:
-            raise ValueError(f"{name}: a grad of layout {g.layout}")
-        if not p.is_contiguous() or not g.is_contiguous():
-            if g.stride() != p.stride():
-                g = torch.empty_like(p).copy_(g)
-                held.append(g)
-        if eight:
-            if m.dtype != torch.uint8 or tuple(m.shape) != (-(-n // MOMENT_BLOCK), MOMENT_BYTES) or not m.is_contiguous():
-                raise ValueError(f"{name}: 8-bit moments must be contiguous uint8 {(-(-n // MOMENT_BLOCK), MOMENT_BYTES)} for "
-                                 f"a param {tuple(p.shape)}, got {m.dtype} {tuple(m.shape)}")
-        else:
-            for t in (m, v):
-                if t.dtype != torch.float32 or t.shape != p.shape or (t.stride() != p.stride() and not (
-                        t.is_contiguous() and p.is_contiguous())):
-                    raise ValueError(f"{name}: moments must be float32 {tuple(p.shape)} of the param's strides "
-                                     f"{tuple(p.stride())}, got {t.dtype} {tuple(t.shape)} of {tuple(t.stride())}")
-        rows += (p.data_ptr(), g.data_ptr(), m.data_ptr(), 0 if eight else v.data_ptr(), n, _float_code(name, "params", p))
-    table = array.array("q", rows)
-    written = [a for k in ((0, 2) if eight else (0, 2, 3)) for a, n in zip(rows[k::6], rows[4::6]) if n]
-    if len(set(written)) != len(written) or not set(written).isdisjoint(rows[1::6]):
+        (ps, gs, ms, vs), index = _lists(name, params=params, grads=grads, exp_avgs=exp_avgs, exp_avg_sqs=exp_avg_sqs)
+    count, dev = len(ps), ps[0].device
+    codes, shapes, sizes = _codes(name, "params", ps), list(map(_shape_of, ps)), list(map(_T.numel, ps))
+    if list(map(_dtype_of, gs)) != list(map(_dtype_of, ps)) or list(map(_shape_of, gs)) != shapes:
+        p, g = next((p, g) for p, g in zip(ps, gs) if g.dtype != p.dtype or g.shape != p.shape)
+        raise ValueError(f"{name}: a grad of {g.dtype} {tuple(g.shape)} for a param of {p.dtype} {tuple(p.shape)}")
+    plain = _contiguous(ps) and _contiguous(gs)
+    if not plain:
+        gs = _ordered_grads(name, ps, gs)
+    if eight:
+        _check_moments8(name, "exp_avgs", ms, sizes)
+    else:
+        for ts in (ms, vs):
+            if set(map(_dtype_of, ts)) != {torch.float32} or list(map(_shape_of, ts)) != shapes or not (
+                    plain and _contiguous(ts)):
+                for p, t in zip(ps, ts):
+                    if t.dtype != torch.float32 or t.shape != p.shape or (t.stride() != p.stride() and not (
+                            t.is_contiguous() and p.is_contiguous())):
+                        raise ValueError(f"{name}: moments must be float32 {tuple(p.shape)} of the param's strides "
+                                         f"{tuple(p.stride())}, got {t.dtype} {tuple(t.shape)} of {tuple(t.stride())}")
+    at_p, at_g, at_m = (list(map(_T.data_ptr, ts)) for ts in (ps, gs, ms))
+    at_v = None if eight else list(map(_T.data_ptr, vs))
+    # an address of its own for everything that is written (0: a tensor without values)
+    written = at_p + at_m if eight else at_p + at_m + at_v
+    different = set(written)
+    if len(different) + written.count(0) - (0 in different) != len(written) or not different.isdisjoint(filter(None, at_g)):
         raise ValueError(f"{name}: a tensor occurs twice")
     t_dev, lr_dev = None, None
     if torch.is_tensor(step):
@@ -1984,7 +2029,8 @@ def adamw(params, grads, exp_avgs, exp_avg_sqs=None, *, step, lr=1e-3, betas=(0.
         raise ValueError(f"{name}: norm must be float32 with one element on {dev}")
     options = _lib.SdmRtAdamwOptions(lr, betas[0], betas[1], eps, weight_decay, step, _ptr(t_dev), _ptr(lr_dev), _ptr(norm),
                                      1.0 if max_norm is None else max_norm, 8 if eight else 32, seed & 0xffffffff)
-    _launch(_lib.load().sdm_rt_adamw, ps[0].get_device(), ctypes.byref(options), table.buffer_info()[0], count)
+    table = _table(count, at_p, at_g, at_m, at_v, sizes, codes)
+    _launch(_lib.load().sdm_rt_adamw, index, ctypes.byref(options), table.buffer_info()[0], count)
     _written(ps)
     _written(ms)
     if not eight:
@@ -1998,17 +2044,13 @@ def read_moments(moments, exp_avgs, exp_avg_sqs):
     """Writes the values that 8-bit moments (new_moments) stand for into exp_avgs and exp_avg_sqs: tensors of the params'
     sizes, contiguous, bfloat16 (which holds them exactly) or float32."""
     name = "read_moments"
-    (ss, ms, vs), dev = _listed(name, moments=moments, exp_avgs=exp_avgs, exp_avg_sqs=exp_avg_sqs)
-    rows = []
-    for s, m, v in zip(ss, ms, vs):
-        n = m.numel()
-        if s.dtype != torch.uint8 or tuple(s.shape) != (-(-n // MOMENT_BLOCK), MOMENT_BYTES) or not s.is_contiguous():
-            raise ValueError(f"{name}: moments must be contiguous uint8 {(-(-n // MOMENT_BLOCK), MOMENT_BYTES)} for {n} values, "
-                             f"got {s.dtype} {tuple(s.shape)}")
-        if v.numel() != n or v.dtype != m.dtype or not m.is_contiguous() or not v.is_contiguous():
-            raise ValueError(f"{name}: exp_avgs and exp_avg_sqs must be contiguous and alike in size and dtype")
-        rows += (m.data_ptr(), 0, s.data_ptr(), v.data_ptr(), n, _float_code(name, "exp_avgs", m))
-    table = array.array("q", rows)
-    _launch(_lib.load().sdm_rt_read_moments, ss[0].get_device(), table.buffer_info()[0], len(ss))
+    (ss, ms, vs), index = _lists(name, moments=moments, exp_avgs=exp_avgs, exp_avg_sqs=exp_avg_sqs)
+    sizes, codes = list(map(_T.numel, ms)), _codes(name, "exp_avgs", ms)
+    if list(map(_T.numel, vs)) != sizes or list(map(_dtype_of, vs)) != list(map(_dtype_of, ms)) or not _contiguous(ms) or (
+            not _contiguous(vs)):
+        raise ValueError(f"{name}: exp_avgs and exp_avg_sqs must be contiguous and alike in size and dtype")
+    _check_moments8(name, "moments", ss, sizes)
+    table = _table(len(ss), map(_T.data_ptr, ms), None, map(_T.data_ptr, ss), map(_T.data_ptr, vs), sizes, codes)
+    _launch(_lib.load().sdm_rt_read_moments, index, table.buffer_info()[0], len(ss))
     _written(ms)
     _written(vs)
