@@ -45,12 +45,48 @@ __device__ __forceinline__ int tensor_of(const StepTable<N>& table, uint32_t chu
   return lo;
 }
 
+// 8, 16 or 32 bytes at any element's address.  THROUGH: what a call streams through leaves the caches to others, and the memory
+// to longer bursts (a step of 110 M float32 values with their moments 620 us, 737 without; a model that the last-level cache
+// holds is better left there)
+template <bool THROUGH, int BYTES>
+__device__ __forceinline__ void load_bytes(const void* p, void* v) {
+  if constexpr (!THROUGH) {
+    __builtin_memcpy(v, p, BYTES);
+  } else if constexpr (BYTES == 8) {
+    const words2 w = __builtin_nontemporal_load(static_cast<const words2*>(p));
+    __builtin_memcpy(v, &w, 8);
+  } else {
+#pragma unroll
+    for (int i = 0; i < BYTES / 16; ++i) {
+      const words4 w = __builtin_nontemporal_load(static_cast<const words4*>(p) + i);
+      __builtin_memcpy(static_cast<char*>(v) + 16 * i, &w, 16);
+    }
+  }
+}
+template <bool THROUGH, int BYTES>
+__device__ __forceinline__ void store_bytes(void* p, const void* v) {
+  if constexpr (!THROUGH) {
+    __builtin_memcpy(p, v, BYTES);
+  } else if constexpr (BYTES == 8) {
+    words2 w;
+    __builtin_memcpy(&w, v, 8);
+    __builtin_nontemporal_store(w, static_cast<words2*>(p));
+  } else {
+#pragma unroll
+    for (int i = 0; i < BYTES / 16; ++i) {
+      words4 w;
+      __builtin_memcpy(&w, static_cast<const char*>(v) + 16 * i, 16);
+      __builtin_nontemporal_store(w, static_cast<words4*>(p) + i);
+    }
+  }
+}
+
 // N values of T at p, of which the first n are there (the others 0)
-template <typename T, int N>
+template <bool THROUGH, typename T, int N>
 __device__ __forceinline__ void load_values(const T* p, int64_t n, float (&v)[N]) {
   if (n >= N) {
     T x[N];
-    __builtin_memcpy(x, p, sizeof(x));
+    load_bytes<THROUGH, sizeof(x)>(p, x);
 #pragma unroll
     for (int e = 0; e < N; ++e) v[e] = to_f32(x[e]);
   } else {
@@ -58,16 +94,16 @@ __device__ __forceinline__ void load_values(const T* p, int64_t n, float (&v)[N]
     for (int e = 0; e < N; ++e) v[e] = e < n ? to_f32(p[e]) : 0.f;
   }
 }
-template <typename T, int N>
+template <bool THROUGH, typename T, int N>
 __device__ __forceinline__ void store_values(T* p, int64_t n, const float (&v)[N]) {
   if (n >= N) {
     if constexpr (sizeof(T) == 2) {
       uint32_t w[N / 2];
 #pragma unroll
       for (int e = 0; e < N / 2; ++e) w[e] = pack_bf16(v[2 * e], v[2 * e + 1]);
-      __builtin_memcpy(p, w, sizeof(w));
+      store_bytes<THROUGH, sizeof(w)>(p, w);
     } else {
-      __builtin_memcpy(p, v, sizeof(v));
+      store_bytes<THROUGH, sizeof(v)>(p, v);
     }
   } else {
 #pragma unroll
@@ -84,15 +120,25 @@ __device__ __forceinline__ double wave_add(double v) {
   return v;
 }
 
+// Eight pieces of a thread under way at once: one at a time left it waiting (220 MB of bfloat16 72 us).
 template <typename T>
 __device__ __forceinline__ double sum_squares(const T* g, int64_t n) {
-  constexpr int kN = 16 / static_cast<int>(sizeof(T));
+  constexpr int kN = 16 / static_cast<int>(sizeof(T)), kAtOnce = 8;
   double s = 0.0;
-  for (int64_t i = threadIdx.x * kN; i < n; i += kStepThreads * kN) {
-    float v[kN];
-    load_values(g + i, n - i, v);
+  for (int64_t i = threadIdx.x * kN; i < n; i += kAtOnce * kStepThreads * kN) {
+    float v[kAtOnce][kN];
 #pragma unroll
-    for (int e = 0; e < kN; ++e) s = fma(static_cast<double>(v[e]), static_cast<double>(v[e]), s);
+    for (int q = 0; q < kAtOnce; ++q) {
+      const int64_t at = i + q * kStepThreads * kN;
+      if (at < n)
+        load_values<false>(g + at, n - at, v[q]);
+      else
+        for (int e = 0; e < kN; ++e) v[q][e] = 0.f;
+    }
+#pragma unroll
+    for (int q = 0; q < kAtOnce; ++q)
+#pragma unroll
+      for (int e = 0; e < kN; ++e) s = fma(static_cast<double>(v[q][e]), static_cast<double>(v[q][e]), s);
   }
   return s;
 }
@@ -144,20 +190,37 @@ __device__ __forceinline__ uint32_t block_exponent(uint32_t bits) {
   const uint32_t e = (bits + 0xfffffu) >> 23;
   return e >= 254 ? 255 : e;
 }
+// 2^(E - 127), 0 for E = 0, NaN for E = 255
 __device__ __forceinline__ float block_scale(uint32_t e) { return __uint_as_float(e == 255 ? 0x7fc00000u : e << 23); }
 
-// A code's bits, put where float32 has its exponent and mantissa, are the value times a power of two: float32's own values
-// below its least normal one do for e = 0.  So decoding is a shift and two products, and encoding two products, the addition
-// of the random bits below the code's last place, and a shift, whatever the value's size.  TOP: the code's largest exponent.
-template <int TOP>
-__device__ __forceinline__ float decode(uint32_t magnitude, uint32_t sign, float scale) {
-  constexpr float up = TOP == 15 ? 0x1p112f : 0x1p96f;   // 2^(127 - TOP)
-  return __uint_as_float(magnitude << 20 | sign) * up * scale;
+// Codes.  The bits of a code of v, put where float32 has its exponent and mantissa, are the value times a power of two, for e =
+// 0 too (float32's values below its least normal one); those of m are a float16 so.  Encoding is the way back: the value
+// times a power of two, random bits added below the code's last place, the bits above taken.  None of it asks for a value's
+// size.
+__device__ __forceinline__ float decode_v(uint32_t codes, int q, int shift) {   // shift: v_shift's
+  const uint32_t bits = (q == 3 ? codes >> 4 : codes << (20 - 8 * q)) & 0x0ff00000u;
+  return __builtin_amdgcn_ldexpf(__uint_as_float(bits), shift);
 }
-template <int TOP>
-__device__ __forceinline__ uint32_t encode(float x, float inv_scale, uint32_t random16) {
-  constexpr float down = TOP == 15 ? 0x1p-112f : 0x1p-96f;
-  return (__float_as_uint(fabsf(x) * inv_scale * down) + (random16 << 4)) >> 20;
+__device__ __forceinline__ int v_shift(uint32_t e) { return e == 0 ? -400 : static_cast<int>(e) - 31; }
+typedef _Float16 halves __attribute__((ext_vector_type(2)));
+typedef short shorts __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ halves decode_m(uint32_t codes, int pair) {   // without the scale of its block
+  const uint32_t apart = __builtin_amdgcn_perm(0u, codes, pair ? 0x030c020cu : 0x010c000cu);   // each in the upper byte of a half
+  const shorts down = __builtin_bit_cast(shorts, apart) >> 1;
+  return __builtin_bit_cast(halves, __builtin_bit_cast(uint32_t, down) & 0xbfffbfffu);
+}
+// the code of a value in the upper byte of a word (shift: 15 - E for m, 31 - E for v, and far below for E = 0: code 0)
+__device__ __forceinline__ uint32_t encode_m(float m, int shift, uint32_t random16) {
+  const uint32_t t = __float_as_uint(__builtin_amdgcn_ldexpf(m, shift)) + (random16 << 4);
+  return (t << 4 & 0x7fffffffu) | (t & 0x80000000u);
+}
+__device__ __forceinline__ uint32_t encode_v(float v, int shift, uint32_t random16) {
+  const uint32_t t = __float_as_uint(__builtin_amdgcn_ldexpf(v, shift)) + (random16 << 4);
+  return max(t, v > 0.f ? 0x00100000u : 0u) << 4;   // a v above 0 has no code 0
+}
+// the upper bytes of four words
+__device__ __forceinline__ uint32_t upper_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return __builtin_amdgcn_perm(__builtin_amdgcn_perm(d, c, 0x07030c0cu), __builtin_amdgcn_perm(b, a, 0x0c0c0703u), 0x07060100u);
 }
 
 // the maximum over a row of 16 lanes, in each of them
@@ -192,20 +255,22 @@ __device__ __forceinline__ void read_step(StepArgs& a) {
   a.key = step_key(a.seed, t);
 }
 
-// One value's new moments and parameter.  Every product and sum of the moments is rounded by itself, as the formula is
-// written: their codes in 8 bits then do not hang on what a compiler fuses.
+// One value's new moments (from the old ones times beta1 and beta2) and parameter.  Every product and sum of the moments is
+// rounded by itself, as the formula is written: their codes in 8 bits then do not hang on what a compiler fuses.
 __device__ __forceinline__ void step_value(const StepArgs& a, float clip, float g, float& p, float& m, float& v) {
+  {
 #pragma clang fp contract(off)
-  g = g * clip;
-  m = m * a.b1 + g * a.c1;
-  v = v * a.b2 + g * g * a.c2;
-  const float d = __builtin_amdgcn_sqrtf(v) * a.r2 + a.eps;
-  p = p * a.decay - m * a.size * __builtin_amdgcn_rcpf(d);
+    g = g * clip;
+    m = m + g * a.c1;
+    v = v + g * g * a.c2;
+  }
+  const float d = fmaf(__builtin_amdgcn_sqrtf(v), a.r2, a.eps);
+  p = fmaf(m * -a.size, __builtin_amdgcn_rcpf(d), p * a.decay);
 }
 
 constexpr int kStepChunk = 4096;
 
-template <typename T>
+template <bool THROUGH, typename T>
 __device__ __forceinline__ void step_chunk32(const StepArgs& a, float clip, const StepTensor& t, int64_t begin, int64_t n) {
   T* p = reinterpret_cast<T*>(t.p) + begin;
   const T* g = reinterpret_cast<const T*>(t.g) + begin;
@@ -213,67 +278,78 @@ __device__ __forceinline__ void step_chunk32(const StepArgs& a, float clip, cons
   float* v = reinterpret_cast<float*>(t.v) + begin;
   for (int64_t i = threadIdx.x * 4; i < n; i += kStepThreads * 4) {
     float pv[4], gv[4], mv[4], vv[4];
-    load_values(p + i, n - i, pv);
-    load_values(g + i, n - i, gv);
-    load_values(m + i, n - i, mv);
-    load_values(v + i, n - i, vv);
+    load_values<THROUGH>(p + i, n - i, pv);
+    load_values<THROUGH>(g + i, n - i, gv);
+    load_values<THROUGH>(m + i, n - i, mv);
+    load_values<THROUGH>(v + i, n - i, vv);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) step_value(a, clip, gv[e], pv[e], mv[e], vv[e]);
-    store_values(p + i, n - i, pv);
-    store_values(m + i, n - i, mv);
-    store_values(v + i, n - i, vv);
+    for (int e = 0; e < 4; ++e) {
+      mv[e] *= a.b1;
+      vv[e] *= a.b2;
+      step_value(a, clip, gv[e], pv[e], mv[e], vv[e]);
+    }
+    store_values<THROUGH>(p + i, n - i, pv);
+    store_values<THROUGH>(m + i, n - i, mv);
+    store_values<THROUGH>(v + i, n - i, vv);
   }
 }
 
-// Sixteen lanes hold a block, 8 values each: its maxima come from four DPP steps.
-template <typename T>
+// Sixteen lanes hold a block, 8 values each: its maxima come from four DPP steps.  Past a tensor's end p, g and the codes are 0
+// and stay so.  What bounds it is instructions as much as memory (110 M bfloat16 values: 240 us at 72 a value).
+template <bool THROUGH, typename T>
 __device__ __forceinline__ void step_chunk8(const StepArgs& a, float clip, const StepTensor& t, int64_t begin, int64_t n) {
   T* p = reinterpret_cast<T*>(t.p) + begin;
   const T* g = reinterpret_cast<const T*>(t.g) + begin;
-  const int64_t whole = (n + kBlock - 1) / kBlock * kBlock;
-  for (int64_t i = threadIdx.x * 8; i < whole; i += kStepThreads * 8) {
-    const int64_t block = (begin + i) / kBlock;
-    char* state = t.m + block * kBlockBytes;
-    const int at = static_cast<int>(i % kBlock);
-    const uint2 cm = *reinterpret_cast<const uint2*>(state + at), cv = *reinterpret_cast<const uint2*>(state + kBlock + at);
+  char* chunk = t.m + begin / kBlock * kBlockBytes;
+  const int whole = static_cast<int>((n + kBlock - 1) / kBlock * kBlock);
+  for (int i = threadIdx.x * 8; i < whole; i += kStepThreads * 8) {
+    char* state = chunk + i / kBlock * kBlockBytes;
+    const int at = i % kBlock;
+    uint32_t cm[2], cv[2];
+    load_bytes<THROUGH, 8>(state + at, cm);
+    load_bytes<THROUGH, 8>(state + kBlock + at, cv);
     const uint32_t e = *reinterpret_cast<const uint16_t*>(state + 2 * kBlock);
     float pv[8], gv[8], mv[8], vv[8];
-    load_values(p + i, n - i, pv);
-    load_values(g + i, n - i, gv);
-    const float sm = block_scale(e & 255), sv = block_scale(e >> 8);
-    const uint32_t counter = t.block * static_cast<uint32_t>(kBlock) + static_cast<uint32_t>(begin + i) + a.key;
-    uint32_t am = 0, av = 0;
+    load_values<THROUGH>(p + i, n - i, pv);
+    load_values<THROUGH>(g + i, n - i, gv);
+    const float b1 = a.b1 * block_scale(e & 255), b2 = e >> 8 == 255 ? NAN : a.b2;
+    const int shift = v_shift(e >> 8);
+    float am = 0.f;
+    uint32_t av = 0;
 #pragma unroll
     for (int q = 0; q < 8; ++q) {
-      const uint32_t wm = (q < 4 ? cm.x : cm.y) >> (8 * (q & 3)), wv = (q < 4 ? cv.x : cv.y) >> (8 * (q & 3));
-      mv[q] = decode<15>(wm & 127, (wm & 128) << 24, sm);
-      vv[q] = decode<31>(wv & 255, 0, sv);
+      const halves h = decode_m(cm[q / 4], q / 2 & 1);
+      mv[q] = fmaf(static_cast<float>(q & 1 ? h.y : h.x), b1, 0.f);
+      vv[q] = decode_v(cv[q / 4], q & 3, shift) * b2;
       step_value(a, clip, gv[q], pv[q], mv[q], vv[q]);
-      if (i + q >= n) mv[q] = vv[q] = 0.f;
-      am = max(am, __float_as_uint(mv[q]) & 0x7fffffffu);
-      av = max(av, __float_as_uint(vv[q]) & 0x7fffffffu);
+      am = fmaxf(am, fabsf(mv[q]));   // passes over NaN: v has it then, or infinity
+      av = max(av, __float_as_uint(vv[q]));
     }
-    store_values(p + i, n - i, pv);
-    const uint32_t em = block_exponent(row16_max(am)), ev = block_exponent(row16_max(av));
-    const float im = __uint_as_float((254 - min(em, 254u)) << 23), iv = __uint_as_float((254 - min(ev, 254u)) << 23);
-    uint2 nm = make_uint2(0, 0), nv = make_uint2(0, 0);
+    store_values<THROUGH>(p + i, n - i, pv);
+    uint32_t em = block_exponent(row16_max(__float_as_uint(am)));
+    const uint32_t ev = block_exponent(row16_max(av));
+    em = ev == 255 ? 255 : em;
+    const int sm = em == 0 ? -400 : 15 - static_cast<int>(em), sv = ev == 0 ? -400 : 31 - static_cast<int>(ev);
+    const uint32_t counter = t.block * static_cast<uint32_t>(kBlock) + static_cast<uint32_t>(begin) + static_cast<uint32_t>(i) + a.key;
+    uint32_t nm[8], nv[8];
 #pragma unroll
     for (int q = 0; q < 8; ++q) {
       const uint32_t u = mix(counter + q);
-      uint32_t c = encode<15>(mv[q], im, u >> 16) | (__float_as_uint(mv[q]) >> 24 & 128);
-      uint32_t d = max(encode<31>(vv[q], iv, u & 0xffff), vv[q] > 0.f ? 1u : 0u);
-      if (em == 0 || em == 255) c = 0;
-      if (ev == 0 || ev == 255) d = 0;
-      (q < 4 ? nm.x : nm.y) |= c << (8 * (q & 3));
-      (q < 4 ? nv.x : nv.y) |= d << (8 * (q & 3));
+      nm[q] = encode_m(mv[q], sm, u >> 16);
+      nv[q] = encode_v(vv[q], sv, u & 0xffff);
     }
-    *reinterpret_cast<uint2*>(state + at) = nm;
-    *reinterpret_cast<uint2*>(state + kBlock + at) = nv;
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      cm[w] = upper_bytes(nm[4 * w], nm[4 * w + 1], nm[4 * w + 2], nm[4 * w + 3]);
+      cv[w] = upper_bytes(nv[4 * w], nv[4 * w + 1], nv[4 * w + 2], nv[4 * w + 3]);
+    }
+    store_bytes<THROUGH, 8>(state + at, cm);
+    store_bytes<THROUGH, 8>(state + kBlock + at, cv);
     if (at == 0) *reinterpret_cast<uint16_t*>(state + 2 * kBlock) = static_cast<uint16_t>(em | ev << 8);
   }
 }
 
-template <int BITS, bool DEVICE>
+template <int BITS, bool DEVICE, bool THROUGH>
 __global__ void __launch_bounds__(kStepThreads) adamw_kernel(StepTable<kStepTensors> table, StepArgs a) {
   if constexpr (DEVICE) read_step(a);
   const StepTensor& t = table.t[tensor_of(table, blockIdx.x)];
@@ -287,48 +363,52 @@ __global__ void __launch_bounds__(kStepThreads) adamw_kernel(StepTable<kStepTens
   }
   if constexpr (BITS == 32) {
     if (t.flags & 1)
-      step_chunk32<bf16_t>(a, clip, t, begin, n);
+      step_chunk32<THROUGH, bf16_t>(a, clip, t, begin, n);
     else
-      step_chunk32<float>(a, clip, t, begin, n);
+      step_chunk32<THROUGH, float>(a, clip, t, begin, n);
   } else {
     if (t.flags & 1)
-      step_chunk8<bf16_t>(a, clip, t, begin, n);
+      step_chunk8<THROUGH, bf16_t>(a, clip, t, begin, n);
     else
-      step_chunk8<float>(a, clip, t, begin, n);
+      step_chunk8<THROUGH, float>(a, clip, t, begin, n);
   }
 }
 
 // -- the values of 8-bit moments --------------------------------------------------------------------------------------
-template <typename T>
+template <bool THROUGH, typename T>
 __device__ __forceinline__ void read_chunk(const StepTensor& t, int64_t begin, int64_t n) {
   T* m = reinterpret_cast<T*>(t.p) + begin;
   T* v = reinterpret_cast<T*>(t.v) + begin;
-  for (int64_t i = threadIdx.x * 8; i < n; i += kStepThreads * 8) {
-    const char* state = t.m + (begin + i) / kBlock * kBlockBytes;
-    const int at = static_cast<int>(i % kBlock);
-    const uint2 cm = *reinterpret_cast<const uint2*>(state + at), cv = *reinterpret_cast<const uint2*>(state + kBlock + at);
+  const char* chunk = t.m + begin / kBlock * kBlockBytes;
+  for (int i = threadIdx.x * 8; i < n; i += kStepThreads * 8) {
+    const char* state = chunk + i / kBlock * kBlockBytes;
+    uint32_t cm[2], cv[2];
+    load_bytes<THROUGH, 8>(state + i % kBlock, cm);
+    load_bytes<THROUGH, 8>(state + kBlock + i % kBlock, cv);
     const uint32_t e = *reinterpret_cast<const uint16_t*>(state + 2 * kBlock);
-    const float sm = block_scale(e & 255), sv = block_scale(e >> 8);
+    const float scale = block_scale(e & 255), nan = e >> 8 == 255 ? NAN : 1.f;
+    const int shift = v_shift(e >> 8);
     float mv[8], vv[8];
 #pragma unroll
     for (int q = 0; q < 8; ++q) {
-      const uint32_t wm = (q < 4 ? cm.x : cm.y) >> (8 * (q & 3)), wv = (q < 4 ? cv.x : cv.y) >> (8 * (q & 3));
-      mv[q] = decode<15>(wm & 127, (wm & 128) << 24, sm);
-      vv[q] = decode<31>(wv & 255, 0, sv);
+      const halves h = decode_m(cm[q / 4], q / 2 & 1);
+      mv[q] = fmaf(static_cast<float>(q & 1 ? h.y : h.x), scale, 0.f);
+      vv[q] = decode_v(cv[q / 4], q & 3, shift) * nan;
     }
-    store_values(m + i, n - i, mv);
-    store_values(v + i, n - i, vv);
+    store_values<THROUGH>(m + i, n - i, mv);
+    store_values<THROUGH>(v + i, n - i, vv);
   }
 }
 
+template <bool THROUGH>
 __global__ void __launch_bounds__(kStepThreads) read_moments_kernel(StepTable<kStepTensors> table) {
   const StepTensor& t = table.t[tensor_of(table, blockIdx.x)];
   const int64_t begin = static_cast<int64_t>(blockIdx.x - t.chunk) * kStepChunk;
   const int64_t n = min(t.n - begin, static_cast<int64_t>(kStepChunk));
   if (t.flags & 1)
-    read_chunk<bf16_t>(t, begin, n);
+    read_chunk<THROUGH, bf16_t>(t, begin, n);
   else
-    read_chunk<float>(t, begin, n);
+    read_chunk<THROUGH, float>(t, begin, n);
 }
 
 // -- host -------------------------------------------------------------------------------------------------------------
@@ -425,11 +505,12 @@ int sdm_rt_adamw(const sdm_rt_adamw_options* o, const sdm_rt_tensor* tensors, in
   if (!o->t_device && o->t < 1) return set_err(SDM_RT_EINVAL, "t must be >= 1");
   if (o->norm && !(o->max_norm > 0.f)) return set_err(SDM_RT_EINVAL, "max_norm must be positive");
   if (o->state_bits != 32 && o->state_bits != 8) return set_err(SDM_RT_EINVAL, "state_bits must be 32 or 8");
-  int64_t total;
+  int64_t total, bytes = 0;   // bytes: of parameters, gradients and moments
   if (int rc = check_tensors(tensors, count, kStepChunk, &total)) return rc;
   for (int32_t i = 0; i < count; ++i) {
     const sdm_rt_tensor& t = tensors[i];
     if (t.n == 0) continue;
+    bytes += t.n * ((t.dtype == SDM_RT_BF16 ? 4 : 8) + (o->state_bits == 32 ? 8 : 2));
     if (!t.param || !t.grad || !t.exp_avg || (o->state_bits == 32) != (t.exp_avg_sq != nullptr))
       return set_err(SDM_RT_EINVAL, "tensor %d: param, grad and exp_avg must not be NULL, exp_avg_sq NULL for 8 bits alone", i);
     if (o->state_bits == 8 && reinterpret_cast<uintptr_t>(t.exp_avg) % 8)
@@ -461,20 +542,28 @@ int sdm_rt_adamw(const sdm_rt_adamw_options* o, const sdm_rt_tensor* tensors, in
   }
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (o->t_device) hipLaunchKernelGGL(count_step_kernel, dim3(1), dim3(1), 0, st, o->t_device);
-  for_tables(tensors, count, kStepChunk, [&](const StepTable<kStepTensors>& table, unsigned chunks, int64_t) {
-    const dim3 grid(chunks), threads(kStepThreads);
-    if (o->state_bits == 32) {
-      if (o->t_device)
-        hipLaunchKernelGGL((adamw_kernel<32, true>), grid, threads, 0, st, table, a);
-      else
-        hipLaunchKernelGGL((adamw_kernel<32, false>), grid, threads, 0, st, table, a);
-    } else {
-      if (o->t_device)
-        hipLaunchKernelGGL((adamw_kernel<8, true>), grid, threads, 0, st, table, a);
-      else
-        hipLaunchKernelGGL((adamw_kernel<8, false>), grid, threads, 0, st, table, a);
-    }
-  });
+  auto launch = [&](auto bits, auto device, auto through) {
+    for_tables(tensors, count, kStepChunk, [&](const StepTable<kStepTensors>& table, unsigned chunks, int64_t) {
+      hipLaunchKernelGGL((adamw_kernel<decltype(bits)::value, decltype(device)::value, decltype(through)::value>), dim3(chunks),
+                         dim3(kStepThreads), 0, st, table, a);
+    });
+  };
+  auto with_device = [&](auto bits, auto through) {
+    if (o->t_device)
+      launch(bits, std::true_type{}, through);
+    else
+      launch(bits, std::false_type{}, through);
+  };
+  auto with_bits = [&](auto through) {
+    if (o->state_bits == 32)
+      with_device(std::integral_constant<int, 32>{}, through);
+    else
+      with_device(std::integral_constant<int, 8>{}, through);
+  };
+  if (bytes > kStreamBytes)
+    with_bits(std::true_type{});
+  else
+    with_bits(std::false_type{});
   return check_launch("adamw");
 }
 
@@ -482,11 +571,12 @@ int64_t sdm_rt_moments_bytes(int64_t n) { return n > 0 ? (n + kBlock - 1) / kBlo
 
 int sdm_rt_read_moments(const sdm_rt_tensor* tensors, int32_t count, void* stream) {
   g_err[0] = 0;
-  int64_t total;
+  int64_t total, bytes = 0;
   if (int rc = check_tensors(tensors, count, kStepChunk, &total)) return rc;
   for (int32_t i = 0; i < count; ++i) {
     const sdm_rt_tensor& t = tensors[i];
     if (t.n == 0) continue;
+    bytes += t.n * (t.dtype == SDM_RT_BF16 ? 6 : 10);
     if (!t.param || !t.exp_avg || !t.exp_avg_sq) return set_err(SDM_RT_EINVAL, "tensor %d: a NULL pointer", i);
     if (reinterpret_cast<uintptr_t>(t.exp_avg) % 8)
       return set_err(SDM_RT_EINVAL, "tensor %d: 8-bit moments must be 8-byte aligned", i);
@@ -494,7 +584,10 @@ int sdm_rt_read_moments(const sdm_rt_tensor* tensors, int32_t count, void* strea
   if (total == 0) return SDM_RT_OK;
   hipStream_t st = static_cast<hipStream_t>(stream);
   for_tables(tensors, count, kStepChunk, [&](const StepTable<kStepTensors>& table, unsigned chunks, int64_t) {
-    hipLaunchKernelGGL(read_moments_kernel, dim3(chunks), dim3(kStepThreads), 0, st, table);
+    if (bytes > kStreamBytes)
+      hipLaunchKernelGGL(read_moments_kernel<true>, dim3(chunks), dim3(kStepThreads), 0, st, table);
+    else
+      hipLaunchKernelGGL(read_moments_kernel<false>, dim3(chunks), dim3(kStepThreads), 0, st, table);
   });
   return check_launch("read_moments");
 }
