@@ -1,9 +1,9 @@
 // sdm_step.hip -- the end of a training step over a whole model's tensors: the norm of the gradients (sdm_rt_grad_norm), the
 // AdamW step with its moments in 32 or in 8 bits (sdm_rt_adamw), and the values of 8-bit moments (sdm_rt_read_moments).
 //
-// A call takes a list of tensors.  Their addresses and sizes ride in the kernel's arguments (4 KB of them at most), some 80
-// to a launch: nothing is copied to the device, a captured launch holds all it needs, and no list has to outlive the call.
-// A tensor is cut into chunks, one a workgroup; a workgroup finds its tensor by its index in the chunks of the launch.
+// A call takes a list of tensors.  Their addresses and sizes ride in the kernel's arguments (under 4 KB of them), some 100 to a
+// launch: nothing is copied to the device, a captured launch holds all it needs, and no list has to outlive the call.  A tensor
+// is cut into chunks, one a workgroup.
 #include "sdm_vocab.h"
 
 namespace sdmrt {
@@ -13,36 +13,33 @@ constexpr int kBlock = 128;                       // values of a block of 8-bit 
 constexpr int kBlockBytes = 2 * kBlock + 8;       // codes of m, codes of v, two exponents, 6 unused
 
 // -- lists of tensors in kernel arguments -----------------------------------------------------------------------------
-struct StepTensor {
-  char* p;
-  const char* g;
-  char* m;
-  char* v;
-  int64_t n;
-  uint32_t chunk;   // its first chunk in this launch
-  uint32_t flags;   // bit 0: bfloat16
-  uint32_t block;   // the blocks of the tensors before it in the call
-  uint32_t pad;
-};
-template <int N>
+template <int P, int N, bool BLOCKS = false>   // addresses of a tensor, tensors at most
 struct StepTable {
-  StepTensor t[N];
-  int count;
+  static constexpr int kAddresses = P, kTensors = N, kSearched = (N + 64) / 64 * 64;
+  static constexpr bool kBlocks = BLOCKS;
+  char* at[P][N];
+  uint32_t chunk[kSearched];         // each tensor's first chunk in the launch, then the number of all, then ~0
+  uint32_t block[BLOCKS ? N : 1];    // blocks of 8-bit moments of the tensors before it in the call
+  uint16_t tail[N];                  // values of its last chunk, less one; bit 15: bfloat16
 };
-constexpr int kStepTensors = 68;   // 56 bytes each and the options: under 4 KB
 
-// the tensor of a chunk: the last one that begins at or before it
-template <int N>
-__device__ __forceinline__ int tensor_of(const StepTable<N>& table, uint32_t chunk) {
-  int lo = 0, hi = table.count - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) / 2;
-    if (table.t[mid].chunk <= chunk)
-      lo = mid;
-    else
-      hi = mid - 1;
-  }
-  return lo;
+// A workgroup's chunk: its tensor, where it begins there and how many values it has.  Every wave finds its tensor at once: a lane
+// looks at each (a search by halves waits for one load after the other).
+struct StepChunk {
+  int tensor;
+  bool bf16;
+  int n;
+  int64_t begin;
+};
+template <int CHUNK, typename TABLE>
+__device__ __forceinline__ StepChunk find_chunk(const TABLE& table, uint32_t index) {
+  int t = -1;
+#pragma unroll
+  for (int i = 0; i < TABLE::kSearched; i += 64) t += __popcll(__ballot(table.chunk[i + (threadIdx.x & 63)] <= index));
+  const uint32_t first = table.chunk[t];
+  const int tail = table.tail[t];
+  return StepChunk{t, (tail & 0x8000) != 0, index + 1 == table.chunk[t + 1] ? (tail & 0x7fff) + 1 : CHUNK,
+                   static_cast<int64_t>(index - first) * CHUNK};
 }
 
 // 8, 16 or 32 bytes at any element's address.  THROUGH: what a call streams through leaves the caches to others, and the memory
@@ -113,7 +110,7 @@ __device__ __forceinline__ void store_values(T* p, int64_t n, const float (&v)[N
 }
 
 // -- the gradients' norm ----------------------------------------------------------------------------------------------
-constexpr int kNormChunk = 16384;
+using NormTable = StepTable<1, 191>;
 
 __device__ __forceinline__ double wave_add(double v) {
   for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d);
@@ -122,14 +119,14 @@ __device__ __forceinline__ double wave_add(double v) {
 
 // Eight pieces of a thread under way at once: one at a time left it waiting (220 MB of bfloat16 72 us).
 template <typename T>
-__device__ __forceinline__ double sum_squares(const T* g, int64_t n) {
+__device__ __forceinline__ double sum_squares(const T* g, int n) {
   constexpr int kN = 16 / static_cast<int>(sizeof(T)), kAtOnce = 8;
   double s = 0.0;
-  for (int64_t i = threadIdx.x * kN; i < n; i += kAtOnce * kStepThreads * kN) {
+  for (int i = threadIdx.x * kN; i < n; i += kAtOnce * kStepThreads * kN) {
     float v[kAtOnce][kN];
 #pragma unroll
     for (int q = 0; q < kAtOnce; ++q) {
-      const int64_t at = i + q * kStepThreads * kN;
+      const int at = i + q * kStepThreads * kN;
       if (at < n)
         load_values<false>(g + at, n - at, v[q]);
       else
@@ -144,13 +141,13 @@ __device__ __forceinline__ double sum_squares(const T* g, int64_t n) {
 }
 
 // Each chunk's sum of squares in float64: no gradient is too large or too small for its square, and the order is fixed.
-__global__ void __launch_bounds__(kStepThreads) norm_kernel(StepTable<kStepTensors> table, double* __restrict__ partial) {
+template <int CHUNK>
+__global__ void __launch_bounds__(kStepThreads) norm_kernel(NormTable table, double* __restrict__ partial) {
   __shared__ double red[kStepThreads / 64];
-  const StepTensor& t = table.t[tensor_of(table, blockIdx.x)];
-  const int64_t begin = static_cast<int64_t>(blockIdx.x - t.chunk) * kNormChunk;
-  const int64_t n = min(t.n - begin, static_cast<int64_t>(kNormChunk));
-  double s = t.flags & 1 ? sum_squares(reinterpret_cast<const bf16_t*>(t.g) + begin, n)
-                         : sum_squares(reinterpret_cast<const float*>(t.g) + begin, n);
+  const StepChunk c = find_chunk<CHUNK>(table, blockIdx.x);
+  const char* g = table.at[0][c.tensor];
+  double s = c.bf16 ? sum_squares(reinterpret_cast<const bf16_t*>(g) + c.begin, c.n)
+                    : sum_squares(reinterpret_cast<const float*>(g) + c.begin, c.n);
   s = wave_add(s);
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
   __syncthreads();
@@ -268,40 +265,44 @@ __device__ __forceinline__ void step_value(const StepArgs& a, float clip, float 
   p = fmaf(m * -a.size, __builtin_amdgcn_rcpf(d), p * a.decay);
 }
 
-constexpr int kStepChunk = 4096;
+using StepTable32 = StepTable<4, 96>;
+using StepTable8 = StepTable<3, 108, true>;
 
-template <bool THROUGH, typename T>
-__device__ __forceinline__ void step_chunk32(const StepArgs& a, float clip, const StepTensor& t, int64_t begin, int64_t n) {
-  T* p = reinterpret_cast<T*>(t.p) + begin;
-  const T* g = reinterpret_cast<const T*>(t.g) + begin;
-  float* m = reinterpret_cast<float*>(t.m) + begin;
-  float* v = reinterpret_cast<float*>(t.v) + begin;
-  for (int64_t i = threadIdx.x * 4; i < n; i += kStepThreads * 4) {
-    float pv[4], gv[4], mv[4], vv[4];
-    load_values<THROUGH>(p + i, n - i, pv);
-    load_values<THROUGH>(g + i, n - i, gv);
-    load_values<THROUGH>(m + i, n - i, mv);
-    load_values<THROUGH>(v + i, n - i, vv);
+// All of a thread's pieces of a chunk are loaded before the first is computed on.
+template <int CHUNK, bool THROUGH, typename T>
+__device__ __forceinline__ void step_chunk32(const StepArgs& a, float clip, T* p, const T* g, float* m, float* v, int n) {
+  constexpr int kPieces = CHUNK / (kStepThreads * 4);
+  float pv[kPieces][4], gv[kPieces][4], mv[kPieces][4], vv[kPieces][4];
+#pragma unroll
+  for (int q = 0; q < kPieces; ++q) {
+    const int i = (q * kStepThreads + threadIdx.x) * 4;
+    if (i >= n) break;
+    load_values<THROUGH>(p + i, n - i, pv[q]);
+    load_values<THROUGH>(g + i, n - i, gv[q]);
+    load_values<THROUGH>(m + i, n - i, mv[q]);
+    load_values<THROUGH>(v + i, n - i, vv[q]);
+  }
+#pragma unroll
+  for (int q = 0; q < kPieces; ++q) {
+    const int i = (q * kStepThreads + threadIdx.x) * 4;
+    if (i >= n) break;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      mv[e] *= a.b1;
-      vv[e] *= a.b2;
-      step_value(a, clip, gv[e], pv[e], mv[e], vv[e]);
+      mv[q][e] *= a.b1;
+      vv[q][e] *= a.b2;
+      step_value(a, clip, gv[q][e], pv[q][e], mv[q][e], vv[q][e]);
     }
-    store_values<THROUGH>(p + i, n - i, pv);
-    store_values<THROUGH>(m + i, n - i, mv);
-    store_values<THROUGH>(v + i, n - i, vv);
+    store_values<THROUGH>(p + i, n - i, pv[q]);
+    store_values<THROUGH>(m + i, n - i, mv[q]);
+    store_values<THROUGH>(v + i, n - i, vv[q]);
   }
 }
 
 // Sixteen lanes hold a block, 8 values each: its maxima come from four DPP steps.  Past a tensor's end p, g and the codes are 0
 // and stay so.  What bounds it is instructions as much as memory (110 M bfloat16 values: 240 us at 72 a value).
 template <bool THROUGH, typename T>
-__device__ __forceinline__ void step_chunk8(const StepArgs& a, float clip, const StepTensor& t, int64_t begin, int64_t n) {
-  T* p = reinterpret_cast<T*>(t.p) + begin;
-  const T* g = reinterpret_cast<const T*>(t.g) + begin;
-  char* chunk = t.m + begin / kBlock * kBlockBytes;
-  const int whole = static_cast<int>((n + kBlock - 1) / kBlock * kBlock);
+__device__ __forceinline__ void step_chunk8(const StepArgs& a, float clip, T* p, const T* g, char* chunk, uint32_t position, int n) {
+  const int whole = (n + kBlock - 1) / kBlock * kBlock;
   for (int i = threadIdx.x * 8; i < whole; i += kStepThreads * 8) {
     char* state = chunk + i / kBlock * kBlockBytes;
     const int at = i % kBlock;
@@ -330,7 +331,7 @@ __device__ __forceinline__ void step_chunk8(const StepArgs& a, float clip, const
     const uint32_t ev = block_exponent(row16_max(av));
     em = ev == 255 ? 255 : em;
     const int sm = em == 0 ? -400 : 15 - static_cast<int>(em), sv = ev == 0 ? -400 : 31 - static_cast<int>(ev);
-    const uint32_t counter = t.block * static_cast<uint32_t>(kBlock) + static_cast<uint32_t>(begin) + static_cast<uint32_t>(i) + a.key;
+    const uint32_t counter = position + static_cast<uint32_t>(i) + a.key;
     uint32_t nm[8], nv[8];
 #pragma unroll
     for (int q = 0; q < 8; ++q) {
@@ -349,37 +350,53 @@ __device__ __forceinline__ void step_chunk8(const StepArgs& a, float clip, const
   }
 }
 
-template <int BITS, bool DEVICE, bool THROUGH>
-__global__ void __launch_bounds__(kStepThreads) adamw_kernel(StepTable<kStepTensors> table, StepArgs a) {
+// a norm that is NaN makes the gradients NaN, as a product with it would
+__device__ __forceinline__ float clip_factor(const StepArgs& a) {
+  if (!a.norm) return 1.f;
+  const float c = a.max_norm / (*a.norm + 1e-6f);
+  return c > 1.f ? 1.f : c;
+}
+
+template <int CHUNK, bool DEVICE, bool THROUGH>
+__global__ void __launch_bounds__(kStepThreads) adamw32_kernel(StepTable32 table, StepArgs a) {
   if constexpr (DEVICE) read_step(a);
-  const StepTensor& t = table.t[tensor_of(table, blockIdx.x)];
-  const int64_t begin = static_cast<int64_t>(blockIdx.x - t.chunk) * kStepChunk;
-  const int64_t n = min(t.n - begin, static_cast<int64_t>(kStepChunk));
-  // a norm that is NaN makes the gradients NaN, as a product with it would
-  float clip = 1.f;
-  if (a.norm) {
-    clip = a.max_norm / (*a.norm + 1e-6f);
-    clip = clip > 1.f ? 1.f : clip;
-  }
-  if constexpr (BITS == 32) {
-    if (t.flags & 1)
-      step_chunk32<THROUGH, bf16_t>(a, clip, t, begin, n);
-    else
-      step_chunk32<THROUGH, float>(a, clip, t, begin, n);
-  } else {
-    if (t.flags & 1)
-      step_chunk8<THROUGH, bf16_t>(a, clip, t, begin, n);
-    else
-      step_chunk8<THROUGH, float>(a, clip, t, begin, n);
-  }
+  const float clip = clip_factor(a);
+  const StepChunk c = find_chunk<CHUNK>(table, blockIdx.x);
+  char* p = table.at[0][c.tensor];
+  const char* g = table.at[1][c.tensor];
+  float* m = reinterpret_cast<float*>(table.at[2][c.tensor]) + c.begin;
+  float* v = reinterpret_cast<float*>(table.at[3][c.tensor]) + c.begin;
+  if (c.bf16)
+    step_chunk32<CHUNK, THROUGH>(a, clip, reinterpret_cast<bf16_t*>(p) + c.begin, reinterpret_cast<const bf16_t*>(g) + c.begin, m,
+                                 v, c.n);
+  else
+    step_chunk32<CHUNK, THROUGH>(a, clip, reinterpret_cast<float*>(p) + c.begin, reinterpret_cast<const float*>(g) + c.begin, m, v,
+                                 c.n);
+}
+
+template <int CHUNK, bool DEVICE, bool THROUGH>
+__global__ void __launch_bounds__(kStepThreads) adamw8_kernel(StepTable8 table, StepArgs a) {
+  if constexpr (DEVICE) read_step(a);
+  const float clip = clip_factor(a);
+  const StepChunk c = find_chunk<CHUNK>(table, blockIdx.x);
+  char* p = table.at[0][c.tensor];
+  const char* g = table.at[1][c.tensor];
+  char* state = table.at[2][c.tensor] + c.begin / kBlock * kBlockBytes;
+  const uint32_t position = table.block[c.tensor] * static_cast<uint32_t>(kBlock) + static_cast<uint32_t>(c.begin);
+  if (c.bf16)
+    step_chunk8<THROUGH>(a, clip, reinterpret_cast<bf16_t*>(p) + c.begin, reinterpret_cast<const bf16_t*>(g) + c.begin, state,
+                         position, c.n);
+  else
+    step_chunk8<THROUGH>(a, clip, reinterpret_cast<float*>(p) + c.begin, reinterpret_cast<const float*>(g) + c.begin, state,
+                         position, c.n);
 }
 
 // -- the values of 8-bit moments --------------------------------------------------------------------------------------
+using ReadTable = StepTable<3, 120>;
+constexpr int kReadChunk = 4096;
+
 template <bool THROUGH, typename T>
-__device__ __forceinline__ void read_chunk(const StepTensor& t, int64_t begin, int64_t n) {
-  T* m = reinterpret_cast<T*>(t.p) + begin;
-  T* v = reinterpret_cast<T*>(t.v) + begin;
-  const char* chunk = t.m + begin / kBlock * kBlockBytes;
+__device__ __forceinline__ void read_chunk(T* m, T* v, const char* chunk, int n) {
   for (int i = threadIdx.x * 8; i < n; i += kStepThreads * 8) {
     const char* state = chunk + i / kBlock * kBlockBytes;
     uint32_t cm[2], cv[2];
@@ -401,63 +418,77 @@ __device__ __forceinline__ void read_chunk(const StepTensor& t, int64_t begin, i
 }
 
 template <bool THROUGH>
-__global__ void __launch_bounds__(kStepThreads) read_moments_kernel(StepTable<kStepTensors> table) {
-  const StepTensor& t = table.t[tensor_of(table, blockIdx.x)];
-  const int64_t begin = static_cast<int64_t>(blockIdx.x - t.chunk) * kStepChunk;
-  const int64_t n = min(t.n - begin, static_cast<int64_t>(kStepChunk));
-  if (t.flags & 1)
-    read_chunk<THROUGH, bf16_t>(t, begin, n);
+__global__ void __launch_bounds__(kStepThreads) read_moments_kernel(ReadTable table) {
+  const StepChunk c = find_chunk<kReadChunk>(table, blockIdx.x);
+  const char* state = table.at[0][c.tensor] + c.begin / kBlock * kBlockBytes;
+  char *m = table.at[1][c.tensor], *v = table.at[2][c.tensor];
+  if (c.bf16)
+    read_chunk<THROUGH>(reinterpret_cast<bf16_t*>(m) + c.begin, reinterpret_cast<bf16_t*>(v) + c.begin, state, c.n);
   else
-    read_chunk<THROUGH, float>(t, begin, n);
+    read_chunk<THROUGH>(reinterpret_cast<float*>(m) + c.begin, reinterpret_cast<float*>(v) + c.begin, state, c.n);
 }
 
 // -- host -------------------------------------------------------------------------------------------------------------
-static_assert(sizeof(StepTable<kStepTensors>) + sizeof(StepArgs) + 16 <= 4096, "kernel arguments");
+static_assert(sizeof(StepTable32) + sizeof(StepArgs) + 16 <= 4096 && sizeof(StepTable8) + sizeof(StepArgs) + 16 <= 4096 &&
+                  sizeof(NormTable) + 32 <= 4096 && sizeof(ReadTable) + 16 <= 4096,
+              "kernel arguments");
 
 inline int64_t chunks_of(int64_t n, int chunk) { return (n + chunk - 1) / chunk; }
 
-// Every check that needs no device; total: the chunks of all tensors.
-inline int check_tensors(const sdm_rt_tensor* t, int32_t count, int chunk, int64_t* total) {
+// Every check that needs no device; values: the sum of the n.  Chunks are at least 1,024 values: fewer than 2^24 in a launch.
+inline int check_tensors(const sdm_rt_tensor* t, int32_t count, int64_t* values) {
   if (count < 0 || (count > 0 && !t)) return set_err(SDM_RT_EINVAL, "count must be >= 0, tensors not NULL");
-  *total = 0;
+  *values = 0;
   for (int32_t i = 0; i < count; ++i) {
     if (t[i].n < 0) return set_err(SDM_RT_EINVAL, "tensor %d: n must be >= 0", i);
     if (t[i].dtype != SDM_RT_F32 && t[i].dtype != SDM_RT_BF16)
       return set_err(SDM_RT_EINVAL, "tensor %d: unknown dtype %lld", i, (long long)t[i].dtype);
-    if (t[i].n > (int64_t{1} << 38)) return set_err(SDM_RT_EUNSUPPORTED, "tensor %d: n must be at most 2^38", i);
-    *total += chunks_of(t[i].n, chunk);
+    if (t[i].n > (int64_t{1} << 33)) return set_err(SDM_RT_EUNSUPPORTED, "tensor %d: n must be at most 2^33", i);
+    *values += t[i].n;
+    if (*values > (int64_t{1} << 34)) return set_err(SDM_RT_EUNSUPPORTED, "more than 2^34 values in one call");
   }
-  if (*total > (int64_t{1} << 23)) return set_err(SDM_RT_EUNSUPPORTED, "too many values in one call");
   return SDM_RT_OK;
 }
 
-// launch(table, chunks of the launch, chunks before it) over the list, as many tensors at a time as a launch takes
-template <typename F>
-void for_tables(const sdm_rt_tensor* t, int32_t count, int chunk, F launch) {
-  StepTable<kStepTensors> table;
-  table.count = 0;
+// launch(table, chunks of the launch, chunks before it) over the list, as many tensors at a time as a launch takes; take(tensor,
+// addresses) says which addresses the kernel needs
+template <typename TABLE, typename TAKE, typename LAUNCH>
+void for_tables(const sdm_rt_tensor* t, int32_t count, int chunk, TAKE take, LAUNCH launch) {
+  TABLE table{};
+  int filled = 0;
   int64_t chunks = 0, before = 0, blocks = 0;
   auto flush = [&] {
-    if (table.count) launch(table, static_cast<unsigned>(chunks), before);
+    if (!filled) return;
+    table.chunk[filled] = static_cast<uint32_t>(chunks);
+    for (int i = filled + 1; i < TABLE::kSearched; ++i) table.chunk[i] = ~0u;
+    launch(table, static_cast<unsigned>(chunks), before);
     before += chunks;
-    chunks = table.count = 0;
+    chunks = filled = 0;
   };
   for (int32_t i = 0; i < count; ++i) {
     if (t[i].n == 0) continue;
-    if (table.count == kStepTensors) flush();
-    StepTensor& s = table.t[table.count++];
-    s.p = static_cast<char*>(t[i].param);
-    s.g = static_cast<const char*>(t[i].grad);
-    s.m = static_cast<char*>(t[i].exp_avg);
-    s.v = static_cast<char*>(t[i].exp_avg_sq);
-    s.n = t[i].n;
-    s.chunk = static_cast<uint32_t>(chunks);
-    s.flags = t[i].dtype == SDM_RT_BF16;
-    s.block = static_cast<uint32_t>(blocks);
+    if (filled == TABLE::kTensors) flush();
+    char* at[TABLE::kAddresses];
+    take(t[i], at);
+    for (int k = 0; k < TABLE::kAddresses; ++k) table.at[k][filled] = at[k];
+    table.chunk[filled] = static_cast<uint32_t>(chunks);
+    table.tail[filled] = static_cast<uint16_t>((t[i].n - 1) % chunk | (t[i].dtype == SDM_RT_BF16 ? 0x8000 : 0));
+    if (TABLE::kBlocks) table.block[filled] = static_cast<uint32_t>(blocks);
     chunks += chunks_of(t[i].n, chunk);
     blocks += chunks_of(t[i].n, kBlock);
+    ++filled;
   }
   flush();
+}
+
+// Few values take small chunks, so that all compute units have some.
+constexpr int64_t kSmallStep = 8 << 20, kSmallNorm = 8 << 20;
+
+inline int norm_chunk(int64_t values) { return values <= kSmallNorm ? 4096 : 16384; }
+inline int64_t norm_partials(const sdm_rt_tensor* t, int32_t count, int64_t values) {
+  int64_t n = 0;
+  for (int32_t i = 0; i < count; ++i) n += chunks_of(t[i].n, norm_chunk(values));
+  return n;
 }
 
 }  // namespace sdmrt
@@ -467,28 +498,36 @@ using namespace sdmrt;
 extern "C" {
 
 size_t sdm_rt_grad_norm_workspace_bytes(const sdm_rt_tensor* tensors, int32_t count) {
-  int64_t total;
-  return check_tensors(tensors, count, kNormChunk, &total) ? 0 : static_cast<size_t>(total) * sizeof(double);
+  int64_t values;
+  return check_tensors(tensors, count, &values) ? 0 : static_cast<size_t>(norm_partials(tensors, count, values)) * sizeof(double);
 }
 
 int sdm_rt_grad_norm(const sdm_rt_tensor* tensors, int32_t count, float* norm, void* workspace, size_t workspace_bytes,
                      void* stream) {
   g_err[0] = 0;
-  int64_t total;
-  if (int rc = check_tensors(tensors, count, kNormChunk, &total)) return rc;
+  int64_t values;
+  if (int rc = check_tensors(tensors, count, &values)) return rc;
   for (int32_t i = 0; i < count; ++i)
     if (tensors[i].n && !tensors[i].grad) return set_err(SDM_RT_EINVAL, "tensor %d: grad is NULL", i);
   if (!norm) return set_err(SDM_RT_EINVAL, "norm is NULL");
-  const size_t need = static_cast<size_t>(total) * sizeof(double);
+  const int64_t partials = norm_partials(tensors, count, values);
+  const size_t need = static_cast<size_t>(partials) * sizeof(double);
   if (need && (!workspace || workspace_bytes < need))
     return set_err(SDM_RT_ENOSPACE, "workspace of %zu bytes, %zu needed", workspace ? workspace_bytes : 0, need);
   if (reinterpret_cast<uintptr_t>(workspace) % 8) return set_err(SDM_RT_EINVAL, "workspace must be 8-byte aligned");
   hipStream_t st = static_cast<hipStream_t>(stream);
   double* partial = static_cast<double*>(workspace);
-  for_tables(tensors, count, kNormChunk, [&](const StepTable<kStepTensors>& table, unsigned chunks, int64_t before) {
-    hipLaunchKernelGGL(norm_kernel, dim3(chunks), dim3(kStepThreads), 0, st, table, partial + before);
-  });
-  hipLaunchKernelGGL(norm_join_kernel, dim3(1), dim3(1024), 0, st, partial, static_cast<int>(total), norm);
+  const int chunk = norm_chunk(values);
+  for_tables<NormTable>(
+      tensors, count, chunk,
+      [](const sdm_rt_tensor& t, char** at) { at[0] = static_cast<char*>(const_cast<void*>(t.grad)); },
+      [&](const NormTable& table, unsigned chunks, int64_t before) {
+        if (chunk == 4096)
+          hipLaunchKernelGGL(norm_kernel<4096>, dim3(chunks), dim3(kStepThreads), 0, st, table, partial + before);
+        else
+          hipLaunchKernelGGL(norm_kernel<16384>, dim3(chunks), dim3(kStepThreads), 0, st, table, partial + before);
+      });
+  hipLaunchKernelGGL(norm_join_kernel, dim3(1), dim3(1024), 0, st, partial, static_cast<int>(partials), norm);
   return check_launch("grad_norm");
 }
 
@@ -505,8 +544,8 @@ int sdm_rt_adamw(const sdm_rt_adamw_options* o, const sdm_rt_tensor* tensors, in
   if (!o->t_device && o->t < 1) return set_err(SDM_RT_EINVAL, "t must be >= 1");
   if (o->norm && !(o->max_norm > 0.f)) return set_err(SDM_RT_EINVAL, "max_norm must be positive");
   if (o->state_bits != 32 && o->state_bits != 8) return set_err(SDM_RT_EINVAL, "state_bits must be 32 or 8");
-  int64_t total, bytes = 0;   // bytes: of parameters, gradients and moments
-  if (int rc = check_tensors(tensors, count, kStepChunk, &total)) return rc;
+  int64_t values, bytes = 0;   // bytes: of parameters, gradients and moments
+  if (int rc = check_tensors(tensors, count, &values)) return rc;
   for (int32_t i = 0; i < count; ++i) {
     const sdm_rt_tensor& t = tensors[i];
     if (t.n == 0) continue;
@@ -516,7 +555,7 @@ int sdm_rt_adamw(const sdm_rt_adamw_options* o, const sdm_rt_tensor* tensors, in
     if (o->state_bits == 8 && reinterpret_cast<uintptr_t>(t.exp_avg) % 8)
       return set_err(SDM_RT_EINVAL, "tensor %d: 8-bit moments must be 8-byte aligned", i);
   }
-  if (total == 0 && !o->t_device) return SDM_RT_OK;
+  if (values == 0 && !o->t_device) return SDM_RT_OK;
   StepArgs a{};
   a.b1 = static_cast<float>(o->beta1);
   a.c1 = static_cast<float>(1.0 - o->beta1);
@@ -542,28 +581,47 @@ int sdm_rt_adamw(const sdm_rt_adamw_options* o, const sdm_rt_tensor* tensors, in
   }
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (o->t_device) hipLaunchKernelGGL(count_step_kernel, dim3(1), dim3(1), 0, st, o->t_device);
-  auto launch = [&](auto bits, auto device, auto through) {
-    for_tables(tensors, count, kStepChunk, [&](const StepTable<kStepTensors>& table, unsigned chunks, int64_t) {
-      hipLaunchKernelGGL((adamw_kernel<decltype(bits)::value, decltype(device)::value, decltype(through)::value>), dim3(chunks),
-                         dim3(kStepThreads), 0, st, table, a);
-    });
+  auto launch = [&](auto small, auto device, auto through) {
+    constexpr bool kSmall = decltype(small)::value, kDevice = decltype(device)::value, kThrough = decltype(through)::value;
+    if (o->state_bits == 32) {
+      constexpr int kChunk = kSmall ? 1024 : 4096;
+      for_tables<StepTable32>(
+          tensors, count, kChunk,
+          [](const sdm_rt_tensor& t, char** at) {
+            at[0] = static_cast<char*>(t.param);
+            at[1] = static_cast<char*>(const_cast<void*>(t.grad));
+            at[2] = static_cast<char*>(t.exp_avg);
+            at[3] = static_cast<char*>(t.exp_avg_sq);
+          },
+          [&](const StepTable32& table, unsigned chunks, int64_t) {
+            hipLaunchKernelGGL((adamw32_kernel<kChunk, kDevice, kThrough>), dim3(chunks), dim3(kStepThreads), 0, st, table, a);
+          });
+    } else {
+      constexpr int kChunk = kSmall ? 2048 : 4096;
+      for_tables<StepTable8>(
+          tensors, count, kChunk,
+          [](const sdm_rt_tensor& t, char** at) {
+            at[0] = static_cast<char*>(t.param);
+            at[1] = static_cast<char*>(const_cast<void*>(t.grad));
+            at[2] = static_cast<char*>(t.exp_avg);
+          },
+          [&](const StepTable8& table, unsigned chunks, int64_t) {
+            hipLaunchKernelGGL((adamw8_kernel<kChunk, kDevice, kThrough>), dim3(chunks), dim3(kStepThreads), 0, st, table, a);
+          });
+    }
   };
-  auto with_device = [&](auto bits, auto through) {
+  auto with_device = [&](auto small, auto through) {
     if (o->t_device)
-      launch(bits, std::true_type{}, through);
+      launch(small, std::true_type{}, through);
     else
-      launch(bits, std::false_type{}, through);
-  };
-  auto with_bits = [&](auto through) {
-    if (o->state_bits == 32)
-      with_device(std::integral_constant<int, 32>{}, through);
-    else
-      with_device(std::integral_constant<int, 8>{}, through);
+      launch(small, std::false_type{}, through);
   };
   if (bytes > kStreamBytes)
-    with_bits(std::true_type{});
+    with_device(std::false_type{}, std::true_type{});
+  else if (values > kSmallStep)
+    with_device(std::false_type{}, std::false_type{});
   else
-    with_bits(std::false_type{});
+    with_device(std::true_type{}, std::false_type{});
   return check_launch("adamw");
 }
 
@@ -571,8 +629,8 @@ int64_t sdm_rt_moments_bytes(int64_t n) { return n > 0 ? (n + kBlock - 1) / kBlo
 
 int sdm_rt_read_moments(const sdm_rt_tensor* tensors, int32_t count, void* stream) {
   g_err[0] = 0;
-  int64_t total, bytes = 0;
-  if (int rc = check_tensors(tensors, count, kStepChunk, &total)) return rc;
+  int64_t values, bytes = 0;
+  if (int rc = check_tensors(tensors, count, &values)) return rc;
   for (int32_t i = 0; i < count; ++i) {
     const sdm_rt_tensor& t = tensors[i];
     if (t.n == 0) continue;
@@ -581,14 +639,21 @@ int sdm_rt_read_moments(const sdm_rt_tensor* tensors, int32_t count, void* strea
     if (reinterpret_cast<uintptr_t>(t.exp_avg) % 8)
       return set_err(SDM_RT_EINVAL, "tensor %d: 8-bit moments must be 8-byte aligned", i);
   }
-  if (total == 0) return SDM_RT_OK;
+  if (values == 0) return SDM_RT_OK;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  for_tables(tensors, count, kStepChunk, [&](const StepTable<kStepTensors>& table, unsigned chunks, int64_t) {
-    if (bytes > kStreamBytes)
-      hipLaunchKernelGGL(read_moments_kernel<true>, dim3(chunks), dim3(kStepThreads), 0, st, table);
-    else
-      hipLaunchKernelGGL(read_moments_kernel<false>, dim3(chunks), dim3(kStepThreads), 0, st, table);
-  });
+  for_tables<ReadTable>(
+      tensors, count, kReadChunk,
+      [](const sdm_rt_tensor& t, char** at) {
+        at[0] = static_cast<char*>(t.exp_avg);
+        at[1] = static_cast<char*>(t.param);
+        at[2] = static_cast<char*>(t.exp_avg_sq);
+      },
+      [&](const ReadTable& table, unsigned chunks, int64_t) {
+        if (bytes > kStreamBytes)
+          hipLaunchKernelGGL(read_moments_kernel<true>, dim3(chunks), dim3(kStepThreads), 0, st, table);
+        else
+          hipLaunchKernelGGL(read_moments_kernel<false>, dim3(chunks), dim3(kStepThreads), 0, st, table);
+      });
   return check_launch("read_moments");
 }
 
