@@ -587,7 +587,7 @@ int sdm_rt_token_logprobs_grad(const sdm_rt_logprob* dims, const void* logits, i
                                void* d_logits, int64_t d_logits_row_stride, void* stream);
 
 /* A tensor of a training step: n values of dtype at each of param and grad, dense and in the same order, any alignment of an
- * element, n at most 2^33 and 2^34 in one call.  exp_avg, exp_avg_sq: float32 [n] each; or exp_avg the 8-bit moments of sdm_rt_moments_bytes(n) bytes, 8-byte
+ * element, at most 2^33 values in one call.  exp_avg, exp_avg_sq: float32 [n] each; or exp_avg the 8-bit moments of sdm_rt_moments_bytes(n) bytes, 8-byte
  * aligned, and exp_avg_sq NULL.  All fields are 64 bits wide. */
 typedef struct {
   void* param;

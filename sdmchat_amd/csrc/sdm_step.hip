@@ -120,7 +120,7 @@ __device__ __forceinline__ double wave_add(double v) {
 // Eight pieces of a thread under way at once: one at a time left it waiting (220 MB of bfloat16 72 us).
 template <typename T>
 __device__ __forceinline__ double sum_squares(const T* g, int n) {
-  constexpr int kN = 16 / static_cast<int>(sizeof(T)), kAtOnce = 8;
+  constexpr int kN = 16 / static_cast<int>(sizeof(T)), kAtOnce = 4;
   double s = 0.0;
   for (int i = threadIdx.x * kN; i < n; i += kAtOnce * kStepThreads * kN) {
     float v[kAtOnce][kN];
@@ -268,14 +268,14 @@ __device__ __forceinline__ void step_value(const StepArgs& a, float clip, float 
 using StepTable32 = StepTable<4, 96>;
 using StepTable8 = StepTable<3, 108, true>;
 
-// All of a thread's pieces of a chunk are loaded before the first is computed on.
+// All of a thread's pieces of a chunk are loaded before the first is computed on: 16 bytes of parameters and gradients each.
 template <int CHUNK, bool THROUGH, typename T>
 __device__ __forceinline__ void step_chunk32(const StepArgs& a, float clip, T* p, const T* g, float* m, float* v, int n) {
-  constexpr int kPieces = CHUNK / (kStepThreads * 4);
-  float pv[kPieces][4], gv[kPieces][4], mv[kPieces][4], vv[kPieces][4];
+  constexpr int kN = 4, kPieces = CHUNK / (kStepThreads * kN);
+  float pv[kPieces][kN], gv[kPieces][kN], mv[kPieces][kN], vv[kPieces][kN];
 #pragma unroll
   for (int q = 0; q < kPieces; ++q) {
-    const int i = (q * kStepThreads + threadIdx.x) * 4;
+    const int i = (q * kStepThreads + threadIdx.x) * kN;
     if (i >= n) break;
     load_values<THROUGH>(p + i, n - i, pv[q]);
     load_values<THROUGH>(g + i, n - i, gv[q]);
@@ -284,10 +284,10 @@ __device__ __forceinline__ void step_chunk32(const StepArgs& a, float clip, T* p
   }
 #pragma unroll
   for (int q = 0; q < kPieces; ++q) {
-    const int i = (q * kStepThreads + threadIdx.x) * 4;
+    const int i = (q * kStepThreads + threadIdx.x) * kN;
     if (i >= n) break;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
+    for (int e = 0; e < kN; ++e) {
       mv[q][e] *= a.b1;
       vv[q][e] *= a.b2;
       step_value(a, clip, gv[q][e], pv[q][e], mv[q][e], vv[q][e]);
@@ -299,7 +299,8 @@ __device__ __forceinline__ void step_chunk32(const StepArgs& a, float clip, T* p
 }
 
 // Sixteen lanes hold a block, 8 values each: its maxima come from four DPP steps.  Past a tensor's end p, g and the codes are 0
-// and stay so.  What bounds it is instructions as much as memory (110 M bfloat16 values: 240 us at 72 a value).
+// and stay so.  The codes do not stream past the caches: their lines are shared by neighbouring lanes' pieces (14 M values 43.5 us,
+// 48.9 if they do).  Bound by memory and instructions alike: 110 M bfloat16 values 217 us, 5.1 TB/s, 52 instructions a value.
 template <bool THROUGH, typename T>
 __device__ __forceinline__ void step_chunk8(const StepArgs& a, float clip, T* p, const T* g, char* chunk, uint32_t position, int n) {
   const int whole = (n + kBlock - 1) / kBlock * kBlock;
@@ -307,8 +308,8 @@ __device__ __forceinline__ void step_chunk8(const StepArgs& a, float clip, T* p,
     char* state = chunk + i / kBlock * kBlockBytes;
     const int at = i % kBlock;
     uint32_t cm[2], cv[2];
-    load_bytes<THROUGH, 8>(state + at, cm);
-    load_bytes<THROUGH, 8>(state + kBlock + at, cv);
+    load_bytes<false, 8>(state + at, cm);
+    load_bytes<false, 8>(state + kBlock + at, cv);
     const uint32_t e = *reinterpret_cast<const uint16_t*>(state + 2 * kBlock);
     float pv[8], gv[8], mv[8], vv[8];
     load_values<THROUGH>(p + i, n - i, pv);
@@ -344,8 +345,8 @@ __device__ __forceinline__ void step_chunk8(const StepArgs& a, float clip, T* p,
       cm[w] = upper_bytes(nm[4 * w], nm[4 * w + 1], nm[4 * w + 2], nm[4 * w + 3]);
       cv[w] = upper_bytes(nv[4 * w], nv[4 * w + 1], nv[4 * w + 2], nv[4 * w + 3]);
     }
-    store_bytes<THROUGH, 8>(state + at, cm);
-    store_bytes<THROUGH, 8>(state + kBlock + at, cv);
+    store_bytes<false, 8>(state + at, cm);
+    store_bytes<false, 8>(state + kBlock + at, cv);
     if (at == 0) *reinterpret_cast<uint16_t*>(state + 2 * kBlock) = static_cast<uint16_t>(em | ev << 8);
   }
 }
@@ -400,8 +401,8 @@ __device__ __forceinline__ void read_chunk(T* m, T* v, const char* chunk, int n)
   for (int i = threadIdx.x * 8; i < n; i += kStepThreads * 8) {
     const char* state = chunk + i / kBlock * kBlockBytes;
     uint32_t cm[2], cv[2];
-    load_bytes<THROUGH, 8>(state + i % kBlock, cm);
-    load_bytes<THROUGH, 8>(state + kBlock + i % kBlock, cv);
+    load_bytes<false, 8>(state + i % kBlock, cm);
+    load_bytes<false, 8>(state + kBlock + i % kBlock, cv);
     const uint32_t e = *reinterpret_cast<const uint16_t*>(state + 2 * kBlock);
     const float scale = block_scale(e & 255), nan = e >> 8 == 255 ? NAN : 1.f;
     const int shift = v_shift(e >> 8);
@@ -435,7 +436,7 @@ static_assert(sizeof(StepTable32) + sizeof(StepArgs) + 16 <= 4096 && sizeof(Step
 
 inline int64_t chunks_of(int64_t n, int chunk) { return (n + chunk - 1) / chunk; }
 
-// Every check that needs no device; values: the sum of the n.  Chunks are at least 1,024 values: fewer than 2^24 in a launch.
+// Every check that needs no device; values: the sum of the n.  Chunks are at least 1,024 values: not much over 2^23 in a launch.
 inline int check_tensors(const sdm_rt_tensor* t, int32_t count, int64_t* values) {
   if (count < 0 || (count > 0 && !t)) return set_err(SDM_RT_EINVAL, "count must be >= 0, tensors not NULL");
   *values = 0;
@@ -443,9 +444,9 @@ inline int check_tensors(const sdm_rt_tensor* t, int32_t count, int64_t* values)
     if (t[i].n < 0) return set_err(SDM_RT_EINVAL, "tensor %d: n must be >= 0", i);
     if (t[i].dtype != SDM_RT_F32 && t[i].dtype != SDM_RT_BF16)
       return set_err(SDM_RT_EINVAL, "tensor %d: unknown dtype %lld", i, (long long)t[i].dtype);
-    if (t[i].n > (int64_t{1} << 33)) return set_err(SDM_RT_EUNSUPPORTED, "tensor %d: n must be at most 2^33", i);
+    if (t[i].n > (int64_t{1} << 33)) return set_err(SDM_RT_EUNSUPPORTED, "tensor %d: n must be at most 2^33", i);   // before the sum
     *values += t[i].n;
-    if (*values > (int64_t{1} << 34)) return set_err(SDM_RT_EUNSUPPORTED, "more than 2^34 values in one call");
+    if (*values > (int64_t{1} << 33)) return set_err(SDM_RT_EUNSUPPORTED, "more than 2^33 values in one call");
   }
   return SDM_RT_OK;
 }
@@ -482,7 +483,7 @@ void for_tables(const sdm_rt_tensor* t, int32_t count, int chunk, TAKE take, LAU
 }
 
 // Few values take small chunks, so that all compute units have some.
-constexpr int64_t kSmallStep = 8 << 20, kSmallNorm = 8 << 20;
+constexpr int64_t kSmallStep = 16 << 20, kSmallNorm = 8 << 20;
 
 inline int norm_chunk(int64_t values) { return values <= kSmallNorm ? 4096 : 16384; }
 inline int64_t norm_partials(const sdm_rt_tensor* t, int32_t count, int64_t values) {
@@ -584,7 +585,7 @@ int sdm_rt_adamw(const sdm_rt_adamw_options* o, const sdm_rt_tensor* tensors, in
   auto launch = [&](auto small, auto device, auto through) {
     constexpr bool kSmall = decltype(small)::value, kDevice = decltype(device)::value, kThrough = decltype(through)::value;
     if (o->state_bits == 32) {
-      constexpr int kChunk = kSmall ? 1024 : 4096;
+      constexpr int kChunk = 1024;   // 110 M float32 values 476 us, 466 with 2,048, 480 with 4,096; 285 M bfloat16 1,040, 1,075, 1,167
       for_tables<StepTable32>(
           tensors, count, kChunk,
           [](const sdm_rt_tensor& t, char** at) {
@@ -597,7 +598,7 @@ int sdm_rt_adamw(const sdm_rt_adamw_options* o, const sdm_rt_tensor* tensors, in
             hipLaunchKernelGGL((adamw32_kernel<kChunk, kDevice, kThrough>), dim3(chunks), dim3(kStepThreads), 0, st, table, a);
           });
     } else {
-      constexpr int kChunk = kSmall ? 2048 : 4096;
+      constexpr int kChunk = kSmall ? 2048 : 4096;   // 14 M values 46.7 us with 2,048, 48.9 with 4,096; 110 M 236 and 220
       for_tables<StepTable8>(
           tensors, count, kChunk,
           [](const sdm_rt_tensor& t, char** at) {

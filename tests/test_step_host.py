@@ -89,7 +89,7 @@ GOOD = (P, P, P, P, 100, 0)
     (dict(), (0, P, P, P, 100, 0), -1, "NULL"), (dict(), (P, 0, P, P, 100, 0), -1, "NULL"), (dict(), (P, P, 0, P, 100, 0), -1, "NULL"),
     (dict(), (P, P, P, 0, 100, 0), -1, "NULL"), (dict(state_bits=8), GOOD, -1, "NULL for 8 bits"),
     (dict(state_bits=8), (P, P, P + 4, 0, 100, 0), -1, "8-byte"), (dict(), (P, P, P, P, -1, 0), -1, "n must"),
-    (dict(), (P, P, P, P, 100, 2), -1, "dtype"), (dict(), (P, P, P, P, (1 << 33) + 1, 0), -3, "2^33")])
+    (dict(), (P, P, P, P, 100, 2), -1, "dtype"), (dict(), (P, P, P, P, (1 << 33) + 1, 0), -3, "2^33"), (dict(), (P, P, P, P, 1 << 33, 0), -3, "more than")])
 def test_adamw_checks(over, row, code, text):
     lib = _lib.load()
     o = _options(**over)
