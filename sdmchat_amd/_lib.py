@@ -4,6 +4,7 @@ The library is loaded from ``sdmchat_amd/lib/libsdm_rt.so`` (built by ``python -
 fallback: if the library is missing or a symbol is absent, loading raises.
 """
 import ctypes
+import importlib.util
 import os
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "lib", "libsdm_rt.so")
@@ -102,9 +103,6 @@ class SdmRtLogprob(ctypes.Structure):
         ("temperature", ctypes.c_float),
         ("ignore_index", c_i64),
     ]
-
-
-TENSOR_FIELDS = 6   # sdm_rt_tensor: param, grad, exp_avg, exp_avg_sq, n, dtype, 64 bits each
 
 
 class SdmRtAdamwOptions(ctypes.Structure):
@@ -290,6 +288,23 @@ def load(path=None):
     if path is None:
         _LIB = lib
     return lib
+
+
+_LISTS = None
+
+
+def lists():
+    """Load (once) and return the extension that packs lists of tensors (csrc/lists.cpp)."""
+    global _LISTS
+    if _LISTS is None:
+        path = os.path.join(os.path.dirname(LIB_PATH), "_lists.so")
+        if not os.path.exists(path):
+            raise RuntimeError(f"run-time SDM HIP library not built: {path} is missing (python -m sdmchat_amd.build)")
+        spec = importlib.util.spec_from_file_location("_lists", path)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        _LISTS = module
+    return _LISTS
 
 
 class SdmRtError(RuntimeError):

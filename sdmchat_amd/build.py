@@ -4,13 +4,15 @@
 
 compiles every ``sdmchat_amd/csrc/*.hip`` translation unit with ``hipcc`` (in parallel) and links
 ``sdmchat_amd/lib/libsdm_rt.so``.  The library is loaded by ``sdmchat_amd._lib`` through ctypes; it exports the C ABI
-declared in ``include/sdm_rt.h``.  ``build(incremental=True)`` recompiles only the units whose source, or a header
-they may include, is newer than their object file.
+declared in ``include/sdm_rt.h``.  Beside it ``csrc/lists.cpp``, a small Python extension on torch's headers (host code
+only), becomes ``sdmchat_amd/lib/_lists.so``.  ``build(incremental=True)`` recompiles only the units whose source, or a
+header they may include, is newer than their object file.
 """
 import glob
 import os
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 
 PKG = os.path.dirname(os.path.abspath(__file__))
@@ -20,6 +22,7 @@ INCLUDE = os.path.join(ROOT, "include")
 LIB_DIR = os.path.join(PKG, "lib")
 OBJ_DIR = os.path.join(LIB_DIR, "obj")
 LIB = os.path.join(LIB_DIR, "libsdm_rt.so")
+LISTS = os.path.join(LIB_DIR, "_lists.so")
 ARCH = "gfx950"
 
 # -packed-fp32-ops keeps the compiler from forming packed FP32 VALU instructions.
@@ -52,6 +55,24 @@ def _compile(src, extra_flags, verbose):
     return src, None
 
 
+def _compile_lists(verbose):
+    import torch
+    from torch.utils.cpp_extension import include_paths
+    libs = os.path.join(os.path.dirname(torch.__file__), "lib")
+    dirs = [INCLUDE, sysconfig.get_paths()["include"], *include_paths()]
+    src = os.path.join(CSRC, "lists.cpp")
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *[a for d in dirs for a in ("-I", d)], src,
+           "-o", LISTS + ".tmp", "-L" + libs, "-ltorch_python", "-ltorch_cpu", "-lc10"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        return src, res.stdout + res.stderr
+    os.replace(LISTS + ".tmp", LISTS)
+    return src, None
+
+
 def build(verbose=False, extra_flags=(), incremental=False, jobs=None):
     """Compile the library and return its path (every unit, unless ``incremental``)."""
     os.makedirs(OBJ_DIR, exist_ok=True)
@@ -64,9 +85,14 @@ def build(verbose=False, extra_flags=(), incremental=False, jobs=None):
         if (not incremental or not os.path.exists(obj)
                 or os.path.getmtime(obj) < max(os.path.getmtime(src), newest_header)):
             todo.append(src)
-    jobs = jobs or min(len(todo) or 1, int(os.environ.get("MAX_JOBS", os.cpu_count() or 4)))
+    newest = max(newest_header, os.path.getmtime(os.path.join(CSRC, "lists.cpp")))
+    lists = not incremental or not os.path.exists(LISTS) or os.path.getmtime(LISTS) < newest
+    jobs = jobs or min(len(todo) + lists or 1, int(os.environ.get("MAX_JOBS", os.cpu_count() or 4)))
     with ThreadPoolExecutor(max_workers=jobs) as ex:
+        ext = ex.submit(_compile_lists, verbose) if lists else None
         failed = [(s, err) for s, err in ex.map(lambda s: _compile(s, extra_flags, verbose), todo) if err]
+        if ext and ext.result()[1]:
+            failed.append(ext.result())
     for s, err in failed:
         sys.stderr.write(f"--- {os.path.basename(s)}\n{err}")
     if failed:

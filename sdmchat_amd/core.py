@@ -7,7 +7,6 @@ stream; nothing synchronises.
 import array
 import ctypes
 import math
-import operator
 import typing
 
 import torch
@@ -1865,104 +1864,105 @@ def _dense(t):
     return True
 
 
-_T = torch.Tensor
-_dtype_of, _shape_of = operator.attrgetter("dtype"), operator.attrgetter("shape")
-
-
 def _lists(name, **lists):
     """Lists of equal length, not empty, on one GPU: (lists, its index)."""
-    out = [v if type(v) is list else list(v) for v in lists.values()]
+    out = list(lists.values())
     first = out[0]
     if not first:
         raise ValueError(f"{name}: no tensors")
     index = first[0].get_device()
     if index < 0:
         raise RuntimeError(f"{name} needs ROCm device tensors")
-    for what, ts in zip(lists, out):
+    for what, ts in lists.items():
         if len(ts) != len(first):
             raise ValueError(f"{name}: {len(ts)} {what} for {len(first)} {next(iter(lists))}")
-        if set(map(_T.get_device, ts)) != {index}:
-            other = next(t for t in ts if t.get_device() != index)
-            raise ValueError(f"{name}: one of the {what} is on {other.device}, expected {first[0].device}")
+        for t in ts:
+            if t.get_device() != index:
+                raise ValueError(f"{name}: one of the {what} is on {t.device}, expected {first[0].device}")
+            if t.layout is not torch.strided:
+                raise ValueError(f"{name}: one of the {what} has layout {t.layout}")
     return out, index
 
 
-def _contiguous(ts):
-    """Whether all are strided and contiguous (a tensor of another layout cannot be asked)."""
-    try:
-        return all(map(_T.is_contiguous, ts))
-    except RuntimeError:
-        return False
+def _code(name, what, t):
+    """The library's code of a tensor's dtype."""
+    code = _DT.get(t.dtype)
+    if code is None:
+        raise ValueError(f"{name}: one of the {what} has dtype {t.dtype}, not float32 or bfloat16")
+    return code
 
 
-def _codes(name, what, ts):
-    """The library's codes of the tensors' dtypes."""
-    try:
-        return [_DT[d] for d in map(_dtype_of, ts)]
-    except KeyError as e:
-        raise ValueError(f"{name}: one of the {what} has dtype {e.args[0]}, not float32 or bfloat16") from None
+def _table(rows):
+    """sdm_rt_tensor rows (param, grad, exp_avg, exp_avg_sq, n, dtype) as the library takes them."""
+    return array.array("q", [v for r in rows for v in r]).tobytes()
 
 
-def _table(n, *columns):
-    """The sdm_rt_tensor array of n tensors from its columns: param, grad, exp_avg, exp_avg_sq, n, dtype."""
-    rows = [0] * (_lib.TENSOR_FIELDS * n)
-    for i, c in enumerate(columns):
-        if c is not None:
-            rows[i::_lib.TENSOR_FIELDS] = c if type(c) is list else list(c)
-    return array.array("q", rows)
-
-
-def _written(tensors):
-    """Tensors that a kernel has written in place: a graph that saved one must not read it again, and what is derived from one
-    is derived anew."""
-    try:
-        torch.autograd.graph.increment_version(tensors)
-    except RuntimeError:   # inference tensors count no versions
-        torch.autograd.graph.increment_version([t for t in tensors if not t.is_inference()])
+def _check_apart(name, spans):
+    """(begin, bytes, written) of tensors: none that is written overlaps another."""
+    end_of_any = end_of_written = 0
+    for begin, size, written in sorted(spans):
+        if size and begin < (end_of_any if written else end_of_written):
+            raise ValueError(f"{name}: two of the tensors overlap, and one of them is written")
+        end_of_any = max(end_of_any, begin + size)
+        if written:
+            end_of_written = max(end_of_written, begin + size)
 
 
 def grad_norm(tensors):
     """The norm of all of these tensors' values together, sqrt(sum of squares): a float32 scalar on their GPU.  float32 or
     bfloat16 tensors, mixed; the squares are summed in float64 in a fixed order (deterministic)."""
-    (ts,), index = _lists("grad_norm", tensors=tensors)
-    codes = _codes("grad_norm", "tensors", ts)
-    if not _contiguous(ts):
-        other = {t.layout for t in ts} - {torch.strided}
-        if other:
-            raise ValueError(f"grad_norm: a tensor of layout {other.pop()}")
-        ts = [t if _dense(t) else t.contiguous() for t in ts]
-    n = len(ts)
-    table = _table(n, None, map(_T.data_ptr, ts), None, None, map(_T.numel, ts), codes)
-    at, lib = table.buffer_info()[0], _lib.load()
+    ts = tensors if type(tensors) is list else list(tensors)
+    packed = _lib.lists().pack(None, ts, None, None, False, False)
+    if packed is None:
+        (ts,), index = _lists("grad_norm", tensors=ts)
+        ts = [t if _dense(t) else t.contiguous() for t in ts]   # which the call below outlives
+        packed = _table([(0, t.data_ptr(), 0, 0, t.numel(), _code("grad_norm", "tensors", t)) for t in ts]), index
+    table, index = packed
+    n, lib = len(ts), _lib.load()
     out = ts[0].new_empty((), dtype=torch.float32)
-    nbytes = lib.sdm_rt_grad_norm_workspace_bytes(at, n)   # 0 outside the limits: the call below reports why
+    nbytes = lib.sdm_rt_grad_norm_workspace_bytes(table, n)   # 0 outside the limits: the call below reports why
     ws = out.new_empty(nbytes // 8, dtype=torch.float64)
-    _launch(lib.sdm_rt_grad_norm, index, at, n, out.data_ptr(), ws.data_ptr(), nbytes)
+    _launch(lib.sdm_rt_grad_norm, index, table, n, out.data_ptr(), ws.data_ptr(), nbytes)
     return out
 
 
-def _ordered_grads(name, ps, gs):
-    """The grads in the order of their params' values in memory: a grad of other strides is copied."""
-    out = []
-    for p, g in zip(ps, gs):
+def _check_moments8(name, m, n):
+    """8-bit moments (new_moments) of n values."""
+    want = (-(-n // MOMENT_BLOCK), MOMENT_BYTES)
+    if m.dtype != torch.uint8 or tuple(m.shape) != want or not m.is_contiguous():
+        raise ValueError(f"{name}: 8-bit moments must be contiguous uint8 {want} for {n} values, got {m.dtype} {tuple(m.shape)}")
+
+
+def _pack_step(name, ps, gs, ms, vs):
+    """adamw's lists, not all of them plain: (table, GPU, grads that the table points to), or what is wrong with them."""
+    lists = dict(params=ps, grads=gs, exp_avgs=ms)
+    if vs is not None:
+        lists["exp_avg_sqs"] = vs
+    index = _lists(name, **lists)[1]
+    rows, spans, held = [], [], []
+    for i, (p, g) in enumerate(zip(ps, gs)):
+        if g.dtype != p.dtype or g.shape != p.shape:
+            raise ValueError(f"{name}: a grad of {g.dtype} {tuple(g.shape)} for a param of {p.dtype} {tuple(p.shape)}")
         if not _dense(p):
             raise ValueError(f"{name}: a param {tuple(p.shape)} of strides {tuple(p.stride())}: its values must be dense")
-        if g.layout is not torch.strided:
-            raise ValueError(f"{name}: a grad of layout {g.layout}")
-        out.append(g if g.stride() == p.stride() or (p.is_contiguous() and g.is_contiguous()) else torch.empty_like(p).copy_(g))
-    return out
-
-
-def _check_moments8(name, what, ms, sizes):
-    """8-bit moments (new_moments) for these numbers of values."""
-    if {m.dtype for m in ms} == {torch.uint8} and _contiguous(ms) and list(map(_shape_of, ms)) == [
-            (-(-n // MOMENT_BLOCK), MOMENT_BYTES) for n in sizes]:
-        return
-    for m, n in zip(ms, sizes):
-        want = (-(-n // MOMENT_BLOCK), MOMENT_BYTES)
-        if m.dtype != torch.uint8 or tuple(m.shape) != want or not m.is_contiguous():
-            raise ValueError(f"{name}: 8-bit moments must be contiguous uint8 {want} for {n} values, got {m.dtype} "
-                             f"{tuple(m.shape)}")
+        if not (p.is_contiguous() and g.is_contiguous()) and g.stride() != p.stride():
+            g = torch.empty_like(p).copy_(g)   # the grad in the order of the param's values
+        held.append(g)
+        if vs is None:
+            _check_moments8(name, ms[i], p.numel())
+            moments = [ms[i]]
+        else:
+            moments = [ms[i], vs[i]]
+            for t in moments:
+                if t.dtype != torch.float32 or t.shape != p.shape or not (
+                        t.stride() == p.stride() or (t.is_contiguous() and p.is_contiguous())):
+                    raise ValueError(f"{name}: moments must be float32 {tuple(p.shape)} of the param's strides "
+                                     f"{tuple(p.stride())}, got {t.dtype} {tuple(t.shape)} of {tuple(t.stride())}")
+        at = [t.data_ptr() for t in moments] + [0]
+        rows.append((p.data_ptr(), g.data_ptr(), at[0], at[1], p.numel(), _code(name, "params", p)))
+        spans += [(t.data_ptr(), t.numel() * t.element_size(), t is not g) for t in (p, g, *moments)]
+    _check_apart(name, spans)
+    return _table(rows), index, held
 
 
 def adamw(params, grads, exp_avgs, exp_avg_sqs=None, *, step, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2,
@@ -1981,62 +1981,36 @@ def adamw(params, grads, exp_avgs, exp_avg_sqs=None, *, step, lr=1e-3, betas=(0.
     element too.  Returns the norm (float32 scalar on the GPU) with max_norm, else None."""
     name = "adamw"
     eight = exp_avg_sqs is None
-    if eight:
-        (ps, gs, ms), index = _lists(name, params=params, grads=grads, exp_avgs=exp_avgs)
+    ps, gs, ms, vs = (ts if type(ts) is list else ts if ts is None else list(ts) for ts in (params, grads, exp_avgs, exp_avg_sqs))
+    native = _lib.lists()
+    try:
+        packed = native.pack(ps, gs, ms, vs, eight, False)
+    except ValueError as e:
+        raise ValueError(f"{name}: {e}") from None
+    if packed is None:
+        table, index, gs = _pack_step(name, ps, gs, ms, vs)
     else:
-        (ps, gs, ms, vs), index = _lists(name, params=params, grads=grads, exp_avgs=exp_avgs, exp_avg_sqs=exp_avg_sqs)
-    count, dev = len(ps), ps[0].device
-    codes, shapes, sizes = _codes(name, "params", ps), list(map(_shape_of, ps)), list(map(_T.numel, ps))
-    if list(map(_dtype_of, gs)) != list(map(_dtype_of, ps)) or list(map(_shape_of, gs)) != shapes:
-        p, g = next((p, g) for p, g in zip(ps, gs) if g.dtype != p.dtype or g.shape != p.shape)
-        raise ValueError(f"{name}: a grad of {g.dtype} {tuple(g.shape)} for a param of {p.dtype} {tuple(p.shape)}")
-    plain = _contiguous(ps) and _contiguous(gs)
-    if not plain:
-        gs = _ordered_grads(name, ps, gs)
-    if eight:
-        _check_moments8(name, "exp_avgs", ms, sizes)
-    else:
-        for ts in (ms, vs):
-            if set(map(_dtype_of, ts)) != {torch.float32} or list(map(_shape_of, ts)) != shapes or not (
-                    plain and _contiguous(ts)):
-                for p, t in zip(ps, ts):
-                    if t.dtype != torch.float32 or t.shape != p.shape or (t.stride() != p.stride() and not (
-                            t.is_contiguous() and p.is_contiguous())):
-                        raise ValueError(f"{name}: moments must be float32 {tuple(p.shape)} of the param's strides "
-                                         f"{tuple(p.stride())}, got {t.dtype} {tuple(t.shape)} of {tuple(t.stride())}")
-    at_p, at_g, at_m = (list(map(_T.data_ptr, ts)) for ts in (ps, gs, ms))
-    at_v = None if eight else list(map(_T.data_ptr, vs))
-    # an address of its own for everything that is written (0: a tensor without values)
-    written = at_p + at_m if eight else at_p + at_m + at_v
-    different = set(written)
-    if len(different) + written.count(0) - (0 in different) != len(written) or not different.isdisjoint(filter(None, at_g)):
-        raise ValueError(f"{name}: a tensor occurs twice")
+        table, index = packed
     t_dev, lr_dev = None, None
-    if torch.is_tensor(step):
-        if step.dtype != torch.int64 or step.numel() != 1 or step.device != dev:
-            raise ValueError(f"{name}: a step on the device must be int64 with one element on {dev}")
+    if type(step) is not int and torch.is_tensor(step):
+        if step.dtype != torch.int64 or step.numel() != 1 or step.get_device() != index:
+            raise ValueError(f"{name}: a step on the device must be int64 with one element on {ps[0].device}")
         t_dev, step = step, 0
-    if torch.is_tensor(lr):
-        if lr.dtype != torch.float32 or lr.numel() != 1 or lr.device != dev or t_dev is None:
-            raise ValueError(f"{name}: an lr on the device must be float32 with one element on {dev}, beside a step there")
+    if type(lr) is not float and torch.is_tensor(lr):
+        if lr.dtype != torch.float32 or lr.numel() != 1 or lr.get_device() != index or t_dev is None:
+            raise ValueError(f"{name}: an lr on the device must be float32 with one element on {ps[0].device}, beside a step there")
         lr_dev, lr = lr, 0.0
     if max_norm is None:
         if norm is not None:
             raise ValueError(f"{name}: norm needs max_norm")
     elif norm is None:
         norm = grad_norm(gs)
-    elif norm.dtype != torch.float32 or norm.numel() != 1 or norm.device != dev:
-        raise ValueError(f"{name}: norm must be float32 with one element on {dev}")
+    elif norm.dtype != torch.float32 or norm.numel() != 1 or norm.get_device() != index:
+        raise ValueError(f"{name}: norm must be float32 with one element on {ps[0].device}")
     options = _lib.SdmRtAdamwOptions(lr, betas[0], betas[1], eps, weight_decay, step, _ptr(t_dev), _ptr(lr_dev), _ptr(norm),
                                      1.0 if max_norm is None else max_norm, 8 if eight else 32, seed & 0xffffffff)
-    table = _table(count, at_p, at_g, at_m, at_v, sizes, codes)
-    _launch(_lib.load().sdm_rt_adamw, index, ctypes.byref(options), table.buffer_info()[0], count)
-    _written(ps)
-    _written(ms)
-    if not eight:
-        _written(vs)
-    if t_dev is not None:
-        _written([t_dev])
+    _launch(_lib.load().sdm_rt_adamw, index, ctypes.byref(options), table, len(ps))
+    native.written(ps, ms, vs or [], [] if t_dev is None else [t_dev])
     return norm
 
 
@@ -2044,13 +2018,23 @@ def read_moments(moments, exp_avgs, exp_avg_sqs):
     """Writes the values that 8-bit moments (new_moments) stand for into exp_avgs and exp_avg_sqs: tensors of the params'
     sizes, contiguous, bfloat16 (which holds them exactly) or float32."""
     name = "read_moments"
-    (ss, ms, vs), index = _lists(name, moments=moments, exp_avgs=exp_avgs, exp_avg_sqs=exp_avg_sqs)
-    sizes, codes = list(map(_T.numel, ms)), _codes(name, "exp_avgs", ms)
-    if list(map(_T.numel, vs)) != sizes or list(map(_dtype_of, vs)) != list(map(_dtype_of, ms)) or not _contiguous(ms) or (
-            not _contiguous(vs)):
-        raise ValueError(f"{name}: exp_avgs and exp_avg_sqs must be contiguous and alike in size and dtype")
-    _check_moments8(name, "moments", ss, sizes)
-    table = _table(len(ss), map(_T.data_ptr, ms), None, map(_T.data_ptr, ss), map(_T.data_ptr, vs), sizes, codes)
-    _launch(_lib.load().sdm_rt_read_moments, index, table.buffer_info()[0], len(ss))
-    _written(ms)
-    _written(vs)
+    ss, ms, vs = (ts if type(ts) is list else list(ts) for ts in (moments, exp_avgs, exp_avg_sqs))
+    native = _lib.lists()
+    try:
+        packed = native.pack(ms, None, ss, vs, True, True)
+    except ValueError as e:
+        raise ValueError(f"{name}: {e}") from None
+    if packed is None:
+        index = _lists(name, moments=ss, exp_avgs=ms, exp_avg_sqs=vs)[1]
+        rows, spans = [], []
+        for s, m, v in zip(ss, ms, vs):
+            if v.numel() != m.numel() or v.dtype != m.dtype or not m.is_contiguous() or not v.is_contiguous():
+                raise ValueError(f"{name}: exp_avgs and exp_avg_sqs must be contiguous and alike in size and dtype")
+            _check_moments8(name, s, m.numel())
+            rows.append((m.data_ptr(), 0, s.data_ptr(), v.data_ptr(), m.numel(), _code(name, "exp_avgs", m)))
+            spans += [(t.data_ptr(), t.numel() * t.element_size(), t is not s) for t in (s, m, v)]
+        _check_apart(name, spans)
+        packed = _table(rows), index
+    table, index = packed
+    _launch(_lib.load().sdm_rt_read_moments, index, table, len(ss))
+    native.written(ms, vs)

@@ -535,9 +535,9 @@ def test_refusals_on_the_gpu():
             (lambda: core.adamw([p], [g], [m[:299]], [v], step=1), "moments must be float32"),
             (lambda: core.adamw([p], [g], [m], step=1), "8-bit moments"),
             (lambda: core.adamw([p], [g], [s[:2]], step=1), "8-bit moments"),
-            (lambda: core.adamw([p, p], [g, g], [m, v], [m.clone(), v.clone()], step=1), "twice"),
-            (lambda: core.adamw([p], [g], [m], [m], step=1), "twice"),
-            (lambda: core.adamw([p], [p], [m], [v], step=1), "twice"),
+            (lambda: core.adamw([p, p], [g, g], [m, v], [m.clone(), v.clone()], step=1), "overlap"),
+            (lambda: core.adamw([p], [g], [m], [m], step=1), "overlap"),
+            (lambda: core.adamw([p], [p], [m], [v], step=1), "overlap"),
             (lambda: core.adamw([p], [g.cpu()], [m], [v], step=1), "is on cpu"),
             (lambda: core.adamw([p], [g.to_sparse()], [m], [v], step=1), "layout"),
             (lambda: core.adamw([p], [g], [m], [v], step=0), "t must be"),
