@@ -93,18 +93,20 @@ struct RowLds {
   uint16_t hot[1024];   // threads with a logit at or above the threshold
 };
 
-// The key t for which k to 5/4 k of the threads' maxima have key >= t (k or more, where ties forbid that), by one wave that
-// halves the range of keys: those maxima are k logits of the row, so all alternatives have keys >= t.  The key of the least
-// finite number if fewer than k maxima are finite.
-template <int PER>
+// The key t for which k to 5/4 k of the threads' maxima (over 512 threads: of those of pairs of threads) have key >= t, or more
+// where ties forbid that, by one wave that halves the range of keys: those maxima are k logits of the row, so all alternatives
+// have keys >= t.  The key of the least finite number if fewer than k maxima are finite.
 __device__ __forceinline__ uint32_t near_kth(const float* top, int threads, int k, float largest) {
+  constexpr int PER = 8;
   const int lane = threadIdx.x & 63;
   uint32_t v[PER];
   float least = INFINITY;
   int n = 0;
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
-    const float x = i * 64 + lane < threads ? top[i * 64 + lane] : -INFINITY;
+    const int at = i * 64 + lane;
+    float x = at < threads ? top[at] : -INFINITY;
+    if (threads > 512) x = fmaxf(x, at + 512 < threads ? top[at + 512] : -INFINITY);
     v[i] = ordered(x);
     const bool there = v[i] != 0;
     least = fminf(least, there ? x : INFINITY);
@@ -227,8 +229,9 @@ __device__ __noinline__ int crowded(int k, const T* z, int n, int first, uint32_
 }
 
 template <typename T, int NV, bool TOP, bool ENT>
-__global__ void __launch_bounds__(1024, 8) logprob_kernel(LogprobArgs a, int slices, int pieces_per_slice, Partial part) {
+__global__ void __launch_bounds__(1024, 8) logprob_kernel(LogprobArgs a, int slices, int pieces_per_slice, Partial part, int slots) {
   constexpr int kN = Piece<T>::kN;
+  extern __shared__ uint4 hot_pieces[];   // TOP: [slots][NV]
   __shared__ typename std::conditional<TOP, RowLds, float[4][16]>::type lds_;
   float(*red)[16];
   if constexpr (TOP)
@@ -314,8 +317,8 @@ __global__ void __launch_bounds__(1024, 8) logprob_kernel(LogprobArgs a, int sli
   if constexpr (ENT) u = wave_add(u);
   if (lane == 0) red[1][wave] = count, red[2][wave] = rest, red[3][wave] = u;
   if constexpr (TOP) {
-    if (wave == 0) {   // its pieces' registers are free by now
-      const uint32_t t = threads <= 512 ? near_kth<8>(lds_.top, threads, a.k, m) : near_kth<16>(lds_.top, threads, a.k, m);
+    if (wave == 0) {
+      const uint32_t t = near_kth(lds_.top, threads, a.k, m);
       if (lane == 0) lds_.threshold = t;
     }
   }
@@ -335,8 +338,9 @@ __global__ void __launch_bounds__(1024, 8) logprob_kernel(LogprobArgs a, int sli
     }
   }
   if constexpr (TOP) {
-    // The threads with a logit at or above the threshold are few (k to 5/4 k of them): their pieces are dealt out to all threads,
-    // which read them again from the caches, and the logits found are listed in any order.
+    // The threads with a logit at or above the threshold are few (k to 5/4 k of them, or somewhat more): they put their pieces
+    // down in LDS, and all threads look through those.  The logits found are listed in any order.  (Read again from memory they
+    // cost a line for every 16 bytes: 2,048 x 151,936 with 64 alternatives 156 us.)
     const uint32_t threshold = lds_.threshold;
     const float from = unordered(threshold);
     const uint64_t hot = __ballot(mine >= from);
@@ -344,32 +348,34 @@ __global__ void __launch_bounds__(1024, 8) logprob_kernel(LogprobArgs a, int sli
       int at = 0;
       if (lane == 0) at = atomicAdd(&lds_.n_hot, __popcll(hot));
       at = __builtin_amdgcn_readfirstlane(at) + __popcll(hot & ((uint64_t{1} << lane) - 1));
-      if (hot >> lane & 1) lds_.hot[at] = static_cast<uint16_t>(threadIdx.x);
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < lds_.n_hot * NV; i += threads) {
-      const int at = ((i % NV) * threads + lds_.hot[i / NV]) * kN;
-      Piece<T> q;
-      if (at + kN <= n)
-        q.load(z + at);
-      else if (at < n)
-        q.load_part(z + at, n - at, from_f32<T>(-INFINITY));
-      else
-        continue;
-      RunningMax<T> most;
-      most.add(q);
-      if (!(most.get() >= from)) continue;
+      if ((hot >> lane & 1) && at < slots) {
+        lds_.hot[at] = static_cast<uint16_t>(threadIdx.x);
 #pragma unroll
-      for (int e = 0; e < kN; ++e) {
-        const float x = q.get(e);
-        if (x >= from) {
-          const int to = atomicAdd(&lds_.n, 1);
-          if (to < kCandidates) lds_.keys[to] = logit_key(x, first * kN + at + e);
-        }
+        for (int v = 0; v < NV; ++v) hot_pieces[at * NV + v] = p[v].r;
       }
     }
     __syncthreads();
-    int found = lds_.n;
+    const int n_hot = lds_.n_hot;
+    if (n_hot <= slots) {
+      for (int i = threadIdx.x; i < n_hot * NV; i += threads) {
+        Piece<T> q;
+        q.r = hot_pieces[i];
+        RunningMax<T> most;
+        most.add(q);
+        if (!(most.get() >= from)) continue;
+        const int at = first * kN + ((i % NV) * threads + lds_.hot[i / NV]) * kN;
+#pragma unroll
+        for (int e = 0; e < kN; ++e) {
+          const float x = q.get(e);
+          if (x >= from) {
+            const int to = atomicAdd(&lds_.n, 1);
+            if (to < kCandidates) lds_.keys[to] = logit_key(x, at + e);
+          }
+        }
+      }
+      __syncthreads();
+    }
+    int found = n_hot <= slots ? lds_.n : kCandidates + 1;
     if (found > kCandidates) {
       found = crowded<T>(a.k, z, n, first * kN, threshold, ordered(m), lds_);
     }
@@ -585,9 +591,10 @@ inline size_t logprob_bytes(int64_t rows, int k, int slices) {
 template <typename T>
 void launch_logprob(const LogprobArgs& a, const RowShape& s, const Partial& part, hipStream_t st) {
   const dim3 grid(static_cast<unsigned>(a.rows * s.slices)), threads(s.threads);
+  const int slots = std::min(s.threads, a.k + a.k / 2 + 8);   // 50 KB at most
   auto launch = [&](auto nv, auto top, auto ent) {
-    hipLaunchKernelGGL((logprob_kernel<T, decltype(nv)::value, decltype(top)::value, decltype(ent)::value>), grid, threads, 0,
-                       st, a, s.slices, s.pieces, part);
+    hipLaunchKernelGGL((logprob_kernel<T, decltype(nv)::value, decltype(top)::value, decltype(ent)::value>), grid, threads,
+                       a.k ? static_cast<size_t>(slots) * decltype(nv)::value * 16 : 0, st, a, s.slices, s.pieces, part, slots);
   };
   auto with_nv = [&](auto top, auto ent) {
     if (s.nv == 2)
