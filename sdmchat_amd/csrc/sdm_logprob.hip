@@ -73,6 +73,7 @@ __device__ __forceinline__ void write_row(const LogprobArgs& a, int64_t r, const
 // -- a row, or a slice of one, by one workgroup -------------------------------------------------------------------------
 // The slice is in registers, NV 16-byte pieces a thread, so the row is read once: its maximum, its sums against that, and its
 // alternatives all come from there.
+constexpr int kMaxSlots = kMaxAlternatives + kMaxAlternatives / 2 + 8;
 constexpr int kCandidates = 1024;   // keys that are ranked against each other
 constexpr uint32_t kLowest = 0x00800000u;   // the key of the least finite number
 
@@ -113,17 +114,28 @@ __device__ __forceinline__ uint32_t near_kth(const float* top, int threads, int 
     n += __popcll(__ballot(there));
   }
   if (n < k) return kLowest;
-  uint32_t lo = ordered(-wave_max(-least)), hi = max(ordered(largest), lo);   // k or more from lo on, none past hi
-  while (lo < hi) {
-    const uint32_t mid = lo + (hi - lo + 1) / 2;
+  // k or more from lo on, fewer past hi.  The counts fall about exponentially, so the first guesses go by their logarithms (2 or 3
+  // of them as a rule, where halving takes 8).
+  least = -wave_max(-least);
+  uint32_t lo = ordered(least), hi = max(ordered(largest), lo);
+  float f_lo = least, f_hi = largest, l_lo = __builtin_amdgcn_logf(static_cast<float>(n)), l_hi = -1.f;
+  const float wanted = __builtin_amdgcn_logf(1.125f * static_cast<float>(k));
+  for (int tries = 0; lo < hi; ++tries) {
+    uint32_t mid = lo + (hi - lo + 1) / 2;
+    if (tries < 5) mid = min(max(ordered(fmaf(f_hi - f_lo, (l_lo - wanted) * __builtin_amdgcn_rcpf(l_lo - l_hi), f_lo)), lo + 1), hi);
+    mid = __builtin_amdgcn_readfirstlane(mid);
     n = 0;
 #pragma unroll
     for (int i = 0; i < PER; ++i) n += __popcll(__ballot(v[i] >= mid));
     if (n >= k) {
       lo = mid;
       if (n <= k + k / 4) break;
+      f_lo = unordered(mid);
+      l_lo = __builtin_amdgcn_logf(static_cast<float>(n));
     } else {
       hi = mid - 1;
+      f_hi = unordered(mid);
+      l_hi = n ? __builtin_amdgcn_logf(static_cast<float>(n)) : -1.f;
     }
   }
   return lo;
@@ -227,6 +239,8 @@ __device__ __noinline__ int crowded(int k, const T* z, int n, int first, uint32_
   __syncthreads();
   return min(lds.n, kCandidates);
 }
+
+static_assert(sizeof(RowLds) + kMaxSlots * 8 * 16 <= 65536, "LDS without asking for more");
 
 template <typename T, int NV, bool TOP, bool ENT>
 __global__ void __launch_bounds__(1024, 8) logprob_kernel(LogprobArgs a, int slices, int pieces_per_slice, Partial part, int slots) {
@@ -379,16 +393,21 @@ __global__ void __launch_bounds__(1024, 8) logprob_kernel(LogprobArgs a, int sli
     if (found > kCandidates) {
       found = crowded<T>(a.k, z, n, first * kN, threshold, ordered(m), lds_);
     }
-    // each key's place among them: how many are greater
+    // each key's place among them: how many are greater, counted by four lanes
     const float log = lds_.log;
     const bool bad = log != log;
-    for (int i = threadIdx.x; i < max(found, a.k); i += threads) {
+    const int quarter = lane & 3;
+    for (int i = threadIdx.x / 4; i < max(found, a.k); i += threads / 4) {
       const uint64_t key = i < found ? lds_.keys[i] : 0;
-      int place = i < found ? 0 : i;
-      if (i < found)
-#pragma unroll 8
-        for (int j = 0; j < found; ++j) place += lds_.keys[j] > key;
-      if (place >= a.k) continue;
+      int place = 0;
+      if (i < found) {
+#pragma unroll 4
+        for (int j = quarter; j < found; j += 4) place += lds_.keys[j] > key;
+      }
+      place += dpp_rows<0xb1, 0xf>(0, place);
+      place += dpp_rows<0x4e, 0xf>(0, place);
+      if (i >= found) place = i;
+      if (place >= a.k || quarter) continue;
       if (slices > 1) {
         part.keys[(r * slices + slice) * a.k + place] = key;
       } else {
@@ -591,7 +610,7 @@ inline size_t logprob_bytes(int64_t rows, int k, int slices) {
 template <typename T>
 void launch_logprob(const LogprobArgs& a, const RowShape& s, const Partial& part, hipStream_t st) {
   const dim3 grid(static_cast<unsigned>(a.rows * s.slices)), threads(s.threads);
-  const int slots = std::min(s.threads, a.k + a.k / 2 + 8);   // 50 KB at most
+  const int slots = std::min(s.threads, a.k + a.k / 2 + 8);   // kMaxSlots at most
   auto launch = [&](auto nv, auto top, auto ent) {
     hipLaunchKernelGGL((logprob_kernel<T, decltype(nv)::value, decltype(top)::value, decltype(ent)::value>), grid, threads,
                        a.k ? static_cast<size_t>(slots) * decltype(nv)::value * 16 : 0, st, a, s.slices, s.pieces, part, slots);
