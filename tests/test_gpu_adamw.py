@@ -555,3 +555,127 @@ def test_refusals_on_the_gpu():
         with pytest.raises((ValueError, RuntimeError), match=text):
             call()
     assert torch.equal(p, keep) and not m.any() and int(count) == 0
+
+
+def test_overlaps():
+    """What overlaps a tensor that is written is refused, in the plain case and where a tensor's strides are not; grads may be one
+    tensor for several params, params may lie next to each other."""
+    buf = torch.randn(1000, device="cuda")
+    z = lambda n=300: torch.zeros(n, device="cuda")  # noqa: E731
+    g = torch.randn(300, device="cuda")
+    keep = buf.clone()
+    for strided in (False, True):
+        more = ([torch.randn(20, 10, device="cuda").t()] if strided else [])
+        extra = [torch.randn(10, 20, device="cuda") for _ in more]
+        zs = lambda: [torch.zeros_like(t) for t in more]  # noqa: E731
+        for ps, gs, ms, vs in [
+                ([buf[:300], buf[299:599]], [g, g], [z(), z()], [z(), z()]),
+                ([buf[:300]], [buf[100:400]], [z()], [z()]),
+                ([buf[:300]], [g], [buf[200:500]], [z()]),
+                ([buf[:300]], [g], [z()], [buf[200:500]])]:
+            with pytest.raises(ValueError, match="overlap"):
+                core.adamw(ps + more, gs + extra, ms + zs(), vs + zs(), step=1)
+        assert torch.equal(buf, keep)
+        a = [buf[:300], buf[300:600]]
+        ms, vs = [z(), z()], [z(), z()]
+        core.adamw(a + more, [g, g] + extra, ms + zs(), vs + zs(), step=1, **HYPER)
+        b = [t.clone() for t in (keep[:300], keep[300:600])]
+        core.adamw(b, [g.clone(), g.clone()], [z(), z()], [z(), z()], step=1, **HYPER)
+        assert all(torch.equal(x, y) for x, y in zip(a, b)) and torch.equal(buf[600:], keep[600:])
+        buf.copy_(keep)
+    s = [core.new_moments(g)]
+    with pytest.raises(ValueError, match="overlap"):
+        core.read_moments(s, [buf[:300]], [buf[299:599]])
+
+
+class Named(torch.Tensor):
+    pass
+
+
+def test_other_kinds_of_tensors():
+    """Subclasses, inference tensors, tuples and iterators in place of lists."""
+    g0 = torch.randn(300, device="cuda")
+    want = torch.ones(300, device="cuda")
+    core.adamw([want], [g0], [torch.zeros_like(want)], [torch.zeros_like(want)], step=1, max_norm=0.1, **HYPER)
+    for wrap in (lambda t: t.as_subclass(Named), lambda t: torch.nn.Parameter(t)):
+        p, g, m, v = (wrap(t) for t in (torch.ones(300, device="cuda"), g0.clone(), torch.zeros_like(g0), torch.zeros_like(g0)))
+        with torch.no_grad():
+            core.adamw((p,), iter([g]), (m,), [v], step=1, max_norm=0.1, **HYPER)
+        assert torch.equal(p.detach().as_subclass(torch.Tensor), want)
+    with torch.inference_mode():
+        p, m, v = torch.ones(300, device="cuda"), torch.zeros(300, device="cuda"), torch.zeros(300, device="cuda")
+        core.adamw([p], [g0], [m], [v], step=1, max_norm=0.1, **HYPER)
+        assert torch.equal(p, want)
+
+
+def test_the_largest_steps_stream():
+    """More values than the last-level cache keeps take other loads and stores: the same bits as in parts."""
+    n = (1 << 25) + 77
+    for bits in (32, 8):
+        for dtype in (torch.float32, torch.bfloat16):
+            gen = torch.Generator(device="cuda").manual_seed(1)
+            p = torch.randn(n, device="cuda", generator=gen).to(dtype)
+            g = torch.randn(n, device="cuda", generator=gen).to(dtype)
+            q = p.clone()
+            cut = 1 << 18   # a whole number of blocks
+            parts = [t.split(cut) for t in (q, g)]
+            if bits == 32:
+                m, v = torch.zeros(n, device="cuda"), torch.zeros(n, device="cuda")
+                m2, v2 = torch.zeros(n, device="cuda"), torch.zeros(n, device="cuda")
+                core.adamw([p], [g], [m], [v], step=1, **HYPER)
+                for a, b, c, d in zip(*parts, m2.split(cut), v2.split(cut)):
+                    core.adamw([a], [b], [c], [d], step=1, **HYPER)
+                assert torch.equal(m, m2) and torch.equal(v, v2)
+            else:
+                s = core.new_moments(p)
+                core.adamw([p], [g], [s], step=1, seed=3, **HYPER)
+                m, v = torch.empty(n, dtype=dtype, device="cuda"), torch.empty(n, dtype=dtype, device="cuda")
+                core.read_moments([s], [m], [v])
+                # the parts in one list have the positions that the whole has
+                small = [core.new_moments(t) for t in parts[0]]
+                core.adamw(list(parts[0]), list(parts[1]), small, step=1, seed=3, **HYPER)
+                assert torch.equal(torch.cat(small), s)
+                m2, v2 = torch.empty_like(m), torch.empty_like(v)
+                for t, a, b in zip(small, m2.split(cut), v2.split(cut)):
+                    core.read_moments([t], [a], [b])
+                assert torch.equal(m, m2) and torch.equal(v, v2)
+            assert torch.equal(p, q)
+            del p, q, g, m, v, m2, v2, parts
+
+
+def test_a_training_run_and_its_decoding():
+    """The operators together, as a program uses them: a loss on given tokens with an entropy bonus, its gradient, the clipped
+    step, the new weights in a captured decode step beside the log probabilities of what it chose."""
+    torch.manual_seed(5)
+    kw = dict(d=64, layers=2, mlp_f=96, heads=4, n_sub=8, d_a=16, k=4)
+    model = OneSdmLM(211, **kw, seed=6).cuda()
+    opt = model.optimizer(3e-3, state_bits=8, max_norm=1.0)
+    idx = torch.randint(0, 211, (4, 33), device="cuda")
+    for _ in range(3):
+        opt.zero_grad()
+        r = model.token_logprobs(idx, entropy=True)
+        (-r.logprobs.sum() / (4 * 32) - 0.01 * r.entropy.mean()).backward()
+        opt.step()
+        assert math.isfinite(float(opt.norm)) and float(opt.norm) > 0
+    with torch.no_grad():
+        state, eager = model.decode_state(4), model.decode_state(4)
+        tok = idx[:, 0].clone()
+        warm = model.decode_state(4)
+        for _ in range(2):
+            r = core.token_logprobs(model.step(tok, warm), tok, top=5)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            logits = model.step(tok, state)
+            nxt = logits.argmax(-1)
+            r = core.token_logprobs(logits, nxt, entropy=True, top=5)
+        t = idx[:, 0].clone()
+        for i in range(5):
+            tok.copy_(t)
+            graph.replay()
+            want = model.step(t, eager)
+            w = core.token_logprobs(want, want.argmax(-1), entropy=True, top=5)
+            torch.cuda.synchronize()
+            assert torch.equal(nxt, want.argmax(-1)) and all(torch.equal(a, b) for a, b in zip(r, w))
+            assert torch.equal(r.top_ids[:, 0], nxt)
+            t = want.argmax(-1)

@@ -162,3 +162,23 @@ def test_model_optimizer_groups():
     assert "emb.weight" in decayed and "mems.0.wk.weight" in decayed and "mlps.0.down.weight" in decayed
     assert "nf.w" in rest and "mems.0.keys1" in rest and "mems.0.onorm_w" in rest and "mems.0.wg.bias" in rest
     assert sorted(decayed + rest) == sorted(n for n, p in model.named_parameters() if p.requires_grad)
+
+
+def test_native_lists():
+    """What the extension does not pack is left to the caller: CPU tensors, other lengths, no tensors at all."""
+    pack = _lib.lists().pack
+    a, b = torch.zeros(3), torch.zeros(3)
+    assert pack(None, [a], None, None, False, False) is None
+    assert pack([a], [a, b], [a], [b], False, False) is None
+    assert pack([], [], [], [], False, False) is None
+    assert pack(None, None, None, None, False, False) is None
+    assert pack([1], [2], [3], [4], False, False) is None
+    assert pack((a,), [a], [a], [b], False, False) is None
+    with pytest.raises(TypeError):
+        pack([a])
+    v = a._version
+    _lib.lists().written([a], [])
+    assert a._version == v + 1 and b._version == 0
+    with torch.inference_mode():
+        c = torch.zeros(3)
+    _lib.lists().written([c])
