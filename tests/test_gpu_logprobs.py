@@ -167,6 +167,37 @@ def test_ties_and_crowded_alternatives(V, dtype, k):
     say(check(z, y, 1.0, k)[2])
 
 
+@pytest.mark.parametrize("V,k", [(300001, 256), (1 << 21, 100), (1 << 21, 256), (1 << 21, 0)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_the_widest_rows(V, k, dtype):
+    """As many slices as there can be, with more keys in them than the join holds in LDS."""
+    z, y, _ = make(2, V, dtype, V + k, 1.5)
+    say(V, dtype, k, check(z, y, 1.1, k)[2])
+
+
+@pytest.mark.parametrize("V", [130, 900, 1500, 6000, 33000, 70000])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("k", [20, 100, 256])
+def test_coarse_logits_and_counts_around_k(V, dtype, k):
+    """Few different values, in any order; rows that leave k - 1, k and k + 1 tokens, spread or side by side; all but a few values
+    of one size."""
+    g = torch.Generator().manual_seed(V + k)
+    rows = [(torch.randn(V, generator=g) * 1.5).round(), (torch.randn(V, generator=g) * 3).round() / 2 - 9,
+            torch.randint(0, 2, (V,), generator=g).float(), torch.randn(V, generator=g) * 0.02 + 5, torch.randn(V, generator=g) * 0.02 - 5]
+    for left in (k - 1, k, k + 1):
+        for spread in (True, False):
+            x = torch.full((V,), -math.inf)
+            at = torch.randperm(V, generator=g)[:left] if spread else torch.arange(V)[V // 3:V // 3 + left]
+            x[at] = torch.randn(len(at), generator=g)
+            rows.append(x)
+    x = torch.zeros(V)
+    x[torch.randperm(V, generator=g)[:max(1, k // 2)]] = 1.0
+    rows += [x, -x]
+    z = torch.stack(rows).to(dtype)
+    y = torch.arange(len(rows)) * 7
+    say(check(z, y, 1.0, k)[2])
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("V", [10, 2100, 40001])
 def test_masked_rows(dtype, V):
