@@ -1740,18 +1740,14 @@ class TokenLogprobs(typing.NamedTuple):
 
 
 def _logprobs(z, zs, targets, dims, entropy, stats):
-    n, k, at, lib = z.size(0), dims.top_k, ctypes.byref(dims), _lib.load()
-    empty = torch.empty
-    dev, code = z.device, _DT[z.dtype]
-    lp = None if targets is None else empty(n, dtype=torch.float32, device=dev)
-    h = empty(n, dtype=torch.float32, device=dev) if entropy else None
-    ids = empty((n, k), dtype=torch.int64, device=dev) if k else None
-    tops = empty((n, k), dtype=torch.float32, device=dev) if k else None
+    n, k, at, lib, code = dims.rows, dims.top_k, ctypes.byref(dims), _lib.load(), _DT[z.dtype]
+    out = lp, h, ids, tops = _lib.lists().new_rows(z, n, k, ("-" if targets is None else "f") + ("f" if entropy else "-") + (
+        "IF" if k else "--"))
     nbytes = lib.sdm_rt_token_logprobs_workspace_bytes(at, code)
-    ws = empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=z.device) if nbytes else None
     _launch(lib.sdm_rt_token_logprobs, z.get_device(), at, z.data_ptr(), zs, code, _ptr(targets), _ptr(lp), _ptr(h), _ptr(ids),
             _ptr(tops), _ptr(stats), _ptr(ws), nbytes)
-    return lp, h, ids, tops
+    return out
 
 
 class LogprobFunction(torch.autograd.Function):

@@ -1,9 +1,11 @@
-// lists.cpp -- lists of torch tensors as the sdm_rt_tensor array that a training step's calls take (a Python extension,
-// sdmchat_amd/lib/_lists.so, loaded by sdmchat_amd/_lib.py).
+// lists.cpp -- what is quicker asked of torch's tensors from here than from Python (an extension, sdmchat_amd/lib/_lists.so,
+// loaded by sdmchat_amd/_lib.py): lists of tensors as the sdm_rt_tensor array that a training step's calls take, and several
+// small outputs at once.
 //
 // A step over a model asks five things of each of some 700 tensors: asked from Python they take longer than the step itself
 // (182 tensors with two moments each: 230 us of host time, from here 20).
 #include <Python.h>
+#include <ATen/Functions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <algorithm>
@@ -131,11 +133,55 @@ PyObject* written(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   Py_RETURN_NONE;
 }
 
+// new_rows(like, n, k, kinds): uninitialised tensors on the GPU of the tensor `like`, one for each letter of kinds: f float32
+// [n], F float32 [n][k], I int64 [n][k]; None for any other.  (Half the time of as many calls from Python: a decode step's token
+// waits for them.)
+PyObject* new_rows(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  if (nargs != 4 || !THPVariable_Check(args[0]) || !PyUnicode_Check(args[3])) {
+    PyErr_SetString(PyExc_TypeError, "new_rows: a tensor, two numbers and the kinds");
+    return nullptr;
+  }
+  const int64_t n = PyLong_AsLongLong(args[1]), k = PyLong_AsLongLong(args[2]);
+  Py_ssize_t count = 0;
+  const char* kinds = PyUnicode_AsUTF8AndSize(args[3], &count);
+  if (!kinds || PyErr_Occurred()) return nullptr;
+  PyObject* out = PyTuple_New(count);
+  if (!out) return nullptr;
+  try {
+    const at::TensorOptions on = THPVariable_Unpack(args[0]).options().requires_grad(false);
+    for (Py_ssize_t i = 0; i < count; ++i) {
+      PyObject* t;
+      if (kinds[i] == 'f') {
+        t = THPVariable_Wrap(at::empty({n}, on.dtype(at::kFloat)));
+      } else if (kinds[i] == 'F') {
+        t = THPVariable_Wrap(at::empty({n, k}, on.dtype(at::kFloat)));
+      } else if (kinds[i] == 'I') {
+        t = THPVariable_Wrap(at::empty({n, k}, on.dtype(at::kLong)));
+      } else {
+        t = Py_None;
+        Py_INCREF(t);
+      }
+      if (!t) {
+        Py_DECREF(out);
+        return nullptr;
+      }
+      PyTuple_SET_ITEM(out, i, t);
+    }
+  } catch (const std::exception& e) {   // no memory
+    Py_DECREF(out);
+    PyErr_SetString(PyExc_RuntimeError, e.what());
+    return nullptr;
+  }
+  return out;
+}
+
 PyMethodDef methods[] = {
     {"pack", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(pack)), METH_FASTCALL,
      "pack(params, grads, exp_avgs, exp_avg_sqs, eight, reading) -> (table, GPU) or None"},
     {"written", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(written)), METH_FASTCALL,
      "written(list of tensors, ...)"},
+    {"new_rows", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(new_rows)), METH_FASTCALL,
+     "new_rows(like, n, k, kinds) -> tensors"},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_lists", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

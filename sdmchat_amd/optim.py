@@ -18,18 +18,19 @@ class AdamW(torch.optim.Optimizer):
         opt.zero_grad()
 
     max_norm: gradients are clipped to this norm over all parameter groups, which must be on one GPU then; the .grad tensors
-    stay as they are.  state_bits: 32, or 8 (core.new_moments: 2.06 bytes a value instead of 8); a parameter group may have its
+    stay as they are (a norm that is NaN reaches every parameter, as a product with it does).  state_bits: 32, or 8 (core.new_moments: 2.06 bytes a value instead of 8); a parameter group may have its
     own, as its own lr, betas, eps and weight_decay.  capturable: the steps are counted on the GPU, so a graph may capture
     step() once it has run; lr may then be a float32 tensor of one element that a schedule writes.  seed: of the 8-bit moments'
     rounding.  bfloat16 parameters are rounded to nearest, so a change below half their last place is lost: keep float32
     parameters and bfloat16 autocast where that matters.  Sparse gradients and parameters whose values are not dense in memory
     are refused."""
 
+    norm = None   # of the last step's gradients
+
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, *, state_bits=32, max_norm=None,
                  capturable=False, seed=0):
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay, state_bits=state_bits,
                                       max_norm=max_norm, capturable=capturable, seed=seed))
-        self.norm = None
 
     def add_param_group(self, param_group):
         super().add_param_group(param_group)
@@ -131,6 +132,8 @@ class AdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict):
         """As torch's, but for the moments' types, which stay what they are: float32, or the bytes of 8-bit moments."""
+        if any(not g.keys() >= self.defaults.keys() for g in state_dict["param_groups"]):
+            raise ValueError("AdamW.load_state_dict: not the state of this optimiser")
         old = [p for g in state_dict["param_groups"] for p in g["params"]]
         new = [p for g in self.param_groups for p in g["params"]]
         bits = [g["state_bits"] for g in state_dict["param_groups"] for _ in g["params"]]

@@ -182,3 +182,18 @@ def test_native_lists():
     with torch.inference_mode():
         c = torch.zeros(3)
     _lib.lists().written([c])
+    rows = _lib.lists().new_rows(torch.zeros(2, dtype=torch.bfloat16), 3, 5, "f-IF")
+    assert [None if t is None else (tuple(t.shape), t.dtype) for t in rows] == [
+        ((3,), torch.float32), None, ((3, 5), torch.int64), ((3, 5), torch.float32)]
+    with pytest.raises(TypeError):
+        _lib.lists().new_rows(1, 2, 3, "f")
+
+
+def test_a_foreign_optimizer_state_is_refused():
+    p = torch.nn.Parameter(torch.zeros(3))
+    other = torch.optim.AdamW([p])
+    with pytest.raises(ValueError, match="not the state"):
+        AdamW([p]).load_state_dict(other.state_dict())
+    import copy
+    opt = copy.deepcopy(AdamW([p], state_bits=8, max_norm=2.0))
+    assert opt.norm is None and opt.defaults["max_norm"] == 2.0 and opt.param_groups[0]["state_bits"] == 8
