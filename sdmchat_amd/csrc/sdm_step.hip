@@ -42,9 +42,8 @@ __device__ __forceinline__ StepChunk find_chunk(const TABLE& table, uint32_t ind
                    static_cast<int64_t>(index - first) * CHUNK};
 }
 
-// 8, 16 or 32 bytes at any element's address.  THROUGH: what a call streams through leaves the caches to others, and the memory
-// to longer bursts (a step of 110 M float32 values with their moments 620 us, 737 without; a model that the last-level cache
-// holds is better left there)
+// 8, 16 or 32 bytes at any element's address.  THROUGH: what a call streams through leaves the caches to others (a step of 110 M
+// float32 values, the norm of their gradients with it, 620 us, 737 without); a model that the last-level cache holds stays there.
 template <bool THROUGH, int BYTES>
 __device__ __forceinline__ void load_bytes(const void* p, void* v) {
   if constexpr (!THROUGH) {
@@ -117,7 +116,8 @@ __device__ __forceinline__ double wave_add(double v) {
   return v;
 }
 
-// Eight pieces of a thread under way at once: one at a time left it waiting (220 MB of bfloat16 72 us).
+// Four pieces of a thread under way at once (220 MB of bfloat16 41 us, 5.3 TB/s): one at a time left it waiting (72), eight left
+// too few waves (50).
 template <typename T>
 __device__ __forceinline__ double sum_squares(const T* g, int n) {
   constexpr int kN = 16 / static_cast<int>(sizeof(T)), kAtOnce = 4;
@@ -482,8 +482,9 @@ void for_tables(const sdm_rt_tensor* t, int32_t count, int chunk, TAKE take, LAU
   flush();
 }
 
-// Few values take small chunks, so that all compute units have some.
-constexpr int64_t kSmallStep = 16 << 20, kSmallNorm = 8 << 20;
+// Few values take small chunks, so that all compute units have some: the norm of 14 M values 13.2 us in chunks of 4,096, 15.0 of
+// 16,384, of 110 M 55 and 41; an 8-bit step of 14 M values 40 us in chunks of 2,048, 42 of 4,096, of 110 M 236 and 220.
+constexpr int64_t kSmallStep = 16 << 20, kSmallNorm = 32 << 20;
 
 inline int norm_chunk(int64_t values) { return values <= kSmallNorm ? 4096 : 16384; }
 inline int64_t norm_partials(const sdm_rt_tensor* t, int32_t count, int64_t values) {
@@ -582,47 +583,53 @@ int sdm_rt_adamw(const sdm_rt_adamw_options* o, const sdm_rt_tensor* tensors, in
   }
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (o->t_device) hipLaunchKernelGGL(count_step_kernel, dim3(1), dim3(1), 0, st, o->t_device);
-  auto launch = [&](auto small, auto device, auto through) {
-    constexpr bool kSmall = decltype(small)::value, kDevice = decltype(device)::value, kThrough = decltype(through)::value;
-    if (o->state_bits == 32) {
-      constexpr int kChunk = 1024;   // 110 M float32 values 476 us, 466 with 2,048, 480 with 4,096; 285 M bfloat16 1,040, 1,075, 1,167
-      for_tables<StepTable32>(
-          tensors, count, kChunk,
-          [](const sdm_rt_tensor& t, char** at) {
-            at[0] = static_cast<char*>(t.param);
-            at[1] = static_cast<char*>(const_cast<void*>(t.grad));
-            at[2] = static_cast<char*>(t.exp_avg);
-            at[3] = static_cast<char*>(t.exp_avg_sq);
-          },
-          [&](const StepTable32& table, unsigned chunks, int64_t) {
-            hipLaunchKernelGGL((adamw32_kernel<kChunk, kDevice, kThrough>), dim3(chunks), dim3(kStepThreads), 0, st, table, a);
-          });
-    } else {
-      constexpr int kChunk = kSmall ? 2048 : 4096;   // 14 M values 46.7 us with 2,048, 48.9 with 4,096; 110 M 236 and 220
-      for_tables<StepTable8>(
-          tensors, count, kChunk,
-          [](const sdm_rt_tensor& t, char** at) {
-            at[0] = static_cast<char*>(t.param);
-            at[1] = static_cast<char*>(const_cast<void*>(t.grad));
-            at[2] = static_cast<char*>(t.exp_avg);
-          },
-          [&](const StepTable8& table, unsigned chunks, int64_t) {
-            hipLaunchKernelGGL((adamw8_kernel<kChunk, kDevice, kThrough>), dim3(chunks), dim3(kStepThreads), 0, st, table, a);
-          });
-    }
+  auto launch32 = [&](auto device, auto through) {
+    constexpr int kChunk = 1024;   // 110 M float32 values 476 us, 466 with 2,048, 480 with 4,096; 285 M bfloat16 1,040, 1,075, 1,167
+    for_tables<StepTable32>(
+        tensors, count, kChunk,
+        [](const sdm_rt_tensor& t, char** at) {
+          at[0] = static_cast<char*>(t.param);
+          at[1] = static_cast<char*>(const_cast<void*>(t.grad));
+          at[2] = static_cast<char*>(t.exp_avg);
+          at[3] = static_cast<char*>(t.exp_avg_sq);
+        },
+        [&](const StepTable32& table, unsigned chunks, int64_t) {
+          hipLaunchKernelGGL((adamw32_kernel<kChunk, decltype(device)::value, decltype(through)::value>), dim3(chunks),
+                             dim3(kStepThreads), 0, st, table, a);
+        });
   };
-  auto with_device = [&](auto small, auto through) {
-    if (o->t_device)
-      launch(small, std::true_type{}, through);
+  auto launch8 = [&](auto chunk, auto device, auto through) {
+    constexpr int kChunk = decltype(chunk)::value;
+    for_tables<StepTable8>(
+        tensors, count, kChunk,
+        [](const sdm_rt_tensor& t, char** at) {
+          at[0] = static_cast<char*>(t.param);
+          at[1] = static_cast<char*>(const_cast<void*>(t.grad));
+          at[2] = static_cast<char*>(t.exp_avg);
+        },
+        [&](const StepTable8& table, unsigned chunks, int64_t) {
+          hipLaunchKernelGGL((adamw8_kernel<kChunk, decltype(device)::value, decltype(through)::value>), dim3(chunks),
+                             dim3(kStepThreads), 0, st, table, a);
+        });
+  };
+  auto with_bits = [&](auto device, auto through) {
+    if (o->state_bits == 32)
+      launch32(device, through);
+    else if (values <= kSmallStep)
+      launch8(std::integral_constant<int, 2048>{}, device, through);
     else
-      launch(small, std::false_type{}, through);
+      launch8(std::integral_constant<int, 4096>{}, device, through);
+  };
+  auto with_device = [&](auto through) {
+    if (o->t_device)
+      with_bits(std::true_type{}, through);
+    else
+      with_bits(std::false_type{}, through);
   };
   if (bytes > kStreamBytes)
-    with_device(std::false_type{}, std::true_type{});
-  else if (values > kSmallStep)
-    with_device(std::false_type{}, std::false_type{});
+    with_device(std::true_type{});
   else
-    with_device(std::true_type{}, std::false_type{});
+    with_device(std::false_type{});
   return check_launch("adamw");
 }
 
