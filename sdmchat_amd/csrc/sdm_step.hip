@@ -182,9 +182,10 @@ __host__ __device__ __forceinline__ uint32_t step_key(uint32_t seed, int64_t t) 
   return mix(seed + static_cast<uint32_t>(t) * 2654435761u);
 }
 
-// the exponent of a block whose largest magnitude has these bits: 255 where it is not finite or from 2^127 on
+// the exponent of a block whose largest magnitude has these bits: 255 where it is not finite or from 2^127 on (a NaN may have
+// its sign set, and is then the greatest of the bits)
 __device__ __forceinline__ uint32_t block_exponent(uint32_t bits) {
-  const uint32_t e = (bits + 0xfffffu) >> 23;
+  const uint32_t e = ((bits & 0x7fffffffu) + 0xfffffu) >> 23;
   return e >= 254 ? 255 : e;
 }
 // 2^(E - 127), 0 for E = 0, NaN for E = 255

@@ -319,6 +319,30 @@ def test_non_finite_gradients():
     assert p.isnan().cpu().tolist() == [False, True, False, False]   # 1 / inf: the others' gradients are 0
 
 
+@pytest.mark.parametrize("dtype,patterns", [(torch.float32, [0x7fc00000, 0xffc00000, 0x7f800001, 0x7fffffff, 0xffffffff, 0xfff00001]),
+                                            (torch.bfloat16, [0x7fc0, 0xffc0, 0x7f81, 0x7fff, 0xffff, 0xfff0])])
+def test_nan_of_any_bits(dtype, patterns):
+    """A NaN is one whatever its sign and payload: for its block's exponents, its parameter and the norm."""
+    whole = torch.int32 if dtype == torch.float32 else torch.int16
+    for bits in patterns:
+        g = torch.ones(300, device="cuda", dtype=dtype)
+        g.view(whole)[140] = bits - (1 << whole.itemsize * 8) if bits >> (whole.itemsize * 8 - 1) else bits
+        assert g.isnan().cpu().nonzero().flatten().tolist() == [140]
+        assert math.isnan(float(core.grad_norm([g])))
+        p = torch.ones_like(g)
+        st = [core.new_moments(p)]
+        core.adamw([p], [g], st, step=1, **HYPER)
+        assert p.isnan().cpu().nonzero().flatten().tolist() == [140], hex(bits)
+        block = torch.zeros(300, dtype=torch.bool)
+        block[128:256] = True
+        for moment in read(st, [p]):
+            assert torch.equal(moment[0].isnan().cpu(), block), hex(bits)
+        m, v = torch.zeros(300, device="cuda"), torch.zeros(300, device="cuda")
+        core.adamw([p], [g], [m], [v], step=1, **HYPER)
+        for moment in (m, v, p):
+            assert moment.isnan().cpu().nonzero().flatten().tolist() == [140], hex(bits)
+
+
 def test_step_and_lr_on_the_device():
     ps, gs = tensors([(300,), (77,)], [torch.float32], 6)
     for bits in (32, 8):

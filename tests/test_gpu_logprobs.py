@@ -250,6 +250,33 @@ def test_nan_and_infinity(dtype, V):
     assert not grad[bad.cuda()].any() and not grad[5].any() and bool(grad[1].any()) and not grad.isnan().any()
 
 
+@pytest.mark.parametrize("dtype,patterns", [(torch.float32, [0x7fc00000, 0xffc00000, 0x7f800001, 0x7fffffff, 0xffffffff, 0xfff00001]),
+                                            (torch.bfloat16, [0x7fc0, 0xffc0, 0x7f81, 0x7fff, 0xffff, 0xfff0])])
+@pytest.mark.parametrize("V", [7, 5000, 40001])
+def test_nan_of_any_bits(dtype, patterns, V):
+    """A NaN is one whatever its sign and payload: among logits, negative logits, masked ones and in a row of its own kind, in the
+    first place, the middle and the last."""
+    whole = torch.int32 if dtype == torch.float32 else torch.int16
+    for bits in patterns:
+        nan = bits - (1 << whole.itemsize * 8) if bits >> (whole.itemsize * 8 - 1) else bits
+        z = torch.randn(10, V, generator=torch.Generator().manual_seed(5)).to(dtype)
+        z[3:6] = -z[3:6].abs() - 1.0
+        z[6:9] = -math.inf
+        w = z.view(whole)
+        for r in range(9):
+            w[r, (0, V // 2, V - 1)[r % 3]] = nan
+        w[9] = nan
+        assert z.isnan().any(1).all()
+        for top, entropy in ((0, False), (0, True), (3, True)):
+            with torch.no_grad():
+                r = core.token_logprobs(z.cuda(), torch.full((10,), 1).cuda(), entropy=entropy, top=top)
+            assert bool(r.logprobs.isnan().all()), hex(bits)
+            if entropy:
+                assert bool(r.entropy.isnan().all()), hex(bits)
+            if top:
+                assert bool(r.top_logprobs.isnan().all()) and bool((r.top_ids == -1).all()), hex(bits)
+
+
 def test_nearly_certain_rows_keep_their_digits():
     """A token of probability 1 - q, q down to 1e-12: log probability -q and entropy of about q (1 + log 1 / q), to relative
     precision: log1p of the others' sum, which is off by U (5 a + 4 + c)."""
