@@ -37,6 +37,10 @@ __device__ __forceinline__ RowLogs row_logs(const RowSums& s) {
   return RowLogs{l, l * kLog2, l - kLn2 * (s.u / (s.count + s.rest))};
 }
 
+// (z - max) / temperature; in halves, since the difference of two float32 of different signs may pass float32's range where its
+// quotient does not
+__device__ __forceinline__ float below_max(float z, float m, float inv_tau) { return (0.5f * z - 0.5f * m) * (2.f * inv_tau); }
+
 // greater for a greater logit, at equal logits for a lower id; 0 for -inf and NaN of either sign
 __device__ __forceinline__ uint32_t ordered(float z) {
   const uint32_t b = __float_as_uint(z + 0.f);   // -0 as 0
@@ -62,7 +66,7 @@ __device__ __forceinline__ int64_t row_target(const LogprobArgs& a, int64_t r) {
 // What becomes of a row's sums, by one thread.
 __device__ __forceinline__ void write_row(const LogprobArgs& a, int64_t r, const RowTarget& y, const RowSums& s, const RowLogs& g) {
   const bool bad = s.m == INFINITY || s.rest != s.rest, none = !bad && s.m == -INFINITY;
-  if (a.logprobs) a.logprobs[r] = y.id < 0 ? 0.f : bad ? NAN : none ? -INFINITY : (y.z - s.m) * a.inv_tau - g.l;
+  if (a.logprobs) a.logprobs[r] = y.id < 0 ? 0.f : bad ? NAN : none ? -INFINITY : below_max(y.z, s.m, a.inv_tau) - g.l;
   const float h = bad ? NAN : none ? 0.f : g.h;
   if (a.entropy) a.entropy[r] = h;
   // a row of -inf: sums that make every p 0
@@ -494,7 +498,7 @@ __global__ void __launch_bounds__(1024, 8) logprob_kernel(LogprobArgs a, int sli
         part.keys[(r * slices + slice) * a.k + place] = key;
       } else {
         a.top_ids[r * a.k + place] = key && !bad ? static_cast<int64_t>(~static_cast<uint32_t>(key)) : -1;
-        a.top_logprobs[r * a.k + place] = bad ? NAN : key ? (unordered(static_cast<uint32_t>(key >> 32)) - m) * a.inv_tau - log : -INFINITY;
+        a.top_logprobs[r * a.k + place] = bad ? NAN : key ? below_max(unordered(static_cast<uint32_t>(key >> 32)), m, a.inv_tau) - log : -INFINITY;
       }
     }
   }
@@ -536,7 +540,7 @@ __device__ __forceinline__ int place_keys(const LogprobArgs& a, int64_t r, int s
     if (place >= a.k) continue;
     ++there;
     a.top_ids[r * a.k + place] = bad ? -1 : static_cast<int64_t>(~static_cast<uint32_t>(key));
-    a.top_logprobs[r * a.k + place] = bad ? NAN : (unordered(static_cast<uint32_t>(key >> 32)) - m) * a.inv_tau - log;
+    a.top_logprobs[r * a.k + place] = bad ? NAN : below_max(unordered(static_cast<uint32_t>(key >> 32)), m, a.inv_tau) - log;
   }
   return there;
 }

@@ -277,6 +277,31 @@ def test_nan_of_any_bits(dtype, patterns, V):
                 assert bool(r.top_logprobs.isnan().all()) and bool((r.top_ids == -1).all()), hex(bits)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V", [5, 70001])
+@pytest.mark.parametrize("tau", [1.0, 1e6, 1e18])
+def test_the_types_largest_values(V, dtype, tau):
+    """Logits at both ends of the type: a difference past float32's range whose quotient by the temperature is not.  Off by the
+    two roundings of the difference and the temperature's reciprocal and the product, 4 U, and the sum's (at most 2^-20)."""
+    big = torch.finfo(dtype).max
+    z = torch.full((3, V), -big, dtype=dtype)
+    z[0, 1] = z[1, V - 1] = big
+    z[2] = torch.linspace(-big / 2, big, V, dtype=torch.float64).to(dtype)
+    y = torch.tensor([0, 2, 0])
+    with torch.no_grad():
+        r = core.token_logprobs(z.cuda(), y.cuda(), temperature=tau, entropy=True, top=3)
+    t = (z.double() - z.double().max(1, keepdim=True).values) / tau
+    l = t - t.exp().sum(1, keepdim=True).log()
+    want = torch.cat([l.gather(1, y[:, None]), l.gather(1, r.top_ids.cpu())], 1)
+    got = torch.cat([r.logprobs[:, None], r.top_logprobs], 1).cpu().double()
+    past = want < -float(torch.finfo(torch.float32).max)
+    assert torch.equal(got == -math.inf, past) and bool((past.any() if tau == 1.0 else ~past.any()))
+    assert bool(((got - want).abs() <= 4 * U * want.abs() + 2.0 ** -20)[~past].all())
+    p = l.exp()
+    h = -torch.where(p > 0, p * l, torch.zeros_like(p)).sum(1)
+    assert bool(((r.entropy.cpu().double() - h).abs() <= 2.0 ** -20 * (1 + h)).all())
+
+
 def test_nearly_certain_rows_keep_their_digits():
     """A token of probability 1 - q, q down to 1e-12: log probability -q and entropy of about q (1 + log 1 / q), to relative
     precision: log1p of the others' sum, which is off by U (5 a + 4 + c)."""
