@@ -254,7 +254,11 @@ __device__ __forceinline__ void read_step(StepArgs& a) {
 }
 
 // One value's new moments (from the old ones times beta1 and beta2) and parameter.  Every product and sum of the moments is
-// rounded by itself, as the formula is written: their codes in 8 bits then do not hang on what a compiler fuses.
+// rounded by itself, as the formula is written: their codes in 8 bits then do not hang on what a compiler fuses.  The instruction
+// for square roots takes a v below float32's least normal value, 2^-126, for 0: 2^-63 in the root, less than a rounding of the
+// denominator unless eps is TINY.  Then the compiler's own root and quotient are taken, in kernels of their own (both in one
+// kernel took a third of the 8-bit step's waves: 110 M values 368 us against 350).
+template <bool TINY>
 __device__ __forceinline__ void step_value(const StepArgs& a, float clip, float g, float& p, float& m, float& v) {
   {
 #pragma clang fp contract(off)
@@ -262,15 +266,19 @@ __device__ __forceinline__ void step_value(const StepArgs& a, float clip, float 
     m = m + g * a.c1;
     v = v + g * g * a.c2;
   }
-  const float d = fmaf(__builtin_amdgcn_sqrtf(v), a.r2, a.eps);
-  p = fmaf(m * -a.size, __builtin_amdgcn_rcpf(d), p * a.decay);
+  if constexpr (TINY) {
+    p = fmaf(m / fmaf(sqrtf(v), a.r2, a.eps), -a.size, p * a.decay);
+  } else {
+    const float d = fmaf(__builtin_amdgcn_sqrtf(v), a.r2, a.eps);
+    p = fmaf(m * -a.size, __builtin_amdgcn_rcpf(d), p * a.decay);
+  }
 }
 
 using StepTable32 = StepTable<4, 96>;
 using StepTable8 = StepTable<3, 108, true>;
 
 // All of a thread's pieces of a chunk are loaded before the first is computed on: 16 bytes of parameters and gradients each.
-template <int CHUNK, bool THROUGH, typename T>
+template <int CHUNK, bool THROUGH, bool TINY, typename T>
 __device__ __forceinline__ void step_chunk32(const StepArgs& a, float clip, T* p, const T* g, float* m, float* v, int n) {
   constexpr int kN = 4, kPieces = CHUNK / (kStepThreads * kN);
   float pv[kPieces][kN], gv[kPieces][kN], mv[kPieces][kN], vv[kPieces][kN];
@@ -291,7 +299,7 @@ __device__ __forceinline__ void step_chunk32(const StepArgs& a, float clip, T* p
     for (int e = 0; e < kN; ++e) {
       mv[q][e] *= a.b1;
       vv[q][e] *= a.b2;
-      step_value(a, clip, gv[q][e], pv[q][e], mv[q][e], vv[q][e]);
+      step_value<TINY>(a, clip, gv[q][e], pv[q][e], mv[q][e], vv[q][e]);
     }
     store_values<THROUGH>(p + i, n - i, pv[q]);
     store_values<THROUGH>(m + i, n - i, mv[q]);
@@ -302,7 +310,7 @@ __device__ __forceinline__ void step_chunk32(const StepArgs& a, float clip, T* p
 // Sixteen lanes hold a block, 8 values each: its maxima come from four DPP steps.  Past a tensor's end p, g and the codes are 0
 // and stay so.  The codes do not stream past the caches: their lines are shared by neighbouring lanes' pieces (14 M values 43.5 us,
 // 48.9 if they do).  Bound by memory and instructions alike: 110 M bfloat16 values 217 us, 5.1 TB/s, 52 instructions a value.
-template <bool THROUGH, typename T>
+template <bool THROUGH, bool TINY, typename T>
 __device__ __forceinline__ void step_chunk8(const StepArgs& a, float clip, T* p, const T* g, char* chunk, uint32_t position, int n) {
   const int whole = (n + kBlock - 1) / kBlock * kBlock;
   for (int i = threadIdx.x * 8; i < whole; i += kStepThreads * 8) {
@@ -324,7 +332,7 @@ __device__ __forceinline__ void step_chunk8(const StepArgs& a, float clip, T* p,
       const halves h = decode_m(cm[q / 4], q / 2 & 1);
       mv[q] = fmaf(static_cast<float>(q & 1 ? h.y : h.x), b1, 0.f);
       vv[q] = decode_v(cv[q / 4], q & 3, shift) * b2;
-      step_value(a, clip, gv[q], pv[q], mv[q], vv[q]);
+      step_value<TINY>(a, clip, gv[q], pv[q], mv[q], vv[q]);
       am = fmaxf(am, fabsf(mv[q]));   // passes over NaN: v has it then, or infinity
       av = max(av, __float_as_uint(vv[q]));
     }
@@ -359,7 +367,7 @@ __device__ __forceinline__ float clip_factor(const StepArgs& a) {
   return c > 1.f ? 1.f : c;
 }
 
-template <int CHUNK, bool DEVICE, bool THROUGH>
+template <int CHUNK, bool DEVICE, bool THROUGH, bool TINY>
 __global__ void __launch_bounds__(kStepThreads) adamw32_kernel(StepTable32 table, StepArgs a) {
   if constexpr (DEVICE) read_step(a);
   const float clip = clip_factor(a);
@@ -369,14 +377,14 @@ __global__ void __launch_bounds__(kStepThreads) adamw32_kernel(StepTable32 table
   float* m = reinterpret_cast<float*>(table.at[2][c.tensor]) + c.begin;
   float* v = reinterpret_cast<float*>(table.at[3][c.tensor]) + c.begin;
   if (c.bf16)
-    step_chunk32<CHUNK, THROUGH>(a, clip, reinterpret_cast<bf16_t*>(p) + c.begin, reinterpret_cast<const bf16_t*>(g) + c.begin, m,
+    step_chunk32<CHUNK, THROUGH, TINY>(a, clip, reinterpret_cast<bf16_t*>(p) + c.begin, reinterpret_cast<const bf16_t*>(g) + c.begin, m,
                                  v, c.n);
   else
-    step_chunk32<CHUNK, THROUGH>(a, clip, reinterpret_cast<float*>(p) + c.begin, reinterpret_cast<const float*>(g) + c.begin, m, v,
+    step_chunk32<CHUNK, THROUGH, TINY>(a, clip, reinterpret_cast<float*>(p) + c.begin, reinterpret_cast<const float*>(g) + c.begin, m, v,
                                  c.n);
 }
 
-template <int CHUNK, bool DEVICE, bool THROUGH>
+template <int CHUNK, bool DEVICE, bool THROUGH, bool TINY>
 __global__ void __launch_bounds__(kStepThreads) adamw8_kernel(StepTable8 table, StepArgs a) {
   if constexpr (DEVICE) read_step(a);
   const float clip = clip_factor(a);
@@ -386,10 +394,10 @@ __global__ void __launch_bounds__(kStepThreads) adamw8_kernel(StepTable8 table, 
   char* state = table.at[2][c.tensor] + c.begin / kBlock * kBlockBytes;
   const uint32_t position = table.block[c.tensor] * static_cast<uint32_t>(kBlock) + static_cast<uint32_t>(c.begin);
   if (c.bf16)
-    step_chunk8<THROUGH>(a, clip, reinterpret_cast<bf16_t*>(p) + c.begin, reinterpret_cast<const bf16_t*>(g) + c.begin, state,
+    step_chunk8<THROUGH, TINY>(a, clip, reinterpret_cast<bf16_t*>(p) + c.begin, reinterpret_cast<const bf16_t*>(g) + c.begin, state,
                          position, c.n);
   else
-    step_chunk8<THROUGH>(a, clip, reinterpret_cast<float*>(p) + c.begin, reinterpret_cast<const float*>(g) + c.begin, state,
+    step_chunk8<THROUGH, TINY>(a, clip, reinterpret_cast<float*>(p) + c.begin, reinterpret_cast<const float*>(g) + c.begin, state,
                          position, c.n);
 }
 
@@ -584,7 +592,7 @@ int sdm_rt_adamw(const sdm_rt_adamw_options* o, const sdm_rt_tensor* tensors, in
   }
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (o->t_device) hipLaunchKernelGGL(count_step_kernel, dim3(1), dim3(1), 0, st, o->t_device);
-  auto launch32 = [&](auto device, auto through) {
+  auto launch32 = [&](auto device, auto through, auto tiny) {
     constexpr int kChunk = 1024;   // 110 M float32 values 476 us, 466 with 2,048, 480 with 4,096; 285 M bfloat16 1,040, 1,075, 1,167
     for_tables<StepTable32>(
         tensors, count, kChunk,
@@ -595,11 +603,11 @@ int sdm_rt_adamw(const sdm_rt_adamw_options* o, const sdm_rt_tensor* tensors, in
           at[3] = static_cast<char*>(t.exp_avg_sq);
         },
         [&](const StepTable32& table, unsigned chunks, int64_t) {
-          hipLaunchKernelGGL((adamw32_kernel<kChunk, decltype(device)::value, decltype(through)::value>), dim3(chunks),
-                             dim3(kStepThreads), 0, st, table, a);
+          hipLaunchKernelGGL((adamw32_kernel<kChunk, decltype(device)::value, decltype(through)::value, decltype(tiny)::value>),
+                             dim3(chunks), dim3(kStepThreads), 0, st, table, a);
         });
   };
-  auto launch8 = [&](auto chunk, auto device, auto through) {
+  auto launch8 = [&](auto chunk, auto device, auto through, auto tiny) {
     constexpr int kChunk = decltype(chunk)::value;
     for_tables<StepTable8>(
         tensors, count, kChunk,
@@ -609,23 +617,29 @@ int sdm_rt_adamw(const sdm_rt_adamw_options* o, const sdm_rt_tensor* tensors, in
           at[2] = static_cast<char*>(t.exp_avg);
         },
         [&](const StepTable8& table, unsigned chunks, int64_t) {
-          hipLaunchKernelGGL((adamw8_kernel<kChunk, decltype(device)::value, decltype(through)::value>), dim3(chunks),
-                             dim3(kStepThreads), 0, st, table, a);
+          hipLaunchKernelGGL((adamw8_kernel<kChunk, decltype(device)::value, decltype(through)::value, decltype(tiny)::value>),
+                             dim3(chunks), dim3(kStepThreads), 0, st, table, a);
         });
   };
-  auto with_bits = [&](auto device, auto through) {
+  auto with_bits = [&](auto device, auto through, auto tiny) {
     if (o->state_bits == 32)
-      launch32(device, through);
+      launch32(device, through, tiny);
     else if (values <= kSmallStep)
-      launch8(std::integral_constant<int, 2048>{}, device, through);
+      launch8(std::integral_constant<int, 2048>{}, device, through, tiny);
     else
-      launch8(std::integral_constant<int, 4096>{}, device, through);
+      launch8(std::integral_constant<int, 4096>{}, device, through, tiny);
+  };
+  auto with_eps = [&](auto device, auto through) {
+    if (o->eps * std::sqrt(1.0 - o->beta2) < 1.82e-12)   // 2^-39: step_value; 1 / sqrt(1 - beta2^t) is largest in the first step
+      with_bits(device, through, std::true_type{});
+    else
+      with_bits(device, through, std::false_type{});
   };
   auto with_device = [&](auto through) {
     if (o->t_device)
-      with_bits(std::true_type{}, through);
+      with_eps(std::true_type{}, through);
     else
-      with_bits(std::false_type{}, through);
+      with_eps(std::false_type{}, through);
   };
   if (bytes > kStreamBytes)
     with_device(std::true_type{});

@@ -319,6 +319,33 @@ def test_non_finite_gradients():
     assert p.isnan().cpu().tolist() == [False, True, False, False]   # 1 / inf: the others' gradients are 0
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("eps", [0.0, 1e-38, 1e-30, 1e-15, 1e-12, 1e-8, 1e3])
+def test_gradients_and_eps_of_every_size(bits, eps):
+    """One value alone in its block, from 1e-38 (v underflows: as the formula does in float32) to 1e18: the parameter is the formula's
+    from float32 moments to the roundings of a root, a quotient and their products (16 U of the move)."""
+    for e in range(-38, 19, 2):
+        g = torch.zeros(4 * 128)
+        g[::128] = torch.tensor([1.0, -1.3, 1.7, 2.0]) * 10.0 ** e
+        p = torch.randn(g.shape, generator=torch.Generator().manual_seed(e + 50))
+        f = np.float32
+        m, v = g.numpy() * f(1 - 0.9), g.numpy() * g.numpy() * f(1 - 0.999)
+        for device in (False, True):
+            q = p.cuda()
+            st = ([torch.zeros_like(q)], [torch.zeros_like(q)]) if bits == 32 else ([core.new_moments(q)],)
+            core.adamw([q], [g.cuda()], *st, step=torch.zeros((), dtype=torch.int64, device="cuda") if device else 1,
+                       **dict(HYPER, eps=eps))
+            with np.errstate(invalid="ignore", divide="ignore"):
+                move = HYPER["lr"] / (1 - 0.9) * (m.astype(np.float64) / (np.sqrt(v.astype(np.float64) / (1 - 0.999)) + eps))
+            old = p.numpy().astype(np.float64)
+            want = old * (1 - HYPER["lr"] * HYPER["weight_decay"]) - move
+            got = q.cpu().numpy().astype(np.float64)
+            with np.errstate(invalid="ignore"):
+                near = np.abs(got - want) <= 3 * U * np.abs(old) + 16 * U * np.abs(move)
+            same = (np.isnan(got) & np.isnan(want)) | (got == want)   # 0 / 0 and m / 0
+            assert (near | same).all(), (e, device, got[::128], want[::128])
+
+
 @pytest.mark.parametrize("dtype,patterns", [(torch.float32, [0x7fc00000, 0xffc00000, 0x7f800001, 0x7fffffff, 0xffffffff, 0xfff00001]),
                                             (torch.bfloat16, [0x7fc0, 0xffc0, 0x7f81, 0x7fff, 0xffff, 0xfff0])])
 def test_nan_of_any_bits(dtype, patterns):
