@@ -587,8 +587,8 @@ int sdm_rt_token_logprobs_grad(const sdm_rt_logprob* dims, const void* logits, i
                                void* d_logits, int64_t d_logits_row_stride, void* stream);
 
 /* A tensor of a training step: n values of dtype at each of param and grad, dense and in the same order, any alignment of an
- * element, at most 2^33 values in one call.  exp_avg, exp_avg_sq: float32 [n] each; or exp_avg the 8-bit moments of sdm_rt_moments_bytes(n) bytes, 8-byte
- * aligned, and exp_avg_sq NULL.  All fields are 64 bits wide. */
+ * element, at most 2^33 values in one call.  exp_avg, exp_avg_sq: float32 [n] each; or exp_avg the 8-bit moments of
+ * sdm_rt_moments_bytes(n) bytes, 8-byte aligned, and exp_avg_sq NULL.  All fields are 64 bits wide. */
 typedef struct {
   void* param;
   const void* grad;
@@ -618,7 +618,7 @@ int sdm_rt_grad_norm(const sdm_rt_tensor* tensors, int32_t count, float* norm, v
  * mantissa, of v 5 and 3: value = 2^(E - 127) (1 + f / 8) 2^(e - 15), of v 2^(e - 31), and with e = 0 that of e = 1 without
  * the 1.  A new value between two codes takes the upper one with the probability that its place between them says, by a hash
  * of its position in the list of tensors, seed and t; a v above 0 has no code 0.  A block with a value that is not finite (or
- * from 2^127 on) reads as NaN. */
+ * from 2^127 on) reads as NaN, one with none from 2^-126 on as 0 (their roots are below 1.1e-19: eps should be above). */
 typedef struct {
   double lr, beta1, beta2, eps, weight_decay;
   int64_t t;             /* the step's number, from 1 on; ignored with t_device */
