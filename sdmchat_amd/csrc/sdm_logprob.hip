@@ -99,7 +99,7 @@ struct RowLds {
   int count[16];
   uint32_t threshold;
   float log;
-  int n, n_hot;
+  int n, n_hot, n_kept;
   uint16_t hot[1024];   // threads with a logit at or above the threshold
 };
 
@@ -474,10 +474,10 @@ __global__ void __launch_bounds__(1024, 8) logprob_kernel(LogprobArgs a, int sli
     if (found > 2 * a.k + 64) {
       if (wave == 0) {
         const int kept = narrowed(lds_.keys, found, a.k);
-        if (lane == 0) lds_.n = kept;
+        if (lane == 0) lds_.n_kept = kept;   // not n, which other waves may be about to read: this branch hangs on it
       }
       __syncthreads();
-      found = lds_.n;
+      found = lds_.n_kept;
     }
     // each key's place among them: how many are greater, counted by four lanes
     const float log = lds_.log;
