@@ -1289,7 +1289,10 @@ def _ids(name, what, t):
 
 def _read_rows(t2):
     """(rows, row stride in elements) of a 2-D tensor as the kernels that read any row stride and any element alignment
-    take it: itself where the last dimension is contiguous, else a copy."""
+    take it: itself where the last dimension is contiguous, else a copy (of a lazily negated one too: the kernels read
+    memory)."""
+    if t2.is_neg():
+        t2 = t2.resolve_neg()
     if t2.is_contiguous():
         return t2, t2.size(1)
     rows, width = t2.shape
@@ -1775,6 +1778,7 @@ class LogprobFunction(torch.autograd.Function):
         z, targets, stats = ctx.saved_tensors
         if dlp is None and dh is None:
             return None, None, None, None
+        dlp, dh = (g if g is None or not g.is_neg() else g.resolve_neg() for g in (dlp, dh))   # as a conjugation leaves them
         dz = z.new_empty(z.shape)
         z, zs = _read_rows(z)
         _launch(_lib.load().sdm_rt_token_logprobs_grad, z.get_device(), ctypes.byref(ctx.dims), z.data_ptr(), zs, _DT[z.dtype],
@@ -1922,6 +1926,13 @@ def grad_norm(tensors):
     return out
 
 
+def _check_written(name, **tensors):
+    """Kernels write memory: a lazily negated tensor would have the values with the other sign."""
+    for what, t in tensors.items():
+        if t.is_neg():
+            raise ValueError(f"{name}: one of the {what} is lazily negated (Tensor.resolve_neg makes it plain)")
+
+
 def _check_moments8(name, m, n):
     """8-bit moments (new_moments) of n values."""
     want = (-(-n // MOMENT_BLOCK), MOMENT_BYTES)
@@ -1941,6 +1952,7 @@ def _pack_step(name, ps, gs, ms, vs):
             raise ValueError(f"{name}: a grad of {g.dtype} {tuple(g.shape)} for a param of {p.dtype} {tuple(p.shape)}")
         if not _dense(p):
             raise ValueError(f"{name}: a param {tuple(p.shape)} of strides {tuple(p.stride())}: its values must be dense")
+        g = g.resolve_neg()
         if not (p.is_contiguous() and g.is_contiguous()) and g.stride() != p.stride():
             g = torch.empty_like(p).copy_(g)   # the grad in the order of the param's values
         held.append(g)
@@ -1954,6 +1966,7 @@ def _pack_step(name, ps, gs, ms, vs):
                         t.stride() == p.stride() or (t.is_contiguous() and p.is_contiguous())):
                     raise ValueError(f"{name}: moments must be float32 {tuple(p.shape)} of the param's strides "
                                      f"{tuple(p.stride())}, got {t.dtype} {tuple(t.shape)} of {tuple(t.stride())}")
+        _check_written(name, params=p, **dict(zip(("exp_avgs", "exp_avg_sqs"), moments)))
         at = [t.data_ptr() for t in moments] + [0]
         rows.append((p.data_ptr(), g.data_ptr(), at[0], at[1], p.numel(), _code(name, "params", p)))
         spans += [(t.data_ptr(), t.numel() * t.element_size(), t is not g) for t in (p, g, *moments)]
@@ -1995,7 +2008,7 @@ def adamw(params, grads, exp_avgs, exp_avg_sqs=None, *, step, lr=1e-3, betas=(0.
     if type(lr) is not float and torch.is_tensor(lr):
         if lr.dtype != torch.float32 or lr.numel() != 1 or lr.get_device() != index or t_dev is None:
             raise ValueError(f"{name}: an lr on the device must be float32 with one element on {ps[0].device}, beside a step there")
-        lr_dev, lr = lr, 0.0
+        lr_dev, lr = lr.resolve_neg(), 0.0
     if max_norm is None:
         if norm is not None:
             raise ValueError(f"{name}: norm needs max_norm")
@@ -2003,6 +2016,8 @@ def adamw(params, grads, exp_avgs, exp_avg_sqs=None, *, step, lr=1e-3, betas=(0.
         norm = grad_norm(gs)
     elif norm.dtype != torch.float32 or norm.numel() != 1 or norm.get_device() != index:
         raise ValueError(f"{name}: norm must be float32 with one element on {ps[0].device}")
+    else:
+        norm = norm.resolve_neg()
     options = _lib.SdmRtAdamwOptions(lr, betas[0], betas[1], eps, weight_decay, step, _ptr(t_dev), _ptr(lr_dev), _ptr(norm),
                                      1.0 if max_norm is None else max_norm, 8 if eight else 32, seed & 0xffffffff)
     _launch(_lib.load().sdm_rt_adamw, index, ctypes.byref(options), table, len(ps))
@@ -2027,6 +2042,7 @@ def read_moments(moments, exp_avgs, exp_avg_sqs):
             if v.numel() != m.numel() or v.dtype != m.dtype or not m.is_contiguous() or not v.is_contiguous():
                 raise ValueError(f"{name}: exp_avgs and exp_avg_sqs must be contiguous and alike in size and dtype")
             _check_moments8(name, s, m.numel())
+            _check_written(name, exp_avgs=m, exp_avg_sqs=v)
             rows.append((m.data_ptr(), 0, s.data_ptr(), v.data_ptr(), m.numel(), _code(name, "exp_avgs", m)))
             spans += [(t.data_ptr(), t.numel() * t.element_size(), t is not s) for t in (s, m, v)]
         _check_apart(name, spans)
