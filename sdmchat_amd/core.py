@@ -62,9 +62,9 @@ def _rows16(t2):
 
 def _own_rows(t2):
     """A 2-D view as rows that the kernels take: itself where the rows are 16-byte aligned (_rows16) and do not overlap (a
-    row broadcast over many has stride 0), else a copy."""
+    row broadcast over many has stride 0), else a copy (of a lazily negated one too: the kernels read memory)."""
     row, step = t2.stride()
-    if step == 1 and row >= t2.shape[1] and row * t2.element_size() % 16 == 0 and t2.data_ptr() % 16 == 0:
+    if not t2.is_neg() and step == 1 and row >= t2.shape[1] and row * t2.element_size() % 16 == 0 and t2.data_ptr() % 16 == 0:
         return t2
     return t2.clone(memory_format=torch.contiguous_format)
 
@@ -72,7 +72,7 @@ def _own_rows(t2):
 def _f32(t, device):
     if t is None:
         return None
-    return t.detach().to(device=device, dtype=torch.float32).contiguous()
+    return t.detach().to(device=device, dtype=torch.float32).contiguous().resolve_neg()
 
 
 def _bytes(reset, device):
@@ -88,6 +88,8 @@ def _rows(x, name, B, T, width):
         raise ValueError(f"{name}: expected [B={B}, T={T}, >={width}], got {tuple(x.shape)}")
     if x.dtype not in _DT:
         raise ValueError(f"{name}: dtype {x.dtype} is not float32 or bfloat16")
+    if x.is_neg():
+        raise ValueError(f"{name}: lazily negated (Tensor.resolve_neg makes it plain)")
     if x.numel() == 0:
         return width
     if x.stride(2) != 1:
@@ -976,6 +978,7 @@ def core_backward(kz, qz, v, gate_logits, saved, dy, *, params, k, read_mode="me
     gs = 0 if gate_logits is None else _rows(gate_logits, "gate_logits", B, T, H)
     if dy.dtype not in _DT:
         dy = dy.float()
+    dy = dy.resolve_neg()
     if dy.dim() != 3 or dy.stride(2) != 1:
         dy = dy.contiguous()
     dys = _rows(dy, "dy", B, T, H * dh)
@@ -1190,6 +1193,7 @@ def table_backward(q, slots, weights, scores, values, dy, *, k, params, workspac
     qs = _rows(q, "q", B, T, H * d_a)
     if dy.dtype not in _DT:
         dy = dy.float()
+    dy = dy.resolve_neg()
     if dy.dim() != 3 or dy.stride(2) != 1:
         dy = dy.contiguous()
     dys = _rows(dy, "dy", B, T, H * dh)
@@ -1400,7 +1404,7 @@ def embedding_backward(idx, dy, vocab, scale=1.0, padding_idx=None):
 
 
 def _embed_backward(ids, dy, vocab, d, scale, pad):
-    if dy.is_contiguous():
+    if dy.is_contiguous() and not dy.is_neg():
         stride = d
     else:
         dy, stride = _read_rows(dy if dy.dim() == 2 else dy.reshape(-1, d))
@@ -1530,7 +1534,7 @@ class DistillFunction(torch.autograd.Function):
         else:
             dz = z.new_empty(z.shape)
         z, zs = _read_rows(z)
-        g = dloss.contiguous()
+        g = dloss.contiguous().resolve_neg()
         _launch(lib.sdm_rt_distill_grad, z.get_device(), at, z.data_ptr(), zs, code, ids.data_ptr(), k, top.data_ptr(),
                 k, _ptr(labels), stats.data_ptr(), g.data_ptr(), unless_one, dz.data_ptr(), V)
         return dz, None, None, None, None
@@ -1580,8 +1584,8 @@ def distill_loss(logits, top_ids, top_logits, *, temperature=1.0, labels=None, a
         _widths("distill_loss", vocab=V, k=k)
     ids = _ids("distill_loss", "top_ids", top_ids)
     top = top_logits.detach() if top_logits.requires_grad else top_logits
-    if top.dtype != torch.float32 or not top.is_contiguous():
-        top = top.to(torch.float32).contiguous()
+    if top.dtype != torch.float32 or not top.is_contiguous() or top.is_neg():
+        top = top.to(torch.float32).contiguous().resolve_neg()
     lab = None if labels is None else _ids("distill_loss", "labels", labels)
     n = lead.numel()
     dims = _lib.SdmRtDistill(n, V, k, temperature, alpha, ignore_index, _REDUCTION[reduction])
@@ -1603,6 +1607,7 @@ def _per_row(name, what, v, B, device):
         raise ValueError(f"{name}: {what} must be a number or a floating-point tensor [B={B}], got {v.dtype} {tuple(v.shape)}")
     if v.device != device:
         raise ValueError(f"{name}: {what} is on {v.device}, expected {device}")
+    v = v.resolve_neg()
     if v.dtype == torch.float32 and v.dim() == 1 and v.shape[0] == B and v.is_contiguous():
         return v, 0.0
     return v.detach().to(torch.float32).reshape(-1).expand(B).contiguous(), 0.0
@@ -1613,7 +1618,7 @@ def _row_or_rows(name, what, t, B, width, dtype):
     shape = t.shape
     if t.dtype != dtype or shape[-1:] != (width,) or len(shape) > 2 or (len(shape) == 2 and shape[0] != B):
         raise ValueError(f"{name}: {what} must be {dtype} [{width}] or [B={B}, {width}], got {t.dtype} {tuple(shape)}")
-    return (t.contiguous(), 0) if len(shape) == 1 else _read_rows(t)
+    return (t.contiguous().resolve_neg(), 0) if len(shape) == 1 else _read_rows(t)
 
 
 def pack_mask(allowed):
@@ -1700,8 +1705,8 @@ def process_logits(logits, tokens=None, lengths=None, *, prompt=None, repetition
     if out is None:
         out = torch.empty(B, V, dtype=logits.dtype, device=dev)
     elif tuple(out.shape) != (B, V) or out.dtype != logits.dtype or (V > 1 and out.stride(1) != 1) or (
-            B > 1 and out.stride(0) < V):
-        raise ValueError(f"{name}: out must be {logits.dtype} [B={B}, {V}] with contiguous rows")
+            B > 1 and out.stride(0) < V) or out.is_neg():
+        raise ValueError(f"{name}: out must be {logits.dtype} [B={B}, {V}] with contiguous rows, not lazily negated")
     elif src.data_ptr() == logits.data_ptr() and not _apart(logits, out):
         raise ValueError(f"{name}: out overlaps logits in part")
     _launch(_lib.load().sdm_rt_process_logits, out.get_device(), ctypes.byref(rules), src.data_ptr(), ls, _DT[logits.dtype],

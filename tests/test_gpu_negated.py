@@ -110,3 +110,55 @@ def test_what_would_be_written_is_refused():
         with pytest.raises(ValueError, match="negated"):
             call()
     assert not s.any()
+
+
+def test_losses_and_embeddings():
+    """The operators on token ids and vocabulary rows."""
+    g = torch.Generator().manual_seed(1)
+    table, dy = torch.randn(50, 16, generator=g).cuda(), torch.randn(7, 16, generator=g).cuda()
+    idx = torch.randint(0, 50, (7,), generator=g).cuda()
+    logits, ids, top = torch.randn(7, 50, generator=g).cuda(), torch.arange(21).view(7, 3).cuda(), torch.randn(7, 3, generator=g).cuda()
+    bias = torch.randn(50, generator=g).cuda()
+    for wrap in (negated, dense_negated):
+        assert torch.equal(core.embedding(idx, wrap(table)), core.embedding(idx, table))
+        assert torch.equal(core.embedding_backward(idx, wrap(dy), 50), core.embedding_backward(idx, dy, 50))
+        assert torch.equal(core.distill_loss(wrap(logits), ids, wrap(top)), core.distill_loss(logits, ids, top))
+        assert torch.equal(core.process_logits(wrap(logits), bias=wrap(bias)), core.process_logits(logits, bias=bias))
+        grads = []
+        for w in (lambda t: t, wrap):
+            for reduction in ("mean", "none"):
+                x = logits.clone().requires_grad_(True)
+                loss = core.distill_loss(x, ids, top, reduction=reduction)
+                grads.append(torch.autograd.grad(loss, x, w(torch.full(loss.shape, 0.7, device="cuda")))[0])
+        assert torch.equal(grads[0], grads[2]) and torch.equal(grads[1], grads[3])
+        with pytest.raises(ValueError, match="negated"):
+            core.process_logits(logits, bias=bias, out=dense_negated(logits.clone()))
+
+
+@pytest.mark.parametrize("wrap", [negated, dense_negated])
+def test_norms_mixers_and_tables(wrap):
+    """Their inputs and the gradients that come into them."""
+    g = torch.Generator().manual_seed(2)
+    x, w, dy = torch.randn(2, 5, 64, generator=g).cuda(), torch.rand(64, generator=g).cuda(), torch.randn(2, 5, 64, generator=g).cuda()
+    assert torch.equal(core.rms_norm(wrap(x), w), core.rms_norm(x, w))
+    assert all(torch.equal(a, b) for a, b in zip(core.rms_norm_backward(wrap(x), w, wrap(dy), 1e-6),
+                                                 core.rms_norm_backward(x, w, dy, 1e-6)))
+    H, dh, d_a, n = 2, 32, 16, 8
+    kz, qz = (torch.randn(2, 5, H * d_a, generator=g).cuda() for _ in range(2))
+    v, gate = torch.randn(2, 5, H * dh, generator=g).cuda(), torch.randn(2, 5, H, generator=g).cuda()
+    k1, k2 = (torch.randn(H, n, d_a // 2, generator=g).cuda() for _ in range(2))
+    scale, decay = torch.full((H,), 2.0).cuda(), torch.full((H,), 0.9).cuda()
+    cfg = dict(k=4, read_mode="mean", out_norm=False, read_eps=1e-3, out_norm_eps=1e-2)
+    table = torch.randn(H, n * n, dh, generator=g).cuda()
+    grads = []
+    for wr in (lambda t: t, wrap):
+        ins = [t.clone().requires_grad_(True) for t in (kz, qz, v, gate, k1, k2)]
+        r = core.SdmCoreFunction.apply(*ins, None, scale, decay, None, None, dict(cfg))
+        one = torch.autograd.grad(r, ins, wr(dy))
+        ins = [t.clone().requires_grad_(True) for t in (qz, k1, k2, scale, table)]
+        r = core.TableSdmFunction.apply(*ins, dict(k=4))
+        grads.append(one + torch.autograd.grad(r, ins, wr(dy)))
+    assert all(torch.equal(a, b) for a, b in zip(*grads))
+    with pytest.raises(ValueError, match="negated"):
+        core.core_forward(wrap(kz) if wrap is dense_negated else dense_negated(kz), qz, v, gate, keys1=k1, keys2=k2, log_scale=scale,
+                          decay=decay, out_norm=False, k=4)
