@@ -8,6 +8,11 @@ import torch
 
 from . import core
 
+# A call's seed is its group's plus this (from the square root of 3) times the place of its first parameter in the optimiser.  The
+# library adds t times another odd number (from the golden ratio) before it hashes: of places under 2,341 apart two steps meet the
+# same sum only 1.7 million steps apart (of places under 36,672, 110,000), so no two calls of a run round by the same bits.
+_CALL = 3144134277
+
 
 class AdamW(torch.optim.Optimizer):
     """AdamW on float32 or bfloat16 parameters of one or more GPUs.
@@ -111,7 +116,7 @@ class AdamW(torch.optim.Optimizer):
         max_norm, self.norm = self.defaults["max_norm"], None
         if max_norm is not None and any(live for _, live in groups):
             self.norm = core.grad_norm([p.grad for _, live in groups for p in live])
-        calls = 0
+        before = 0   # parameters of the groups before
         for group, live in groups:
             for step, members in self._clocks(group, live, capturing):
                 ps = [p for p, _ in members]
@@ -120,14 +125,15 @@ class AdamW(torch.optim.Optimizer):
                 else:
                     moments = [[st["exp_avg"] for _, st in members], [st["exp_avg_sq"] for _, st in members]]
                 on_device = torch.is_tensor(step)
-                # a call's positions begin at 0: each has a seed of its own
+                # a call's positions begin at 0: each has a seed of its own, whatever else takes part in the step
+                place = before + next(i for i, p in enumerate(group["params"]) if p is ps[0])
                 core.adamw(ps, [p.grad for p in ps], *moments, step=step if on_device else step + 1, lr=group["lr"],
                            betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"], max_norm=max_norm,
-                           norm=self.norm, seed=group["seed"] + 0x9E3779B1 * calls)
-                calls += 1
+                           norm=self.norm, seed=group["seed"] + _CALL * place)
                 if not on_device:
                     for _, st in members:
                         st["step"] = step + 1
+            before += len(group["params"])
         return loss
 
     def load_state_dict(self, state_dict):
