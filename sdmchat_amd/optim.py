@@ -39,7 +39,13 @@ class AdamW(torch.optim.Optimizer):
 
     def add_param_group(self, param_group):
         super().add_param_group(param_group)
-        group = self.param_groups[-1]
+        try:
+            self._check_group(self.param_groups[-1])
+        except Exception:
+            self.param_groups.pop()   # a refused group is none of the optimiser's
+            raise
+
+    def _check_group(self, group):
         lr, betas = group["lr"], group["betas"]
         if torch.is_tensor(lr) and not group["capturable"]:
             raise ValueError("AdamW: an lr on the device needs capturable")

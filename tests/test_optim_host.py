@@ -73,3 +73,22 @@ def test_seeds_do_not_hang_on_what_else_steps(calls):
     step(opt, ps[1:])
     first, second, alone = calls
     assert first[2] == 11 and second[0][0] is alone[0][0] is ps[1] and second[2] == alone[2] != 11
+
+
+@pytest.mark.parametrize("over", [dict(betas=(0.9, 1.5)), dict(betas=0.9), dict(lr=-1.0), dict(eps=-1.0), dict(weight_decay=-0.1),
+                                  dict(state_bits=4), dict(max_norm=2.0), dict(lr=torch.ones(())), dict(capturable=True)])
+def test_a_refused_group_is_not_kept(calls, over):
+    a, b = params(3, 4)
+    opt = AdamW([a], lr=1e-3)
+    with pytest.raises((ValueError, TypeError)):
+        opt.add_param_group(dict(dict(params=[b]), **over))
+    with pytest.raises(ValueError, match="float64"):
+        opt.add_param_group(dict(params=[torch.nn.Parameter(torch.zeros(3, dtype=torch.float64))]))
+    with pytest.raises(ValueError):
+        opt.add_param_group(dict(params=[a]))   # torch's own refusal
+    assert [g["params"] for g in opt.param_groups] == [[a]]
+    step(opt, [a, b])
+    assert [c[0] for c in calls] == [[a]]
+    opt.add_param_group(dict(params=[b], lr=1e-2))   # a refusal does not spoil the parameter
+    step(opt, [a, b])
+    assert [c[0] for c in calls] == [[a], [a], [b]]
