@@ -31,6 +31,7 @@ class AdamW(torch.optim.Optimizer):
     that matters.  Sparse gradients and parameters whose values are not dense in memory are refused."""
 
     norm = None   # of the last step's gradients
+    _OPTIONS = {"lr", "betas", "eps", "weight_decay", "state_bits", "max_norm", "capturable", "seed"}   # of a parameter group
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, *, state_bits=32, max_norm=None,
                  capturable=False, seed=0):
@@ -144,7 +145,7 @@ class AdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict):
         """As torch's, but for the moments' types, which stay what they are: float32, or the bytes of 8-bit moments."""
-        if any(not g.keys() >= self.defaults.keys() for g in state_dict["param_groups"]):
+        if any(not g.keys() >= self._OPTIONS for g in state_dict["param_groups"]):
             raise ValueError("AdamW.load_state_dict: not the state of this optimiser")
         old = [p for g in state_dict["param_groups"] for p in g["params"]]
         new = [p for g in self.param_groups for p in g["params"]]

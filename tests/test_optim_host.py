@@ -1,5 +1,8 @@
 """The AdamW optimiser's own work on the CPU, with core.adamw replaced by a record of its calls: the seeds of the calls' rounding,
 parameter groups that are refused, states that are loaded."""
+import copy
+import pickle
+
 import numpy as np
 import pytest
 import torch
@@ -92,3 +95,17 @@ def test_a_refused_group_is_not_kept(calls, over):
     opt.add_param_group(dict(params=[b], lr=1e-2))   # a refusal does not spoil the parameter
     step(opt, [a, b])
     assert [c[0] for c in calls] == [[a], [a], [b]]
+
+
+@pytest.mark.parametrize("capturable", [False, True])
+def test_states_are_loaded_again(calls, capturable):
+    """A second state after a first, and one into a copy of the optimiser: torch adds options of its own to those that a loaded or
+    copied optimiser has, which no state of this one holds."""
+    ps = params(300, 200)
+    opt = AdamW(ps, lr=1e-3, state_bits=8, capturable=capturable)
+    step(opt, ps)
+    first = opt.state_dict()
+    for other in (opt, copy.deepcopy(opt), pickle.loads(pickle.dumps(opt))):
+        for _ in range(2):
+            other.load_state_dict(first)
+        assert [int(st["step"]) for st in other.state.values()] == [1, 1]
