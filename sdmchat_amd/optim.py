@@ -144,41 +144,68 @@ class AdamW(torch.optim.Optimizer):
         return loss
 
     def load_state_dict(self, state_dict):
-        """As torch's, but for the moments' types, which stay what they are: float32, or the bytes of 8-bit moments."""
-        if any(not g.keys() >= self._OPTIONS for g in state_dict["param_groups"]):
-            raise ValueError("AdamW.load_state_dict: not the state of this optimiser")
-        old = [p for g in state_dict["param_groups"] for p in g["params"]]
-        new = [p for g in self.param_groups for p in g["params"]]
-        bits = [g["state_bits"] for g in state_dict["param_groups"] for _ in g["params"]]
-        for key, p, b in zip(old, new, bits):   # before anything changes
-            st = state_dict["state"].get(key)
+        """As torch's, but for the moments' types, which stay what they are (float32, or the bytes of 8-bit moments), and an lr
+        that is a tensor here: it stays, and takes the loaded value.  The moments and counts are new tensors: a graph that
+        captured a step holds the old ones.  What is refused changes nothing."""
+        mine, loaded = [g["lr"] for g in self.param_groups], {}
+
+        def check(_, state_dict):   # after the hooks before
+            loaded.update(self._loaded_state(state_dict))
+            return dict(state_dict, state={})
+
+        def fill(_):   # before the hooks after
+            self.state.update(loaded)
+            for group, lr in zip(self.param_groups, mine):
+                if torch.is_tensor(lr):
+                    lr.detach().fill_(float(group["lr"]))
+                    group["lr"] = lr
+                elif torch.is_tensor(group["lr"]) and group["params"]:
+                    group["lr"] = group["lr"].to(group["params"][0].device)
+        hooks = [self.register_load_state_dict_pre_hook(check), self.register_load_state_dict_post_hook(fill, prepend=True)]
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            for hook in hooks:
+                hook.remove()
+
+    def _loaded_state(self, state_dict):
+        """The state that a state dict holds, {parameter: its own copies}; ValueError for what is not this optimiser's kind."""
+        name, on_device = "AdamW.load_state_dict", self.defaults["capturable"]
+        groups = state_dict["param_groups"]
+        if any(not g.keys() >= self._OPTIONS for g in groups):
+            raise ValueError(f"{name}: not the state of this optimiser")
+        if [len(g["params"]) for g in groups] != [len(g["params"]) for g in self.param_groups]:
+            raise ValueError(f"{name}: parameter groups of other sizes")
+        if any(g["max_norm"] != self.defaults["max_norm"] or g["capturable"] != on_device for g in groups):
+            raise ValueError(f"{name}: max_norm and capturable must be the optimiser's own")
+        if any(torch.is_tensor(g["lr"]) and g["lr"].numel() != 1 for g in groups):
+            raise ValueError(f"{name}: an lr of several values")
+        found = [(i, group["state_bits"], p, state_dict["state"].get(key)) for i, (group, own) in enumerate(
+            zip(groups, self.param_groups)) for key, p in zip(group["params"], own["params"])]
+        for _, bits, p, st in found:
             if not st:
                 continue
-            want = {"moments": ((-(-p.numel() // core.MOMENT_BLOCK), core.MOMENT_BYTES), torch.uint8)} if b == 8 else {
+            want = {"moments": ((-(-p.numel() // core.MOMENT_BLOCK), core.MOMENT_BYTES), torch.uint8)} if bits == 8 else {
                 "exp_avg": (tuple(p.shape), torch.float32), "exp_avg_sq": (tuple(p.shape), torch.float32)}
-            if {k: (tuple(v.shape), v.dtype) for k, v in st.items() if k != "step"} != want:
-                raise ValueError(f"AdamW.load_state_dict: the state of a parameter {tuple(p.shape)} is not {want}")
-        if any(g["max_norm"] != self.defaults["max_norm"] or g["capturable"] != self.defaults["capturable"]
-               for g in state_dict["param_groups"]):
-            raise ValueError("AdamW.load_state_dict: max_norm and capturable must be the optimiser's own")
-        super().load_state_dict({"state": {}, "param_groups": state_dict["param_groups"]})
-        self.state.clear()
-        clocks = {}
-        for key, p in zip(old, new):
-            st = state_dict["state"].get(key)
+            if {k: (tuple(v.shape), v.dtype) if torch.is_tensor(v) else v for k, v in st.items() if k != "step"} != want:
+                raise ValueError(f"{name}: the state of a parameter {tuple(p.shape)} is not {want}")
+            step = st.get("step")
+            if not (isinstance(step, int) or (torch.is_tensor(step) and step.numel() == 1)) or step < 0:
+                raise ValueError(f"{name}: a parameter's step must be a whole number from 0 on, got {step}")
+        state, clocks = {}, {}
+        for i, _, p, st in found:
             if not st:
                 continue
             count = int(st["step"])
-            if self.defaults["capturable"]:
-                group = next(i for i, g in enumerate(self.param_groups) if any(q is p for q in g["params"]))
-                at = (group, count, p.device)
+            if on_device:
+                at = (i, count, p.device)
                 if at not in clocks:
                     clocks[at] = torch.full((), count, dtype=torch.int64, device=p.device)
                 count = clocks[at]
-            mine = {"step": count}
+            state[p] = {"step": count}
             for k, v in st.items():
                 if k == "moments":
-                    mine[k] = v.detach().to(p.device, copy=True).contiguous()
+                    state[p][k] = v.detach().to(p.device, copy=True).contiguous()
                 elif k != "step":
-                    mine[k] = torch.empty_like(p, dtype=torch.float32, requires_grad=False).copy_(v.detach())
-            self.state[p] = mine
+                    state[p][k] = torch.empty_like(p, dtype=torch.float32, requires_grad=False).copy_(v.detach())
+        return state

@@ -109,3 +109,103 @@ def test_states_are_loaded_again(calls, capturable):
         for _ in range(2):
             other.load_state_dict(first)
         assert [int(st["step"]) for st in other.state.values()] == [1, 1]
+
+
+def trained(bits, capturable, lr):
+    ps = params(300, 200)
+    opt = AdamW([dict(params=ps[:1]), dict(params=ps[1:])], lr=lr, state_bits=bits, capturable=capturable)
+    step(opt, ps)
+    step(opt, ps[:1])
+    for st in opt.state.values():
+        for k, v in st.items():
+            if k != "step":
+                v.fill_(3)
+    return ps, opt
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("mine", ["number", "tensor", "row"])
+@pytest.mark.parametrize("loaded", ["number", "tensor", "row"])
+def test_a_rate_that_is_a_tensor_is_loaded_into(calls, bits, mine, loaded):
+    """The tensor that a schedule writes and a graph holds stays the group's and takes the loaded value; a number becomes a copy
+    of a loaded tensor."""
+    def rate(kind, value):
+        return value if kind == "number" else torch.full(() if kind == "tensor" else (1,), value)
+    _, old = trained(bits, True, rate(loaded, 0.25))
+    lr = rate(mine, 0.5)
+    ps, new = trained(bits, True, lr)
+    sd = old.state_dict()
+    new.load_state_dict(sd)
+    for g, s in zip(new.param_groups, sd["param_groups"]):
+        assert float(g["lr"]) == 0.25 and torch.is_tensor(g["lr"]) == (mine != "number" or loaded != "number")
+        if mine != "number":
+            assert g["lr"] is lr
+            lr.fill_(0.125)
+            assert float(s["lr"]) == 0.25   # the checkpoint's is another
+            lr.fill_(0.25)
+        elif loaded != "number":
+            assert g["lr"] is not s["lr"] and g["lr"].device == g["params"][0].device
+    step(new, ps)
+    assert float(calls[-1][3]) == 0.25
+    if mine != "number":   # its own state again
+        new.load_state_dict(new.state_dict())
+        assert all(g["lr"] is lr for g in new.param_groups) and float(lr) == 0.25
+
+
+def test_a_rate_of_several_values_is_refused(calls):
+    _, opt = trained(32, True, torch.full((), 0.5))
+    sd = opt.state_dict()
+    sd["param_groups"][1]["lr"] = torch.ones(2)
+    with pytest.raises(ValueError, match="lr"):
+        opt.load_state_dict(sd)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("capturable", [False, True])
+@pytest.mark.parametrize("what", ["no step", "step of another kind", "negative step", "no moments", "another size", "a number", "groups"])
+def test_a_refused_state_changes_nothing(calls, bits, capturable, what):
+    ps, opt = trained(bits, capturable, 0.5)
+    keep = {p: {k: v.clone() if torch.is_tensor(v) else v for k, v in st.items()} for p, st in opt.state.items()}
+    held = {p: dict(st) for p, st in opt.state.items()}
+    sd = trained(bits, capturable, 0.25)[1].state_dict()
+    sd["state"] = {k: dict(st) for k, st in sd["state"].items()}
+    key = "moments" if bits == 8 else "exp_avg"
+    if what == "no step":
+        del sd["state"][1]["step"]
+    elif what == "step of another kind":
+        sd["state"][1]["step"] = torch.ones(2) if capturable else "many"
+    elif what == "negative step":
+        sd["state"][1]["step"] = -1
+    elif what == "no moments":
+        del sd["state"][1][key]
+    elif what == "another size":
+        sd["state"][1][key] = sd["state"][1][key][:1]
+    elif what == "a number":
+        sd["state"][1][key] = 3.0
+    else:
+        sd["param_groups"] = sd["param_groups"][:1]
+    with pytest.raises(ValueError):
+        opt.load_state_dict(sd)
+    assert [g["lr"] for g in opt.param_groups] == [0.5, 0.5] and list(opt.state) == list(keep)
+    for p, st in opt.state.items():
+        assert all(held[p][k] is v for k, v in st.items())
+        assert all(torch.equal(v, keep[p][k]) if torch.is_tensor(v) else v == keep[p][k] for k, v in st.items())
+
+
+@pytest.mark.parametrize("capturable", [False, True])
+def test_hooks_of_a_loaded_state(calls, capturable):
+    """A hook before sees, and may replace, the whole state; one after finds the new state in place."""
+    _, old = trained(8, capturable, 0.25)
+    ps, new = trained(8, capturable, 0.5)
+    seen = []
+
+    def before(opt, sd):
+        seen.append(sorted(sd["state"]))
+        return dict(sd, state={k: dict(st, step=st["step"] + 5) for k, st in sd["state"].items()})
+    new.register_load_state_dict_pre_hook(before)
+    new.register_load_state_dict_post_hook(lambda opt: seen.append([int(opt.state[p]["step"]) for p in ps]))
+    new.load_state_dict(old.state_dict())
+    assert seen == [[0, 1], [7, 6]]
+    assert [int(new.state[p]["step"]) for p in ps] == [7, 6]
+    new.load_state_dict(old.state_dict())   # the optimiser's own hooks were for one call
+    assert seen[2:] == [[0, 1], [7, 6]] and len(seen) == 4
