@@ -614,11 +614,12 @@ int sdm_rt_grad_norm(const sdm_rt_tensor* tensors, int32_t count, float* norm, v
  *
  * Moments in 8 bits (state_bits 8): ceil(n / 128) blocks of 264 bytes, each the codes of 128 consecutive values of m, those
  * of v, an exponent E of each, 6 bytes unused.  2^(E - 127) is the block's largest magnitude without its mantissa (twice that
- * where the mantissa is over 1.875; E = 0: all zero).  A code of m is a sign bit, 4 bits e of exponent and 3 bits f of
+ * where the mantissa is over 1.875), at least 2^-126; E = 0: all zero, E = 255: all NaN.  A code of m is a sign bit, 4 bits e of exponent and 3 bits f of
  * mantissa, of v 5 and 3: value = 2^(E - 127) (1 + f / 8) 2^(e - 15), of v 2^(e - 31), and with e = 0 that of e = 1 without
  * the 1.  A new value between two codes takes the upper one with the probability that its place between them says, by a hash
- * of its position in the list of tensors, seed and t; a v above 0 has no code 0.  A block with a value that is not finite (or
- * from 2^127 on) reads as NaN, one with none from 2^-126 on as 0 (their roots are below 1.1e-19: eps should be above). */
+ * of its position in the list of tensors, seed and t; a v above 0 has no code 0.  A block with a value above 1.875 2^126 (an
+ * infinity or NaN among them) reads as NaN, both moments; a moment's block whose largest magnitude is at most 0.875 2^-126 as 0
+ * (of v, their roots are below 1.1e-19: eps should be above). */
 typedef struct {
   double lr, beta1, beta2, eps, weight_decay;
   int64_t t;             /* the step's number, from 1 on; ignored with t_device */

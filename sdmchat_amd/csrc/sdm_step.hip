@@ -182,8 +182,8 @@ __host__ __device__ __forceinline__ uint32_t step_key(uint32_t seed, int64_t t) 
   return mix(seed + static_cast<uint32_t>(t) * 2654435761u);
 }
 
-// the exponent of a block whose largest magnitude has these bits: 255 where it is not finite or from 2^127 on (a NaN may have
-// its sign set, and is then the greatest of the bits)
+// the exponent of a block whose largest magnitude has these bits: 255 where it is above 1.875 2^126, whose codes would be infinite,
+// or not finite (a NaN may have its sign set, and is then the greatest of the bits); 0 up to 0.875 2^-126
 __device__ __forceinline__ uint32_t block_exponent(uint32_t bits) {
   const uint32_t e = ((bits & 0x7fffffffu) + 0xfffffu) >> 23;
   return e >= 254 ? 255 : e;
