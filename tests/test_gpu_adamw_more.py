@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from sdmchat_amd import AdamW, core
-from tests.test_gpu_adamw import SIZES, mix, read, regrad, tensors
+from tests.test_gpu_adamw import HYPER, SIZES, Twin, mix, read, regrad, tensors
 
 pytestmark = pytest.mark.gpu
 
@@ -114,3 +114,31 @@ def test_the_ends_of_the_8_bit_range():
         assert np.isnan(v).all() == (i >= len(ends)), i
         for got, want in ((ms[i], m), (vs[i], v)):
             assert np.array_equal(got, want.astype(np.float32), equal_nan=True), (i, row[17])
+
+
+@pytest.mark.parametrize("full", [96, 108, 120, 191])
+@pytest.mark.parametrize("more", [-1, 0, 1])
+@pytest.mark.parametrize("copies", [1, 2])
+def test_lists_at_the_edges_of_a_launch(full, more, copies):
+    """Lists of as many tensors as a launch of the 32-bit step takes (96), of the 8-bit step (108), of read_moments (120), of the
+    norm (191), one fewer and one more, and twice that; tensors without values among them, at the ends and at the edge."""
+    count = full * copies + more
+    gen = torch.Generator().manual_seed(count)
+    sizes = [(int(n),) for n in torch.randint(1, 5000, (count,), generator=gen)]
+    for at in (0, full - 1, full, count):   # which no launch's table holds
+        sizes.insert(at, (0,))
+    ps, gs = tensors(sizes, [torch.float32, torch.bfloat16, torch.bfloat16], count)
+    want = sum(float(g.double().square().sum()) for g in gs) ** 0.5
+    assert abs(float(core.grad_norm(gs)) - want) <= 2.0 ** -24 * 1.01 * want
+    for bits in (32, 8):
+        qs = [p.clone() for p in ps]
+        twin = Twin(qs, bits, 5)
+        if bits == 32:
+            ms, vs = ([torch.zeros(p.shape, device="cuda") for p in qs] for _ in range(2))
+            core.adamw(qs, gs, ms, vs, step=1, max_norm=1.0, **HYPER)
+        else:
+            st = [core.new_moments(p) for p in qs]
+            core.adamw(qs, gs, st, step=1, max_norm=1.0, seed=5, **HYPER)
+            ms, vs = read(st, qs)
+        twin.step(gs, 1.0)
+        twin.compare(qs, ms, vs)
