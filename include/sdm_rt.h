@@ -579,6 +579,7 @@ int sdm_rt_token_logprobs(const sdm_rt_logprob* dims, const void* logits, int64_
 /* d_logits [rows][vocab] in dtype, every row written: the gradient of logprobs and entropy for d_logprobs and d_entropy,
  * float32 on the device, [rows] with a stride in elements (0: one value for all), or NULL:
  *   d z_j = (d_logprob (1[j = target] - p_j) - d_entropy p_j (l_j + entropy)) / temperature
+ * stats: of the same logits, targets and dims; with d_entropy of a call that asked for the entropy (else the gradient is NaN).
  * A row whose two gradients are 0 (d_logprob counts as 0 without a target) has gradient 0 whatever its logits hold.  It must
  * not overlap the logits. */
 int sdm_rt_token_logprobs_grad(const sdm_rt_logprob* dims, const void* logits, int64_t logits_row_stride,

@@ -69,9 +69,11 @@ __device__ __forceinline__ void write_row(const LogprobArgs& a, int64_t r, const
   if (a.logprobs) a.logprobs[r] = y.id < 0 ? 0.f : bad ? NAN : none ? -INFINITY : below_max(y.z, s.m, a.inv_tau) - g.l;
   const float h = bad ? NAN : none ? 0.f : g.h;
   if (a.entropy) a.entropy[r] = h;
-  // a row of -inf: sums that make every p 0
+  // a row of -inf: sums that make every p 0; the entropy is summed only where it is asked
   if (a.stats)
-    a.stats[r] = bad ? make_float4(NAN, NAN, NAN, 0.f) : none ? make_float4(0.f, INFINITY, 0.f, 0.f) : make_float4(s.m, g.l2, h, 0.f);
+    a.stats[r] = bad    ? make_float4(NAN, NAN, NAN, 0.f)
+                 : none ? make_float4(0.f, INFINITY, 0.f, 0.f)
+                        : make_float4(s.m, g.l2, a.entropy ? h : NAN, 0.f);
 }
 
 // -- a row, or a slice of one, by one workgroup -------------------------------------------------------------------------
@@ -622,6 +624,7 @@ __global__ void __launch_bounds__(kGradThreads) logprob_grad_kernel(LogprobGradA
     const float gb = a.dh ? a.dh[r * a.dh_stride] * a.inv_tau : 0.f;
     const bool live = !(ga == 0.f && gb == 0.f);
     const float4 s = a.stats[r];
+    const float entropy = a.dh ? s.z : 0.f;
     const int y = given && s.y != INFINITY ? static_cast<int>(y64) : -1;
     Piece<T> p[kGradPieces];
     if (live) {
@@ -642,7 +645,7 @@ __global__ void __launch_bounds__(kGradThreads) logprob_grad_kernel(LogprobGradA
 #pragma unroll
       for (int e = 0; e < kN; ++e) {
         const float t = (p[v].get(e) - s.x) * a.c - s.y, w = __builtin_amdgcn_exp2f(t);
-        o[e] = live ? -w * fmaf(gb, fmaf(fmaxf(t, -1000.f), kLn2, s.z), ga) : 0.f;
+        o[e] = live ? -w * fmaf(gb, fmaf(fmaxf(t, -1000.f), kLn2, entropy), ga) : 0.f;
       }
       if (static_cast<unsigned>(y - at) < static_cast<unsigned>(kN)) {
 #pragma unroll
