@@ -24,11 +24,12 @@ class AdamW(torch.optim.Optimizer):
 
     max_norm: gradients are clipped to this norm over all parameter groups, which must be on one GPU then; the .grad tensors
     stay as they are (a norm that is NaN reaches every parameter, as a product with it does).  state_bits: 32, or 8
-    (core.new_moments: 2.06 bytes a value instead of 8); a parameter group may have its own, as its own lr, betas, eps and
-    weight_decay.  capturable: the steps are counted on the GPU, so a graph may capture step() once it has run; lr may then be
-    a float32 tensor of one element that a schedule writes.  seed: of the 8-bit moments' rounding.  bfloat16 parameters are
-    rounded to nearest, so a change below half their last place is lost: keep float32 parameters and bfloat16 autocast where
-    that matters.  Sparse gradients and parameters whose values are not dense in memory are refused."""
+    (core.new_moments: 2.06 bytes a value instead of 8, in the order of the parameter's values in memory, which has to stay what
+    it is); a parameter group may have its own, as its own lr, betas, eps and weight_decay.  capturable: the steps are counted on
+    the GPU, so a graph may capture step() once it has run; lr may then be a float32 tensor of one element that a schedule
+    writes.  seed: of the 8-bit moments' rounding.  bfloat16 parameters are rounded to nearest, so a change below half their last
+    place is lost: keep float32 parameters and bfloat16 autocast where that matters.  Sparse gradients and parameters whose values
+    are not dense in memory are refused."""
 
     norm = None   # of the last step's gradients
     _OPTIONS = {"lr", "betas", "eps", "weight_decay", "state_bits", "max_norm", "capturable", "seed"}   # of a parameter group
