@@ -132,9 +132,30 @@ def _params(device, keys1, keys2, addr_b, log_scale, decay, onorm_w, gate_bias, 
     return prm, held
 
 
+graph_writes = False   # whether a captured step (adamw) writes any parameters
+_GRAPH_WRITTEN = WeakIdKeyDictionary()   # these
+
+
+def written_by_graphs(tensors):
+    """Whether a captured step writes one of these tensors: its replays count up no version, so nothing that is prepared from
+    them may be kept.  Asked only where graph_writes is set."""
+    return any(t is not None and t in _GRAPH_WRITTEN for t in tensors)
+
+
+def _mark_captured(params, index):
+    """Keeps in mind what a step writes that is being captured on GPU ``index``."""
+    global graph_writes
+    if torch.cuda.is_current_stream_capturing() if _current_device() == index else _lib.load().sdm_rt_capture_id(_raw_stream(index)):
+        graph_writes = True
+        for p in params:
+            _GRAPH_WRITTEN[p] = True
+            if p._base is not None:
+                _GRAPH_WRITTEN[p._base] = True
+
+
 class ParamCache:
     """The float32, contiguous copies of a module's core parameters and their SdmRtParams, rebuilt only when one of
-    the source tensors changes (data pointer or version)."""
+    the source tensors changes (data pointer or version; always, where a graph writes one)."""
 
     def __init__(self):
         self.key = None
@@ -144,7 +165,7 @@ class ParamCache:
         """decay may be a callable computing it; decay_source is then the tensor it derives from (the cache key)."""
         srcs = (keys1, keys2, addr_b, log_scale, decay_source if callable(decay) else decay, onorm_w, gate_bias)
         key = (device,) + tuple(None if t is None else (t.data_ptr(), t._version, t.dtype) for t in srcs)
-        if self.key != key:
+        if self.key != key or (graph_writes and written_by_graphs(srcs)):
             dec = decay() if callable(decay) else decay
             self.value = _params(device, keys1, keys2, addr_b, log_scale, dec, onorm_w, gate_bias)
             self.key = key
@@ -561,7 +582,8 @@ def _f32_weight(w, device):
     if w.dtype == torch.float32 and w.device == device and w.is_contiguous():
         return w.detach()
     hit = _W32.get(w)
-    if hit is not None and hit[0] == w._version and hit[1].device == device:
+    if hit is not None and hit[0] == w._version and hit[1].device == device and not (
+            graph_writes and w in _GRAPH_WRITTEN):
         return hit[1]
     f = w.detach().to(device=device, dtype=torch.float32).contiguous()
     _W32[w] = (w._version, f)
@@ -2027,6 +2049,7 @@ def adamw(params, grads, exp_avgs, exp_avg_sqs=None, *, step, lr=1e-3, betas=(0.
                                      1.0 if max_norm is None else max_norm, 8 if eight else 32, seed & 0xffffffff)
     _launch(_lib.load().sdm_rt_adamw, index, ctypes.byref(options), table, len(ps))
     native.written(ps, ms, vs or [], [] if t_dev is None else [t_dev])
+    _mark_captured(ps, index)
     return norm
 
 

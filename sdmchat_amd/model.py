@@ -47,8 +47,9 @@ class SwiGLU(nn.Module):
 
     def _gate_up(self):
         """[gate; up] stacked, cached until either changes."""
-        key = tuple((w.data_ptr(), w._version, w.dtype) for w in (self.gate.weight, self.up.weight))
-        if self._gu is None or self._gu[0] != key:
+        ws = (self.gate.weight, self.up.weight)
+        key = tuple((w.data_ptr(), w._version, w.dtype) for w in ws)
+        if self._gu is None or self._gu[0] != key or (core.graph_writes and core.written_by_graphs(ws)):
             self._gu = (key, torch.cat([self.gate.weight.detach(), self.up.weight.detach()], 0))
         return self._gu[1]
 

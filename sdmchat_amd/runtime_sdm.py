@@ -122,7 +122,7 @@ class RunTimeSdm(nn.Module):
         ws = (self.wk.weight, self.wq.weight, self.wg.weight, self.wv.weight)
         srcs = ws + (self.wg.bias, self.wo.weight)
         key = (dtype, ws[0].device, self.write_gate) + tuple((t.data_ptr(), t._version) for t in srcs)
-        if self._fused is not None and self._fused[0] == key:
+        if self._fused is not None and self._fused[0] == key and not (core.graph_writes and core.written_by_graphs(srcs)):
             return self._fused[1:]
         H, d_a, d = self.h, self.d_a, self.d
         ra = self._rows_a()

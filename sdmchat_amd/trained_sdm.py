@@ -69,7 +69,7 @@ class TrainedSdm(nn.Module):
         """wq and wo in the compute dtype, cached until either changes."""
         ws = (self.wq.weight, self.wo.weight)
         key = (dt,) + tuple((w.data_ptr(), w._version) for w in ws)
-        if self._cast is None or self._cast[0] != key:
+        if self._cast is None or self._cast[0] != key or (core.graph_writes and core.written_by_graphs(ws)):
             self._cast = (key,) + tuple(w.detach().to(dt) for w in ws)
         return self._cast[1], self._cast[2]
 
