@@ -172,6 +172,19 @@ class ParamCache:
         return self.value
 
 
+def prepared(module):
+    """What a module's layers have prepared of their weights, and their workspaces: tensors that a graph captured now reads and
+    writes where they are, and that the layers let go of when a weight changes or a larger call comes."""
+    out = [_W32.get(p) for p in module.parameters()]
+    for m in module.modules():
+        for v in vars(m).values():
+            if isinstance(v, (ParamCache, CoreWorkspace)):
+                out.append(v.value if isinstance(v, ParamCache) else v.buf)
+            elif isinstance(v, tuple):
+                out.append(v)
+    return out
+
+
 def workspace_bytes(dims):
     return _lib.load().sdm_rt_workspace_bytes(ctypes.byref(dims))
 

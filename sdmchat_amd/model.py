@@ -444,7 +444,8 @@ class DecodeGraph:
     every workspace and parameter cache exists before capture and nothing allocates inside the graph.  rules: a
     TokenRules of the B streams that every step's logits pass.  The graph reads and writes the tensors that rules had at
     capture where they are, and keeps them: what is written into them reaches the next replay, another tensor or number put
-    in their place does not."""
+    in their place does not.  It keeps what the layers have prepared of the model's weights, too: after a change of the
+    parameters, capture a new one."""
 
     def __init__(self, model, state, steps=1, rules=None):
         dev = model.emb.weight.device
@@ -463,6 +464,7 @@ class DecodeGraph:
             with torch.cuda.graph(self.graph):
                 outs = [model.step(self.tokens[t], state, **kw) for t in range(steps)]
                 self.logits = torch.stack(outs) if steps > 1 else outs[0]
+        self._held = core.prepared(model)
         state.pos -= steps   # capture ran no step
 
     def run(self, tokens):
@@ -481,8 +483,8 @@ class ForwardGraph:
     ``run(idx)`` copies the tokens into the graph's input, replays it and returns the graph's logits tensor
     (overwritten by the next run).  Capture first runs the forward twice on the same shapes, so that every workspace
     and parameter cache exists before capture; replays launch the whole forward at once, without the host's
-    per-kernel work between launches.  Inference only; the model's parameters must not be replaced while the graph
-    is in use (in-place updates are seen by the replays)."""
+    per-kernel work between launches.  Inference only; the graph keeps what the layers have prepared of the model's weights
+    at capture: after a change of the parameters, in place too, capture a new one."""
 
     def __init__(self, model, B, T):
         dev = model.emb.weight.device
@@ -498,6 +500,7 @@ class ForwardGraph:
             self.graph = torch.cuda.CUDAGraph()
             with torch.cuda.graph(self.graph):
                 self.logits = model(self.idx)
+        self._held = core.prepared(model)
 
     def run(self, idx):
         """idx [B, T] int64 -> logits [B, T, V]."""
