@@ -175,6 +175,8 @@ class ParamCache:
 def prepared(module):
     """What a module's layers have prepared of their weights, and their workspaces: tensors that a graph captured now reads and
     writes where they are, and that the layers let go of when a weight changes or a larger call comes."""
+    if not isinstance(module, torch.nn.Module):   # a model of another kind, with a step of its own
+        return []
     out = [_W32.get(p) for p in module.parameters()]
     for m in module.modules():
         for v in vars(m).values():
