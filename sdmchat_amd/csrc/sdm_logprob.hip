@@ -78,12 +78,15 @@ __device__ __forceinline__ void write_row(const LogprobArgs& a, int64_t r, const
 
 // -- a row, or a slice of one, by one workgroup -------------------------------------------------------------------------
 // The slice is in registers, NV 16-byte pieces a thread, so the row is read once: its maximum, its sums against that, and its
-// alternatives all come from there.  At most 64 registers a thread, so that four workgroups of a 32,768-logit bf16 row are on a
-// compute unit and load while others compute.  Without alternatives memory bounds it (16,384 x 32,768 bf16 with entropies 184 us,
-// 5.8 TB/s: what reading alone reaches here); a logit takes 4 instructions in the sums, one of them an exponential of four
-// issue slots, and 1 in the maximum.  With them instructions do (2,048 x 151,936 bf16, 64 alternatives, 141 us at 4.4 TB/s: some
-// 300 of a wave's 750 instructions are not the sums'), and a single row the chain of its phases (32,768 logits 7 us).  Slices of
-// 65,536 logits take that case to 189 us, of 16,384 to 173; a row of 32,768 in two slices and a join 12.6 us in place of 8.8.
+// alternatives all come from there.  At most 64 registers a thread, so that four workgroups of a 32,768-logit bf16 row are on
+// a compute unit and load while others compute.  Without alternatives memory bounds it (16,384 x 32,768 bf16 with entropies
+// 182 us call after call, 5.9 TB/s: what reading alone reaches here; a profiled training step's, behind a gradient, 245 in the
+// median); a logit takes 4 instructions in the sums, one of them an exponential of four issue slots, and 1 in the maximum.
+// With half of each row masked the entropies' sums are made twice (0 times -inf): 274 us, 192 without entropies.  With
+// alternatives instructions bound it (2,048 x 151,936 bf16, 64 of them, 141 us at 4.4 TB/s: some 300 of a wave's 750
+// instructions are not the sums'; with the join 64 take 143 us, 96 160, 128 186, 192 292, 256 525: a workgroup's LDS grows to
+// 65 KB), and a single row the chain of its phases (32,768 logits 7 us).  Slices of 65,536 logits take the case of 64 to 189
+// us, of 16,384 to 173; a row of 32,768 in two slices and a join 12.6 us in place of 8.8.
 constexpr int kMaxSlots = kMaxAlternatives + kMaxAlternatives / 2 + 8;
 constexpr int kCandidates = 1024;   // keys that are ranked against each other
 constexpr uint32_t kLowest = 0x00800000u;   // the key of the least finite number
@@ -196,8 +199,9 @@ __device__ __forceinline__ void in_turn(Piece<T>& p) {
 // Ties in great number, or the best logits in a few threads' pieces: more than kCandidates logits at or above the threshold.
 // The workgroup halves the range of keys until k to kCandidates logits are at or above one, or it is down to the k-th greatest
 // key itself, of which it then takes as many as are wanted in the order of their ids.  The slice's pieces are read again each
-// time, from the caches (held in registers they made the whole kernel spill); all threads get here together.  Returns how many keys it has listed.  64 x 32,768
-// bf16 rows of few different values, 20 alternatives: 30 us; counting from memory each time 210.
+// time, from the caches (held in registers they made the whole kernel spill); all threads get here together.  Returns how many
+// keys it has listed.  64 x 32,768 bf16 rows of few different values, 20 alternatives: 30 us; counting from memory each time
+// 210.
 template <typename T, int NV>
 __device__ __noinline__ int crowded(int k, const T* z, int n, int first, uint32_t lo, uint32_t hi, RowLds& lds) {
   constexpr int kN = Piece<T>::kN, kDrop = sizeof(T) == 2 ? 16 : 0;   // bits that a key of bfloat16 does not use
@@ -605,8 +609,9 @@ struct LogprobGradArgs {
 };
 
 // -- the gradient -------------------------------------------------------------------------------------------------------
-// One workgroup per segment of a row, kGradPieces pieces a thread: a logit in, its gradient out, bound by memory (16,384 x 32,768
-// bf16 343 us, 6.3 TB/s read and written; rows in reverse, to meet what the forward left in the caches, the same).
+// One workgroup per segment of a row, kGradPieces pieces a thread: a logit in, its gradient out, bound by memory (16,384 x
+// 32,768 bf16 343 us in the median of a profiled step, 6.3 TB/s read and written; rows in reverse, to meet what the forward
+// left in the caches, the same).
 constexpr int kGradThreads = 256, kGradPieces = 4;
 
 template <typename T, bool THROUGH>

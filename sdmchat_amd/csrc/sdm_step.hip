@@ -307,9 +307,10 @@ __device__ __forceinline__ void step_chunk32(const StepArgs& a, float clip, T* p
   }
 }
 
-// Sixteen lanes hold a block, 8 values each: its maxima come from four DPP steps.  Past a tensor's end p, g and the codes are 0
-// and stay so.  The codes do not stream past the caches: their lines are shared by neighbouring lanes' pieces (14 M values 43.5 us,
-// 48.9 if they do).  Bound by memory and instructions alike: 110 M bfloat16 values 217 us, 5.1 TB/s, 52 instructions a value.
+// Sixteen lanes hold a block, 8 values each: its maxima come from four DPP steps.  Past a tensor's end p, g and the codes are
+// 0 and stay so.  The codes do not stream past the caches: their lines are shared by neighbouring lanes' pieces (14 M values
+// 43.5 us, 48.9 if they do).  Bound by memory and instructions alike: 110 M bfloat16 values 210 us call after call, 5.3 TB/s,
+// 52 instructions a value (a profiled step's, behind the norm and before read_moments, 237 in the median).
 template <bool THROUGH, bool TINY, typename T>
 __device__ __forceinline__ void step_chunk8(const StepArgs& a, float clip, T* p, const T* g, char* chunk, uint32_t position, int n) {
   const int whole = (n + kBlock - 1) / kBlock * kBlock;
@@ -491,8 +492,11 @@ void for_tables(const sdm_rt_tensor* t, int32_t count, int chunk, TAKE take, LAU
   flush();
 }
 
-// Few values take small chunks, so that all compute units have some: the norm of 14 M values 13.2 us in chunks of 4,096, 15.0 of
-// 16,384, of 110 M 55 and 41; an 8-bit step of 14 M values 40 us in chunks of 2,048, 42 of 4,096, of 110 M 236 and 220.
+// Few values take small chunks, so that all compute units have some: a model's 14 M float32 values' norm 13.2 us in chunks of
+// 4,096, 15.0 of 16,384, their 8-bit step 40 us in chunks of 2,048, 42 of 4,096.  One bfloat16 tensor would cross over
+// earlier: norms of 4, 8, 16, 32 and 105 Mi values 9.8, 10.2, 11.0, 19.6, 50.8 us in small chunks, 11.6, 9.9, 9.7, 15.7, 36.9
+// in large ones, 8-bit steps 11.2, 23.2, 38.0, 73.1, 211 and 11.4, 19.4, 35.4, 66.5, 192; lists of many tensors between the
+// two sizes were not compared.
 constexpr int64_t kSmallStep = 16 << 20, kSmallNorm = 32 << 20;
 
 inline int norm_chunk(int64_t values) { return values <= kSmallNorm ? 4096 : 16384; }
