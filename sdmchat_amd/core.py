@@ -1644,10 +1644,9 @@ def _per_row(name, what, v, B, device):
         raise ValueError(f"{name}: {what} must be a number or a floating-point tensor [B={B}], got {v.dtype} {tuple(v.shape)}")
     if v.device != device:
         raise ValueError(f"{name}: {what} is on {v.device}, expected {device}")
-    v = v.resolve_neg()
-    if v.dtype == torch.float32 and v.dim() == 1 and v.shape[0] == B and v.is_contiguous():
+    if v.dtype == torch.float32 and v.dim() == 1 and v.shape[0] == B and v.is_contiguous() and not v.is_neg():
         return v, 0.0
-    return v.detach().to(torch.float32).reshape(-1).expand(B).contiguous(), 0.0
+    return v.detach().resolve_neg().to(torch.float32).reshape(-1).expand(B).contiguous(), 0.0
 
 
 def _row_or_rows(name, what, t, B, width, dtype):
@@ -1655,7 +1654,11 @@ def _row_or_rows(name, what, t, B, width, dtype):
     shape = t.shape
     if t.dtype != dtype or shape[-1:] != (width,) or len(shape) > 2 or (len(shape) == 2 and shape[0] != B):
         raise ValueError(f"{name}: {what} must be {dtype} [{width}] or [B={B}, {width}], got {t.dtype} {tuple(shape)}")
-    return (t.contiguous().resolve_neg(), 0) if len(shape) == 1 else _read_rows(t)
+    if len(shape) > 1:
+        return _read_rows(t)
+    if not t.is_contiguous():
+        t = t.contiguous()
+    return (t.resolve_neg() if dtype is torch.float32 and t.is_neg() else t), 0
 
 
 def pack_mask(allowed):
