@@ -142,15 +142,14 @@ def written_by_graphs(tensors):
     return any(t is not None and t in _GRAPH_WRITTEN for t in tensors)
 
 
-def _mark_captured(params, index):
-    """Keeps in mind what a step writes that is being captured on GPU ``index``."""
+def _mark_captured(params):
+    """Keeps in mind what a step writes that is being captured."""
     global graph_writes
-    if torch.cuda.is_current_stream_capturing() if _current_device() == index else _lib.load().sdm_rt_capture_id(_raw_stream(index)):
-        graph_writes = True
-        for p in params:
-            _GRAPH_WRITTEN[p] = True
-            if p._base is not None:
-                _GRAPH_WRITTEN[p._base] = True
+    graph_writes = True
+    for p in params:
+        _GRAPH_WRITTEN[p] = True
+        if p._base is not None:
+            _GRAPH_WRITTEN[p._base] = True
 
 
 class ParamCache:
@@ -2065,9 +2064,11 @@ def adamw(params, grads, exp_avgs, exp_avg_sqs=None, *, step, lr=1e-3, betas=(0.
         norm = norm.resolve_neg()
     options = _lib.SdmRtAdamwOptions(lr, betas[0], betas[1], eps, weight_decay, step, _ptr(t_dev), _ptr(lr_dev), _ptr(norm),
                                      1.0 if max_norm is None else max_norm, 8 if eight else 32, seed & 0xffffffff)
-    _launch(_lib.load().sdm_rt_adamw, index, ctypes.byref(options), table, len(ps))
+    lib = _lib.load()
+    _launch(lib.sdm_rt_adamw, index, ctypes.byref(options), table, len(ps))
     native.written(ps, ms, vs or [], [] if t_dev is None else [t_dev])
-    _mark_captured(ps, index)
+    if lib.sdm_rt_capture_id(_raw_stream(index)):
+        _mark_captured(ps)
     return norm
 
 
